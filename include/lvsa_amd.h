@@ -285,6 +285,104 @@ LVSA_API int lvsa_gather_frames(const void* src, const int64_t src_str[3], void*
                        const int32_t* frames, int32_t n_frames, int32_t P,
                        int32_t B, int32_t H, int32_t D, int32_t elem_bytes, hipStream_t stream);
 
+/* ───────────────────────── paged key/value cache ───────────────────────── */
+
+/* Keys and values of many sequences in pages of `page_size` token slots.
+ * Page p, slot t, head h of a 16-bit cache: D elements at
+ * k + (p * k_str[0] + t * k_str[1] + h * k_str[2]) elements.  A 4-bit cache
+ * holds E2M1 codes there (element d in byte d / 2, the low four bits for even
+ * d; strides in bytes) and, at k_scale with ks_str, one byte for every 32
+ * elements: the scale 2^(byte - 127), 255 for a group of NaN.  Row addresses
+ * are multiples of 16 bytes (the scales' of one).
+ * `status` (optional, one int32, never cleared by a call): calls set
+ * LVSA_PAGED_* bits in it for what they find on the device.                  */
+typedef struct lvsa_paged_cache {
+  void* k; void* v;
+  void* k_scale; void* v_scale;          /* 4 bits only                         */
+  int64_t k_str[3], v_str[3], ks_str[3], vs_str[3];   /* page, slot, head        */
+  int32_t n_pages, page_size, Hkv, D;    /* D = 64, 96, 128, 192 or 256          */
+  int32_t bits;                          /* 16 or 4                             */
+  int32_t dtype;                         /* of the caller's tensors (and of a
+                                            16-bit cache): LVSA_BF16 / LVSA_FP16 */
+  int32_t* status;
+} lvsa_paged_cache;
+
+#define LVSA_PAGED_BAD_PAGE 1     /* a page number outside [0, n_pages)            */
+#define LVSA_PAGED_BAD_LENGTH 2   /* kv_lens negative or beyond the table's pages  */
+#define LVSA_PAGED_BAD_CU 4       /* cu_seqlens not ascending within [0, N]        */
+#define LVSA_PAGED_BAD_APPEND 8   /* more new tokens than kv_lens counts           */
+#define LVSA_PAGED_BAD_POSITION 16 /* a rotation position outside the angle table  */
+
+/* A batch over a cache, all device memory.  Sequence b has kv_lens[b] cached
+ * tokens, position p in slot p % page_size of page page_table[b * table_stride
+ * + p / page_size].  Of N packed rows, cu_seqlens[b] .. cu_seqlens[b + 1] - 1
+ * are its newest tokens: row cu_seqlens[b] + i is position kv_lens[b] -
+ * (cu_seqlens[b + 1] - cu_seqlens[b]) + i.  Rows from cu_seqlens[B] on belong
+ * to no sequence.                                                           */
+typedef struct lvsa_paged_batch {
+  const int32_t* cu_seqlens;      /* [B + 1]                                      */
+  const int32_t* kv_lens;         /* [B]                                          */
+  const int32_t* page_table;      /* [B] rows of max_pages                        */
+  int64_t table_stride;
+  int32_t B, max_pages, N;
+} lvsa_paged_batch;
+
+/* Writes new tokens' keys and values to the cache (kv_lens counts them
+ * already), keys turned by their positions, and the turned queries to q_out.
+ * k / v [N, Hkv, D], q / q_out [N, H, D] (null: none); strides of token and
+ * head in elements.  Row p of cos / sin [n_angles, rot / 2] (fp32, null: no
+ * rotation) belongs to position p; `positions` [N] (null: the position in the
+ * cache) names another row.  The first `rot` dimensions turn (a multiple of 16):
+ * (a, b) -> (a cos - b sin, b cos + a sin) with pairs (2i, 2i + 1) if
+ * `interleaved`, else (i, i + rot / 2).  Tokens with a bad page, length, row range or
+ * position are not written, and their q_out is NaN.  Two tokens of a call must
+ * not share a slot.  The reference has neither cache nor rotation here: its
+ * adapters rotate Q and K before the attention call (lvsa/rope.py:10-27).     */
+typedef struct lvsa_paged_append_args {
+  lvsa_paged_cache cache;
+  lvsa_paged_batch batch;
+  const void* k; const void* v; const void* q; void* q_out;
+  int64_t k_str[2], v_str[2], q_str[2], qo_str[2];
+  const float* cos; const float* sin;
+  const int32_t* positions;
+  int32_t H, rot, interleaved, n_angles;
+} lvsa_paged_append_args;
+LVSA_API int lvsa_paged_append(const lvsa_paged_append_args* a, hipStream_t stream);
+
+/* Reads every sequence's cached keys and values into k_out / v_out
+ * [B, max_len, Hkv, D] (contiguous, in `dtype` of the cache struct); zeros
+ * behind a sequence's end, NaN where its page is bad.  cu_seqlens and N of the
+ * batch are not used.  The paged counterpart of lvsa_gather_frames.           */
+LVSA_API int lvsa_paged_gather(const lvsa_paged_cache* cache, const lvsa_paged_batch* batch, void* k_out, void* v_out,
+                               int32_t max_len, hipStream_t stream);
+
+/* Attention of the N newest tokens over the cache: q / o [N, H, D] (H a multiple
+ * of Hkv), row at position p attends its sequence's keys below kv_lens and, if
+ * `causal`, up to p.  o = sum_j softmax_j(scale q.k_j) v_j, lse (optional,
+ * [N, H], contiguous) its natural log-sum-exp; a row without keys gets 0 and
+ * -inf, a row of a sequence with a bad page or length NaN.  Keys
+ * that a row does not attend have no effect on it, infinities and NaN
+ * included.  Rows of no sequence are zeroed (lse -inf) if `fill_tail`, else
+ * left as they are.  `max_q_len` and `max_kv_len` (0: unknown) only choose a kernel and its
+ * split; results hold whatever they say.  Workspace: device memory of
+ * lvsa_paged_attn_workspace_query bytes, 16-byte aligned, any contents,
+ * not shared by calls that overlap.                                          */
+typedef struct lvsa_paged_attn_args {
+  lvsa_paged_cache cache;
+  lvsa_paged_batch batch;
+  const void* q; void* o; float* lse;
+  int64_t q_str[2], o_str[2];
+  float scale;
+  int32_t H, causal, fill_tail, max_q_len, max_kv_len;
+  void* workspace;
+  int64_t workspace_bytes;
+} lvsa_paged_attn_args;
+LVSA_API int lvsa_paged_attn_fwd(const lvsa_paged_attn_args* a, hipStream_t stream);
+
+/* Bytes of workspace lvsa_paged_attn_fwd needs for `a` on the current device
+ * (a->workspace and workspace_bytes are not read); host only.                 */
+LVSA_API int lvsa_paged_attn_workspace_query(const lvsa_paged_attn_args* a, int64_t* bytes);
+
 /* Library identification and error reporting. */
 LVSA_API const char* lvsa_version(void);
 LVSA_API const char* lvsa_last_error(void);

@@ -21,12 +21,16 @@ _SPARSE = (
 _BLOCK = ("BlockSparseAttentionWrapper", "single_prefill_with_kv_cache", "HipDualStreamRunner",
           "get_shared_runner")
 
+_PAGED = ("PagedKVCache", "paged_kv_append", "paged_kv_gather", "paged_attention")
+
 
 def __getattr__(name):
     if name in _SPARSE:
         from . import sparse_attention as m
     elif name in _BLOCK:
         from . import block_sparse as m
+    elif name in _PAGED:
+        from . import paged_kv as m
     elif name == "build_global_kv":
         from . import global_kv as m
     elif name == "DistributedLVSAProcessor":
@@ -40,4 +44,4 @@ def __getattr__(name):
     return value
 
 
-__all__ = list(_SPARSE) + list(_BLOCK) + ["build_global_kv", "DistributedLVSAProcessor", "step_attention"]
+__all__ = list(_SPARSE) + list(_BLOCK) + list(_PAGED) + ["build_global_kv", "DistributedLVSAProcessor", "step_attention"]

@@ -105,6 +105,48 @@ class AttnArgs(C.Structure):
     ]
 
 
+# Bits of a paged cache's status word (LVSA_PAGED_*).
+PAGED_BAD_PAGE, PAGED_BAD_LENGTH, PAGED_BAD_CU, PAGED_BAD_APPEND, PAGED_BAD_POSITION = 1, 2, 4, 8, 16
+
+_Str2 = C.c_int64 * 2
+
+
+class PagedCache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("k_str", _Str3), ("v_str", _Str3), ("ks_str", _Str3), ("vs_str", _Str3),
+        ("n_pages", C.c_int32), ("page_size", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32),
+        ("bits", C.c_int32), ("dtype", C.c_int32), ("status", C.c_void_p),
+    ]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [
+        ("cu_seqlens", C.c_void_p), ("kv_lens", C.c_void_p), ("page_table", C.c_void_p),
+        ("table_stride", C.c_int64), ("B", C.c_int32), ("max_pages", C.c_int32), ("N", C.c_int32),
+    ]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("batch", PagedBatch),
+        ("k", C.c_void_p), ("v", C.c_void_p), ("q", C.c_void_p), ("q_out", C.c_void_p),
+        ("k_str", _Str2), ("v_str", _Str2), ("q_str", _Str2), ("qo_str", _Str2),
+        ("cos", C.c_void_p), ("sin", C.c_void_p), ("positions", C.c_void_p),
+        ("H", C.c_int32), ("rot", C.c_int32), ("interleaved", C.c_int32), ("n_angles", C.c_int32),
+    ]
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("batch", PagedBatch),
+        ("q", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p), ("q_str", _Str2), ("o_str", _Str2),
+        ("scale", C.c_float), ("H", C.c_int32), ("causal", C.c_int32), ("fill_tail", C.c_int32),
+        ("max_q_len", C.c_int32), ("max_kv_len", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
 # Every symbol the header declares, with its ctypes signature.
 SIGNATURES = {
     "lvsa_mask_sizes_query": (C.c_int, [C.POINTER(MaskParams), C.POINTER(MaskSizes)]),
@@ -122,6 +164,11 @@ SIGNATURES = {
     "lvsa_gather_frames": (C.c_int, [C.c_void_p, C.POINTER(C.c_int64), C.c_void_p, C.POINTER(C.c_int64),
                                      C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                      C.c_int32, C.c_void_p]),
+    "lvsa_paged_append": (C.c_int, [C.POINTER(PagedAppendArgs), C.c_void_p]),
+    "lvsa_paged_gather": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedBatch), C.c_void_p, C.c_void_p, C.c_int32,
+                                    C.c_void_p]),
+    "lvsa_paged_attn_fwd": (C.c_int, [C.POINTER(PagedAttnArgs), C.c_void_p]),
+    "lvsa_paged_attn_workspace_query": (C.c_int, [C.POINTER(PagedAttnArgs), C.POINTER(C.c_int64)]),
     "lvsa_version": (C.c_char_p, []),
     "lvsa_last_error": (C.c_char_p, []),
 }

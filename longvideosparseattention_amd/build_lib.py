@@ -39,6 +39,12 @@ SOURCES = {
     "lvsa_attn_d192.hip": MAXOCC,
     "lvsa_attn_d256.hip": MAXOCC,
     "lvsa_attn_f32.hip": [],
+    "lvsa_paged.hip": [],
+    "lvsa_paged_d64.hip": [],
+    "lvsa_paged_d96.hip": [],
+    "lvsa_paged_d128.hip": [],
+    "lvsa_paged_d192.hip": [],
+    "lvsa_paged_d256.hip": [],
 }
 
 HIPCC_FLAGS = [

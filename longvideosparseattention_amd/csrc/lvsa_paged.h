@@ -1,0 +1,177 @@
+// What the kernels over the paged key/value cache share (lvsa_paged.hip:
+// append, gather, merge and the C ABI; lvsa_paged_attn.h: attention, one unit
+// per head size): the cache and batch as the device sees them, the lookup of
+// rows through the page table, and the number format of 4-bit pages.
+//
+// Nothing read from device memory is trusted: page numbers, lengths and row
+// ranges are checked where they are used, so that no address leaves the
+// cache's pages or the batch's rows; what is found is reported in the cache's
+// status word (LVSA_PAGED_*).
+#pragma once
+#include "lvsa_common.h"
+
+namespace lvsa {
+
+struct PagedView {
+  // 16-bit elements or E2M1 codes and their scales; strides in bytes
+  char* k; char* v;
+  uint8_t* ks; uint8_t* vs;
+  int64_t k_str[3], v_str[3], ks_str[3], vs_str[3];
+  int32_t n_pages, page_size, Hkv;
+  uint32_t ps_mul, ps_shift;     // p / page_size = (p * ps_mul) >> ps_shift for 0 <= p < 2^31
+  int32_t* status;
+  const int32_t* cu;
+  const int32_t* lens;
+  const int32_t* table;
+  int64_t table_str;
+  int32_t B, max_pages, N;
+};
+
+struct PagedAttnParams {
+  PagedView c;
+  const char* q; char* o; float* lse;
+  int64_t q_str[2], o_str[2];    // bytes
+  float scale_log2;              // scale * log2(e)
+  int32_t H, group, causal, fill_tail;
+  // Decode kernel: `grid` work-groups share the launch's key blocks; each has
+  // two slots of row-tile partials.  Prefill kernel: `tiles` bounds the row
+  // tiles of all sequences, every tile's key blocks run as `splits` parts with
+  // a slot each.  Partials: fp32 O [slot][rows][D], then (max, sum) pairs.
+  int32_t grid, tiles, splits;
+  float* ws_o; float* ws_ml;
+};
+
+// Attention launches per head size.  rows: 16 or 32 (decode kernel, row tiles
+// of that many rows) or 128 (prefill kernel).
+int paged_attn_d64(const PagedAttnParams& p, int bits, int rows, bool bf16, hipStream_t stream);
+int paged_attn_d96(const PagedAttnParams& p, int bits, int rows, bool bf16, hipStream_t stream);
+int paged_attn_d128(const PagedAttnParams& p, int bits, int rows, bool bf16, hipStream_t stream);
+int paged_attn_d192(const PagedAttnParams& p, int bits, int rows, bool bf16, hipStream_t stream);
+int paged_attn_d256(const PagedAttnParams& p, int bits, int rows, bool bf16, hipStream_t stream);
+
+// Keys that the four waves of a decode work-group take per step.
+__host__ __device__ constexpr int paged_decode_keys(int D) { return 4 * (D >= 192 ? 16 : 32); }
+constexpr int kPagedTile = 128;        // rows of a prefill tile
+constexpr int kPagedBlock = 64;        // its keys per step
+
+// The running maximum of a row that has seen no key: below every finite score,
+// and still finite, so that differences to it are never NaN.
+constexpr float kNoKeys = -3.0e38f;
+
+// ── lookups, alike on host and device (tests/native/paged_map_check.cpp) ─────
+
+__host__ __device__ inline int page_of(const PagedView& c, int pos) {
+  return (int)(((uint64_t)(uint32_t)pos * c.ps_mul) >> c.ps_shift);
+}
+
+// Sequence s: its rows [t0, t0 + n) of the packed ones, its cached length, and
+// the position of row t0.  Ranges and lengths outside what the caller
+// allocated are cut to it and flagged.
+struct PagedSeq {
+  int t0, n, L, first;
+  int flags;
+};
+__host__ __device__ inline PagedSeq paged_seq(const PagedView& c, int s) {
+  PagedSeq r;
+  const int a = c.cu[s], e = c.cu[s + 1], len = c.lens[s];
+  const int64_t cap = (int64_t)c.max_pages * c.page_size;
+  r.flags = 0;
+  r.L = len;
+  if (len < 0) r.L = 0;
+  if (len > cap) r.L = (int)cap;
+  if (r.L != len) r.flags |= LVSA_PAGED_BAD_LENGTH;
+  const int lo = a < 0 ? 0 : a, hi = e > c.N ? c.N : e;
+  if (a < 0 || e > c.N || e < a) r.flags |= LVSA_PAGED_BAD_CU;
+  r.t0 = lo;
+  r.n = hi > lo ? hi - lo : 0;
+  const int64_t first = (int64_t)r.L - ((int64_t)e - lo);
+  r.first = first < -(1 << 30) ? -(1 << 30) : first > INT32_MAX ? INT32_MAX : (int)first;
+  return r;
+}
+
+// Key position that a kernel reads for `pos`: past the end the last key, whose
+// weight is masked away.  L >= 1.
+__host__ __device__ inline int key_within(int pos, int L) { return pos < L ? pos : L - 1; }
+
+// Page and slot of position `pos` whose table entry is `page`; a page outside
+// the cache is read as page 0.
+struct PagedRow {
+  int64_t page, slot;
+  bool ok;
+};
+__host__ __device__ inline PagedRow paged_row(const PagedView& c, int pos, int page) {
+  PagedRow r;
+  r.slot = pos - page_of(c, pos) * c.page_size;
+  r.ok = (uint32_t)page < (uint32_t)c.n_pages;
+  r.page = r.ok ? page : 0;
+  return r;
+}
+
+// Work units of a sequence in the decode kernel: (row tiles) x (key heads) x
+// (key steps), key steps innermost.
+__host__ __device__ inline int64_t decode_units(const PagedAttnParams& p, const PagedSeq& q, int rows, int keys) {
+  const int64_t rt = ((int64_t)q.n * p.group + rows - 1) / rows;
+  return rt * p.c.Hkv * (((int64_t)q.L + keys - 1) / keys);
+}
+
+// Shares of U > 0 units over a grid: none is empty, so that the work-groups a
+// row tile spans all have a partial of it.
+__host__ __device__ inline int unit_shares(int64_t U, int grid) { return U < grid ? (int)U : grid; }
+// First unit of share w of G over U units, and the share of unit u.
+__host__ __device__ inline int64_t unit_start(int64_t U, int G, int w) { return w * U / G; }
+__host__ __device__ inline int wg_of_unit(int64_t U, int G, int64_t u) { return (int)(((u + 1) * G - 1) / U); }
+
+// Partials of the row tile whose key steps are units [u0, u0 + nb): none if one
+// work-group has them all, else one per work-group, in the first of its two
+// slots but where it came to the tile from another one.
+struct DecodeSlots {
+  int count;
+  int64_t first, rest;      // slot of partial 0; slot of partial i > 0: rest + 2 i
+};
+__host__ __device__ inline DecodeSlots decode_slots(int64_t U, int G, int64_t u0, int nb) {
+  const int wa = wg_of_unit(U, G, u0), wb = wg_of_unit(U, G, u0 + nb - 1);
+  if (wa == wb) return DecodeSlots{0, 0, 0};
+  return DecodeSlots{wb - wa + 1, 2 * (int64_t)wa + (unit_start(U, G, wa) < u0 ? 1 : 0), 2 * (int64_t)wa};
+}
+
+// p / d as (p * mul) >> shift, exact for 0 <= p < 2^31: with 2^l >= d and mul =
+// floor(2^(31 + l) / d) + 1, mul * d exceeds 2^(31 + l) by at most 2^l.
+inline void set_page_size(PagedView* v, int page_size) {
+  int l = 0;
+  while ((1LL << l) < page_size) ++l;
+  v->page_size = page_size;
+  v->ps_mul = (uint32_t)((1ULL << (31 + l)) / (uint64_t)page_size + 1);
+  v->ps_shift = (uint32_t)(31 + l);
+}
+
+namespace {
+
+__device__ __forceinline__ void paged_flag(const PagedView& c, int bit) {
+  if (c.status) atomicOr(c.status, bit);
+}
+
+// The sequence that row t belongs to (the same for every lane of the wave; t
+// uniform), or -1.
+__device__ __forceinline__ int paged_seq_of_row(const PagedView& c, int t, int lane) {
+  for (int s0 = 0; s0 < c.B; s0 += 64) {
+    const int s = s0 + lane;
+    bool in = false;
+    if (s < c.B) in = c.cu[s] <= t && t < c.cu[s + 1];
+    const uint64_t m = __builtin_amdgcn_ballot_w64(in);
+    if (m) return s0 + __builtin_ctzll(m);
+  }
+  return -1;
+}
+
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ int64_t wave_scan(int64_t x, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+}  // namespace
+}  // namespace lvsa

@@ -1,0 +1,691 @@
+// Paged key/value cache on gfx950: appending new tokens (rotation by position
+// and 4-bit quantisation on the way), reading a cache back, the merge of
+// attention partials, and the C ABI.  The attention kernels are in
+// lvsa_paged_attn.h.
+#include "lvsa_paged.h"
+
+#include <mutex>
+
+using namespace lvsa;
+
+namespace lvsa {
+namespace {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kMaxGrid = 1 << 20;      // work-groups of a launch that walks its rows
+
+template <typename E> struct Half;
+template <> struct Half<__bf16> {
+  static constexpr uint32_t kNaN = 0x7fc0u;
+  __device__ static void unpack(u32x4 u, float* x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __builtin_bit_cast(float, u[i] << 16);
+      x[2 * i + 1] = __builtin_bit_cast(float, u[i] & 0xffff0000u);
+    }
+  }
+};
+template <> struct Half<_Float16> {
+  static constexpr uint32_t kNaN = 0x7e00u;
+  __device__ static void unpack(u32x4 u, float* x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)u[i]);
+      x[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(u[i] >> 16));
+    }
+  }
+};
+template <typename E>
+__device__ __forceinline__ u32x4 pack8(const float* x) {
+  u32x4 u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    typedef E v2 __attribute__((ext_vector_type(2)));
+    u[i] = __builtin_bit_cast(uint32_t, v2{(E)x[2 * i], (E)x[2 * i + 1]});
+  }
+  return u;
+}
+
+// Eight 4-bit values at byte scale `s` (2^(s - 127), 255: NaN).  Exact in both
+// types for the scales that the append writes.
+template <typename E>
+__device__ __forceinline__ u32x4 unpack_e2m1(uint32_t codes, uint32_t s) {
+  const float f = __builtin_bit_cast(float, s << 23);
+  u32x4 u;
+  if constexpr (__is_same(E, __bf16)) {
+    u[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, f, 0));
+    u[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, f, 1));
+    u[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, f, 2));
+    u[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, f, 3));
+  } else {
+    u[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, f, 0));
+    u[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, f, 1));
+    u[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, f, 2));
+    u[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, f, 3));
+  }
+  return u;
+}
+
+// x in 32 bits, rounded to odd: the two neighbours' sticky bit is kept, so that
+// a later rounding to few bits (and a comparison with a number of few bits)
+// comes out as if it had been made from the 64-bit value.
+__device__ __forceinline__ float to_odd(double x) {
+  float f = (float)x;
+  if (__builtin_isinf(f) && !__builtin_isinf(x)) return __builtin_copysignf(3.0e38f, f);
+  const double back = (double)f;
+  if (back != x) {       // false for NaN with NaN's payload only: handled by the caller's non-finite test
+    uint32_t b = __builtin_bit_cast(uint32_t, f);
+    if (__builtin_fabs(back) > __builtin_fabs(x)) b -= 1;   // |f| rounded up: back to the neighbour below
+    f = __builtin_bit_cast(float, b | 1u);
+  }
+  return f;
+}
+
+// ──────────────────────────────── append ───────────────────────────────────
+
+struct AppendParams {
+  PagedView c;
+  const char* k; const char* v; const char* q; char* qo;
+  int64_t k_str[2], v_str[2], q_str[2], qo_str[2];   // bytes
+  const float* cos; const float* sin;
+  const int32_t* positions;
+  int H, rot, interleaved, n_angles;
+};
+
+// One work-group per token; a thread holds chunk `c` (8 elements) of every
+// RPP-th row, where the rows are the token's keys, values and queries.  The
+// chunk's angles are read once and serve all of them.  A rotated element
+// needs its partner: in the same chunk with interleaved pairs, else rot / 2
+// elements away, which is a second 16-byte load of a line that the neighbours
+// fetch anyway.  Bound by memory.
+//
+// 16-bit caches: turned in fp32, one rounding at the end.  4-bit caches: the
+// turned key is formed in 64 bits, where both products are exact and the sum
+// rounds once, and goes to odd-rounded fp32 for the converter: a key next to
+// the border of two codes or of two scales comes out as the exact value's
+// would, on every device and in every order of evaluation.
+template <int D, typename E, int BITS>
+__device__ __forceinline__ void append_token(const AppendParams& p, int t) {
+  constexpr int CH = D / 8, RPP = 256 / CH;
+  const int lane = threadIdx.x & 63;
+  const int s = paged_seq_of_row(p.c, t, lane);
+  if (s < 0) return;                        // a row of no sequence: left alone
+  const PagedSeq sq = paged_seq(p.c, s);
+  const int64_t pos = (int64_t)sq.first + (t - sq.t0);
+  int flags = sq.flags;
+  int64_t page = 0, slot = 0;
+  if (pos < 0) flags |= LVSA_PAGED_BAD_APPEND;
+  if (!(flags & (LVSA_PAGED_BAD_LENGTH | LVSA_PAGED_BAD_APPEND | LVSA_PAGED_BAD_CU))) {
+    const PagedRow row = paged_row(p.c, (int)pos, p.c.table[s * p.c.table_str + page_of(p.c, (int)pos)]);
+    page = row.page;
+    slot = row.slot;
+    if (!row.ok) flags |= LVSA_PAGED_BAD_PAGE;
+  }
+  int64_t angle = pos;
+  if (p.rot) {
+    if (p.positions) angle = p.positions[t];
+    if (angle < 0 || angle >= p.n_angles) flags |= LVSA_PAGED_BAD_POSITION;
+  }
+  const bool bad = flags != 0;
+  if (bad && threadIdx.x == 0) paged_flag(p.c, flags);
+
+  const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
+  if (r0 >= RPP) return;                    // D = 96 and 192 leave a few threads over; whole groups of four
+  const int half = p.rot / 2;
+  const bool turn = 8 * c < p.rot;
+  float cs[8], sn[8];
+  int partner = 0;
+  bool second = false;                      // this chunk holds the second elements of its pairs
+  if (turn && !bad) {
+    const int64_t base = angle * half;
+    if (p.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        cs[i] = p.cos[base + 4 * c + i];
+        sn[i] = p.sin[base + 4 * c + i];
+      }
+    } else {
+      second = 8 * c >= half;
+      const int i0 = second ? 8 * c - half : 8 * c;
+      partner = second ? -half : half;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        cs[i] = p.cos[base + i0 + i];
+        sn[i] = second ? p.sin[base + i0 + i] : -p.sin[base + i0 + i];
+      }
+    }
+  }
+
+  const int Hkv = p.c.Hkv, rows = 2 * Hkv + (p.q ? p.H : 0);
+  for (int r = r0; r < rows; r += RPP) {
+    const bool is_k = r < Hkv, is_q = r >= 2 * Hkv;
+    const int h = is_k ? r : is_q ? r - 2 * Hkv : r - Hkv;
+    const char* src = is_k ? p.k + t * p.k_str[0] + h * p.k_str[1]
+                    : is_q ? p.q + t * p.q_str[0] + h * p.q_str[1]
+                           : p.v + t * p.v_str[0] + h * p.v_str[1];
+    if (bad) {
+      if (is_q) {
+        const uint32_t n2 = Half<E>::kNaN * 0x10001u;
+        *reinterpret_cast<u32x4*>(p.qo + t * p.qo_str[0] + h * p.qo_str[1] + 16 * c) = u32x4{n2, n2, n2, n2};
+      }
+      continue;
+    }
+    const u32x4 raw = *reinterpret_cast<const u32x4*>(src + 16 * c);
+    const bool turned = turn && (is_k || is_q);
+    float x[8];
+    Half<E>::unpack(raw, x);
+    float y[8];
+    if (turned && !p.interleaved) Half<E>::unpack(*reinterpret_cast<const u32x4*>(src + 16 * c + 2 * partner), y);
+    if (BITS == 16 || is_q) {
+      u32x4 w = raw;
+      if (turned) {
+        float z[8];
+        if (p.interleaved) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            z[2 * i] = __builtin_fmaf(x[2 * i], cs[i], -(x[2 * i + 1] * sn[i]));
+            z[2 * i + 1] = __builtin_fmaf(x[2 * i + 1], cs[i], x[2 * i] * sn[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z[i] = __builtin_fmaf(x[i], cs[i], y[i] * sn[i]);
+        }
+        w = pack8<E>(z);
+      }
+      char* dst = is_q ? p.qo + t * p.qo_str[0] + h * p.qo_str[1]
+                       : (is_k ? p.c.k + page * p.c.k_str[0] + slot * p.c.k_str[1] + h * p.c.k_str[2]
+                               : p.c.v + page * p.c.v_str[0] + slot * p.c.v_str[1] + h * p.c.v_str[2]);
+      *reinterpret_cast<u32x4*>(dst + 16 * c) = w;
+    } else {
+      if (turned) {
+        if (p.interleaved) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const double a = x[2 * i], b = x[2 * i + 1], cc = cs[i], ss = sn[i];
+            x[2 * i] = to_odd(__builtin_fma(a, cc, -(b * ss)));
+            x[2 * i + 1] = to_odd(__builtin_fma(b, cc, a * ss));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = to_odd(__builtin_fma((double)x[i], (double)cs[i], (double)y[i] * (double)sn[i]));
+        }
+      }
+      // the largest of the 32 values that four neighbouring threads hold; a
+      // NaN or an infinity among them as infinity
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float a = __builtin_fabsf(x[i]);
+        m = a <= 3.4028235e38f ? (a > m ? a : m) : __builtin_inff();
+      }
+      m = __builtin_fmaxf(m, __shfl_xor(m, 1));
+      m = __builtin_fmaxf(m, __shfl_xor(m, 2));
+      // smallest e with 6 * 2^e >= m: of m = f * 2^k, 1 <= f < 2, that is k - 2
+      // for f <= 1.5 and k - 1 above
+      const uint32_t mb = __builtin_bit_cast(uint32_t, m);
+      int e = (int)(mb >> 23) - 127 - 2 + ((mb & 0x7fffffu) > 0x400000u ? 1 : 0);
+      e = e < -23 ? -23 : e > 13 ? 13 : e;
+      const float scale = __builtin_bit_cast(float, (uint32_t)(e + 127) << 23);
+      uint32_t codes = 0;
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], scale, 0);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], scale, 1);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], scale, 2);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], scale, 3);
+      const bool finite = m <= 3.4028235e38f;
+      char* dst = is_k ? p.c.k + page * p.c.k_str[0] + slot * p.c.k_str[1] + h * p.c.k_str[2]
+                       : p.c.v + page * p.c.v_str[0] + slot * p.c.v_str[1] + h * p.c.v_str[2];
+      uint8_t* sd = is_k ? p.c.ks + page * p.c.ks_str[0] + slot * p.c.ks_str[1] + h * p.c.ks_str[2]
+                         : p.c.vs + page * p.c.vs_str[0] + slot * p.c.vs_str[1] + h * p.c.vs_str[2];
+      *reinterpret_cast<uint32_t*>(dst + 4 * c) = finite ? codes : 0u;
+      if ((c & 3) == 0) sd[c >> 2] = finite ? (uint8_t)(e + 127) : (uint8_t)255;
+    }
+  }
+}
+
+template <int D, typename E, int BITS>
+__global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
+  for (int t = blockIdx.x; t < p.c.N; t += gridDim.x) append_token<D, E, BITS>(p, t);
+}
+
+// ──────────────────────────────── gather ───────────────────────────────────
+
+// Work-groups of grid.x walk (position, head, chunk) of sequence blockIdx.y in
+// the order of the output, so that the writes, two thirds or more of the
+// traffic, are contiguous; blockIdx.z: keys, values.  Bound by memory.
+template <int D, typename E, int BITS>
+__global__ __launch_bounds__(256) void paged_gather_kernel(PagedView c, char* ko, char* vo, int max_len) {
+  constexpr int CH = D / 8;
+  const int b = blockIdx.y;
+  const bool is_v = blockIdx.z;
+  int L = c.lens[b];
+  const int64_t cap = (int64_t)c.max_pages * c.page_size;
+  const bool bad_len = L < 0 || L > cap;
+  if (bad_len && blockIdx.x == 0 && threadIdx.x == 0) paged_flag(c, LVSA_PAGED_BAD_LENGTH);
+  if (L > max_len) L = max_len;
+  const char* src = is_v ? c.v : c.k;
+  const uint8_t* sc = is_v ? c.vs : c.ks;
+  const int64_t s0 = is_v ? c.v_str[0] : c.k_str[0], s1 = is_v ? c.v_str[1] : c.k_str[1],
+                s2 = is_v ? c.v_str[2] : c.k_str[2];
+  const int64_t c0 = is_v ? c.vs_str[0] : c.ks_str[0], c1 = is_v ? c.vs_str[1] : c.ks_str[1],
+                c2 = is_v ? c.vs_str[2] : c.ks_str[2];
+  u32x4* out = reinterpret_cast<u32x4*>((is_v ? vo : ko) + (int64_t)b * max_len * c.Hkv * (2 * D));
+  const uint32_t per = (uint32_t)c.Hkv * CH;                 // chunks of one position
+  const int64_t total = (int64_t)max_len * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int pos = (int)(i / per);
+    const uint32_t rest = (uint32_t)(i - (int64_t)pos * per), h = rest / CH, ch = rest % CH;
+    u32x4 w = {0, 0, 0, 0};
+    if (bad_len) {
+      const uint32_t n2 = Half<E>::kNaN * 0x10001u;
+      w = u32x4{n2, n2, n2, n2};
+    } else if (pos < L) {
+      const PagedRow at = paged_row(c, pos, c.table[b * c.table_str + page_of(c, pos)]);
+      if (!at.ok) {
+        paged_flag(c, LVSA_PAGED_BAD_PAGE);
+        const uint32_t n2 = Half<E>::kNaN * 0x10001u;
+        w = u32x4{n2, n2, n2, n2};
+      } else {
+        const char* row = src + at.page * s0 + at.slot * s1 + h * s2;
+        if constexpr (BITS == 16) {
+          w = *reinterpret_cast<const u32x4*>(row + 16 * ch);
+        } else {
+          const uint32_t codes = *reinterpret_cast<const uint32_t*>(row + 4 * ch);
+          w = unpack_e2m1<E>(codes, sc[at.page * c0 + at.slot * c1 + h * c2 + (ch >> 2)]);
+        }
+      }
+    }
+    out[i] = w;
+  }
+}
+
+// ───────────────────────── merge of the partials ───────────────────────────
+
+// One work-group per output row: finds the row's sequence, tile and the slots
+// that hold partials of it, and merges them: o = sum_i 2^(m_i - M) o_i / sum_i
+// 2^(m_i - M) l_i.  The four waves take the slots in turn and are summed in
+// their order, so results do not depend on timing.  Rows whose tile one
+// work-group of the decode kernel did whole are written already.  Rows without
+// keys and rows of no sequence are this kernel's too.
+template <typename E>
+__device__ __forceinline__ void merge_row(const PagedAttnParams& p, int row, int D, int rows, int keys,
+                                          float (*acc_s)[256], float (*ml_s)[2]) {
+  const int t = row / p.H, hq = row % p.H;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  E* out = reinterpret_cast<E*>(p.o + t * p.o_str[0] + hq * p.o_str[1]);
+  float* lse = p.lse ? p.lse + (int64_t)t * p.H + hq : nullptr;
+  const int s = paged_seq_of_row(p.c, t, lane);
+  if (s < 0) {
+    if (p.fill_tail) {
+      for (int d = threadIdx.x; d < D; d += 256) out[d] = (E)0.f;
+      if (lse && threadIdx.x == 0) *lse = -__builtin_inff();
+    }
+    return;
+  }
+  const PagedSeq sq = paged_seq(p.c, s);
+  const int h = hq / p.group;
+  const int r = (t - sq.t0) * p.group + hq % p.group;
+  DecodeSlots parts = {0, 0, 0};
+  int step = 2;
+  if (p.splits == 0) {         // decode kernel
+    int64_t U = 0, base = 0;
+    for (int s0 = 0; s0 < p.c.B; s0 += 64) {
+      const int i = s0 + lane;
+      int64_t n = 0;
+      if (i < p.c.B) n = decode_units(p, paged_seq(p.c, i), rows, keys);
+      const int64_t incl = wave_scan(n, lane);
+      if (s >= s0 && s < s0 + 64) base = U + __shfl(incl - n, s - s0);
+      U += __shfl(incl, 63);
+    }
+    const int nb = (int)(((int64_t)sq.L + keys - 1) / keys);
+    if (nb > 0) {
+      parts = decode_slots(U, unit_shares(U, p.grid), base + ((int64_t)(r / rows) * p.c.Hkv + h) * nb, nb);
+      if (parts.count == 0) return;        // written by the attention kernel
+    }
+  } else {                     // prefill kernel, tiles in `splits` parts
+    int64_t base = 0;
+    for (int s0 = 0; s0 <= s; s0 += 64) {
+      const int i = s0 + lane;
+      int64_t n = 0;
+      if (i < s) n = ((int64_t)paged_seq(p.c, i).n * p.group + rows - 1) / rows;
+      base += __shfl(wave_scan(n, lane), 63);
+    }
+    const int64_t tile = base + r / rows;
+    if (tile >= p.tiles) return;           // row ranges that overlap: more tiles than the batch's rows give
+    const int64_t at = (tile * p.c.Hkv + h) * p.splits;
+    parts = DecodeSlots{p.splits, at, at};
+    step = 1;
+  }
+  const int count = parts.count;
+  const int rr = r % rows;
+  auto slot_of = [&](int i) { return i == 0 ? parts.first : parts.rest + i * step; };
+
+  float M = kNoKeys;
+  for (int i = wave; i < count; i += 4) {
+    const float m = p.ws_ml[2 * (slot_of(i) * rows + rr)];
+    M = __builtin_fmaxf(M, m);
+  }
+  if (lane == 0) ml_s[wave][0] = M;
+  __syncthreads();
+  M = __builtin_fmaxf(__builtin_fmaxf(ml_s[0][0], ml_s[1][0]), __builtin_fmaxf(ml_s[2][0], ml_s[3][0]));
+  float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = wave; i < count; i += 4) {
+    const int64_t at = slot_of(i) * rows + rr;
+    const float w = __builtin_amdgcn_exp2f(p.ws_ml[2 * at] - M);
+    l = __builtin_fmaf(w, p.ws_ml[2 * at + 1], l);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int d = lane + 64 * k;
+      if (d < D) acc[k] = __builtin_fmaf(w, p.ws_o[at * D + d], acc[k]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) acc_s[wave][lane + 64 * k] = acc[k];
+  if (lane == 0) ml_s[wave][1] = l;
+  __syncthreads();
+  l = (ml_s[0][1] + ml_s[1][1]) + (ml_s[2][1] + ml_s[3][1]);
+  if (sq.flags & LVSA_PAGED_BAD_LENGTH) l = __builtin_nanf("");
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  for (int d = threadIdx.x; d < D; d += 256)
+    out[d] = (E)(((acc_s[0][d] + acc_s[1][d]) + (acc_s[2][d] + acc_s[3][d])) * inv);
+  if (lse && threadIdx.x == 0) *lse = l == 0.f ? -__builtin_inff() : (M + __log2f(l)) * 0.69314718055994530942f;
+}
+
+template <typename E>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnParams p, int D, int rows, int keys) {
+  __shared__ float acc_s[4][256];
+  __shared__ float ml_s[4][2];
+  for (int row = blockIdx.x; row < p.c.N * p.H; row += gridDim.x) {
+    merge_row<E>(p, row, D, rows, keys, acc_s, ml_s);
+    __syncthreads();             // the next row writes the same LDS
+  }
+}
+
+// ─────────────────────────────── host side ─────────────────────────────────
+
+int cu_count() {
+  static std::mutex mu;
+  static int cached[64] = {0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) {
+    (void)hipGetLastError();       // no device: sizes are still answered
+    return 256;
+  }
+  std::lock_guard<std::mutex> lock(mu);
+  if (cached[dev] == 0) {
+    int n = 0;
+    cached[dev] = hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && n > 0 ? n : 256;
+  }
+  return cached[dev];
+}
+
+bool aligned16(int64_t x) { return (x & 15) == 0; }
+
+// Checks a cache and a batch and forms the device's view of them.
+int paged_view(const char* what, const lvsa_paged_cache* c, const lvsa_paged_batch* b, bool rows, PagedView* v) {
+  LVSA_REQUIRE(c->D == 64 || c->D == 96 || c->D == 128 || c->D == 192 || c->D == 256, LVSA_ERR_UNSUPPORTED,
+               "%s: head_dim %d not supported (64, 96, 128, 192, 256)", what, c->D);
+  LVSA_REQUIRE(c->bits == 16 || c->bits == 4, LVSA_ERR_UNSUPPORTED, "%s: caches hold 16 or 4 bits, not %d", what, c->bits);
+  LVSA_REQUIRE(c->dtype == LVSA_BF16 || c->dtype == LVSA_FP16, LVSA_ERR_UNSUPPORTED, "%s: dtype %d: bf16 or fp16", what,
+               c->dtype);
+  LVSA_REQUIRE(c->n_pages >= 1 && c->page_size >= 1 && c->Hkv >= 1, LVSA_ERR_INVALID_ARG,
+               "%s: %d pages of %d slots, %d heads", what, c->n_pages, c->page_size, c->Hkv);
+  LVSA_REQUIRE(c->k && c->v && (c->bits == 16 || (c->k_scale && c->v_scale)), LVSA_ERR_INVALID_ARG,
+               "%s: null cache pointer", what);
+  LVSA_REQUIRE(b->B >= 0 && b->max_pages >= 0 && b->N >= 0 && b->table_stride >= b->max_pages, LVSA_ERR_INVALID_ARG,
+               "%s: batch of %d sequences, %d pages (rows %lld apart), %d rows", what, b->B, b->max_pages,
+               (long long)b->table_stride, b->N);
+  LVSA_REQUIRE(b->B == 0 || (b->kv_lens && (b->page_table || b->max_pages == 0) && (!rows || b->cu_seqlens)),
+               LVSA_ERR_INVALID_ARG, "%s: null batch pointer", what);
+  LVSA_REQUIRE((int64_t)b->max_pages * c->page_size < (1LL << 31) - 4096, LVSA_ERR_UNSUPPORTED,
+               "%s: %d pages of %d slots: positions must stay below 2^31 - 4096", what, b->max_pages, c->page_size);
+  const int64_t unit = c->bits == 16 ? 2 : 1;
+  v->k = (char*)c->k;
+  v->v = (char*)c->v;
+  v->ks = (uint8_t*)c->k_scale;
+  v->vs = (uint8_t*)c->v_scale;
+  bool ok = aligned16((int64_t)(uintptr_t)c->k) && aligned16((int64_t)(uintptr_t)c->v);
+  for (int i = 0; i < 3; ++i) {
+    v->k_str[i] = c->k_str[i] * unit;
+    v->v_str[i] = c->v_str[i] * unit;
+    v->ks_str[i] = c->ks_str[i];
+    v->vs_str[i] = c->vs_str[i];
+    ok = ok && aligned16(v->k_str[i]) && aligned16(v->v_str[i]);
+  }
+  LVSA_REQUIRE(ok, LVSA_ERR_INVALID_ARG, "%s: cache rows must start at multiples of 16 bytes", what);
+  v->n_pages = c->n_pages;
+  v->Hkv = c->Hkv;
+  set_page_size(v, c->page_size);
+  v->status = c->status;
+  v->cu = b->cu_seqlens;
+  v->lens = b->kv_lens;
+  v->table = b->page_table;
+  v->table_str = b->table_stride;
+  v->B = b->B;
+  v->max_pages = b->max_pages;
+  v->N = b->N;
+  return LVSA_OK;
+}
+
+template <template <int, typename, int> class L, typename... A>
+int by_type(int D, int dtype, int bits, A&&... a) {
+#define LVSA_PAGED_CASE(d)                                                             \
+  case d:                                                                              \
+    if (dtype == LVSA_BF16) return bits == 16 ? L<d, __bf16, 16>::go(a...) : L<d, __bf16, 4>::go(a...); \
+    return bits == 16 ? L<d, _Float16, 16>::go(a...) : L<d, _Float16, 4>::go(a...);
+  switch (D) {
+    LVSA_PAGED_CASE(64)
+    LVSA_PAGED_CASE(96)
+    LVSA_PAGED_CASE(128)
+    LVSA_PAGED_CASE(192)
+    LVSA_PAGED_CASE(256)
+  }
+#undef LVSA_PAGED_CASE
+  return LVSA_ERR_UNSUPPORTED;
+}
+
+template <int D, typename E, int BITS> struct Append {
+  static int go(const AppendParams& p, hipStream_t stream) {
+    hipLaunchKernelGGL((paged_append_kernel<D, E, BITS>), dim3((unsigned)(p.c.N < kMaxGrid ? p.c.N : kMaxGrid)), dim3(256), 0,
+                       stream, p);
+    return launch_status("lvsa_paged_append");
+  }
+};
+template <int D, typename E, int BITS> struct Gather {
+  static int go(const PagedView& c, void* ko, void* vo, int max_len, hipStream_t stream) {
+    const int64_t chunks = (int64_t)max_len * c.Hkv * (D / 8);
+    const int64_t want = ceil_div(chunks, 256);
+    const unsigned gx = (unsigned)(want < 4096 ? want : 4096);
+    hipLaunchKernelGGL((paged_gather_kernel<D, E, BITS>), dim3(gx, (unsigned)c.B, 2), dim3(256), 0, stream, c, (char*)ko,
+                       (char*)vo, max_len);
+    return launch_status("lvsa_paged_gather");
+  }
+};
+
+// How an attention call runs: row tiles of 16 or 32 rows on the decode kernel
+// or 128 on the prefill kernel, and the launch's size.
+struct AttnShape {
+  int rows, grid, tiles, splits;
+  int64_t o_elems, ml_elems;
+};
+
+AttnShape attn_shape(const lvsa_paged_attn_args* a) {
+  AttnShape s{};
+  const int group = a->H / a->cache.Hkv, D = a->cache.D;
+  const int64_t N = a->batch.N, cus = cu_count();
+  const int64_t cap = (int64_t)a->batch.max_pages * a->cache.page_size;
+  const int64_t kv = a->max_kv_len > 0 && a->max_kv_len < cap ? a->max_kv_len : cap;
+  const int64_t q = a->max_q_len > 0 && a->max_q_len < N ? a->max_q_len : N;
+  const int64_t tile_rows = q * group;
+  if (tile_rows <= 32) {
+    s.rows = tile_rows <= 16 ? 16 : 32;
+    const int keys = paged_decode_keys(D);
+    const int64_t per_cu = 2;
+    const int64_t units = ceil_div(kv, keys) * a->cache.Hkv * (int64_t)(a->batch.B < N ? a->batch.B : N);
+    s.grid = (int)(units < cus * per_cu ? (units > 0 ? units : 1) : cus * per_cu);
+    s.splits = 0;
+    s.o_elems = 2LL * s.grid * s.rows * D;
+    s.ml_elems = 2LL * 2 * s.grid * s.rows;
+  } else {
+    s.rows = kPagedTile;
+    const int64_t B = a->batch.B < N ? a->batch.B : N;
+    s.tiles = (int)(ceil_div(N * group, kPagedTile) + B);
+    const int64_t tiles = ceil_div(N * group, kPagedTile) * a->cache.Hkv;
+    const int64_t slots = cus * (D >= 192 ? 1 : 2);
+    int64_t sp = tiles > 0 ? slots / tiles : 1;
+    const int64_t most = ceil_div(kv, 4 * kPagedBlock);
+    sp = sp < most ? sp : most;
+    sp = sp < 64 ? sp : 64;
+    s.splits = (int)(sp > 1 ? sp : 1);
+    const int64_t slots_ws = s.splits > 1 ? (int64_t)s.tiles * a->cache.Hkv * s.splits : 0;
+    s.o_elems = slots_ws * kPagedTile * D;
+    s.ml_elems = slots_ws * kPagedTile * 2;
+  }
+  return s;
+}
+
+int attn_check(const lvsa_paged_attn_args* a, PagedView* v) {
+  const char* what = "lvsa_paged_attn_fwd";
+  LVSA_REQUIRE(a != nullptr, LVSA_ERR_INVALID_ARG, "%s: null args", what);
+  const int rc = paged_view(what, &a->cache, &a->batch, true, v);
+  if (rc) return rc;
+  LVSA_REQUIRE(a->H >= 1 && a->H % a->cache.Hkv == 0, LVSA_ERR_INVALID_ARG, "%s: %d heads over %d key heads", what, a->H,
+               a->cache.Hkv);
+  LVSA_REQUIRE((int64_t)a->batch.N * a->H < (1LL << 31) - 4096, LVSA_ERR_UNSUPPORTED, "%s: %d rows of %d heads", what,
+               a->batch.N, a->H);
+  LVSA_REQUIRE(a->scale > 0.f && a->scale <= 3.4028235e38f, LVSA_ERR_INVALID_ARG, "%s: scale %g must be positive and finite",
+               what, (double)a->scale);
+  return LVSA_OK;
+}
+
+}  // namespace
+}  // namespace lvsa
+
+extern "C" {
+
+int lvsa_paged_append(const lvsa_paged_append_args* a, hipStream_t stream) {
+  clear_error();
+  const char* what = "lvsa_paged_append";
+  LVSA_REQUIRE(a != nullptr, LVSA_ERR_INVALID_ARG, "%s: null args", what);
+  AppendParams p{};
+  const int rc = paged_view(what, &a->cache, &a->batch, true, &p.c);
+  if (rc) return rc;
+  LVSA_REQUIRE(a->batch.N == 0 || (a->k && a->v), LVSA_ERR_INVALID_ARG, "%s: null keys or values", what);
+  LVSA_REQUIRE((a->q == nullptr) == (a->q_out == nullptr), LVSA_ERR_INVALID_ARG, "%s: q and q_out go together", what);
+  LVSA_REQUIRE(!a->q || a->H >= 1, LVSA_ERR_INVALID_ARG, "%s: %d query heads", what, a->H);
+  LVSA_REQUIRE((a->cos == nullptr) == (a->sin == nullptr), LVSA_ERR_INVALID_ARG, "%s: cos and sin go together", what);
+  LVSA_REQUIRE(!a->cos || (a->rot >= 16 && a->rot % 16 == 0 && a->rot <= a->cache.D && a->n_angles >= 0), LVSA_ERR_INVALID_ARG,
+               "%s: %d rotated dimensions of %d (a multiple of 16), %d angle rows", what, a->rot, a->cache.D, a->n_angles);
+  const void* ptrs[4] = {a->k, a->v, a->q, a->q_out};
+  const int64_t* strs[4] = {a->k_str, a->v_str, a->q_str, a->qo_str};
+  int64_t* outs[4] = {p.k_str, p.v_str, p.q_str, p.qo_str};
+  for (int i = 0; i < 4; ++i) {
+    if (!ptrs[i]) continue;
+    outs[i][0] = 2 * strs[i][0];
+    outs[i][1] = 2 * strs[i][1];
+    LVSA_REQUIRE(aligned16((int64_t)(uintptr_t)ptrs[i]) && aligned16(outs[i][0]) && aligned16(outs[i][1]),
+                 LVSA_ERR_INVALID_ARG, "%s: rows must start at multiples of 16 bytes", what);
+  }
+  if (a->batch.N == 0 || a->batch.B == 0) return LVSA_OK;
+  p.k = (const char*)a->k;
+  p.v = (const char*)a->v;
+  p.q = (const char*)a->q;
+  p.qo = (char*)a->q_out;
+  p.cos = a->cos;
+  p.sin = a->sin;
+  p.positions = a->positions;
+  p.H = a->H;
+  p.rot = a->cos ? a->rot : 0;
+  p.interleaved = a->interleaved;
+  p.n_angles = a->n_angles;
+  return by_type<Append>(a->cache.D, a->cache.dtype, a->cache.bits, p, stream);
+}
+
+int lvsa_paged_gather(const lvsa_paged_cache* cache, const lvsa_paged_batch* batch, void* k_out, void* v_out,
+                      int32_t max_len, hipStream_t stream) {
+  clear_error();
+  const char* what = "lvsa_paged_gather";
+  LVSA_REQUIRE(cache && batch, LVSA_ERR_INVALID_ARG, "%s: null args", what);
+  PagedView c{};
+  const int rc = paged_view(what, cache, batch, false, &c);
+  if (rc) return rc;
+  LVSA_REQUIRE(max_len >= 0 && batch->B <= 65535, LVSA_ERR_INVALID_ARG, "%s: %d sequences of %d tokens", what, batch->B,
+               max_len);
+  if (batch->B == 0 || max_len == 0) return LVSA_OK;
+  LVSA_REQUIRE(k_out && v_out && aligned16((int64_t)(uintptr_t)k_out) && aligned16((int64_t)(uintptr_t)v_out),
+               LVSA_ERR_INVALID_ARG, "%s: outputs must be non-null and 16-byte aligned", what);
+  return by_type<Gather>(cache->D, cache->dtype, cache->bits, c, k_out, v_out, max_len, stream);
+}
+
+int lvsa_paged_attn_workspace_query(const lvsa_paged_attn_args* a, int64_t* bytes) {
+  clear_error();
+  LVSA_REQUIRE(bytes != nullptr, LVSA_ERR_INVALID_ARG, "lvsa_paged_attn_workspace_query: null output");
+  PagedView v{};
+  const int rc = attn_check(a, &v);
+  if (rc) return rc;
+  const AttnShape s = attn_shape(a);
+  *bytes = a->batch.N == 0 ? 0 : 4 * (s.o_elems + s.ml_elems);
+  return LVSA_OK;
+}
+
+int lvsa_paged_attn_fwd(const lvsa_paged_attn_args* a, hipStream_t stream) {
+  clear_error();
+  const char* what = "lvsa_paged_attn_fwd";
+  PagedAttnParams p{};
+  int rc = attn_check(a, &p.c);
+  if (rc) return rc;
+  if (a->batch.N == 0) return LVSA_OK;
+  LVSA_REQUIRE(a->q && a->o, LVSA_ERR_INVALID_ARG, "%s: null q or o", what);
+  bool ok = aligned16((int64_t)(uintptr_t)a->q) && aligned16((int64_t)(uintptr_t)a->o);
+  for (int i = 0; i < 2; ++i) {
+    p.q_str[i] = 2 * a->q_str[i];
+    p.o_str[i] = 2 * a->o_str[i];
+    ok = ok && aligned16(p.q_str[i]) && aligned16(p.o_str[i]);
+  }
+  LVSA_REQUIRE(ok, LVSA_ERR_INVALID_ARG, "%s: rows must start at multiples of 16 bytes", what);
+  const AttnShape s = attn_shape(a);
+  LVSA_REQUIRE((int64_t)s.tiles * a->cache.Hkv < (1 << 24), LVSA_ERR_UNSUPPORTED, "%s: %d row tiles of %d key heads", what,
+               s.tiles, a->cache.Hkv);
+  const int64_t need = 4 * (s.o_elems + s.ml_elems);
+  LVSA_REQUIRE(need == 0 || (a->workspace && aligned16((int64_t)(uintptr_t)a->workspace)), LVSA_ERR_INVALID_ARG,
+               "%s: %lld bytes of 16-byte aligned workspace needed", what, (long long)need);
+  LVSA_REQUIRE(need == 0 || a->workspace_bytes >= need, LVSA_ERR_CAPACITY, "%s: workspace of %lld bytes < %lld", what,
+               (long long)a->workspace_bytes, (long long)need);
+  p.q = (const char*)a->q;
+  p.o = (char*)a->o;
+  p.lse = a->lse;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.H = a->H;
+  p.group = a->H / a->cache.Hkv;
+  p.causal = a->causal;
+  p.fill_tail = a->fill_tail;
+  p.grid = s.grid;
+  p.tiles = s.tiles;
+  p.splits = s.splits;
+  p.ws_o = (float*)a->workspace;
+  p.ws_ml = p.ws_o ? p.ws_o + s.o_elems : nullptr;
+  const bool bf16 = a->cache.dtype == LVSA_BF16;
+  if (a->batch.B > 0) {
+    switch (a->cache.D) {
+      case 64: rc = paged_attn_d64(p, a->cache.bits, s.rows, bf16, stream); break;
+      case 96: rc = paged_attn_d96(p, a->cache.bits, s.rows, bf16, stream); break;
+      case 128: rc = paged_attn_d128(p, a->cache.bits, s.rows, bf16, stream); break;
+      case 192: rc = paged_attn_d192(p, a->cache.bits, s.rows, bf16, stream); break;
+      default: rc = paged_attn_d256(p, a->cache.bits, s.rows, bf16, stream); break;
+    }
+    if (rc) return rc;
+  }
+  // the prefill kernel writes every row itself unless its tiles run in parts
+  if (s.rows == kPagedTile && s.splits == 1 && a->batch.B > 0) return LVSA_OK;
+  const int out_rows = a->batch.N * a->H;
+  const dim3 grid((unsigned)(out_rows < kMaxGrid ? out_rows : kMaxGrid));
+  const int keys = paged_decode_keys(a->cache.D);
+  if (bf16) {
+    hipLaunchKernelGGL((paged_merge_kernel<__bf16>), grid, dim3(256), 0, stream, p, a->cache.D, s.rows, keys);
+  } else {
+    hipLaunchKernelGGL((paged_merge_kernel<_Float16>), grid, dim3(256), 0, stream, p, a->cache.D, s.rows, keys);
+  }
+  return launch_status(what);
+}
+
+}  // extern "C"
