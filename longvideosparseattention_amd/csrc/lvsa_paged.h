@@ -42,7 +42,7 @@ struct PagedAttnParams {
 };
 
 // Attention launches per head size.  rows: 16 or 32 (decode kernel, row tiles
-// of that many rows) or 128 (prefill kernel).
+// of that many rows), 128 or 256 (prefill kernels).
 int paged_attn_d64(const PagedAttnParams& p, int bits, int rows, bool bf16, hipStream_t stream);
 int paged_attn_d96(const PagedAttnParams& p, int bits, int rows, bool bf16, hipStream_t stream);
 int paged_attn_d128(const PagedAttnParams& p, int bits, int rows, bool bf16, hipStream_t stream);
@@ -52,6 +52,7 @@ int paged_attn_d256(const PagedAttnParams& p, int bits, int rows, bool bf16, hip
 // Keys that the four waves of a decode work-group take per step.
 __host__ __device__ constexpr int paged_decode_keys(int D) { return 4 * (D >= 192 ? 16 : 32); }
 constexpr int kPagedTile = 128;        // rows of a prefill tile
+constexpr int kPagedTall = 256;        // rows of a tall one (head sizes up to 128)
 constexpr int kPagedBlock = 64;        // its keys per step
 
 // The running maximum of a row that has seen no key: below every finite score,

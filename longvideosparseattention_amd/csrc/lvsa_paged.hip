@@ -503,7 +503,7 @@ template <int D, typename E, int BITS> struct Gather {
 };
 
 // How an attention call runs: row tiles of 16 or 32 rows on the decode kernel
-// or 128 on the prefill kernel, and the launch's size.
+// or 128 or 256 on the prefill kernels, and the launch's size.
 struct AttnShape {
   int rows, grid, tiles, splits;
   int64_t o_elems, ml_elems;
@@ -527,19 +527,19 @@ AttnShape attn_shape(const lvsa_paged_attn_args* a) {
     s.o_elems = 2LL * s.grid * s.rows * D;
     s.ml_elems = 2LL * 2 * s.grid * s.rows;
   } else {
-    s.rows = kPagedTile;
+    s.rows = D <= 128 && tile_rows > kPagedTile ? kPagedTall : kPagedTile;
     const int64_t B = a->batch.B < N ? a->batch.B : N;
-    s.tiles = (int)(ceil_div(N * group, kPagedTile) + B);
-    const int64_t tiles = ceil_div(N * group, kPagedTile) * a->cache.Hkv;
-    const int64_t slots = cus * (D >= 192 ? 1 : 2);
+    s.tiles = (int)(ceil_div(N * group, s.rows) + B);
+    const int64_t tiles = ceil_div(N * group, s.rows) * a->cache.Hkv;
+    const int64_t slots = cus * (D >= 192 || s.rows == kPagedTall ? 1 : 2);
     int64_t sp = tiles > 0 ? slots / tiles : 1;
     const int64_t most = ceil_div(kv, 4 * kPagedBlock);
     sp = sp < most ? sp : most;
     sp = sp < 64 ? sp : 64;
     s.splits = (int)(sp > 1 ? sp : 1);
     const int64_t slots_ws = s.splits > 1 ? (int64_t)s.tiles * a->cache.Hkv * s.splits : 0;
-    s.o_elems = slots_ws * kPagedTile * D;
-    s.ml_elems = slots_ws * kPagedTile * 2;
+    s.o_elems = slots_ws * s.rows * D;
+    s.ml_elems = slots_ws * s.rows * 2;
   }
   return s;
 }
@@ -676,7 +676,7 @@ int lvsa_paged_attn_fwd(const lvsa_paged_attn_args* a, hipStream_t stream) {
     if (rc) return rc;
   }
   // the prefill kernel writes every row itself unless its tiles run in parts
-  if (s.rows == kPagedTile && s.splits == 1 && a->batch.B > 0) return LVSA_OK;
+  if (s.splits == 1 && a->batch.B > 0) return LVSA_OK;
   const int out_rows = a->batch.N * a->H;
   const dim3 grid((unsigned)(out_rows < kMaxGrid ? out_rows : kMaxGrid));
   const int keys = paged_decode_keys(a->cache.D);

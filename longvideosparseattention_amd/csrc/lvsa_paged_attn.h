@@ -114,10 +114,11 @@ __device__ __forceinline__ bool any_nonfinite(shortx8 x) {
 
 // Infinities and NaN among the values of keys that only some rows attend: the
 // zero weight of a row that does not attend the key would carry them into it
-// (0 * inf is NaN).  Blocks with masked keys are searched for such values; if
-// there are any, they are added to the rows that attend them by themselves
-// (add_nonfinite) and the matrix product runs on the tile with zeros in their
-// place (finite8).
+// (0 * inf is NaN).  Blocks with masked keys are searched for such values on
+// their way into LDS, and the matrix product runs on zeros in their place
+// (finite8).  Where any were found, they are added at the end, from memory, to
+// the rows that attend them (add_nonfinite): no sum of finite terms changes an
+// infinity or a NaN, so the order does not matter.
 template <typename E>
 __device__ __forceinline__ shortx8 finite8(shortx8 x) {
 #pragma unroll
@@ -128,6 +129,33 @@ template <typename E>
 __device__ __forceinline__ float add_nonfinite(float o, uint32_t bits, bool seen) {
   const float v = (float)__builtin_bit_cast(E, (uint16_t)bits);
   return seen && (bits & Mat<E>::kExp) == Mat<E>::kExp ? o + v : o;
+}
+
+// Adds what keys [k0, k1) hold besides finite numbers to a row that attends
+// keys below `lim`: quad q of the row's elements, d0 + q * step .. + 3, in
+// o(q).  Rare, and slow: a key at a time.
+template <typename E, int BITS, int NQ, typename O>
+__device__ __forceinline__ void add_nonfinite_keys(const PagedView& c, const int32_t* table, int h, int k0, int k1,
+                                                   int lim, int d0, int step, O o) {
+#pragma unroll 1
+  for (int k = k0; k < k1; ++k) {
+    const PagedRow at = paged_row(c, k, table[page_of(c, k)]);
+    const char* row = c.v + at.page * c.v_str[0] + at.slot * c.v_str[1] + h * c.v_str[2];
+    const bool seen = k < lim;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int d = d0 + q * step;
+      u32x2 v;
+      if constexpr (BITS == 16) {
+        v = *reinterpret_cast<const u32x2*>(row + 2 * d);
+      } else {
+        const bool nan = c.vs[at.page * c.vs_str[0] + at.slot * c.vs_str[1] + h * c.vs_str[2] + d / 32] == 255;
+        v = nan ? u32x2{0x7fff7fffu, 0x7fff7fffu} : u32x2{0u, 0u};
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o(q, r, (v[r >> 1] >> (16 * (r & 1))) & 0xffffu, seen);
+    }
+  }
 }
 
 // Row r of a (sequence, key head) pair: its q and o / lse, and the end of the
@@ -276,7 +304,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 192 && NT == 2)) ? 1 : 2) v
 #pragma unroll
       for (int i = 0; i < NO; ++i) o[n][i] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
-    bool bad = (sq.flags & LVSA_PAGED_BAD_LENGTH) != 0;
+    bool bad = (sq.flags & LVSA_PAGED_BAD_LENGTH) != 0, odd_keys = false;
 
     const char* kbase = p.c.k + h * p.c.k_str[2];
     const char* vbase = p.c.v + h * p.c.v_str[2];
@@ -331,8 +359,8 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 192 && NT == 2)) ? 1 : 2) v
       const int key0 = b * KEYS + wave * KW;
       if (key0 >= sq.L) return;                // the last step's waves past the end
       // V to LDS, chunk by chunk
-      bool odd_v = false;
       const bool masked = key0 + KW > lim_min;
+      bool odd = false;
 #pragma unroll
       for (int j = 0; j < T; ++j)
 #pragma unroll
@@ -346,9 +374,13 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 192 && NT == 2)) ? 1 : 2) v
             w = decode8<E>(st.v[j][i], scale_of(st.vs[j], i));
             c = ND * g + i;
           }
-          if (masked) odd_v |= any_nonfinite<E>(w);
+          if (masked) {
+            odd |= any_nonfinite<E>(w);
+            w = finite8<E>(w);
+          }
           *reinterpret_cast<__attribute__((address_space(3))) shortx8*>(vbuf + lds_chunk(TB, 16 * j + x, c)) = w;
         }
+      if (masked) odd_keys |= odd;
       // S^T: row 4 g + r of tile j, column x
       floatx4 s[NT][T];
 #pragma unroll
@@ -423,25 +455,6 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 192 && NT == 2)) ? 1 : 2) v
         }
         return a;
       };
-      if (__builtin_expect(masked && __builtin_amdgcn_ballot_w64(odd_v) != 0, 0)) {
-        typedef __attribute__((address_space(3))) u32x2 lds4;
-        typedef __attribute__((address_space(3))) shortx8 lds8;
-#pragma unroll 1
-        for (int k = 0; k < KW; ++k) {
-#pragma unroll
-          for (int i = 0; i < NO; ++i) {
-            const u32x2 v = *reinterpret_cast<const lds4*>(vbuf + lds_chunk(TB, k, 2 * i + (g >> 1)) + 8 * (g & 1));
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                o[n][i][r] = add_nonfinite<E>(o[n][i][r], (v[r >> 1] >> (16 * (r & 1))) & 0xffffu, key0 + k < lim[n]);
-          }
-        }
-#pragma unroll 1
-        for (int at = 16 * lane; at < T * TB; at += 1024)
-          *reinterpret_cast<lds8*>(vbuf + at) = finite8<E>(*reinterpret_cast<const lds8*>(vbuf + at));
-      }
 #pragma unroll
       for (int i = 0; i < NO; ++i) {
         const vp a = vfrag(i);
@@ -473,6 +486,20 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 192 && NT == 2)) ? 1 : 2) v
           __builtin_amdgcn_sched_barrier(0);
           compute(b + 1, sb);
         }
+      }
+    }
+
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd_keys) != 0, 0)) {
+      const int from = lim_min / KEYS > blk0 ? lim_min / KEYS : blk0;
+      for (int b = from; b < blk1; ++b) {
+        const int k0 = b * KEYS + wave * KW, k1 = k0 + KW < sq.L ? k0 + KW : sq.L;
+        if (k0 + KW <= lim_min) continue;             // not masked: its values are in the sums already
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          add_nonfinite_keys<E, BITS, NO>(p.c, table, h, k0, k1, lim[n], 4 * g, 16,
+                                          [&](int q, int r, uint32_t v, bool seen) __attribute__((always_inline)) {
+                                            o[n][q][r] = add_nonfinite<E>(o[n][q][r], v, seen);
+                                          });
       }
     }
 
@@ -538,6 +565,90 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 192 && NT == 2)) ? 1 : 2) v
 
 // ─────────────────────────────── prefill ───────────────────────────────────
 
+// Rows before the first and behind the last sequence: 0 and -inf.
+__device__ __forceinline__ void fill_tail_rows(const PagedAttnParams& p, int D, int lane, int wave, int waves) {
+  const int head = p.c.cu[0] < 0 ? 0 : p.c.cu[0] > p.c.N ? p.c.N : p.c.cu[0];
+  const int tail = p.c.cu[p.c.B] < head ? head : p.c.cu[p.c.B] > p.c.N ? p.c.N : p.c.cu[p.c.B];
+  const int64_t n = (int64_t)(head + p.c.N - tail) * p.H;
+  const int64_t wg = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, wgs = (int64_t)gridDim.x * gridDim.y;
+  for (int64_t i = wg * waves + wave; i < n; i += waves * wgs) {
+    const int64_t r = i / p.H, hq = i - r * p.H, t = r < head ? r : tail + (r - head);
+    for (int d = lane; d < D; d += 64) reinterpret_cast<uint16_t*>(p.o + t * p.o_str[0] + hq * p.o_str[1])[d] = 0;
+    if (p.lse && lane == 0) p.lse[t * p.H + hq] = -__builtin_inff();
+  }
+}
+
+// Row tile and key head of this work-group, or false past the last tile (the
+// launch is sized by a bound).  Tiles run from the last to the first: with a
+// causal order the later ones are the longer ones, and a launch that ends on
+// short tiles ends evenly.  Consecutive work-groups, which go to different
+// XCDs, are the key heads of one tile, so an XCD keeps to a few heads and
+// their keys stay in its L2.
+struct TileRef {
+  PagedSeq sq;
+  int seq, h, r0;
+  int64_t index;
+};
+__device__ __forceinline__ bool find_tile(const PagedAttnParams& p, int rows, int lane, int wave, TileRef* t) {
+  t->h = (int)(blockIdx.x % (uint32_t)p.c.Hkv);
+  t->index = p.tiles - 1 - (int64_t)(blockIdx.x / (uint32_t)p.c.Hkv);
+  int64_t base = 0;
+  int flags = 0;
+  t->seq = -1;
+  for (int s0 = 0; s0 < p.c.B; s0 += 64) {
+    int64_t n = 0;
+    if (s0 + lane < p.c.B) {
+      const PagedSeq q = paged_seq(p.c, s0 + lane);
+      n = ((int64_t)q.n * p.group + rows - 1) / rows;
+      flags |= q.flags;
+    }
+    const int64_t incl = wave_scan(n, lane);
+    const uint64_t above = __builtin_amdgcn_ballot_w64(base + incl > t->index);
+    if (above && t->seq < 0) {
+      const int at = __builtin_ctzll(above);
+      t->seq = s0 + at;
+      t->r0 = (int)(t->index - (base + __shfl(incl - n, at))) * rows;
+      if (blockIdx.x != 0 || blockIdx.y != 0) break;   // the first work-group looks at every sequence's flags
+    }
+    base += __shfl(incl, 63);
+  }
+  if (blockIdx.x == 0 && blockIdx.y == 0 && wave == 0 && flags) paged_flag(p.c, flags);
+  if (t->seq < 0) return false;
+  t->sq = paged_seq(p.c, t->seq);
+  return true;
+}
+
+// A row's result, or its partial sums where its tile runs in parts: O of
+// element 32 dt + 8 q + 4 half + i in o[dt][4 q + i].
+template <int D, typename E>
+__device__ __forceinline__ void store_rows(const PagedAttnParams& p, int64_t slot, int rows, int r, int half,
+                                           const RowRef& ref, const floatx16* o, float m_run, float l) {
+  if (p.splits > 1) {
+    const int64_t at = slot * rows + r;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<floatx4*>(p.ws_o + at * D + 32 * dt + 8 * q + 4 * half) =
+            floatx4{o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]};
+    if (half == 0) {
+      p.ws_ml[2 * at] = m_run;
+      p.ws_ml[2 * at + 1] = l;
+    }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  char* op = p.o + ref.tok * p.o_str[0] + ref.head * p.o_str[1];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<u32x2*>(op + 2 * (32 * dt + 8 * q + 4 * half)) =
+          u32x2{pack2<E>(o[dt][4 * q] * inv, o[dt][4 * q + 1] * inv), pack2<E>(o[dt][4 * q + 2] * inv, o[dt][4 * q + 3] * inv)};
+  if (p.lse && half == 0)
+    p.lse[ref.tok * p.H + ref.head] = l == 0.f ? -__builtin_inff() : (m_run + __log2f(l)) * 0.69314718055994530942f;
+}
+
 // 16 bytes per lane, global -> LDS at `l` + 16 * lane, past the registers.  In
 // asm, so that the compiler does not wait for it before LDS reads it cannot
 // tell apart; the kernel orders the copies by its own wait and barrier.
@@ -547,6 +658,21 @@ __device__ __forceinline__ void copy16(const char* from, const lds_char* l) {
 #pragma clang diagnostic ignored "-Winline-asm"
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(la) : "m0", "memory");
 #pragma clang diagnostic pop
+}
+
+// Puts zeros in the place of what a wave's own tile of V holds besides finite
+// numbers; whether there was any.
+template <typename E>
+__device__ __forceinline__ bool search_tile(lds_char* tile, int bytes, int lane) {
+  typedef __attribute__((address_space(3))) shortx8 lds8;
+  bool odd = false;
+#pragma unroll 1
+  for (int at = 16 * lane; at < bytes; at += 1024) odd |= any_nonfinite<E>(*reinterpret_cast<const lds8*>(tile + at));
+  if (!__builtin_amdgcn_ballot_w64(odd)) return false;
+#pragma unroll 1
+  for (int at = 16 * lane; at < bytes; at += 1024)
+    *reinterpret_cast<lds8*>(tile + at) = finite8<E>(*reinterpret_cast<const lds8*>(tile + at));
+  return true;
 }
 
 // Four waves of 32 rows.  Key blocks of 64 keys in two LDS stages: wave w
@@ -567,51 +693,12 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   const int half = lane >> 5, i32 = lane & 31;       // S^T: column (row of the tile) i32
   const int g = lane >> 4, x = lane & 15;
 
-  // rows before the first and behind the last sequence
-  if (p.fill_tail) {
-    const int head = p.c.cu[0] < 0 ? 0 : p.c.cu[0] > p.c.N ? p.c.N : p.c.cu[0];
-    const int tail = p.c.cu[p.c.B] < head ? head : p.c.cu[p.c.B] > p.c.N ? p.c.N : p.c.cu[p.c.B];
-    const int64_t n = (int64_t)(head + p.c.N - tail) * p.H;
-    const int64_t wg = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, wgs = (int64_t)gridDim.x * gridDim.y;
-    for (int64_t i = wg * 4 + wave; i < n; i += 4 * wgs) {
-      const int64_t r = i / p.H, hq = i - r * p.H, t = r < head ? r : tail + (r - head);
-      for (int d = lane; d < D; d += 64) reinterpret_cast<uint16_t*>(p.o + t * p.o_str[0] + hq * p.o_str[1])[d] = 0;
-      if (p.lse && lane == 0) p.lse[t * p.H + hq] = -__builtin_inff();
-    }
-  }
-
-  // Tile and key head of this work-group.  Tiles run from the last to the
-  // first: with a causal order the later ones are the longer ones, and a
-  // launch that ends on short tiles ends evenly.  Consecutive work-groups,
-  // which go to different XCDs, are the key heads of one tile, so an XCD keeps
-  // to a few heads and their keys stay in its L2.
-  const int h = (int)(blockIdx.x % (uint32_t)p.c.Hkv);
-  const int64_t want = p.tiles - 1 - (int64_t)(blockIdx.x / (uint32_t)p.c.Hkv);
-  int seq = -1;
-  int64_t base = 0;
-  int flags = 0;
-  for (int s0 = 0; s0 < p.c.B; s0 += 64) {
-    int64_t n = 0;
-    if (s0 + lane < p.c.B) {
-      const PagedSeq q = paged_seq(p.c, s0 + lane);
-      n = ((int64_t)q.n * p.group + kPagedTile - 1) / kPagedTile;
-      flags |= q.flags;
-    }
-    const int64_t incl = wave_scan(n, lane);
-    const uint64_t above = __builtin_amdgcn_ballot_w64(base + incl > want);
-    if (above) {
-      const int at = __builtin_ctzll(above);
-      seq = s0 + at;
-      base += __shfl(incl - n, at);
-      break;
-    }
-    base += __shfl(incl, 63);
-  }
-  if (blockIdx.x == 0 && blockIdx.y == 0 && wave == 0 && flags) paged_flag(p.c, flags);
-  if (seq < 0) return;                              // the launch's bound, past the last tile
-  const PagedSeq sq = paged_seq(p.c, seq);
+  if (p.fill_tail) fill_tail_rows(p, D, lane, wave, 4);
+  TileRef tile;
+  if (!find_tile(p, kPagedTile, lane, wave, &tile)) return;
+  const PagedSeq sq = tile.sq;
+  const int h = tile.h, r0 = tile.r0;
   const int nrows = sq.n * p.group;
-  const int r0 = (int)(want - base) * kPagedTile;
   const int r_last = r0 + kPagedTile < nrows ? r0 + kPagedTile - 1 : nrows - 1;
   const int lim_min = key_limit(p, sq, r0), lim_max = key_limit(p, sq, r_last);
   const int nb = (lim_max + kPagedBlock - 1) / kPagedBlock;
@@ -630,7 +717,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
 
   const char* kbase = p.c.k + h * p.c.k_str[2];
   const char* vbase = p.c.v + h * p.c.v_str[2];
-  const int32_t* table = p.c.table + seq * p.c.table_str;
+  const int32_t* table = p.c.table + tile.seq * p.c.table_str;
   // The key of tile `wave` that this lane brings (past the end: the last key).
   // 16 bits: chunks 4 i + g of key x ^ 8 (g & 1), so that a copy's fixed order
   // in LDS is the tile's layout.
@@ -760,37 +847,15 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
       const shortx4 a = read_tr(vs + voff0 + st * TB + 1024 * dt), c = read_tr(vs + voff1 + st * TB + 1024 * dt);
       return __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    bool odd = false;
-    if (masked) {
-      #pragma unroll 1
-      for (int i = lane; i < MAT / 16; i += 64) odd |= any_nonfinite<E>(*reinterpret_cast<lds8*>(vs + 16 * i));
-    }
-    if (__builtin_expect(masked && __builtin_amdgcn_ballot_w64(odd) != 0, 0)) {   // alike in all four waves
-      typedef __attribute__((address_space(3))) u32x2 lds4;
-#pragma unroll 1
-      for (int k = 0; k < kPagedBlock; ++k) {
-        const bool seen = b * kPagedBlock + k < lim;
-#pragma unroll
-        for (int q = 0; q < 4 * NO; ++q) {
-          const u32x2 v = *reinterpret_cast<const lds4*>(vs + lds_chunk(TB, k, q) + 8 * half);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            o[q >> 2][4 * (q & 3) + r] =
-                add_nonfinite<E>(o[q >> 2][4 * (q & 3) + r], (v[r >> 1] >> (16 * (r & 1))) & 0xffffu, seen);
-        }
-      }
-      __syncthreads();
-#pragma unroll 1
-      for (int at = 16 * (int)threadIdx.x; at < MAT; at += 4096)
-        *reinterpret_cast<__attribute__((address_space(3))) shortx8*>(vs + at) = finite8<E>(*reinterpret_cast<lds8*>(vs + at));
-      __syncthreads();
-    }
 #pragma unroll
     for (int st = 0; st < 4; ++st)
 #pragma unroll
       for (int dt = 0; dt < NO; ++dt) o[dt] = Mat<E>::mfma32(vfrag(st, dt), pb[st], o[dt]);
   };
 
+  __shared__ int bad_s, odd_s;
+  if (threadIdx.x == 0) bad_s = odd_s = 0;
+  __syncthreads();
   if (blk0 < blk1) {
     int page = table[page_of(p.c, key_pos(blk0))];
     if constexpr (BITS == 16) {
@@ -802,6 +867,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
     page = table[page_of(p.c, key_pos(blk0 + 1))];
     auto step = [&](int b, lds_char* cur, lds_char* nxt) __attribute__((always_inline)) {
       __builtin_amdgcn_s_waitcnt(0x0F70);           // vmcnt(0): this wave's copies of block b have landed
+      if ((b + 1) * kPagedBlock > lim_min && search_tile<E>(cur + MAT + wave * TB, TB, lane)) odd_s = 1;
       __syncthreads();                              // everyone's; and the other stage has been read
       if (b + 1 < blk1) {
         if constexpr (BITS == 16) bring16(b + 1, page, nxt);
@@ -820,47 +886,359 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   }
 
   // A bad page seen by any wave spoils the tile.
-  __shared__ int bad_s;
-  if (threadIdx.x == 0) bad_s = 0;
-  __syncthreads();
   if (__builtin_amdgcn_ballot_w64(bad) && lane == 0) bad_s = 1;
   __syncthreads();
   if (bad_s && threadIdx.x == 0 && !(sq.flags & LVSA_PAGED_BAD_LENGTH)) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
 
+  if (__builtin_expect(odd_s != 0, 0)) {
+    const int from = lim_min / kPagedBlock > blk0 ? lim_min / kPagedBlock : blk0;
+    const int k1 = blk1 * kPagedBlock < lim_max ? blk1 * kPagedBlock : lim_max;
+    add_nonfinite_keys<E, BITS, 4 * NO>(p.c, table, h, from * kPagedBlock, k1, lim, 4 * half, 8,
+                                        [&](int q, int r, uint32_t v, bool seen) __attribute__((always_inline)) {
+                                          o[q >> 2][4 * (q & 3) + r] = add_nonfinite<E>(o[q >> 2][4 * (q & 3) + r], v, seen);
+                                        });
+  }
   float l = l_run + __shfl_xor(l_run, 32);
   if (bad_s) l = __builtin_nanf("");
-  if (row >= nrows) return;
-  if (p.splits > 1) {
-    const int64_t slot = (want * p.c.Hkv + h) * p.splits + blockIdx.y;
-    const int64_t at = slot * kPagedTile + (row - r0);
+  if (row < nrows) store_rows<D, E>(p, (tile.index * p.c.Hkv + h) * p.splits + blockIdx.y, kPagedTile, row - r0, half, ref, o, m_run, l);
+}
+
+// ──────────────────────────── prefill, tall tiles ──────────────────────────
+
+// Workgroup barrier that nothing crosses: the memory clobber orders LDS and
+// global accesses, the scheduling barriers keep a phase's arithmetic in it.
+__device__ __forceinline__ void phase_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+// Materialise x here, so that the compiler does not sink its computation into
+// the phase that uses it.
+template <typename T>
+__device__ __forceinline__ void keep(T& x) {
+  asm volatile("" : "+v"(x));
+}
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  static_assert(N >= 0 && N < 16, "vmcnt immediate");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | N);
+}
+// 4 bytes per lane, global -> LDS at `l` + 4 * lane (see copy16).
+__device__ __forceinline__ void copy4(const void* from, const lds_char* l) {
+  const uint32_t la = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)l);
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(from), "s"(la) : "m0", "memory");
+#pragma clang diagnostic pop
+}
+
+// Eight waves of 32 rows in two groups of four that alternate between a phase
+// of matrix products and a phase of softmax, one barrier after each: on every
+// SIMD one wave keeps the matrix core busy while the other one's
+// exponentials run, which two independent work-groups do only by chance.
+//
+//   M(j)  S(j) = K(j) Q^T and O += V(j-1) P(j-1) as one stream of matrix
+//         instructions whose LDS operands are read LA instructions ahead
+//   S(j)  masks, maximum, P(j), row sums
+//
+// Group 0 runs M(j) in phase 2 j and S(j) in phase 2 j + 1, group 1 one phase
+// later.  LDS holds four blocks of 64 keys of K and of V; group 0 brings K,
+// group 1 V, wave w of each the block's tile w, two blocks ahead: block j + 2
+// goes where block j - 2 was, whose last readers (group 1's M(j - 1) in phase
+// 2 j - 1) are done before M(j).
+//   16 bits: copies past the registers, issued between the matrix
+//   instructions of M(j) and waited for at the end of S(j + 1), with the page
+//   numbers of block j + 4 behind them on the same way, so that no wait of the
+//   compiler's own for an ordinary load ever drains the copies.
+//   4 bits: codes of block j + 3 are loaded in M(j), decoded and written to LDS
+//   in S(j + 1).
+template <int D, typename E, int BITS>
+__global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
+  constexpr int ND = D / 32, NK = D / 16, NO = D / 32;
+  constexpr int TB = 32 * D, MAT = 4 * TB;
+  constexpr int VB = 4 * MAT, PB = 8 * MAT;
+  constexpr bool kTwoScales = D == 96;
+  // K and V rings, page numbers [wave][4][64]
+  __shared__ __attribute__((aligned(1024))) char smem_raw[PB + (BITS == 16 ? 8 * 4 * 256 : 0)];
+  __shared__ int bad_s, odd_s;
+  lds_char* smem = (lds_char*)smem_raw;
+  typedef __attribute__((address_space(3))) shortx8 lds8;
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int grp = wave >> 2, dw = wave & 3;
+  const int half = lane >> 5, i32 = lane & 31;
+  const int g = lane >> 4, x = lane & 15;
+
+  if (p.fill_tail) fill_tail_rows(p, D, lane, wave, 8);
+  TileRef tile;
+  if (!find_tile(p, kPagedTall, lane, wave, &tile)) return;
+  const PagedSeq sq = tile.sq;
+  const int h = tile.h, r0 = tile.r0, nrows = sq.n * p.group;
+  const int r_last = r0 + kPagedTall < nrows ? r0 + kPagedTall - 1 : nrows - 1;
+  const int lim_min = key_limit(p, sq, r0), lim_max = key_limit(p, sq, r_last);
+  const int nb = (lim_max + kPagedBlock - 1) / kPagedBlock;
+  const int blk0 = (int)((int64_t)nb * blockIdx.y / p.splits), blk1 = (int)((int64_t)nb * (blockIdx.y + 1) / p.splits);
+  const int n = blk1 - blk0;
+
+  const int row = r0 + 32 * wave + i32;
+  const int rc = row < nrows ? row : nrows - 1;
+  const RowRef ref = row_ref(p, sq, h, rc);
+  const int lim = key_limit(p, sq, rc);
+
+  const char* src = grp == 0 ? p.c.k + h * p.c.k_str[2] : p.c.v + h * p.c.v_str[2];
+  const int64_t str0 = grp == 0 ? p.c.k_str[0] : p.c.v_str[0], str1 = grp == 0 ? p.c.k_str[1] : p.c.v_str[1];
+  const uint8_t* scl = BITS == 16 ? nullptr : grp == 0 ? p.c.ks + h * p.c.ks_str[2] : p.c.vs + h * p.c.vs_str[2];
+  const int64_t sst0 = grp == 0 ? p.c.ks_str[0] : p.c.vs_str[0], sst1 = grp == 0 ? p.c.ks_str[1] : p.c.vs_str[1];
+  const int32_t* table = p.c.table + tile.seq * p.c.table_str;
+  lds_char* ring = smem + grp * VB + dw * TB;           // this wave's tile of stage 0
+  lds_char* pids = smem + PB + wave * 1024;
+  const int my_key = 16 * dw + (BITS == 16 ? x ^ (8 * (g & 1)) : x);
+  auto key_pos = [&](int j) __attribute__((always_inline)) { return key_within((blk0 + j) * kPagedBlock + my_key, sq.L); };
+  bool bad = (sq.flags & LVSA_PAGED_BAD_LENGTH) != 0;
+  auto row_at = [&](int j, int page, int64_t& sc) __attribute__((always_inline)) {
+    const PagedRow at = paged_row(p.c, key_pos(j), page);
+    bad |= !at.ok;
+    if constexpr (BITS == 4) sc = at.page * sst0 + at.slot * sst1;
+    return src + at.page * str0 + at.slot * str1;
+  };
+
+  if (threadIdx.x == 0) bad_s = odd_s = 0;
+  __syncthreads();
+  // V of the block before the first (stage 3): read by M(0) with P = 0
+  for (int at = 16 * (int)threadIdx.x; at < MAT; at += 8192) *reinterpret_cast<lds8*>(smem + VB + 3 * MAT + at) = shortx8{0};
+
+  shortx8 qf[NK];
+  {
+    const char* qp = p.q + ref.tok * p.q_str[0] + ref.head * p.q_str[1] + 16 * half;
 #pragma unroll
-    for (int dt = 0; dt < NO; ++dt)
+    for (int c = 0; c < NK; ++c) qf[c] = *reinterpret_cast<const shortx8*>(qp + 32 * c);
+    wait_copies<0>();                                   // no load of the compiler's own is left for the loop to wait for
 #pragma unroll
-      for (int rq = 0; rq < 4; ++rq)
-        *reinterpret_cast<floatx4*>(p.ws_o + at * D + 32 * dt + 8 * rq + 4 * half) =
-            floatx4{o[dt][4 * rq], o[dt][4 * rq + 1], o[dt][4 * rq + 2], o[dt][4 * rq + 3]};
-    if (half == 0) {
-      p.ws_ml[2 * at] = m_run;
-      p.ws_ml[2 * at + 1] = l;
-    }
-    return;
+    for (int c = 0; c < NK; ++c) keep(qf[c]);
   }
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  char* op = p.o + ref.tok * p.o_str[0] + ref.head * p.o_str[1];
+
+  // 4 bits: codes and scales of the next block to decode, and of the one after it.
+  struct Codes {
+    uint32_t w[ND], s[2];
+  } here4, coming;
+  int page_next = 0;                                    // 4 bits: page number of the next block to load
+  auto load4 = [&](int j, int page, Codes& c) __attribute__((always_inline)) {
+    int64_t sc = 0;
+    const char* r = row_at(j, page, sc) + (D / 8) * g;
 #pragma unroll
-  for (int dt = 0; dt < NO; ++dt)
+    for (int i = 0; i < ND; ++i) c.w[i] = reinterpret_cast<const uint32_t*>(r)[i];
+    c.s[0] = scl[sc + (D / 4) * g / 32];
+    c.s[1] = kTwoScales ? scl[sc + ((D / 4) * g + D / 4 - 1) / 32] : 0;
+  };
+  auto is_masked = [&](int j) __attribute__((always_inline)) { return (blk0 + j + 1) * kPagedBlock > lim_min; };
+  auto store4 = [&](int j, int stage, const Codes& c) __attribute__((always_inline)) {
+    const bool masked = grp == 1 && is_masked(j);
 #pragma unroll
-    for (int rq = 0; rq < 4; ++rq)
-      *reinterpret_cast<u32x2*>(op + 2 * (32 * dt + 8 * rq + 4 * half)) =
-          u32x2{pack2<E>(o[dt][4 * rq] * inv, o[dt][4 * rq + 1] * inv),
-                pack2<E>(o[dt][4 * rq + 2] * inv, o[dt][4 * rq + 3] * inv)};
-  if (p.lse && half == 0)
-    p.lse[ref.tok * p.H + ref.head] = l == 0.f ? -__builtin_inff() : (m_run + __log2f(l)) * 0.69314718055994530942f;
+    for (int i = 0; i < ND; ++i) {
+      const bool up = kTwoScales && ((D / 4) * g + 8 * i) / 32 != (D / 4) * g / 32;
+      const uint32_t sb = up ? c.s[1] : c.s[0];
+      shortx8 w = decode8<E>(c.w[i], sb);
+      if (masked && sb == 255) {                        // NaN: see finite8
+        w = shortx8{0};
+        odd_s = 1;
+      }
+      *reinterpret_cast<lds8*>(ring + stage * MAT + lds_chunk(TB, x, ND * g + i)) = w;
+    }
+  };
+
+  // LDS reads (see paged_prefill_kernel).
+  const int koff = lds_chunk(TB, i32, half);
+  const int vrow = 4 * half + (x >> 2), vc = 2 * (g & 1) + ((x & 3) >> 1);
+  const int voff0 = VB + lds_chunk(TB, vrow, vc) + 8 * (x & 1), voff1 = VB + lds_chunk(TB, vrow + 8, vc) + 8 * (x & 1);
+
+  floatx16 o[NO];
+#pragma unroll
+  for (int i = 0; i < NO; ++i) o[i] = floatx16{0};
+  floatx16 s0 = floatx16{0}, s1 = floatx16{0};
+  shortx8 pb[4];
+#pragma unroll
+  for (int st = 0; st < 4; ++st) pb[st] = shortx8{0};
+  float m_run = kNoKeys, l4[4] = {0.f, 0.f, 0.f, 0.f};
+
+  constexpr int LA = D == 128 ? 3 : 4;
+  constexpr int NQK = 2 * NK, NM = NQK + 4 * NO;
+  auto mphase = [&](int j) __attribute__((always_inline)) {
+    const int kat = koff + (j & 3) * MAT, vst = ((j + 3) & 3) * MAT, v0 = voff0 + vst, v1 = voff1 + vst;
+    lds_char* to = ring + ((j + 2) & 3) * MAT;
+    const char* from = nullptr;
+    if constexpr (BITS == 16) {
+      int64_t none;
+      from = row_at(j + 2, *reinterpret_cast<const __attribute__((address_space(3))) int*>(pids + 256 * ((j + 2) & 3) + 4 * lane), none) + 16 * g;
+    } else {
+      const int page = page_next;
+      page_next = table[page_of(p.c, key_pos(j + 4))];
+      load4(j + 3, page, coming);
+    }
+    shortx8 opa[NM];
+    s0 = floatx16{0};
+    s1 = floatx16{0};
+#pragma unroll
+    for (int i = -LA; i < NM; ++i) {
+      const int li = i + LA;
+      if (li < NM) {
+        if (li < NQK) {
+          opa[li] = *reinterpret_cast<const lds8*>(smem + kat + 512 * (li >> 1) + (li & 1) * 2 * TB);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        } else {
+          const int k = li - NQK, st = k / NO, dt = k % NO;
+          const shortx4 a = read_tr(smem + v0 + st * TB + 1024 * dt), c = read_tr(smem + v1 + st * TB + 1024 * dt);
+          opa[li] = __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+      }
+      if (i >= 0) {
+        if (i < NQK) {
+          if (i & 1) s1 = Mat<E>::mfma32(opa[i], qf[i >> 1], s1);
+          else s0 = Mat<E>::mfma32(opa[i], qf[i >> 1], s0);
+        } else {
+          const int k = i - NQK;
+          o[k % NO] = Mat<E>::mfma32(opa[i], pb[k / NO], o[k % NO]);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if constexpr (BITS == 16) {
+          if (i % 4 == 3 && i / 4 < ND) copy16(from + 64 * (i / 4), to + 1024 * (i / 4));
+          if (i == 4 * ND) copy4(table + page_of(p.c, key_pos(j + 4)), pids + 256 * (j & 3));
+        }
+      }
+    }
+    keep(s0);
+    keep(s1);
+#pragma unroll
+    for (int dt = 0; dt < NO; ++dt) keep(o[dt]);
+  };
+
+  auto sphase = [&](int j) __attribute__((always_inline)) {
+    if (is_masked(j)) {
+      const int here = lim - (blk0 + j) * kPagedBlock - 4 * half;   // keys of this block that the row attends, from 4 half on
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int k = 8 * (r >> 2) + (r & 3);
+        s0[r] = k < here ? s0[r] : -__builtin_inff();
+        s1[r] = k + 32 < here ? s1[r] : -__builtin_inff();
+      }
+    }
+    float t[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float m = __builtin_fmaxf(s0[4 * c], s0[4 * c + 1]);
+      m = __builtin_fmaxf(__builtin_fmaxf(m, s0[4 * c + 2]), s0[4 * c + 3]);
+      m = __builtin_fmaxf(__builtin_fmaxf(m, s1[4 * c]), s1[4 * c + 1]);
+      t[c] = __builtin_fmaxf(__builtin_fmaxf(m, s1[4 * c + 2]), s1[4 * c + 3]);
+    }
+    float top = __builtin_fmaxf(__builtin_fmaxf(t[0], t[1]), __builtin_fmaxf(t[2], t[3])) * p.scale_log2;
+    if (__builtin_amdgcn_ballot_w64(top > m_run + 8.0f)) {
+      top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+      const float m_new = __builtin_fmaxf(m_run, top);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l4[i] *= alpha;
+#pragma unroll
+      for (int i = 0; i < NO; ++i) o[i] *= alpha;
+      m_run = m_new;
+    }
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+      const floatx16& s = st < 2 ? s0 : s1;
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * (st & 1) + 2 * i], p.scale_log2, -m_run));
+        const float c = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * (st & 1) + 2 * i + 1], p.scale_log2, -m_run));
+        l4[i] += a + c;
+        w[i] = pack2<E>(a, c);
+      }
+      pb[st] = __builtin_bit_cast(shortx8, w);
+    }
+    if constexpr (BITS == 4) {
+      store4(j + 2, (j + 2) & 3, here4);
+      here4 = coming;
+    } else {
+      wait_copies<ND + 1>();                            // block j + 1 and the page numbers of block j + 3 have landed
+      if (grp == 1 && is_masked(j + 1) && search_tile<E>(ring + ((j + 1) & 3) * MAT, TB, lane)) odd_s = 1;
+    }
+#pragma unroll
+    for (int st = 0; st < 4; ++st) keep(pb[st]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) keep(l4[i]);
+    keep(m_run);
+#pragma unroll
+    for (int dt = 0; dt < NO; ++dt) keep(o[dt]);
+    // LDS writes of this phase are in place for the others' reads after the barrier
+    if (BITS == 4 || grp == 1) __builtin_amdgcn_s_waitcnt(0xC07F);
+  };
+
+  if (n > 0) {
+    if constexpr (BITS == 16) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) copy4(table + page_of(p.c, key_pos(j)), pids + 256 * j);
+      wait_copies<0>();
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        int64_t none;
+        const char* from = row_at(j, *reinterpret_cast<const __attribute__((address_space(3))) int*>(pids + 256 * j + 4 * lane), none) + 16 * g;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) copy16(from + 64 * i, ring + j * MAT + 1024 * i);
+      }
+      wait_copies<ND>();                                // block 0
+      if (grp == 1 && is_masked(0) && search_tile<E>(ring, TB, lane)) odd_s = 1;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        load4(j, table[page_of(p.c, key_pos(j))], here4);
+        store4(j, j, here4);
+      }
+      load4(2, table[page_of(p.c, key_pos(2))], here4);
+      page_next = table[page_of(p.c, key_pos(3))];
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);                 // LDS writes: V of stage 3, tiles, notes
+    phase_barrier();
+    if (grp == 1) phase_barrier();
+    // Each group passes n softmax phases and n + 1 matrix phases; the barriers
+    // (2 n + 1 for both after the first) pair phase with phase.
+    // (One copy of each phase: with the ring's stages as constants, four copies,
+    // the compiler spilled hundreds of registers where the loop's exits meet.)
+    for (int j = 0;; ++j) {
+      mphase(j);
+      if (j >= n) break;
+      phase_barrier();
+      sphase(j);
+      phase_barrier();
+    }
+    if (grp == 0) phase_barrier();
+    wait_copies<0>();                                   // copies past the last block land before the work-group ends
+  }
+
+  if (__builtin_amdgcn_ballot_w64(bad) && lane == 0) bad_s = 1;
+  __syncthreads();
+  if (bad_s && threadIdx.x == 0 && !(sq.flags & LVSA_PAGED_BAD_LENGTH)) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
+  if (__builtin_expect(odd_s != 0, 0)) {
+    const int from = lim_min / kPagedBlock > blk0 ? lim_min / kPagedBlock : blk0;
+    const int k1 = blk1 * kPagedBlock < lim_max ? blk1 * kPagedBlock : lim_max;
+    add_nonfinite_keys<E, BITS, 4 * NO>(p.c, table, h, from * kPagedBlock, k1, lim, 4 * half, 8,
+                                        [&](int q, int r, uint32_t v, bool seen) __attribute__((always_inline)) {
+                                          o[q >> 2][4 * (q & 3) + r] = add_nonfinite<E>(o[q >> 2][4 * (q & 3) + r], v, seen);
+                                        });
+  }
+  const float l_run = (l4[0] + l4[1]) + (l4[2] + l4[3]);
+  float l = l_run + __shfl_xor(l_run, 32);
+  if (bad_s) l = __builtin_nanf("");
+  if (row < nrows) store_rows<D, E>(p, (tile.index * p.c.Hkv + h) * p.splits + blockIdx.y, kPagedTall, row - r0, half, ref, o, m_run, l);
 }
 
 template <int D, typename E, int BITS>
 int paged_launch(const PagedAttnParams& p, int rows, hipStream_t stream) {
-  if (rows == kPagedTile) {
+  if (rows == kPagedTall) {
+    if constexpr (D <= 128)
+      hipLaunchKernelGGL((paged_tall_kernel<D, E, BITS>), dim3((unsigned)(p.tiles * p.c.Hkv), (unsigned)p.splits), dim3(512), 0,
+                         stream, p);
+  } else if (rows == kPagedTile) {
     hipLaunchKernelGGL((paged_prefill_kernel<D, E, BITS>), dim3((unsigned)(p.tiles * p.c.Hkv), (unsigned)p.splits),
                        dim3(256), 0, stream, p);
   } else if (rows == 16) {
