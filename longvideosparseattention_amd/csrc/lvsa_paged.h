@@ -27,18 +27,37 @@ struct PagedView {
   int32_t B, max_pages, N;
 };
 
+// What paged_plan_kernel writes for the prefill kernels, at the start of the
+// workspace: the row tiles of all sequences (each is done once per key head),
+// the units (key blocks) before each, and where each share of the launch's
+// units ends.  Units are ordered by key head, tile and key block; a tile
+// without keys counts as one.
+struct PlanHead {
+  int64_t per_head;              // units of one key head
+  int32_t tiles, shares;
+};
+struct PlanTile {
+  int32_t seq, r0, units, blocks;
+};
+struct PlanEnd {
+  int32_t h, tile, blk, pad;     // the share's last unit is unit blk - 1 of this tile
+};
+
 struct PagedAttnParams {
   PagedView c;
   const char* q; char* o; float* lse;
   int64_t q_str[2], o_str[2];    // bytes
   float scale_log2;              // scale * log2(e)
   int32_t H, group, causal, fill_tail;
-  // Decode kernel: `grid` work-groups share the launch's key blocks; each has
-  // two slots of row-tile partials.  Prefill kernel: `tiles` bounds the row
-  // tiles of all sequences, every tile's key blocks run as `splits` parts with
-  // a slot each.  Partials: fp32 O [slot][rows][D], then (max, sum) pairs.
-  int32_t grid, tiles, splits;
+  // The launch's key blocks are cut into equal shares for `grid` work-groups,
+  // each with two slots of row-tile partials: fp32 O [slot][rows][D], then
+  // (max, sum) pairs.  Prefill kernels: `tiles` bounds the row tiles.
+  int32_t grid, tiles;
   float* ws_o; float* ws_ml;
+  PlanHead* head;
+  PlanTile* plan_tiles;
+  int64_t* before;               // [tiles + 1]
+  PlanEnd* ends;                 // [grid]
 };
 
 // Attention launches per head size.  rows: 16 or 32 (decode kernel, row tiles
@@ -54,6 +73,7 @@ __host__ __device__ constexpr int paged_decode_keys(int D) { return 4 * (D >= 19
 constexpr int kPagedTile = 128;        // rows of a prefill tile
 constexpr int kPagedTall = 256;        // rows of a tall one (head sizes up to 128)
 constexpr int kPagedBlock = 64;        // its keys per step
+constexpr int kPagedLeast = 4;         // fewest steps of a share that is worth its partials
 
 // The running maximum of a row that has seen no key: below every finite score,
 // and still finite, so that differences to it are never NaN.
@@ -115,9 +135,12 @@ __host__ __device__ inline int64_t decode_units(const PagedAttnParams& p, const 
   return rt * p.c.Hkv * (((int64_t)q.L + keys - 1) / keys);
 }
 
-// Shares of U > 0 units over a grid: none is empty, so that the work-groups a
-// row tile spans all have a partial of it.
-__host__ __device__ inline int unit_shares(int64_t U, int grid) { return U < grid ? (int)U : grid; }
+// Shares of U > 0 units over a grid, of at least `least` units each: none is
+// empty, so that the work-groups a row tile spans all have a partial of it.
+__host__ __device__ inline int unit_shares(int64_t U, int grid, int least = 1) {
+  const int64_t n = U / least;
+  return n < 1 ? 1 : n < grid ? (int)n : grid;
+}
 // First unit of share w of G over U units, and the share of unit u.
 __host__ __device__ inline int64_t unit_start(int64_t U, int G, int w) { return w * U / G; }
 __host__ __device__ inline int wg_of_unit(int64_t U, int G, int64_t u) { return (int)(((u + 1) * G - 1) / U); }
@@ -145,7 +168,25 @@ inline void set_page_size(PagedView* v, int page_size) {
   v->ps_shift = (uint32_t)(31 + l);
 }
 
+// End of the keys that row r attends, and the key blocks of the tile of rows
+// [r0, r1].
+__host__ __device__ inline int key_limit(const PagedAttnParams& p, const PagedSeq& s, int r) {
+  if (!p.causal) return s.L;
+  const int64_t e = (int64_t)s.first + r / p.group + 1;
+  return e < 0 ? 0 : e > s.L ? s.L : (int)e;
+}
+__host__ __device__ inline int tile_blocks(const PagedAttnParams& p, const PagedSeq& s, int r0, int rows) {
+  const int end = s.n * p.group, last = r0 + rows < end ? r0 + rows - 1 : end - 1;
+  return (int)(((int64_t)key_limit(p, s, last) + kPagedBlock - 1) / kPagedBlock);
+}
+
 namespace {
+
+// A value that is the same in every lane, in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ PagedSeq uniform(const PagedSeq& s) {
+  return PagedSeq{uniform(s.t0), uniform(s.n), uniform(s.L), uniform(s.first), uniform(s.flags)};
+}
 
 __device__ __forceinline__ void paged_flag(const PagedView& c, int bit) {
   if (c.status) atomicOr(c.status, bit);

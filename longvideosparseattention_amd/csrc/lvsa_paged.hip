@@ -326,39 +326,23 @@ __device__ __forceinline__ void merge_row(const PagedAttnParams& p, int row, int
   const int h = hq / p.group;
   const int r = (t - sq.t0) * p.group + hq % p.group;
   DecodeSlots parts = {0, 0, 0};
-  int step = 2;
-  if (p.splits == 0) {         // decode kernel
-    int64_t U = 0, base = 0;
-    for (int s0 = 0; s0 < p.c.B; s0 += 64) {
-      const int i = s0 + lane;
-      int64_t n = 0;
-      if (i < p.c.B) n = decode_units(p, paged_seq(p.c, i), rows, keys);
-      const int64_t incl = wave_scan(n, lane);
-      if (s >= s0 && s < s0 + 64) base = U + __shfl(incl - n, s - s0);
-      U += __shfl(incl, 63);
-    }
-    const int nb = (int)(((int64_t)sq.L + keys - 1) / keys);
-    if (nb > 0) {
-      parts = decode_slots(U, unit_shares(U, p.grid), base + ((int64_t)(r / rows) * p.c.Hkv + h) * nb, nb);
-      if (parts.count == 0) return;        // written by the attention kernel
-    }
-  } else {                     // prefill kernel, tiles in `splits` parts
-    int64_t base = 0;
-    for (int s0 = 0; s0 <= s; s0 += 64) {
-      const int i = s0 + lane;
-      int64_t n = 0;
-      if (i < s) n = ((int64_t)paged_seq(p.c, i).n * p.group + rows - 1) / rows;
-      base += __shfl(wave_scan(n, lane), 63);
-    }
-    const int64_t tile = base + r / rows;
-    if (tile >= p.tiles) return;           // row ranges that overlap: more tiles than the batch's rows give
-    const int64_t at = (tile * p.c.Hkv + h) * p.splits;
-    parts = DecodeSlots{p.splits, at, at};
-    step = 1;
+  int64_t U = 0, base = 0;
+  for (int s0 = 0; s0 < p.c.B; s0 += 64) {
+    const int i = s0 + lane;
+    int64_t n = 0;
+    if (i < p.c.B) n = decode_units(p, paged_seq(p.c, i), rows, keys);
+    const int64_t incl = wave_scan(n, lane);
+    if (s >= s0 && s < s0 + 64) base = U + __shfl(incl - n, s - s0);
+    U += __shfl(incl, 63);
+  }
+  const int nb = (int)(((int64_t)sq.L + keys - 1) / keys);
+  if (nb > 0) {
+    parts = decode_slots(U, unit_shares(U, p.grid), base + ((int64_t)(r / rows) * p.c.Hkv + h) * nb, nb);
+    if (parts.count == 0) return;          // written by the attention kernel
   }
   const int count = parts.count;
   const int rr = r % rows;
-  auto slot_of = [&](int i) { return i == 0 ? parts.first : parts.rest + i * step; };
+  auto slot_of = [&](int i) { return i == 0 ? parts.first : parts.rest + 2 * i; };
 
   float M = kNoKeys;
   for (int i = wave; i < count; i += 4) {
@@ -398,6 +382,145 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnParams p, int
   for (int row = blockIdx.x; row < p.c.N * p.H; row += gridDim.x) {
     merge_row<E>(p, row, D, rows, keys, acc_s, ml_s);
     __syncthreads();             // the next row writes the same LDS
+  }
+}
+
+// ───────────────────────── plan of a prefill launch ────────────────────────
+
+// Sum over the work-group's 1024 threads before this one, and the total.
+__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* lds, int64_t* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t incl = wave_scan(x, lane);
+  __syncthreads();
+  if (lane == 63) lds[wave] = incl;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    before += w < wave ? lds[w] : 0;
+    all += lds[w];
+  }
+  *total = all;
+  return before + incl - x;
+}
+
+// One work-group: lists the row tiles with their key blocks, and where the
+// shares end.  Latency: a few dependent reads and scans, 5 us beside launches
+// of 30 us and more; with it every work-group of those gets the same number of
+// key blocks, whatever the lengths, where tiles as units leave the last round
+// to a few (516 tiles on 256 CUs: three rounds for two rounds' work).
+__global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int rows) {
+  __shared__ int64_t lds[16];
+  __shared__ int64_t shares_s;
+  int64_t done = 0;              // tiles before this chunk of sequences
+  for (int s0 = 0; s0 < p.c.B; s0 += 1024) {
+    const int s = s0 + threadIdx.x;
+    int64_t nt = 0;
+    if (s < p.c.B) {
+      const PagedSeq q = paged_seq(p.c, s);
+      if (q.flags) paged_flag(p.c, q.flags);
+      nt = ((int64_t)q.n * p.group + rows - 1) / rows;
+    }
+    int64_t all;
+    const int64_t at = done + block_scan(nt, lds, &all);
+    // row ranges that overlap give more tiles than the bound: the rest is dropped
+    for (int64_t i = 0; i < nt && at + i < p.tiles; ++i) p.plan_tiles[at + i] = PlanTile{s, (int)(i * rows), 0, 0};
+    done += all;
+  }
+  const int tiles = (int)(done < p.tiles ? done : p.tiles);
+  __syncthreads();               // the list is read by other threads than its writers
+  int64_t units = 0;
+  for (int t0 = 0; t0 < tiles; t0 += 1024) {
+    const int t = t0 + threadIdx.x;
+    int n = 0;
+    if (t < tiles) {
+      const PlanTile w = p.plan_tiles[t];
+      const int b = tile_blocks(p, paged_seq(p.c, w.seq), w.r0, rows);
+      n = b > 0 ? b : 1;
+      p.plan_tiles[t].units = n;
+      p.plan_tiles[t].blocks = b;
+    }
+    int64_t all;
+    const int64_t at = units + block_scan(n, lds, &all);
+    if (t < tiles) p.before[t] = at;
+    units += all;
+  }
+  if (threadIdx.x == 0) {
+    const int64_t U = units * p.c.Hkv;
+    shares_s = U > 0 ? unit_shares(U, p.grid, kPagedLeast) : 0;
+    p.before[tiles] = units;
+    *p.head = PlanHead{units, tiles, (int)shares_s};
+  }
+  __syncthreads();
+  const int shares = (int)shares_s;
+  for (int w = threadIdx.x; w < shares; w += 1024) {
+    const int64_t u = unit_start(units * p.c.Hkv, shares, w + 1) - 1;
+    const int64_t h = u / units, rest = u - h * units;
+    int lo = 0, hi = tiles - 1;  // last tile with before <= rest
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (p.before[mid] <= rest) lo = mid;
+      else hi = mid - 1;
+    }
+    p.ends[w] = PlanEnd{(int)h, lo, (int)(rest - p.before[lo]) + 1, 0};
+  }
+}
+
+// Joins the partials of the row tile that share blockIdx.x ends in, if the
+// share is also where the tile starts: one of the shares it spans does it.
+// blockIdx.y: 16 rows of the tile, four per wave, whose loads are in flight
+// together (latency bounds this kernel, not the 67 MB that a launch's partials
+// come to at most: one row at a time per wave, it took 130 us).
+template <typename E>
+__global__ __launch_bounds__(256) void paged_merge_tiles_kernel(PagedAttnParams p, int D, int rows) {
+  const PlanHead hd = *p.head;
+  const int w = blockIdx.x;
+  if (w + 1 >= hd.shares) return;
+  const PlanEnd end = p.ends[w];
+  const PlanTile tile = p.plan_tiles[end.tile];
+  if (end.blk == tile.units) return;       // with a tile's last part
+  const int64_t U = hd.per_head * p.c.Hkv, u0 = end.h * hd.per_head + p.before[end.tile];
+  if (wg_of_unit(U, hd.shares, u0) != w) return;
+  const DecodeSlots parts = decode_slots(U, hd.shares, u0, tile.units);
+  const PagedSeq sq = paged_seq(p.c, tile.seq);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int r0 = 16 * blockIdx.y + 4 * wave, last = sq.n * p.group - tile.r0;
+  float M[4], l[4], acc[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    M[j] = kNoKeys;
+    l[j] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[j][k] = 0.f;
+  }
+  for (int i = 0; i < parts.count; ++i) {
+    const int64_t at = (i == 0 ? parts.first : parts.rest + 2 * i) * rows + r0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) M[j] = __builtin_fmaxf(M[j], p.ws_ml[2 * (at + j)]);
+  }
+  for (int i = 0; i < parts.count; ++i) {
+    const int64_t at = (i == 0 ? parts.first : parts.rest + 2 * i) * rows + r0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float wt = __builtin_amdgcn_exp2f(p.ws_ml[2 * (at + j)] - M[j]);
+      l[j] = __builtin_fmaf(wt, p.ws_ml[2 * (at + j) + 1], l[j]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (64 * k < D && lane + 64 * k < D) acc[j][k] = __builtin_fmaf(wt, p.ws_o[(at + j) * D + lane + 64 * k], acc[j][k]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (r0 + j >= last) continue;          // rows past the sequence's end: their slots hold nothing
+    const int i = (tile.r0 + r0 + j) / p.group, hq = end.h * p.group + (tile.r0 + r0 + j) - i * p.group;
+    const int64_t t = (int64_t)sq.t0 + i;
+    const float inv = l[j] == 0.f ? 0.f : 1.0f / l[j];
+    E* out = reinterpret_cast<E*>(p.o + t * p.o_str[0] + hq * p.o_str[1]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (lane + 64 * k < D) out[lane + 64 * k] = (E)(acc[j][k] * inv);
+    if (p.lse && lane == 0)
+      p.lse[t * p.H + hq] = l[j] == 0.f ? -__builtin_inff() : (M[j] + __log2f(l[j])) * 0.69314718055994530942f;
   }
 }
 
@@ -503,44 +626,43 @@ template <int D, typename E, int BITS> struct Gather {
 };
 
 // How an attention call runs: row tiles of 16 or 32 rows on the decode kernel
-// or 128 or 256 on the prefill kernels, and the launch's size.
+// or 128 or 256 on the prefill kernels, the work-groups that share its key
+// blocks, and its workspace.
 struct AttnShape {
-  int rows, grid, tiles, splits;
-  int64_t o_elems, ml_elems;
+  int rows, grid, tiles;
+  int64_t o_elems, ml_elems, plan_bytes;
+  int64_t bytes() const { return 4 * (o_elems + ml_elems) + plan_bytes; }
 };
+int64_t plan_offset(const AttnShape& s, int part) {
+  const int64_t head = 64, tiles = head + (int64_t)s.tiles * sizeof(PlanTile),
+                before = tiles + ((int64_t)s.tiles + 2) * 8, ends = before + (int64_t)s.grid * sizeof(PlanEnd);
+  const int64_t at[] = {0, head, tiles, before, ends};
+  return ceil_div(at[part], 16) * 16;
+}
 
 AttnShape attn_shape(const lvsa_paged_attn_args* a) {
   AttnShape s{};
   const int group = a->H / a->cache.Hkv, D = a->cache.D;
-  const int64_t N = a->batch.N, cus = cu_count();
+  const int64_t N = a->batch.N, cus = cu_count(), B = a->batch.B < N ? a->batch.B : N;
   const int64_t cap = (int64_t)a->batch.max_pages * a->cache.page_size;
-  const int64_t kv = a->max_kv_len > 0 && a->max_kv_len < cap ? a->max_kv_len : cap;
   const int64_t q = a->max_q_len > 0 && a->max_q_len < N ? a->max_q_len : N;
   const int64_t tile_rows = q * group;
   if (tile_rows <= 32) {
     s.rows = tile_rows <= 16 ? 16 : 32;
-    const int keys = paged_decode_keys(D);
-    const int64_t per_cu = 2;
-    const int64_t units = ceil_div(kv, keys) * a->cache.Hkv * (int64_t)(a->batch.B < N ? a->batch.B : N);
-    s.grid = (int)(units < cus * per_cu ? (units > 0 ? units : 1) : cus * per_cu);
-    s.splits = 0;
-    s.o_elems = 2LL * s.grid * s.rows * D;
-    s.ml_elems = 2LL * 2 * s.grid * s.rows;
+    const int64_t kv = a->max_kv_len > 0 && a->max_kv_len < cap ? a->max_kv_len : cap;
+    const int64_t units = ceil_div(kv, paged_decode_keys(D)) * a->cache.Hkv * B, slots = 2 * cus;
+    s.grid = (int)(units < slots ? (units > 0 ? units : 1) : slots);
   } else {
     s.rows = D <= 128 && tile_rows > kPagedTile ? kPagedTall : kPagedTile;
-    const int64_t B = a->batch.B < N ? a->batch.B : N;
     s.tiles = (int)(ceil_div(N * group, s.rows) + B);
-    const int64_t tiles = ceil_div(N * group, s.rows) * a->cache.Hkv;
+    const int64_t units = s.tiles * ceil_div(cap > 0 ? cap : 1, kPagedBlock) * a->cache.Hkv;
     const int64_t slots = cus * (D >= 192 || s.rows == kPagedTall ? 1 : 2);
-    int64_t sp = tiles > 0 ? slots / tiles : 1;
-    const int64_t most = ceil_div(kv, 4 * kPagedBlock);
-    sp = sp < most ? sp : most;
-    sp = sp < 64 ? sp : 64;
-    s.splits = (int)(sp > 1 ? sp : 1);
-    const int64_t slots_ws = s.splits > 1 ? (int64_t)s.tiles * a->cache.Hkv * s.splits : 0;
-    s.o_elems = slots_ws * s.rows * D;
-    s.ml_elems = slots_ws * s.rows * 2;
+    // a multiple of the XCDs: see share_of
+    s.grid = (int)(8 * ceil_div(units < slots ? units : slots, 8));
+    s.plan_bytes = plan_offset(s, 4);
   }
+  s.o_elems = 2LL * s.grid * s.rows * D;
+  s.ml_elems = 2LL * 2 * s.grid * s.rows;
   return s;
 }
 
@@ -624,7 +746,7 @@ int lvsa_paged_attn_workspace_query(const lvsa_paged_attn_args* a, int64_t* byte
   const int rc = attn_check(a, &v);
   if (rc) return rc;
   const AttnShape s = attn_shape(a);
-  *bytes = a->batch.N == 0 ? 0 : 4 * (s.o_elems + s.ml_elems);
+  *bytes = a->batch.N == 0 ? 0 : s.bytes();
   return LVSA_OK;
 }
 
@@ -644,9 +766,7 @@ int lvsa_paged_attn_fwd(const lvsa_paged_attn_args* a, hipStream_t stream) {
   }
   LVSA_REQUIRE(ok, LVSA_ERR_INVALID_ARG, "%s: rows must start at multiples of 16 bytes", what);
   const AttnShape s = attn_shape(a);
-  LVSA_REQUIRE((int64_t)s.tiles * a->cache.Hkv < (1 << 24), LVSA_ERR_UNSUPPORTED, "%s: %d row tiles of %d key heads", what,
-               s.tiles, a->cache.Hkv);
-  const int64_t need = 4 * (s.o_elems + s.ml_elems);
+  const int64_t need = s.bytes();
   LVSA_REQUIRE(need == 0 || (a->workspace && aligned16((int64_t)(uintptr_t)a->workspace)), LVSA_ERR_INVALID_ARG,
                "%s: %lld bytes of 16-byte aligned workspace needed", what, (long long)need);
   LVSA_REQUIRE(need == 0 || a->workspace_bytes >= need, LVSA_ERR_CAPACITY, "%s: workspace of %lld bytes < %lld", what,
@@ -661,11 +781,20 @@ int lvsa_paged_attn_fwd(const lvsa_paged_attn_args* a, hipStream_t stream) {
   p.fill_tail = a->fill_tail;
   p.grid = s.grid;
   p.tiles = s.tiles;
-  p.splits = s.splits;
-  p.ws_o = (float*)a->workspace;
-  p.ws_ml = p.ws_o ? p.ws_o + s.o_elems : nullptr;
+  char* ws = (char*)a->workspace;
+  p.head = (PlanHead*)(ws + plan_offset(s, 0));
+  p.plan_tiles = (PlanTile*)(ws + plan_offset(s, 1));
+  p.before = (int64_t*)(ws + plan_offset(s, 2));
+  p.ends = (PlanEnd*)(ws + plan_offset(s, 3));
+  p.ws_o = (float*)(ws + s.plan_bytes);
+  p.ws_ml = p.ws_o + s.o_elems;
   const bool bf16 = a->cache.dtype == LVSA_BF16;
   if (a->batch.B > 0) {
+    if (s.tiles > 0) {
+      hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(1024), 0, stream, p, s.rows);
+      rc = launch_status(what);
+      if (rc) return rc;
+    }
     switch (a->cache.D) {
       case 64: rc = paged_attn_d64(p, a->cache.bits, s.rows, bf16, stream); break;
       case 96: rc = paged_attn_d96(p, a->cache.bits, s.rows, bf16, stream); break;
@@ -675,8 +804,15 @@ int lvsa_paged_attn_fwd(const lvsa_paged_attn_args* a, hipStream_t stream) {
     }
     if (rc) return rc;
   }
-  // the prefill kernel writes every row itself unless its tiles run in parts
-  if (s.splits == 1 && a->batch.B > 0) return LVSA_OK;
+  if (s.tiles > 0 && a->batch.B > 0) {
+    const dim3 merge((unsigned)s.grid, (unsigned)(s.rows / 16));
+    if (bf16) {
+      hipLaunchKernelGGL((paged_merge_tiles_kernel<__bf16>), merge, dim3(256), 0, stream, p, a->cache.D, s.rows);
+    } else {
+      hipLaunchKernelGGL((paged_merge_tiles_kernel<_Float16>), merge, dim3(256), 0, stream, p, a->cache.D, s.rows);
+    }
+    return launch_status(what);
+  }
   const int out_rows = a->batch.N * a->H;
   const dim3 grid((unsigned)(out_rows < kMaxGrid ? out_rows : kMaxGrid));
   const int keys = paged_decode_keys(a->cache.D);

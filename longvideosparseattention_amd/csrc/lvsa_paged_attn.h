@@ -158,8 +158,7 @@ __device__ __forceinline__ void add_nonfinite_keys(const PagedView& c, const int
   }
 }
 
-// Row r of a (sequence, key head) pair: its q and o / lse, and the end of the
-// keys it attends.
+// Row r of a (sequence, key head) pair: its token and query head.
 struct RowRef {
   int64_t tok;
   int head;
@@ -168,12 +167,6 @@ __device__ __forceinline__ RowRef row_ref(const PagedAttnParams& p, const PagedS
   const int i = r / p.group;
   return RowRef{(int64_t)s.t0 + i, h * p.group + (r - i * p.group)};
 }
-__device__ __forceinline__ int key_limit(const PagedAttnParams& p, const PagedSeq& s, int r) {
-  if (!p.causal) return s.L;
-  const int64_t e = (int64_t)s.first + r / p.group + 1;
-  return e < 0 ? 0 : e > s.L ? s.L : (int)e;
-}
-
 // ─────────────────────────────── decode ────────────────────────────────────
 
 // Keys and values of one step of a wave, on their way from memory: T tiles of
@@ -257,7 +250,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 192 && NT == 2)) ? 1 : 2) v
 
   const int64_t u_first = u;
   while (u < u_end && seq < p.c.B) {
-    const PagedSeq sq = paged_seq(p.c, seq);
+    const PagedSeq sq = uniform(paged_seq(p.c, seq));
     const int64_t units = decode_units(p, sq, ROWS, KEYS);
     if (u >= base + units) {
       base += units;
@@ -570,7 +563,7 @@ __device__ __forceinline__ void fill_tail_rows(const PagedAttnParams& p, int D, 
   const int head = p.c.cu[0] < 0 ? 0 : p.c.cu[0] > p.c.N ? p.c.N : p.c.cu[0];
   const int tail = p.c.cu[p.c.B] < head ? head : p.c.cu[p.c.B] > p.c.N ? p.c.N : p.c.cu[p.c.B];
   const int64_t n = (int64_t)(head + p.c.N - tail) * p.H;
-  const int64_t wg = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, wgs = (int64_t)gridDim.x * gridDim.y;
+  const int64_t wg = blockIdx.x, wgs = gridDim.x;
   for (int64_t i = wg * waves + wave; i < n; i += waves * wgs) {
     const int64_t r = i / p.H, hq = i - r * p.H, t = r < head ? r : tail + (r - head);
     for (int d = lane; d < D; d += 64) reinterpret_cast<uint16_t*>(p.o + t * p.o_str[0] + hq * p.o_str[1])[d] = 0;
@@ -578,52 +571,20 @@ __device__ __forceinline__ void fill_tail_rows(const PagedAttnParams& p, int D, 
   }
 }
 
-// Row tile and key head of this work-group, or false past the last tile (the
-// launch is sized by a bound).  Tiles run from the last to the first: with a
-// causal order the later ones are the longer ones, and a launch that ends on
-// short tiles ends evenly.  Consecutive work-groups, which go to different
-// XCDs, are the key heads of one tile, so an XCD keeps to a few heads and
-// their keys stay in its L2.
-struct TileRef {
-  PagedSeq sq;
-  int seq, h, r0;
-  int64_t index;
-};
-__device__ __forceinline__ bool find_tile(const PagedAttnParams& p, int rows, int lane, int wave, TileRef* t) {
-  t->h = (int)(blockIdx.x % (uint32_t)p.c.Hkv);
-  t->index = p.tiles - 1 - (int64_t)(blockIdx.x / (uint32_t)p.c.Hkv);
-  int64_t base = 0;
-  int flags = 0;
-  t->seq = -1;
-  for (int s0 = 0; s0 < p.c.B; s0 += 64) {
-    int64_t n = 0;
-    if (s0 + lane < p.c.B) {
-      const PagedSeq q = paged_seq(p.c, s0 + lane);
-      n = ((int64_t)q.n * p.group + rows - 1) / rows;
-      flags |= q.flags;
-    }
-    const int64_t incl = wave_scan(n, lane);
-    const uint64_t above = __builtin_amdgcn_ballot_w64(base + incl > t->index);
-    if (above && t->seq < 0) {
-      const int at = __builtin_ctzll(above);
-      t->seq = s0 + at;
-      t->r0 = (int)(t->index - (base + __shfl(incl - n, at))) * rows;
-      if (blockIdx.x != 0 || blockIdx.y != 0) break;   // the first work-group looks at every sequence's flags
-    }
-    base += __shfl(incl, 63);
-  }
-  if (blockIdx.x == 0 && blockIdx.y == 0 && wave == 0 && flags) paged_flag(p.c, flags);
-  if (t->seq < 0) return false;
-  t->sq = paged_seq(p.c, t->seq);
-  return true;
+// Share of a work-group.  Consecutive work-groups go to the eight XCDs in turn:
+// an XCD gets consecutive shares, few key heads' tiles, whose keys its L2 then
+// serves to all of them.
+__device__ __forceinline__ int share_of(int wg, int shares) {
+  const int per = (shares + 7) / 8, s = (wg & 7) * per + (wg >> 3);
+  return (wg >> 3) < per && s < shares ? s : -1;
 }
 
-// A row's result, or its partial sums where its tile runs in parts: O of
+// A row's result, or its partial sums where shares divide its tile: O of
 // element 32 dt + 8 q + 4 half + i in o[dt][4 q + i].
 template <int D, typename E>
-__device__ __forceinline__ void store_rows(const PagedAttnParams& p, int64_t slot, int rows, int r, int half,
+__device__ __forceinline__ void store_rows(const PagedAttnParams& p, bool whole, int64_t slot, int rows, int r, int half,
                                            const RowRef& ref, const floatx16* o, float m_run, float l) {
-  if (p.splits > 1) {
+  if (!whole) {
     const int64_t at = slot * rows + r;
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
@@ -686,6 +647,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   constexpr int TB = 32 * D, MAT = 4 * TB, STAGE = 2 * MAT;   // 16-key tile, 64-key matrix, K and V
   constexpr bool kTwoScales = D == 96 || D >= 192;
   __shared__ __attribute__((aligned(1024))) char smem_raw[2 * STAGE];
+  __shared__ int bad_s, odd_s;
   lds_char* smem = (lds_char*)smem_raw;
 
   const int lane = threadIdx.x & 63;
@@ -694,15 +656,27 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   const int g = lane >> 4, x = lane & 15;
 
   if (p.fill_tail) fill_tail_rows(p, D, lane, wave, 4);
-  TileRef tile;
-  if (!find_tile(p, kPagedTile, lane, wave, &tile)) return;
-  const PagedSeq sq = tile.sq;
-  const int h = tile.h, r0 = tile.r0;
+  const PlanHead hd = *p.head;
+  const int shares = uniform(hd.shares), share = share_of(blockIdx.x, shares);
+  if (share < 0) return;
+  // The share's tiles from the last to the first: the part that it ends with
+  // starts at its tile's first key block and the one it starts with ends at the
+  // last, so that the work-groups of an XCD walk a head's keys at about the
+  // same place at the same time, and its L2 serves them.
+  const int64_t per_head = hd.per_head, U = per_head * p.c.Hkv, u_first = unit_start(U, shares, share);
+  int left = uniform((int)(unit_start(U, shares, share + 1) - u_first));
+  int h = uniform(p.ends[share].h), ti = uniform(p.ends[share].tile), blk_end = uniform(p.ends[share].blk);
+  for (;;) {
+  const PlanTile tile = p.plan_tiles[ti];
+  const int seq = uniform(tile.seq), r0 = uniform(tile.r0), units = uniform(tile.units), nb = uniform(tile.blocks);
+  const PagedSeq sq = uniform(paged_seq(p.c, seq));
+  const int blk0 = left < blk_end ? blk_end - left : 0;
+  const bool whole = blk0 == 0 && blk_end == units;
+  const int64_t slot = 2 * (int64_t)share + (u_first < h * per_head + p.before[ti] ? 1 : 0);   // see decode_slots
+  const int blk1 = blk_end < nb ? blk_end : nb;
   const int nrows = sq.n * p.group;
   const int r_last = r0 + kPagedTile < nrows ? r0 + kPagedTile - 1 : nrows - 1;
   const int lim_min = key_limit(p, sq, r0), lim_max = key_limit(p, sq, r_last);
-  const int nb = (lim_max + kPagedBlock - 1) / kPagedBlock;
-  const int blk0 = (int)((int64_t)nb * blockIdx.y / p.splits), blk1 = (int)((int64_t)nb * (blockIdx.y + 1) / p.splits);
 
   const int row = r0 + 32 * wave + i32;             // this lane's row of the pair
   const int rc = row < nrows ? row : nrows - 1;
@@ -717,7 +691,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
 
   const char* kbase = p.c.k + h * p.c.k_str[2];
   const char* vbase = p.c.v + h * p.c.v_str[2];
-  const int32_t* table = p.c.table + tile.seq * p.c.table_str;
+  const int32_t* table = p.c.table + seq * p.c.table_str;
   // The key of tile `wave` that this lane brings (past the end: the last key).
   // 16 bits: chunks 4 i + g of key x ^ 8 (g & 1), so that a copy's fixed order
   // in LDS is the tile's layout.
@@ -853,7 +827,6 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
       for (int dt = 0; dt < NO; ++dt) o[dt] = Mat<E>::mfma32(vfrag(st, dt), pb[st], o[dt]);
   };
 
-  __shared__ int bad_s, odd_s;
   if (threadIdx.x == 0) bad_s = odd_s = 0;
   __syncthreads();
   if (blk0 < blk1) {
@@ -900,7 +873,16 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   }
   float l = l_run + __shfl_xor(l_run, 32);
   if (bad_s) l = __builtin_nanf("");
-  if (row < nrows) store_rows<D, E>(p, (tile.index * p.c.Hkv + h) * p.splits + blockIdx.y, kPagedTile, row - r0, half, ref, o, m_run, l);
+  if (row < nrows) store_rows<D, E>(p, whole, slot, kPagedTile, row - r0, half, ref, o, m_run, l);
+  left -= blk_end - blk0;
+  if (left <= 0) break;
+  if (--ti < 0) {
+    ti = hd.tiles - 1;
+    --h;
+  }
+  blk_end = uniform(p.plan_tiles[ti].units);
+  __syncthreads();                                      // LDS of this tile has been read
+  }
 }
 
 // ──────────────────────────── prefill, tall tiles ──────────────────────────
@@ -971,14 +953,27 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
   const int g = lane >> 4, x = lane & 15;
 
   if (p.fill_tail) fill_tail_rows(p, D, lane, wave, 8);
-  TileRef tile;
-  if (!find_tile(p, kPagedTall, lane, wave, &tile)) return;
-  const PagedSeq sq = tile.sq;
-  const int h = tile.h, r0 = tile.r0, nrows = sq.n * p.group;
+  const PlanHead hd = *p.head;
+  const int shares = uniform(hd.shares), share = share_of(blockIdx.x, shares);
+  if (share < 0) return;
+  // The share's tiles from the last to the first: the part that it ends with
+  // starts at its tile's first key block and the one it starts with ends at the
+  // last, so that the work-groups of an XCD walk a head's keys at about the
+  // same place at the same time, and its L2 serves them.
+  const int64_t per_head = hd.per_head, U = per_head * p.c.Hkv, u_first = unit_start(U, shares, share);
+  int left = uniform((int)(unit_start(U, shares, share + 1) - u_first));
+  int h = uniform(p.ends[share].h), ti = uniform(p.ends[share].tile), blk_end = uniform(p.ends[share].blk);
+  for (;;) {
+  const PlanTile tile = p.plan_tiles[ti];
+  const int seq = uniform(tile.seq), r0 = uniform(tile.r0), units = uniform(tile.units), nb = uniform(tile.blocks);
+  const PagedSeq sq = uniform(paged_seq(p.c, seq));
+  const int blk0 = left < blk_end ? blk_end - left : 0;
+  const bool whole = blk0 == 0 && blk_end == units;
+  const int64_t slot = 2 * (int64_t)share + (u_first < h * per_head + p.before[ti] ? 1 : 0);   // see decode_slots
+  const int blk1 = blk_end < nb ? blk_end : nb;
+  const int nrows = sq.n * p.group;
   const int r_last = r0 + kPagedTall < nrows ? r0 + kPagedTall - 1 : nrows - 1;
   const int lim_min = key_limit(p, sq, r0), lim_max = key_limit(p, sq, r_last);
-  const int nb = (lim_max + kPagedBlock - 1) / kPagedBlock;
-  const int blk0 = (int)((int64_t)nb * blockIdx.y / p.splits), blk1 = (int)((int64_t)nb * (blockIdx.y + 1) / p.splits);
   const int n = blk1 - blk0;
 
   const int row = r0 + 32 * wave + i32;
@@ -990,7 +985,7 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
   const int64_t str0 = grp == 0 ? p.c.k_str[0] : p.c.v_str[0], str1 = grp == 0 ? p.c.k_str[1] : p.c.v_str[1];
   const uint8_t* scl = BITS == 16 ? nullptr : grp == 0 ? p.c.ks + h * p.c.ks_str[2] : p.c.vs + h * p.c.vs_str[2];
   const int64_t sst0 = grp == 0 ? p.c.ks_str[0] : p.c.vs_str[0], sst1 = grp == 0 ? p.c.ks_str[1] : p.c.vs_str[1];
-  const int32_t* table = p.c.table + tile.seq * p.c.table_str;
+  const int32_t* table = p.c.table + seq * p.c.table_str;
   lds_char* ring = smem + grp * VB + dw * TB;           // this wave's tile of stage 0
   lds_char* pids = smem + PB + wave * 1024;
   const int my_key = 16 * dw + (BITS == 16 ? x ^ (8 * (g & 1)) : x);
@@ -1200,16 +1195,27 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
     __builtin_amdgcn_s_waitcnt(0xC07F);                 // LDS writes: V of stage 3, tiles, notes
     phase_barrier();
     if (grp == 1) phase_barrier();
-    // Each group passes n softmax phases and n + 1 matrix phases; the barriers
-    // (2 n + 1 for both after the first) pair phase with phase.
-    // (One copy of each phase: with the ring's stages as constants, four copies,
-    // the compiler spilled hundreds of registers where the loop's exits meet.)
-    for (int j = 0;; ++j) {
+    // Each group passes n matrix and n softmax phases, and the last block's
+    // second product; the barriers (2 n + 1 for both after the first) pair phase
+    // with phase.  One copy of each phase and one exit, at the bottom: with the
+    // ring's stages as constants (four copies) the compiler spilled hundreds of
+    // registers, and with the exit after M(n) it moved O to and fro in every
+    // step (64 moves).
+    for (int j = 0; j < n; ++j) {
       mphase(j);
-      if (j >= n) break;
       phase_barrier();
       sphase(j);
       phase_barrier();
+    }
+    {
+      const int vst = ((n + 3) & 3) * MAT, v0 = voff0 + vst, v1 = voff1 + vst;
+#pragma unroll
+      for (int st = 0; st < 4; ++st)
+#pragma unroll
+        for (int dt = 0; dt < NO; ++dt) {
+          const shortx4 a = read_tr(smem + v0 + st * TB + 1024 * dt), c = read_tr(smem + v1 + st * TB + 1024 * dt);
+          o[dt] = Mat<E>::mfma32(__builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7), pb[st], o[dt]);
+        }
     }
     if (grp == 0) phase_barrier();
     wait_copies<0>();                                   // copies past the last block land before the work-group ends
@@ -1229,18 +1235,25 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
   const float l_run = (l4[0] + l4[1]) + (l4[2] + l4[3]);
   float l = l_run + __shfl_xor(l_run, 32);
   if (bad_s) l = __builtin_nanf("");
-  if (row < nrows) store_rows<D, E>(p, (tile.index * p.c.Hkv + h) * p.splits + blockIdx.y, kPagedTall, row - r0, half, ref, o, m_run, l);
+  if (row < nrows) store_rows<D, E>(p, whole, slot, kPagedTall, row - r0, half, ref, o, m_run, l);
+  left -= blk_end - blk0;
+  if (left <= 0) break;
+  if (--ti < 0) {
+    ti = hd.tiles - 1;
+    --h;
+  }
+  blk_end = uniform(p.plan_tiles[ti].units);
+  __syncthreads();                                      // LDS of this tile has been read
+  }
 }
 
 template <int D, typename E, int BITS>
 int paged_launch(const PagedAttnParams& p, int rows, hipStream_t stream) {
   if (rows == kPagedTall) {
     if constexpr (D <= 128)
-      hipLaunchKernelGGL((paged_tall_kernel<D, E, BITS>), dim3((unsigned)(p.tiles * p.c.Hkv), (unsigned)p.splits), dim3(512), 0,
-                         stream, p);
+      hipLaunchKernelGGL((paged_tall_kernel<D, E, BITS>), dim3((unsigned)p.grid), dim3(512), 0, stream, p);
   } else if (rows == kPagedTile) {
-    hipLaunchKernelGGL((paged_prefill_kernel<D, E, BITS>), dim3((unsigned)(p.tiles * p.c.Hkv), (unsigned)p.splits),
-                       dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((paged_prefill_kernel<D, E, BITS>), dim3((unsigned)p.grid), dim3(256), 0, stream, p);
   } else if (rows == 16) {
     hipLaunchKernelGGL((paged_decode_kernel<D, E, BITS, 1>), dim3((unsigned)p.grid), dim3(256), 0, stream, p);
   } else {

@@ -421,14 +421,19 @@ def test_bad_appends_leave_the_cache_alone(gpu, bits):
 
 @pytest.mark.parametrize("n", [2, 100])
 def test_bad_lengths_and_row_ranges(gpu, n):
+    """A bad length spoils its sequence; the others stay within the definition's tolerance (which work-groups share a
+    sequence, and so its sums' order, depends on the whole batch's lengths)."""
     b = Batch(gpu, [(n, 150), (n, 140), (n, 133)], 128, 4, 2, 16, BF)
     q = b.randn(b.N, 4, 128)
-    good, _ = _attend(b, q, max_q_len=n)
+    _attend(b, q, max_q_len=n)
+    want, _, tol, _ = ref.attention(b, q)
     for bad in (-1, -2 ** 31, 2 ** 31 - 1, 161):
         lens = b.lens.clone()
         lens[1] = bad
         o = lv.paged_attention(q, b.cache, b.cu, lens, b.table_dev, max_q_len=n)
-        assert torch.isnan(o[n:2 * n]).all() and torch.equal(o[:n], good[:n]) and torch.equal(o[2 * n:], good[2 * n:])
+        assert torch.isnan(o[n:2 * n]).all()
+        for r in (slice(0, n), slice(2 * n, 3 * n)):
+            ref.check_close(o[r], want[r], tol[r], f"beside length {bad}")
         with pytest.raises(ValueError, match="kv_lens"):
             b.cache.check()
     for cu in ([0, n, 2 * n, 3 * n + 50], [0, 2 * n, n, 3 * n], [-5, n, 2 * n, 3 * n], [0, n, 2 ** 31 - 1, 3 * n]):
