@@ -27,20 +27,34 @@ struct PagedView {
   int32_t B, max_pages, N;
 };
 
+// Sequence s: its rows [t0, t0 + n) of the packed ones, its cached length, and
+// the position of row t0 (paged_seq).
+struct PagedSeq {
+  int t0, n, L, first;
+  int flags;
+};
+
 // What paged_plan_kernel writes for the prefill kernels, at the start of the
 // workspace: the row tiles of all sequences (each is done once per key head),
-// the units (key blocks) before each, and where each share of the launch's
-// units ends.  Units are ordered by key head, tile and key block; a tile
-// without keys counts as one.
+// the units (key blocks) before each, where each share of the launch's units
+// ends, and what the tile it ends in is to be joined from.  Units are ordered
+// by key head, tile and key block; a tile without keys counts as one.
 struct PlanHead {
   int64_t per_head;              // units of one key head
   int32_t tiles, shares;
 };
 struct PlanTile {
   int32_t seq, r0, units, blocks;
+  PagedSeq sq;
+  int32_t pad[3];
 };
 struct PlanEnd {
   int32_t h, tile, blk, pad;     // the share's last unit is unit blk - 1 of this tile
+};
+struct PlanJoin {
+  int64_t first, rest;           // see DecodeSlots
+  int32_t count;                 // 0: nothing to join
+  int32_t h, r0, rows, t0, pad[3];
 };
 
 struct PagedAttnParams {
@@ -49,6 +63,7 @@ struct PagedAttnParams {
   int64_t q_str[2], o_str[2];    // bytes
   float scale_log2;              // scale * log2(e)
   int32_t H, group, causal, fill_tail;
+  int32_t short_rows;            // 16 slots of a page lie within 2^31 bytes
   // The launch's key blocks are cut into equal shares for `grid` work-groups,
   // each with two slots of row-tile partials: fp32 O [slot][rows][D], then
   // (max, sum) pairs.  Prefill kernels: `tiles` bounds the row tiles.
@@ -58,6 +73,7 @@ struct PagedAttnParams {
   PlanTile* plan_tiles;
   int64_t* before;               // [tiles + 1]
   PlanEnd* ends;                 // [grid]
+  PlanJoin* joins;               // [grid]
 };
 
 // Attention launches per head size.  rows: 16 or 32 (decode kernel, row tiles
@@ -85,13 +101,8 @@ __host__ __device__ inline int page_of(const PagedView& c, int pos) {
   return (int)(((uint64_t)(uint32_t)pos * c.ps_mul) >> c.ps_shift);
 }
 
-// Sequence s: its rows [t0, t0 + n) of the packed ones, its cached length, and
-// the position of row t0.  Ranges and lengths outside what the caller
-// allocated are cut to it and flagged.
-struct PagedSeq {
-  int t0, n, L, first;
-  int flags;
-};
+// Sequence s.  Ranges and lengths outside what the caller allocated are cut to
+// it and flagged.
 __host__ __device__ inline PagedSeq paged_seq(const PagedView& c, int s) {
   PagedSeq r;
   const int a = c.cu[s], e = c.cu[s + 1], len = c.lens[s];

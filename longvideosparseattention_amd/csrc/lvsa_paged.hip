@@ -404,123 +404,150 @@ __device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* lds, int64_t* 
   return before + incl - x;
 }
 
-// One work-group: lists the row tiles with their key blocks, and where the
-// shares end.  Latency: a few dependent reads and scans, 5 us beside launches
-// of 30 us and more; with it every work-group of those gets the same number of
-// key blocks, whatever the lengths, where tiles as units leave the last round
-// to a few (516 tiles on 256 CUs: three rounds for two rounds' work).
+// One work-group: lists the row tiles with their key blocks, where the shares
+// end and what is to be joined there.  Latency only: two dependent reads of
+// memory, scans and searches in LDS (searches in memory past kPlanLds tiles); 4
+// us beside launches of 30 us and more.  With it every work-group of those
+// gets the same number of key blocks, whatever the lengths, where tiles as units
+// leave the last round to a few (516 tiles on 256 CUs: three rounds for two
+// rounds' work).
+constexpr int kPlanLds = 4096;
 __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int rows) {
   __shared__ int64_t lds[16];
-  __shared__ int64_t shares_s;
-  int64_t done = 0;              // tiles before this chunk of sequences
+  __shared__ int64_t before_s[kPlanLds];
+  __shared__ PagedSeq seq_s[1024];
+  __shared__ int64_t first_s[1024];                    // tiles before a sequence of the chunk
+  int64_t done = 0, units = 0;                          // tiles and units before this chunk of sequences
   for (int s0 = 0; s0 < p.c.B; s0 += 1024) {
-    const int s = s0 + threadIdx.x;
+    const int s = s0 + threadIdx.x, ns = p.c.B - s0 < 1024 ? p.c.B - s0 : 1024;
     int64_t nt = 0;
+    PagedSeq q = {};
     if (s < p.c.B) {
-      const PagedSeq q = paged_seq(p.c, s);
+      q = paged_seq(p.c, s);
       if (q.flags) paged_flag(p.c, q.flags);
       nt = ((int64_t)q.n * p.group + rows - 1) / rows;
     }
     int64_t all;
-    const int64_t at = done + block_scan(nt, lds, &all);
+    const int64_t at = block_scan(nt, lds, &all);
+    first_s[threadIdx.x] = at;
+    seq_s[threadIdx.x] = q;
+    __syncthreads();
     // row ranges that overlap give more tiles than the bound: the rest is dropped
-    for (int64_t i = 0; i < nt && at + i < p.tiles; ++i) p.plan_tiles[at + i] = PlanTile{s, (int)(i * rows), 0, 0};
-    done += all;
-  }
-  const int tiles = (int)(done < p.tiles ? done : p.tiles);
-  __syncthreads();               // the list is read by other threads than its writers
-  int64_t units = 0;
-  for (int t0 = 0; t0 < tiles; t0 += 1024) {
-    const int t = t0 + threadIdx.x;
-    int n = 0;
-    if (t < tiles) {
-      const PlanTile w = p.plan_tiles[t];
-      const int b = tile_blocks(p, paged_seq(p.c, w.seq), w.r0, rows);
-      n = b > 0 ? b : 1;
-      p.plan_tiles[t].units = n;
-      p.plan_tiles[t].blocks = b;
+    if (done + all > p.tiles) all = p.tiles - done;
+    for (int64_t t0 = 0; t0 < all; t0 += 1024) {
+      const int64_t t = t0 + threadIdx.x;
+      PlanTile w = {};
+      if (t < all) {
+        int lo = 0, hi = ns - 1;                        // last sequence with first <= t
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (first_s[mid] <= t) lo = mid;
+          else hi = mid - 1;
+        }
+        w.seq = s0 + lo;
+        w.sq = seq_s[lo];
+        w.r0 = (int)((t - first_s[lo]) * rows);
+        w.blocks = tile_blocks(p, w.sq, w.r0, rows);
+        w.units = w.blocks > 0 ? w.blocks : 1;
+      }
+      int64_t sum;
+      const int64_t u = units + block_scan(w.units, lds, &sum);
+      if (t < all) {
+        p.plan_tiles[done + t] = w;
+        p.before[done + t] = u;
+        if (done + t < kPlanLds) before_s[done + t] = u;
+      }
+      units += sum;
     }
-    int64_t all;
-    const int64_t at = units + block_scan(n, lds, &all);
-    if (t < tiles) p.before[t] = at;
-    units += all;
+    done += all;
+    __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    const int64_t U = units * p.c.Hkv;
-    shares_s = U > 0 ? unit_shares(U, p.grid, kPagedLeast) : 0;
-    p.before[tiles] = units;
-    *p.head = PlanHead{units, tiles, (int)shares_s};
-  }
-  __syncthreads();
-  const int shares = (int)shares_s;
+  const int tiles = (int)done;
+  const int64_t U = units * p.c.Hkv;
+  const int shares = U > 0 ? unit_shares(U, p.grid, kPagedLeast) : 0;
+  if (threadIdx.x == 0) *p.head = PlanHead{units, tiles, shares};
+  const bool in_lds = tiles <= kPlanLds;
   for (int w = threadIdx.x; w < shares; w += 1024) {
-    const int64_t u = unit_start(units * p.c.Hkv, shares, w + 1) - 1;
+    const int64_t u = unit_start(U, shares, w + 1) - 1;
     const int64_t h = u / units, rest = u - h * units;
     int lo = 0, hi = tiles - 1;  // last tile with before <= rest
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (p.before[mid] <= rest) lo = mid;
+      if ((in_lds ? before_s[mid] : p.before[mid]) <= rest) lo = mid;
       else hi = mid - 1;
     }
-    p.ends[w] = PlanEnd{(int)h, lo, (int)(rest - p.before[lo]) + 1, 0};
+    const int64_t b = in_lds ? before_s[lo] : p.before[lo];
+    const PlanTile tile = p.plan_tiles[lo];
+    const int blk = (int)(rest - b) + 1;
+    p.ends[w] = PlanEnd{(int)h, lo, blk, 0};
+    // a tile that shares divide is joined by the one it starts in
+    PlanJoin j = {};
+    const int64_t u0 = h * units + b;
+    if (blk < tile.units && wg_of_unit(U, shares, u0) == w) {
+      const DecodeSlots d = decode_slots(U, shares, u0, tile.units);
+      const int left = tile.sq.n * p.group - tile.r0;
+      j = PlanJoin{d.first, d.rest, d.count, (int)h, tile.r0, left < rows ? left : rows, tile.sq.t0, {0, 0, 0}};
+    }
+    p.joins[w] = j;
   }
 }
 
-// Joins the partials of the row tile that share blockIdx.x ends in, if the
-// share is also where the tile starts: one of the shares it spans does it.
-// blockIdx.y: 16 rows of the tile, four per wave, whose loads are in flight
-// together (latency bounds this kernel, not the 67 MB that a launch's partials
-// come to at most: one row at a time per wave, it took 130 us).
-template <typename E>
-__global__ __launch_bounds__(256) void paged_merge_tiles_kernel(PagedAttnParams p, int D, int rows) {
-  const PlanHead hd = *p.head;
-  const int w = blockIdx.x;
-  if (w + 1 >= hd.shares) return;
-  const PlanEnd end = p.ends[w];
-  const PlanTile tile = p.plan_tiles[end.tile];
-  if (end.blk == tile.units) return;       // with a tile's last part
-  const int64_t U = hd.per_head * p.c.Hkv, u0 = end.h * hd.per_head + p.before[end.tile];
-  if (wg_of_unit(U, hd.shares, u0) != w) return;
-  const DecodeSlots parts = decode_slots(U, hd.shares, u0, tile.units);
-  const PagedSeq sq = paged_seq(p.c, tile.seq);
+// Joins the partials of the row tile that share blockIdx.x ends in, where the
+// plan says so.  blockIdx.y: 32 rows of the tile.  A lane has four elements of
+// a row and a wave R rows at a time, so that every partial is one 16-byte load
+// per lane with the next ones in flight behind it: what bounds it is the bytes,
+// 67 MB for a launch whose 256 shares all end inside a tile of 256 rows of 128.
+template <int D, typename E>
+__global__ __launch_bounds__(256) void paged_merge_tiles_kernel(PagedAttnParams p, int rows) {
+  typedef float f4 __attribute__((ext_vector_type(4)));
+  typedef E e4 __attribute__((ext_vector_type(4)));
+  constexpr int LR = D / 4, R = 64 / LR;               // lanes per row, rows per wave
+  if ((int)blockIdx.x >= p.head->shares) return;
+  const PlanJoin j = p.joins[blockIdx.x];
+  if (j.count == 0) return;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int r0 = 16 * blockIdx.y + 4 * wave, last = sq.n * p.group - tile.r0;
-  float M[4], l[4], acc[4][4];
+  const int sub = lane / LR, d = 4 * (lane % LR);
+  if (sub >= R) return;
+  constexpr int STEPS = 8 / R;
+  float M[STEPS], l[STEPS];
+  f4 o[STEPS];
+  int r[STEPS];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    M[j] = kNoKeys;
-    l[j] = 0.f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) acc[j][k] = 0.f;
+  for (int k = 0; k < STEPS; ++k) {
+    r[k] = 32 * blockIdx.y + 8 * wave + R * k + sub;
+    M[k] = kNoKeys;
+    l[k] = 0.f;
+    o[k] = f4{0.f, 0.f, 0.f, 0.f};
   }
-  for (int i = 0; i < parts.count; ++i) {
-    const int64_t at = (i == 0 ? parts.first : parts.rest + 2 * i) * rows + r0;
+  for (int i = 0; i < j.count; ++i) {
+    const int64_t slot = (i == 0 ? j.first : j.rest + 2 * i) * rows;
+    float m[STEPS], s[STEPS];
+    f4 x[STEPS];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) M[j] = __builtin_fmaxf(M[j], p.ws_ml[2 * (at + j)]);
-  }
-  for (int i = 0; i < parts.count; ++i) {
-    const int64_t at = (i == 0 ? parts.first : parts.rest + 2 * i) * rows + r0;
+    for (int k = 0; k < STEPS; ++k) {
+      m[k] = p.ws_ml[2 * (slot + r[k])];
+      s[k] = p.ws_ml[2 * (slot + r[k]) + 1];
+      x[k] = *reinterpret_cast<const f4*>(p.ws_o + (slot + r[k]) * D + d);
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float wt = __builtin_amdgcn_exp2f(p.ws_ml[2 * (at + j)] - M[j]);
-      l[j] = __builtin_fmaf(wt, p.ws_ml[2 * (at + j) + 1], l[j]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (64 * k < D && lane + 64 * k < D) acc[j][k] = __builtin_fmaf(wt, p.ws_o[(at + j) * D + lane + 64 * k], acc[j][k]);
+    for (int k = 0; k < STEPS; ++k) {
+      const float top = __builtin_fmaxf(M[k], m[k]);
+      const float a = __builtin_amdgcn_exp2f(M[k] - top), b = __builtin_amdgcn_exp2f(m[k] - top);
+      l[k] = l[k] * a + s[k] * b;
+      o[k] = o[k] * a + x[k] * b;
+      M[k] = top;
     }
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (r0 + j >= last) continue;          // rows past the sequence's end: their slots hold nothing
-    const int i = (tile.r0 + r0 + j) / p.group, hq = end.h * p.group + (tile.r0 + r0 + j) - i * p.group;
-    const int64_t t = (int64_t)sq.t0 + i;
-    const float inv = l[j] == 0.f ? 0.f : 1.0f / l[j];
-    E* out = reinterpret_cast<E*>(p.o + t * p.o_str[0] + hq * p.o_str[1]);
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (lane + 64 * k < D) out[lane + 64 * k] = (E)(acc[j][k] * inv);
-    if (p.lse && lane == 0)
-      p.lse[t * p.H + hq] = l[j] == 0.f ? -__builtin_inff() : (M[j] + __log2f(l[j])) * 0.69314718055994530942f;
+  for (int k = 0; k < STEPS; ++k) {
+    if (r[k] >= j.rows) continue;          // rows past the sequence's end: their slots hold nothing
+    const int i = (j.r0 + r[k]) / p.group, hq = j.h * p.group + (j.r0 + r[k]) - i * p.group;
+    const int64_t t = (int64_t)j.t0 + i;
+    const float inv = l[k] == 0.f ? 0.f : 1.0f / l[k];
+    *reinterpret_cast<e4*>(p.o + t * p.o_str[0] + hq * p.o_str[1] + 2 * d) =
+        e4{(E)(o[k][0] * inv), (E)(o[k][1] * inv), (E)(o[k][2] * inv), (E)(o[k][3] * inv)};
+    if (p.lse && d == 0)
+      p.lse[t * p.H + hq] = l[k] == 0.f ? -__builtin_inff() : (M[k] + __log2f(l[k])) * 0.69314718055994530942f;
   }
 }
 
@@ -635,8 +662,9 @@ struct AttnShape {
 };
 int64_t plan_offset(const AttnShape& s, int part) {
   const int64_t head = 64, tiles = head + (int64_t)s.tiles * sizeof(PlanTile),
-                before = tiles + ((int64_t)s.tiles + 2) * 8, ends = before + (int64_t)s.grid * sizeof(PlanEnd);
-  const int64_t at[] = {0, head, tiles, before, ends};
+                before = tiles + ((int64_t)s.tiles + 2) * 8, ends = before + (int64_t)s.grid * sizeof(PlanEnd),
+                joins = ends + (int64_t)s.grid * sizeof(PlanJoin);
+  const int64_t at[] = {0, head, tiles, before, ends, joins};
   return ceil_div(at[part], 16) * 16;
 }
 
@@ -659,12 +687,20 @@ AttnShape attn_shape(const lvsa_paged_attn_args* a) {
     const int64_t slots = cus * (D >= 192 || s.rows == kPagedTall ? 1 : 2);
     // a multiple of the XCDs: see share_of
     s.grid = (int)(8 * ceil_div(units < slots ? units : slots, 8));
-    s.plan_bytes = plan_offset(s, 4);
+    s.plan_bytes = plan_offset(s, 5);
   }
   s.o_elems = 2LL * s.grid * s.rows * D;
   s.ml_elems = 2LL * 2 * s.grid * s.rows;
   return s;
 }
+
+template <int D, typename E, int BITS> struct MergeTiles {
+  static int go(const PagedAttnParams& p, const AttnShape& s, hipStream_t stream) {
+    hipLaunchKernelGGL((paged_merge_tiles_kernel<D, E>), dim3((unsigned)s.grid, (unsigned)(s.rows / 32)), dim3(256), 0, stream,
+                       p, s.rows);
+    return launch_status("lvsa_paged_attn_fwd");
+  }
+};
 
 int attn_check(const lvsa_paged_attn_args* a, PagedView* v) {
   const char* what = "lvsa_paged_attn_fwd";
@@ -778,6 +814,7 @@ int lvsa_paged_attn_fwd(const lvsa_paged_attn_args* a, hipStream_t stream) {
   p.H = a->H;
   p.group = a->H / a->cache.Hkv;
   p.causal = a->causal;
+  p.short_rows = p.c.k_str[1] >= 0 && p.c.k_str[1] < (1 << 26) && p.c.v_str[1] >= 0 && p.c.v_str[1] < (1 << 26);
   p.fill_tail = a->fill_tail;
   p.grid = s.grid;
   p.tiles = s.tiles;
@@ -786,6 +823,7 @@ int lvsa_paged_attn_fwd(const lvsa_paged_attn_args* a, hipStream_t stream) {
   p.plan_tiles = (PlanTile*)(ws + plan_offset(s, 1));
   p.before = (int64_t*)(ws + plan_offset(s, 2));
   p.ends = (PlanEnd*)(ws + plan_offset(s, 3));
+  p.joins = (PlanJoin*)(ws + plan_offset(s, 4));
   p.ws_o = (float*)(ws + s.plan_bytes);
   p.ws_ml = p.ws_o + s.o_elems;
   const bool bf16 = a->cache.dtype == LVSA_BF16;
@@ -805,13 +843,7 @@ int lvsa_paged_attn_fwd(const lvsa_paged_attn_args* a, hipStream_t stream) {
     if (rc) return rc;
   }
   if (s.tiles > 0 && a->batch.B > 0) {
-    const dim3 merge((unsigned)s.grid, (unsigned)(s.rows / 16));
-    if (bf16) {
-      hipLaunchKernelGGL((paged_merge_tiles_kernel<__bf16>), merge, dim3(256), 0, stream, p, a->cache.D, s.rows);
-    } else {
-      hipLaunchKernelGGL((paged_merge_tiles_kernel<_Float16>), merge, dim3(256), 0, stream, p, a->cache.D, s.rows);
-    }
-    return launch_status(what);
+    return by_type<MergeTiles>(a->cache.D, a->cache.dtype, 16, p, s, stream);
   }
   const int out_rows = a->batch.N * a->H;
   const dim3 grid((unsigned)(out_rows < kMaxGrid ? out_rows : kMaxGrid));

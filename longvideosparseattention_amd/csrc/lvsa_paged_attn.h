@@ -18,11 +18,18 @@
 // step is permuted alike on both operands.  V^T comes out of LDS by
 // transposing reads.
 //
-// LDS tile of 16 keys (K or V): 16-byte chunk c (elements 8c .. 8c + 7) of key
-// r at 256 c + 16 (r ^ 8 (c & 1)).  A lane that copies key r always holds that
-// one key, so it looks its page up once per tile; reading 16 keys of a chunk
-// covers all 64 banks, and so does a transposing read of 4 or 8 keys over two
-// chunks (with 16 r alone its two chunks would share half the banks).
+// LDS tiles of K and V, in 16-byte chunks (chunk c: elements 8c .. 8c + 7):
+//   decode    16 keys: key r of chunk c at 256 c + 16 (r ^ 8 (c & 1)).  A lane
+//             loads whole pieces of one key, so it looks one page up per tile.
+//   prefill   8 keys (tile t of the matrix): 128 (c ^ (t & 1)) + 16 (r ^ 4 ((c >>
+//             1) & 1)).  One copy instruction brings 128 bytes of each of 8
+//             keys (16 keys x 64 bytes, as in decode, cost the L1 twice the
+//             lookups and 100 of frames_chunk's 800 us).  Head size 96, whose 12
+//             chunks do not divide by 8, keeps 16 keys x 64 bytes with 4 (c & 3)
+//             in the place of 8 (c & 1).
+// In each, what 16 lanes of a 16-byte read, or 32 of a transposing read (8 keys
+// of two chunks in decode, 4 keys of four in prefill), take in one cycle covers
+// the 64 banks once.
 #pragma once
 #include "lvsa_paged.h"
 
@@ -90,8 +97,14 @@ __device__ __forceinline__ shortx8 decode8(uint32_t codes, uint32_t scale_byte) 
                                            Mat<E>::template decode<2>(codes, s), Mat<E>::template decode<3>(codes, s)});
 }
 
-__device__ __forceinline__ int lds_chunk(int tile_bytes, int r, int c) {
-  return (r >> 4) * tile_bytes + 256 * c + 16 * ((r & 15) ^ (8 * (c & 1)));
+__device__ __forceinline__ int decode_chunk(int D, int r, int c) {
+  return (r >> 4) * 32 * D + 256 * c + 16 * ((r & 15) ^ (8 * (c & 1)));
+}
+template <int D>
+__device__ __forceinline__ int prefill_chunk(int r, int c) {
+  if constexpr (D == 96) return (r >> 4) * 32 * D + 256 * c + 16 * ((r & 15) ^ (4 * (c & 3)));
+  const int t = r >> 3;
+  return t * 16 * D + 128 * (c ^ (t & 1)) + 16 * ((r & 7) ^ (4 * ((c >> 1) & 1)));
 }
 
 // Four keys (rows of the tile) x 16 elements of V, transposed: the lane's
@@ -371,7 +384,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 192 && NT == 2)) ? 1 : 2) v
             odd |= any_nonfinite<E>(w);
             w = finite8<E>(w);
           }
-          *reinterpret_cast<__attribute__((address_space(3))) shortx8*>(vbuf + lds_chunk(TB, 16 * j + x, c)) = w;
+          *reinterpret_cast<__attribute__((address_space(3))) shortx8*>(vbuf + decode_chunk(D, 16 * j + x, c)) = w;
         }
       if (masked) odd_keys |= odd;
       // S^T: row 4 g + r of tile j, column x
@@ -439,9 +452,9 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 192 && NT == 2)) ? 1 : 2) v
       auto vfrag = [&](int i) __attribute__((always_inline)) {
         const int c = 2 * i + (half >> 1);
         vp a;
-        const shortx4 a0 = read_tr(vbuf + lds_chunk(TB, row, c) + 8 * (half & 1));
+        const shortx4 a0 = read_tr(vbuf + decode_chunk(D, row, c) + 8 * (half & 1));
         if constexpr (T == 2) {
-          const shortx4 a1 = read_tr(vbuf + lds_chunk(TB, 16 + row, c) + 8 * (half & 1));
+          const shortx4 a1 = read_tr(vbuf + decode_chunk(D, 16 + row, c) + 8 * (half & 1));
           a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
         } else {
           a = a0;
@@ -621,6 +634,34 @@ __device__ __forceinline__ void copy16(const char* from, const lds_char* l) {
 #pragma clang diagnostic pop
 }
 
+// The same from a uniform base and a 32-bit offset per lane.
+__device__ __forceinline__ void copy16(const char* base, uint32_t off, const lds_char* l) {
+  const uint32_t la = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)l);
+  const uint64_t b = (uint64_t)base;
+  const uint64_t sb = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32)) << 32) |
+                      (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(sb), "s"(la) : "m0", "memory");
+#pragma clang diagnostic pop
+}
+
+// How a wave copies its 16 keys of a 64-key matrix: instruction i of lane l
+// brings chunk(i) of key key(i), counted in the tile, to 16 l behind 1024 i.
+template <int D>
+struct CopyMap {
+  static constexpr int N = D / 32;                  // instructions
+  int lane;
+  __device__ __forceinline__ int key(int i) const {
+    if constexpr (D == 96) return (lane & 15) ^ (4 * (lane >> 4));
+    return ((lane & 7) ^ (4 * ((lane >> 4) & 1))) + 8 * (i / (D / 64));
+  }
+  __device__ __forceinline__ int chunk(int i) const {
+    if constexpr (D == 96) return 4 * i + (lane >> 4);
+    return 8 * (i % (D / 64)) + ((lane >> 3) ^ (i / (D / 64)));
+  }
+};
+
 // Puts zeros in the place of what a wave's own tile of V holds besides finite
 // numbers; whether there was any.
 template <typename E>
@@ -669,7 +710,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   for (;;) {
   const PlanTile tile = p.plan_tiles[ti];
   const int seq = uniform(tile.seq), r0 = uniform(tile.r0), units = uniform(tile.units), nb = uniform(tile.blocks);
-  const PagedSeq sq = uniform(paged_seq(p.c, seq));
+  const PagedSeq sq = uniform(tile.sq);
   const int blk0 = left < blk_end ? blk_end - left : 0;
   const bool whole = blk0 == 0 && blk_end == units;
   const int64_t slot = 2 * (int64_t)share + (u_first < h * per_head + p.before[ti] ? 1 : 0);   // see decode_slots
@@ -692,36 +733,54 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   const char* kbase = p.c.k + h * p.c.k_str[2];
   const char* vbase = p.c.v + h * p.c.v_str[2];
   const int32_t* table = p.c.table + seq * p.c.table_str;
-  // The key of tile `wave` that this lane brings (past the end: the last key).
-  // 16 bits: chunks 4 i + g of key x ^ 8 (g & 1), so that a copy's fixed order
-  // in LDS is the tile's layout.
-  const int my_key = 16 * wave + (BITS == 16 ? x ^ (8 * (g & 1)) : x);
-  auto key_pos = [&](int b) __attribute__((always_inline)) {
-    return key_within(b * kPagedBlock + my_key, sq.L);
+  // Wave w brings keys 16 w .. 16 w + 15 of a block (past the end: the last key).
+  auto key_pos = [&](int b, int key) __attribute__((always_inline)) {
+    return key_within(b * kPagedBlock + 16 * wave + key, sq.L);
   };
   bool bad = (sq.flags & LVSA_PAGED_BAD_LENGTH) != 0;
-  auto row_of = [&](int b, int page, int64_t& pg, int64_t& slot) __attribute__((always_inline)) {
-    const PagedRow at = paged_row(p.c, key_pos(b), page);
+  auto row_of = [&](int b, int key, int page, int64_t& pg, int64_t& slot) __attribute__((always_inline)) {
+    const PagedRow at = paged_row(p.c, key_pos(b, key), page);
     bad |= !at.ok;
     pg = at.page;
     slot = at.slot;
   };
+  const CopyMap<D> map{lane};
+  uint32_t koffs[ND], voffs[ND];                    // of a lane's copies within keys of one page
+#pragma unroll
+  for (int i = 0; i < ND; ++i) {
+    koffs[i] = (uint32_t)map.key(i) * (uint32_t)p.c.k_str[1] + 16 * map.chunk(i);
+    voffs[i] = (uint32_t)map.key(i) * (uint32_t)p.c.v_str[1] + 16 * map.chunk(i);
+  }
+  // pages: of keys x and x of the block, one per lane (x = lane % 16)
   auto bring16 = [&](int b, int page, lds_char* st) __attribute__((always_inline)) {
-    int64_t pg, slot;
-    row_of(b, page, pg, slot);
-    const char* kr = kbase + pg * p.c.k_str[0] + slot * p.c.k_str[1] + 16 * g;
-    const char* vr = vbase + pg * p.c.v_str[0] + slot * p.c.v_str[1] + 16 * g;
+    const int key0 = b * kPagedBlock + 16 * wave, slot0 = key0 - page_of(p.c, key0) * p.c.page_size;
+    if (p.short_rows && key0 + 16 <= sq.L && slot0 + 16 <= p.c.page_size) {   // the 16 keys lie in one page
+      const int pg0 = uniform(page);
+      const bool ok = (uint32_t)pg0 < (uint32_t)p.c.n_pages;
+      bad |= !ok;
+      const int64_t pg = ok ? pg0 : 0;
+      const char* kr = kbase + pg * p.c.k_str[0] + slot0 * p.c.k_str[1];
+      const char* vr = vbase + pg * p.c.v_str[0] + slot0 * p.c.v_str[1];
 #pragma unroll
-    for (int i = 0; i < ND; ++i) copy16(kr + 64 * i, st + wave * TB + 1024 * i);
+      for (int i = 0; i < ND; ++i) copy16(kr, koffs[i], st + wave * TB + 1024 * i);
 #pragma unroll
-    for (int i = 0; i < ND; ++i) copy16(vr + 64 * i, st + MAT + wave * TB + 1024 * i);
+      for (int i = 0; i < ND; ++i) copy16(vr, voffs[i], st + MAT + wave * TB + 1024 * i);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      int64_t pg, slot;
+      row_of(b, map.key(i), __shfl(page, map.key(i)), pg, slot);
+      copy16(kbase + pg * p.c.k_str[0] + slot * p.c.k_str[1] + 16 * map.chunk(i), st + wave * TB + 1024 * i);
+      copy16(vbase + pg * p.c.v_str[0] + slot * p.c.v_str[1] + 16 * map.chunk(i), st + MAT + wave * TB + 1024 * i);
+    }
   };
   struct Codes {
     uint32_t k[ND], v[ND], ks[2], vs[2];
   } codes;
   auto load4 = [&](int b, int page) __attribute__((always_inline)) {
     int64_t pg, slot;
-    row_of(b, page, pg, slot);
+    row_of(b, x, page, pg, slot);
     const uint32_t* kw = reinterpret_cast<const uint32_t*>(kbase + pg * p.c.k_str[0] + slot * p.c.k_str[1] + (D / 8) * g);
     const uint32_t* vw = reinterpret_cast<const uint32_t*>(vbase + pg * p.c.v_str[0] + slot * p.c.v_str[1] + (D / 8) * g);
 #pragma unroll
@@ -741,7 +800,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
       const bool up = kTwoScales && ((D / 4) * g + 8 * i) / 32 != (D / 4) * g / 32;
-      const int at = lds_chunk(TB, 16 * wave + x, ND * g + i);
+      const int at = prefill_chunk<D>(16 * wave + x, ND * g + i);
       typedef __attribute__((address_space(3))) shortx8 lds8;
       *reinterpret_cast<lds8*>(st + at) = decode8<E>(codes.k[i], up ? codes.ks[1] : codes.ks[0]);
       *reinterpret_cast<lds8*>(st + MAT + at) = decode8<E>(codes.v[i], up ? codes.vs[1] : codes.vs[0]);
@@ -751,9 +810,10 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   // LDS reads.  K: key i32 (+ 32), elements 16 c + 8 half .. + 7.  V: keys 4
   // half + (x >> 2) (+ 8) of tile st, elements 32 dt + 16 ((lane >> 4) & 1) +
   // 4 (x & 3) .. + 3; the transposing read hands lane x element x of them.
-  const int koff = lds_chunk(TB, i32, half);
+  constexpr int KS = D == 96 ? 512 : 256, VS = 2 * KS;   // bytes from chunk to chunk + 2, to chunk + 4
+  const int koff[2] = {prefill_chunk<D>(i32, half), prefill_chunk<D>(i32, 2 + half) - KS};   // even and odd c
   const int vrow = 4 * half + (x >> 2), vc = 2 * (g & 1) + ((x & 3) >> 1);
-  const int voff0 = lds_chunk(TB, vrow, vc) + 8 * (x & 1), voff1 = lds_chunk(TB, vrow + 8, vc) + 8 * (x & 1);
+  const int voff0 = prefill_chunk<D>(vrow, vc) + 8 * (x & 1), voff1 = prefill_chunk<D>(vrow + 8, vc) + 8 * (x & 1);
 
   floatx16 o[NO];
 #pragma unroll
@@ -766,8 +826,8 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
     floatx16 s0 = floatx16{0}, s1 = floatx16{0};
 #pragma unroll
     for (int c = 0; c < NK; ++c) {
-      const shortx8 a0 = *reinterpret_cast<lds8*>(ks + koff + 512 * c);
-      const shortx8 a1 = *reinterpret_cast<lds8*>(ks + koff + 512 * c + 2 * TB);
+      const shortx8 a0 = *reinterpret_cast<lds8*>(ks + koff[c & 1] + KS * c);
+      const shortx8 a1 = *reinterpret_cast<lds8*>(ks + koff[c & 1] + KS * c + 2 * TB);
       s0 = Mat<E>::mfma32(a0, qf[c], s0);
       s1 = Mat<E>::mfma32(a1, qf[c], s1);
     }
@@ -818,7 +878,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
     l_run += (ls[0] + ls[1]) + (ls[2] + ls[3]);
 
     auto vfrag = [&](int st, int dt) __attribute__((always_inline)) {
-      const shortx4 a = read_tr(vs + voff0 + st * TB + 1024 * dt), c = read_tr(vs + voff1 + st * TB + 1024 * dt);
+      const shortx4 a = read_tr(vs + voff0 + st * TB + VS * dt), c = read_tr(vs + voff1 + st * TB + VS * dt);
       return __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7);
     };
 #pragma unroll
@@ -830,14 +890,14 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   if (threadIdx.x == 0) bad_s = odd_s = 0;
   __syncthreads();
   if (blk0 < blk1) {
-    int page = table[page_of(p.c, key_pos(blk0))];
+    int page = table[page_of(p.c, key_pos(blk0, x))];
     if constexpr (BITS == 16) {
       bring16(blk0, page, smem);
     } else {
       load4(blk0, page);
       store4(smem);
     }
-    page = table[page_of(p.c, key_pos(blk0 + 1))];
+    page = table[page_of(p.c, key_pos(blk0 + 1, x))];
     auto step = [&](int b, lds_char* cur, lds_char* nxt) __attribute__((always_inline)) {
       __builtin_amdgcn_s_waitcnt(0x0F70);           // vmcnt(0): this wave's copies of block b have landed
       if ((b + 1) * kPagedBlock > lim_min && search_tile<E>(cur + MAT + wave * TB, TB, lane)) odd_s = 1;
@@ -845,7 +905,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
       if (b + 1 < blk1) {
         if constexpr (BITS == 16) bring16(b + 1, page, nxt);
         else load4(b + 1, page);
-        page = table[page_of(p.c, key_pos(b + 2))];
+        page = table[page_of(p.c, key_pos(b + 2, x))];
       }
       compute(b, cur);
       if constexpr (BITS == 4) {
@@ -928,10 +988,10 @@ __device__ __forceinline__ void copy4(const void* from, const lds_char* l) {
 // group 1 V, wave w of each the block's tile w, two blocks ahead: block j + 2
 // goes where block j - 2 was, whose last readers (group 1's M(j - 1) in phase
 // 2 j - 1) are done before M(j).
-//   16 bits: copies past the registers, issued between the matrix
-//   instructions of M(j) and waited for at the end of S(j + 1), with the page
-//   numbers of block j + 4 behind them on the same way, so that no wait of the
-//   compiler's own for an ordinary load ever drains the copies.
+//   16 bits: copies past the registers, issued in the middle of M(j) and waited
+//   for at the end of S(j + 1), with the page numbers of block j + 4 behind them
+//   on the same way, so that no wait of the compiler's own for an ordinary load
+//   ever drains the copies.
 //   4 bits: codes of block j + 3 are loaded in M(j), decoded and written to LDS
 //   in S(j + 1).
 template <int D, typename E, int BITS>
@@ -966,7 +1026,7 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
   for (;;) {
   const PlanTile tile = p.plan_tiles[ti];
   const int seq = uniform(tile.seq), r0 = uniform(tile.r0), units = uniform(tile.units), nb = uniform(tile.blocks);
-  const PagedSeq sq = uniform(paged_seq(p.c, seq));
+  const PagedSeq sq = uniform(tile.sq);
   const int blk0 = left < blk_end ? blk_end - left : 0;
   const bool whole = blk0 == 0 && blk_end == units;
   const int64_t slot = 2 * (int64_t)share + (u_first < h * per_head + p.before[ti] ? 1 : 0);   // see decode_slots
@@ -988,14 +1048,45 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
   const int32_t* table = p.c.table + seq * p.c.table_str;
   lds_char* ring = smem + grp * VB + dw * TB;           // this wave's tile of stage 0
   lds_char* pids = smem + PB + wave * 1024;
-  const int my_key = 16 * dw + (BITS == 16 ? x ^ (8 * (g & 1)) : x);
-  auto key_pos = [&](int j) __attribute__((always_inline)) { return key_within((blk0 + j) * kPagedBlock + my_key, sq.L); };
+  auto key_pos = [&](int j, int key) __attribute__((always_inline)) {
+    return key_within((blk0 + j) * kPagedBlock + 16 * dw + key, sq.L);
+  };
   bool bad = (sq.flags & LVSA_PAGED_BAD_LENGTH) != 0;
-  auto row_at = [&](int j, int page, int64_t& sc) __attribute__((always_inline)) {
-    const PagedRow at = paged_row(p.c, key_pos(j), page);
+  auto row_at = [&](int j, int key, int page, int64_t& sc) __attribute__((always_inline)) {
+    const PagedRow at = paged_row(p.c, key_pos(j, key), page);
     bad |= !at.ok;
     if constexpr (BITS == 4) sc = at.page * sst0 + at.slot * sst1;
     return src + at.page * str0 + at.slot * str1;
+  };
+  // 16 bits: brings keys 16 dw .. + 15 of block j.  Keys of one page, the usual
+  // case: one uniform address, made on the scalar unit.
+  const CopyMap<D> map{lane};
+  uint32_t offs[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) offs[i] = (uint32_t)map.key(i) * (uint32_t)str1 + 16 * map.chunk(i);
+  typedef const __attribute__((address_space(3))) int lds_int;
+  auto bring16 = [&](int j) __attribute__((always_inline)) {
+    const lds_char* at = pids + 256 * (j & 3);
+    lds_char* to = ring + (j & 3) * MAT;
+    const int key0 = (blk0 + j) * kPagedBlock + 16 * dw, slot0 = key0 - page_of(p.c, key0) * p.c.page_size;
+    if (p.short_rows && key0 + 16 <= sq.L && slot0 + 16 <= p.c.page_size) {
+      const int pg0 = uniform(*reinterpret_cast<lds_int*>(at));
+      const bool ok = (uint32_t)pg0 < (uint32_t)p.c.n_pages;
+      bad |= !ok;
+      const char* base = src + (int64_t)(ok ? pg0 : 0) * str0 + slot0 * str1;
+#pragma unroll
+      for (int i = 0; i < ND; ++i) copy16(base, offs[i], to + 1024 * i);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      int64_t none;
+      const int key = map.key(i);
+      copy16(row_at(j, key, *reinterpret_cast<lds_int*>(at + 4 * key), none) + 16 * map.chunk(i), to + 1024 * i);
+    }
+  };
+  auto bring_pages = [&](int j) __attribute__((always_inline)) {
+    copy4(table + page_of(p.c, key_pos(j, x)), pids + 256 * (j & 3));
   };
 
   if (threadIdx.x == 0) bad_s = odd_s = 0;
@@ -1020,7 +1111,7 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
   int page_next = 0;                                    // 4 bits: page number of the next block to load
   auto load4 = [&](int j, int page, Codes& c) __attribute__((always_inline)) {
     int64_t sc = 0;
-    const char* r = row_at(j, page, sc) + (D / 8) * g;
+    const char* r = row_at(j, x, page, sc) + (D / 8) * g;
 #pragma unroll
     for (int i = 0; i < ND; ++i) c.w[i] = reinterpret_cast<const uint32_t*>(r)[i];
     c.s[0] = scl[sc + (D / 4) * g / 32];
@@ -1038,14 +1129,15 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
         w = shortx8{0};
         odd_s = 1;
       }
-      *reinterpret_cast<lds8*>(ring + stage * MAT + lds_chunk(TB, x, ND * g + i)) = w;
+      *reinterpret_cast<lds8*>(ring + stage * MAT + prefill_chunk<D>(x, ND * g + i)) = w;
     }
   };
 
   // LDS reads (see paged_prefill_kernel).
-  const int koff = lds_chunk(TB, i32, half);
+  constexpr int KS = D == 96 ? 512 : 256, VS = 2 * KS;   // bytes from chunk to chunk + 2, to chunk + 4
+  const int koff[2] = {prefill_chunk<D>(i32, half), prefill_chunk<D>(i32, 2 + half) - KS};   // even and odd c
   const int vrow = 4 * half + (x >> 2), vc = 2 * (g & 1) + ((x & 3) >> 1);
-  const int voff0 = VB + lds_chunk(TB, vrow, vc) + 8 * (x & 1), voff1 = VB + lds_chunk(TB, vrow + 8, vc) + 8 * (x & 1);
+  const int voff0 = VB + prefill_chunk<D>(vrow, vc) + 8 * (x & 1), voff1 = VB + prefill_chunk<D>(vrow + 8, vc) + 8 * (x & 1);
 
   floatx16 o[NO];
 #pragma unroll
@@ -1059,15 +1151,10 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
   constexpr int LA = D == 128 ? 3 : 4;
   constexpr int NQK = 2 * NK, NM = NQK + 4 * NO;
   auto mphase = [&](int j) __attribute__((always_inline)) {
-    const int kat = koff + (j & 3) * MAT, vst = ((j + 3) & 3) * MAT, v0 = voff0 + vst, v1 = voff1 + vst;
-    lds_char* to = ring + ((j + 2) & 3) * MAT;
-    const char* from = nullptr;
-    if constexpr (BITS == 16) {
-      int64_t none;
-      from = row_at(j + 2, *reinterpret_cast<const __attribute__((address_space(3))) int*>(pids + 256 * ((j + 2) & 3) + 4 * lane), none) + 16 * g;
-    } else {
+    const int kst = (j & 3) * MAT, kat[2] = {koff[0] + kst, koff[1] + kst}, vst = ((j + 3) & 3) * MAT, v0 = voff0 + vst, v1 = voff1 + vst;
+    if constexpr (BITS == 4) {
       const int page = page_next;
-      page_next = table[page_of(p.c, key_pos(j + 4))];
+      page_next = table[page_of(p.c, key_pos(j + 4, x))];
       load4(j + 3, page, coming);
     }
     shortx8 opa[NM];
@@ -1078,11 +1165,11 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
       const int li = i + LA;
       if (li < NM) {
         if (li < NQK) {
-          opa[li] = *reinterpret_cast<const lds8*>(smem + kat + 512 * (li >> 1) + (li & 1) * 2 * TB);
+          opa[li] = *reinterpret_cast<const lds8*>(smem + kat[(li >> 1) & 1] + KS * (li >> 1) + (li & 1) * 2 * TB);
           __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         } else {
           const int k = li - NQK, st = k / NO, dt = k % NO;
-          const shortx4 a = read_tr(smem + v0 + st * TB + 1024 * dt), c = read_tr(smem + v1 + st * TB + 1024 * dt);
+          const shortx4 a = read_tr(smem + v0 + st * TB + VS * dt), c = read_tr(smem + v1 + st * TB + VS * dt);
           opa[li] = __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7);
           __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
@@ -1095,11 +1182,11 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
           const int k = i - NQK;
           o[k % NO] = Mat<E>::mfma32(opa[i], pb[k / NO], o[k % NO]);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        if constexpr (BITS == 16) {
-          if (i % 4 == 3 && i / 4 < ND) copy16(from + 64 * (i / 4), to + 1024 * (i / 4));
-          if (i == 4 * ND) copy4(table + page_of(p.c, key_pos(j + 4)), pids + 256 * (j & 3));
+        if (BITS == 16 && i == NQK - 1) {
+          bring16(j + 2);
+          bring_pages(j + 4);
         }
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       }
     }
     keep(s0);
@@ -1170,27 +1257,20 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
 
   if (n > 0) {
     if constexpr (BITS == 16) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) copy4(table + page_of(p.c, key_pos(j)), pids + 256 * j);
+      for (int j = 0; j < 4; ++j) bring_pages(j);
       wait_copies<0>();
-      asm volatile("" ::: "memory");
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        int64_t none;
-        const char* from = row_at(j, *reinterpret_cast<const __attribute__((address_space(3))) int*>(pids + 256 * j + 4 * lane), none) + 16 * g;
-#pragma unroll
-        for (int i = 0; i < ND; ++i) copy16(from + 64 * i, ring + j * MAT + 1024 * i);
-      }
+      bring16(0);
+      bring16(1);
       wait_copies<ND>();                                // block 0
       if (grp == 1 && is_masked(0) && search_tile<E>(ring, TB, lane)) odd_s = 1;
     } else {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        load4(j, table[page_of(p.c, key_pos(j))], here4);
+        load4(j, table[page_of(p.c, key_pos(j, x))], here4);
         store4(j, j, here4);
       }
-      load4(2, table[page_of(p.c, key_pos(2))], here4);
-      page_next = table[page_of(p.c, key_pos(3))];
+      load4(2, table[page_of(p.c, key_pos(2, x))], here4);
+      page_next = table[page_of(p.c, key_pos(3, x))];
     }
     __builtin_amdgcn_s_waitcnt(0xC07F);                 // LDS writes: V of stage 3, tiles, notes
     phase_barrier();
@@ -1202,7 +1282,9 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
     // registers, and with the exit after M(n) it moved O to and fro in every
     // step (64 moves).
     for (int j = 0; j < n; ++j) {
+      __builtin_amdgcn_s_setprio(1);                    // the matrix instructions before the other group's exponentials: 3%
       mphase(j);
+      __builtin_amdgcn_s_setprio(0);
       phase_barrier();
       sphase(j);
       phase_barrier();
@@ -1213,7 +1295,7 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
       for (int st = 0; st < 4; ++st)
 #pragma unroll
         for (int dt = 0; dt < NO; ++dt) {
-          const shortx4 a = read_tr(smem + v0 + st * TB + 1024 * dt), c = read_tr(smem + v1 + st * TB + 1024 * dt);
+          const shortx4 a = read_tr(smem + v0 + st * TB + VS * dt), c = read_tr(smem + v1 + st * TB + VS * dt);
           o[dt] = Mat<E>::mfma32(__builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7), pb[st], o[dt]);
         }
     }
