@@ -33,6 +33,8 @@
 #pragma once
 #include "lvsa_paged.h"
 
+#include <type_traits>
+
 namespace lvsa {
 namespace {
 
@@ -677,17 +679,37 @@ __device__ __forceinline__ bool search_tile(lds_char* tile, int bytes, int lane)
   return true;
 }
 
-// Four waves of 32 rows.  Key blocks of 64 keys in two LDS stages: wave w
-// brings tile w (16 keys) of the next block while all four work on the current
-// one.  16-bit pages are copied without passing registers; of 4-bit pages the
-// codes are loaded at the start of a step and written to LDS as 16-bit values
-// at its end, so every row is decoded once for 128 query rows.
+// Workgroup barrier that nothing crosses: the memory clobber orders LDS and
+// global accesses, the scheduling barriers keep a phase's arithmetic in it.
+__device__ __forceinline__ void phase_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+// Materialise x here, so that the compiler does not sink its computation into
+// the phase that uses it.
+template <typename T>
+__device__ __forceinline__ void keep(T& x) {
+  asm volatile("" : "+v"(x));
+}
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  static_assert(N >= 0 && N < 16, "vmcnt immediate");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | N);
+}
+// Four waves of 32 rows, the matrix core of each SIMD with one or two of them:
+// a wave feeds it by itself, with the products of the blocks before and after
+// while it forms the weights of its own block between them.  Two LDS places
+// each for K and V of a block of 64 keys; wave w brings tile w (16 keys).
+// 16-bit pages are copied without passing registers; of 4-bit pages the codes
+// are loaded a step ahead and written to LDS as 16-bit values, so every row is
+// decoded once for 128 query rows.
 template <int D, typename E, int BITS>
 __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(PagedAttnParams p) {
   constexpr int ND = D / 32, NK = D / 16, NO = D / 32;
-  constexpr int TB = 32 * D, MAT = 4 * TB, STAGE = 2 * MAT;   // 16-key tile, 64-key matrix, K and V
+  constexpr int TB = 32 * D, MAT = 4 * TB;           // 16-key tile, 64-key matrix
   constexpr bool kTwoScales = D == 96 || D >= 192;
-  __shared__ __attribute__((aligned(1024))) char smem_raw[2 * STAGE];
+  __shared__ __attribute__((aligned(1024))) char smem_raw[4 * MAT];   // K of even and odd blocks, V of them
   __shared__ int bad_s, odd_s;
   lds_char* smem = (lds_char*)smem_raw;
 
@@ -751,59 +773,52 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
     koffs[i] = (uint32_t)map.key(i) * (uint32_t)p.c.k_str[1] + 16 * map.chunk(i);
     voffs[i] = (uint32_t)map.key(i) * (uint32_t)p.c.v_str[1] + 16 * map.chunk(i);
   }
-  // pages: of keys x and x of the block, one per lane (x = lane % 16)
-  auto bring16 = [&](int b, int page, lds_char* st) __attribute__((always_inline)) {
+  // Copies keys 16 w .. + 15 of block b of one matrix; `page`: key x's, per lane.
+  auto bring16 = [&](int b, int page, const char* base, const int64_t* str, const uint32_t* offs, lds_char* to)
+      __attribute__((always_inline)) {
     const int key0 = b * kPagedBlock + 16 * wave, slot0 = key0 - page_of(p.c, key0) * p.c.page_size;
     if (p.short_rows && key0 + 16 <= sq.L && slot0 + 16 <= p.c.page_size) {   // the 16 keys lie in one page
       const int pg0 = uniform(page);
       const bool ok = (uint32_t)pg0 < (uint32_t)p.c.n_pages;
       bad |= !ok;
-      const int64_t pg = ok ? pg0 : 0;
-      const char* kr = kbase + pg * p.c.k_str[0] + slot0 * p.c.k_str[1];
-      const char* vr = vbase + pg * p.c.v_str[0] + slot0 * p.c.v_str[1];
+      const char* r = base + (int64_t)(ok ? pg0 : 0) * str[0] + slot0 * str[1];
 #pragma unroll
-      for (int i = 0; i < ND; ++i) copy16(kr, koffs[i], st + wave * TB + 1024 * i);
-#pragma unroll
-      for (int i = 0; i < ND; ++i) copy16(vr, voffs[i], st + MAT + wave * TB + 1024 * i);
+      for (int i = 0; i < ND; ++i) copy16(r, offs[i], to + 1024 * i);
       return;
     }
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
       int64_t pg, slot;
       row_of(b, map.key(i), __shfl(page, map.key(i)), pg, slot);
-      copy16(kbase + pg * p.c.k_str[0] + slot * p.c.k_str[1] + 16 * map.chunk(i), st + wave * TB + 1024 * i);
-      copy16(vbase + pg * p.c.v_str[0] + slot * p.c.v_str[1] + 16 * map.chunk(i), st + MAT + wave * TB + 1024 * i);
+      copy16(base + pg * str[0] + slot * str[1] + 16 * map.chunk(i), to + 1024 * i);
     }
   };
   struct Codes {
-    uint32_t k[ND], v[ND], ks[2], vs[2];
-  } codes;
-  auto load4 = [&](int b, int page) __attribute__((always_inline)) {
+    uint32_t w[ND], s[2];
+  };
+  auto load4 = [&](int b, int page, const char* base, const int64_t* str, const uint8_t* sbase, const int64_t* sstr, Codes& c)
+      __attribute__((always_inline)) {
     int64_t pg, slot;
     row_of(b, x, page, pg, slot);
-    const uint32_t* kw = reinterpret_cast<const uint32_t*>(kbase + pg * p.c.k_str[0] + slot * p.c.k_str[1] + (D / 8) * g);
-    const uint32_t* vw = reinterpret_cast<const uint32_t*>(vbase + pg * p.c.v_str[0] + slot * p.c.v_str[1] + (D / 8) * g);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(base + pg * str[0] + slot * str[1] + (D / 8) * g);
 #pragma unroll
-    for (int i = 0; i < ND; ++i) {
-      codes.k[i] = kw[i];
-      codes.v[i] = vw[i];
-    }
-    const uint8_t* ks = p.c.ks + h * p.c.ks_str[2] + pg * p.c.ks_str[0] + slot * p.c.ks_str[1];
-    const uint8_t* vs = p.c.vs + h * p.c.vs_str[2] + pg * p.c.vs_str[0] + slot * p.c.vs_str[1];
-    const int lo = (D / 4) * g / 32, hi = ((D / 4) * g + D / 4 - 1) / 32;
-    codes.ks[0] = ks[lo];
-    codes.vs[0] = vs[lo];
-    codes.ks[1] = kTwoScales ? ks[hi] : 0;
-    codes.vs[1] = kTwoScales ? vs[hi] : 0;
+    for (int i = 0; i < ND; ++i) c.w[i] = w[i];
+    const uint8_t* s = sbase + h * sstr[2] + pg * sstr[0] + slot * sstr[1];
+    c.s[0] = s[(D / 4) * g / 32];
+    c.s[1] = kTwoScales ? s[((D / 4) * g + D / 4 - 1) / 32] : 0;
   };
-  auto store4 = [&](lds_char* st) __attribute__((always_inline)) {
+  typedef __attribute__((address_space(3))) shortx8 lds8;
+  auto store4 = [&](const Codes& c, bool masked, lds_char* to) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
       const bool up = kTwoScales && ((D / 4) * g + 8 * i) / 32 != (D / 4) * g / 32;
-      const int at = prefill_chunk<D>(16 * wave + x, ND * g + i);
-      typedef __attribute__((address_space(3))) shortx8 lds8;
-      *reinterpret_cast<lds8*>(st + at) = decode8<E>(codes.k[i], up ? codes.ks[1] : codes.ks[0]);
-      *reinterpret_cast<lds8*>(st + MAT + at) = decode8<E>(codes.v[i], up ? codes.vs[1] : codes.vs[0]);
+      const uint32_t sb = up ? c.s[1] : c.s[0];
+      shortx8 w = decode8<E>(c.w[i], sb);
+      if (masked && sb == 255) {                        // NaN: see finite8
+        w = shortx8{0};
+        odd_s = 1;
+      }
+      *reinterpret_cast<lds8*>(to + prefill_chunk<D>(x, ND * g + i)) = w;
     }
   };
 
@@ -818,104 +833,183 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   floatx16 o[NO];
 #pragma unroll
   for (int i = 0; i < NO; ++i) o[i] = floatx16{0};
-  float m_run = kNoKeys, l_run = 0.f;
+  float m_run = kNoKeys, l4[4] = {0.f, 0.f, 0.f, 0.f};
+  struct Scores {
+    floatx16 a, b;                                      // keys 0 .. 31 and 32 .. 63 of a block
+  };
+  struct Weights {
+    shortx8 w[4];
+  };
+  auto kread = [&](const lds_char* m, int k) __attribute__((always_inline)) {   // operand k of the 2 NK of a block
+    return *reinterpret_cast<const lds8*>(m + koff[(k >> 1) & 1] + KS * (k >> 1) + (k & 1) * 2 * TB);
+  };
+  auto vread = [&](const lds_char* m, int k) __attribute__((always_inline)) {   // operand k of the 4 NO
+    const int st = k / NO, dt = k % NO;
+    const shortx4 a = read_tr(m + voff0 + st * TB + VS * dt), c = read_tr(m + voff1 + st * TB + VS * dt);
+    return __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto is_masked = [&](int j) __attribute__((always_inline)) { return (blk0 + j + 1) * kPagedBlock > lim_min; };
 
-  auto compute = [&](int b, lds_char* ks) __attribute__((always_inline)) {
-    lds_char* vs = ks + MAT;
-    typedef const __attribute__((address_space(3))) shortx8 lds8;
-    floatx16 s0 = floatx16{0}, s1 = floatx16{0};
-#pragma unroll
-    for (int c = 0; c < NK; ++c) {
-      const shortx8 a0 = *reinterpret_cast<lds8*>(ks + koff[c & 1] + KS * c);
-      const shortx8 a1 = *reinterpret_cast<lds8*>(ks + koff[c & 1] + KS * c + 2 * TB);
-      s0 = Mat<E>::mfma32(a0, qf[c], s0);
-      s1 = Mat<E>::mfma32(a1, qf[c], s1);
+  constexpr int NPV = 4 * NO, NQK = 2 * NK, NM = NPV + NQK, LA = 6, NE = 16;
+  Codes kc, vc4;                                        // 4 bits: of blocks j + 2 and j on their way
+  int page[4];                                          // key x's page of blocks j .. j + 3
+  // Block j: O += V(j - 1) P(j - 1) and S(j + 1) on the matrix core while P(j) is
+  // formed from S(j); K(j + 2) and V(j) are brought meanwhile, to where K(j) and
+  // V(j - 2) were.  S: parity of j, a constant.
+  auto step = [&](auto par, int j, Scores& s, Weights& pv, Scores& sn, Weights& pn) __attribute__((always_inline)) {
+    constexpr int S = decltype(par)::value;
+    lds_char* kto = smem + S * MAT + wave * TB;
+    lds_char* vto = smem + (2 + S) * MAT + wave * TB;
+    const lds_char* kfrom = smem + (1 - S) * MAT;
+    const lds_char* vfrom = smem + (3 - S) * MAT;
+    if constexpr (BITS == 16) {
+      bring16(blk0 + j + 2, page[2], kbase, p.c.k_str, koffs, kto);
+      bring16(blk0 + j, page[0], vbase, p.c.v_str, voffs, vto);
+    } else {
+      store4(kc, false, kto);
+      store4(vc4, is_masked(j), vto);
+      load4(blk0 + j + 3, page[3], kbase, p.c.k_str, p.c.ks, p.c.ks_str, kc);
+      load4(blk0 + j + 1, page[1], vbase, p.c.v_str, p.c.vs, p.c.vs_str, vc4);
     }
-    const bool masked = (b + 1) * kPagedBlock > lim_min;
-    const int here = lim - b * kPagedBlock - 4 * half;   // keys of this block that the row attends, from 4 half on
-    if (masked) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) page[i] = page[i + 1];
+    page[3] = table[page_of(p.c, key_pos(blk0 + j + 4, x))];
+
+    if (is_masked(j)) {
+      const int here = lim - (blk0 + j) * kPagedBlock - 4 * half;   // keys of this block that the row attends, from 4 half on
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int k = 8 * (r >> 2) + (r & 3);
-        s0[r] = k < here ? s0[r] : -__builtin_inff();
-        s1[r] = k + 32 < here ? s1[r] : -__builtin_inff();
+        s.a[r] = k < here ? s.a[r] : -__builtin_inff();
+        s.b[r] = k + 32 < here ? s.b[r] : -__builtin_inff();
       }
     }
     float t[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      float m = __builtin_fmaxf(s0[4 * c], s0[4 * c + 1]);
-      m = __builtin_fmaxf(__builtin_fmaxf(m, s0[4 * c + 2]), s0[4 * c + 3]);
-      m = __builtin_fmaxf(__builtin_fmaxf(m, s1[4 * c]), s1[4 * c + 1]);
-      t[c] = __builtin_fmaxf(__builtin_fmaxf(m, s1[4 * c + 2]), s1[4 * c + 3]);
+      float m = __builtin_fmaxf(s.a[4 * c], s.a[4 * c + 1]);
+      m = __builtin_fmaxf(__builtin_fmaxf(m, s.a[4 * c + 2]), s.a[4 * c + 3]);
+      m = __builtin_fmaxf(__builtin_fmaxf(m, s.b[4 * c]), s.b[4 * c + 1]);
+      t[c] = __builtin_fmaxf(__builtin_fmaxf(m, s.b[4 * c + 2]), s.b[4 * c + 3]);
     }
     float top = __builtin_fmaxf(__builtin_fmaxf(t[0], t[1]), __builtin_fmaxf(t[2], t[3])) * p.scale_log2;
     // the running maximum moves only when some score exceeds it by 2^8
-    if (__builtin_amdgcn_ballot_w64(top > m_run + 8.0f)) {
-      top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m_run + 8.0f) != 0, 0)) {
+      // It is kept a whole number, so that this factor is a power of two and the
+      // weights of block j - 1, rounded already, scale exactly.
+      top = __builtin_ceilf(__builtin_fmaxf(top, __shfl_xor(top, 32)));
       const float m_new = __builtin_fmaxf(m_run, top);
       const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-      l_run *= alpha;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l4[i] *= alpha;
 #pragma unroll
       for (int i = 0; i < NO; ++i) o[i] *= alpha;
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        typedef E v8e __attribute__((ext_vector_type(8)));
+        v8e w = __builtin_bit_cast(v8e, pv.w[st]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = (E)((float)w[i] * alpha);
+        pv.w[st] = __builtin_bit_cast(shortx8, w);
+      }
       m_run = m_new;
     }
-    shortx8 pb[4];
-    float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int st = 0; st < 4; ++st) {
-      const floatx16& s = st < 2 ? s0 : s1;
-      u32x4 w;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * (st & 1) + 2 * j], p.scale_log2, -m_run));
-        const float c = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * (st & 1) + 2 * j + 1], p.scale_log2, -m_run));
-        ls[j] += a + c;
-        w[j] = pack2<E>(a, c);
-      }
-      pb[st] = __builtin_bit_cast(shortx8, w);
-    }
-    l_run += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+    __builtin_amdgcn_sched_barrier(0);
 
-    auto vfrag = [&](int st, int dt) __attribute__((always_inline)) {
-      const shortx4 a = read_tr(vs + voff0 + st * TB + VS * dt), c = read_tr(vs + voff1 + st * TB + VS * dt);
-      return __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
+    shortx8 opa[NM];
+    sn.a = floatx16{0};
+    sn.b = floatx16{0};
+    int done = 0;
 #pragma unroll
-    for (int st = 0; st < 4; ++st)
+    for (int i = 0; i < LA; ++i) opa[i] = vread(vfrom, i);
+    // Nothing moves from one matrix instruction's slot to another: left to itself
+    // the scheduler puts every LDS read right before its use.
 #pragma unroll
-      for (int dt = 0; dt < NO; ++dt) o[dt] = Mat<E>::mfma32(vfrag(st, dt), pb[st], o[dt]);
+    for (int i = 0; i < NM; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (i < NPV) {
+        o[i % NO] = Mat<E>::mfma32(opa[i], pv.w[i / NO], o[i % NO]);
+      } else {
+        const int k = i - NPV;
+        if (k & 1) sn.b = Mat<E>::mfma32(opa[i], qf[k >> 1], sn.b);
+        else sn.a = Mat<E>::mfma32(opa[i], qf[k >> 1], sn.a);
+      }
+      const int li = i + LA;
+      if (li < NPV) opa[li] = vread(vfrom, li);
+      else if (li < NM) opa[li] = kread(kfrom, li - NPV);
+      // the weights of two keys, and their share of the row sum, in every few slots
+#pragma unroll
+      for (; done < (i + 1) * NE / NM; ++done) {
+        const int st = done / 4, q = done % 4;
+        const floatx16& y = st < 2 ? s.a : s.b;
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(y[8 * (st & 1) + 2 * q], p.scale_log2, -m_run));
+        const float c = __builtin_amdgcn_exp2f(__builtin_fmaf(y[8 * (st & 1) + 2 * q + 1], p.scale_log2, -m_run));
+        l4[q] += a + c;
+        u32x4 w = __builtin_bit_cast(u32x4, pn.w[st]);
+        w[q] = pack2<E>(a, c);
+        pn.w[st] = __builtin_bit_cast(shortx8, w);
+      }
+    }
+#pragma unroll
+    for (int st = 0; st < 4; ++st) keep(pn.w[st]);      // formed here, not where they are used
+#pragma unroll
+    for (int q = 0; q < 4; ++q) keep(l4[q]);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (BITS == 16) {
+      wait_copies<0>();
+      if (is_masked(j) && search_tile<E>(vto, TB, lane)) odd_s = 1;
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);                 // LDS writes are in place for the others' reads
+    phase_barrier();
   };
 
   if (threadIdx.x == 0) bad_s = odd_s = 0;
   __syncthreads();
-  if (blk0 < blk1) {
-    int page = table[page_of(p.c, key_pos(blk0, x))];
+  const int n = blk1 - blk0;
+  if (n > 0) {
+    // K of blocks 0 and 1; V of the block before the first: zeros, with P = 0
+    for (int at = 16 * (int)threadIdx.x; at < MAT; at += 4096) *reinterpret_cast<lds8*>(smem + 3 * MAT + at) = shortx8{0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) page[i] = table[page_of(p.c, key_pos(blk0 + i, x))];
     if constexpr (BITS == 16) {
-      bring16(blk0, page, smem);
+      bring16(blk0, page[0], kbase, p.c.k_str, koffs, smem + wave * TB);
+      bring16(blk0 + 1, page[1], kbase, p.c.k_str, koffs, smem + MAT + wave * TB);
+      wait_copies<0>();
     } else {
-      load4(blk0, page);
-      store4(smem);
+      load4(blk0, page[0], kbase, p.c.k_str, p.c.ks, p.c.ks_str, kc);
+      load4(blk0 + 1, page[1], kbase, p.c.k_str, p.c.ks, p.c.ks_str, vc4);
+      store4(kc, false, smem + wave * TB);
+      store4(vc4, false, smem + MAT + wave * TB);
+      load4(blk0 + 2, page[2], kbase, p.c.k_str, p.c.ks, p.c.ks_str, kc);
+      load4(blk0, page[0], vbase, p.c.v_str, p.c.vs, p.c.vs_str, vc4);
     }
-    page = table[page_of(p.c, key_pos(blk0 + 1, x))];
-    auto step = [&](int b, lds_char* cur, lds_char* nxt) __attribute__((always_inline)) {
-      __builtin_amdgcn_s_waitcnt(0x0F70);           // vmcnt(0): this wave's copies of block b have landed
-      if ((b + 1) * kPagedBlock > lim_min && search_tile<E>(cur + MAT + wave * TB, TB, lane)) odd_s = 1;
-      __syncthreads();                              // everyone's; and the other stage has been read
-      if (b + 1 < blk1) {
-        if constexpr (BITS == 16) bring16(b + 1, page, nxt);
-        else load4(b + 1, page);
-        page = table[page_of(p.c, key_pos(b + 2, x))];
-      }
-      compute(b, cur);
-      if constexpr (BITS == 4) {
-        if (b + 1 < blk1) store4(nxt);
-      }
-    };
-    for (int b = blk0; b < blk1; b += 2) {
-      step(b, smem, smem + STAGE);
-      if (b + 1 < blk1) step(b + 1, smem + STAGE, smem);
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    phase_barrier();
+    Scores sa, sb;
+    Weights wa, wb;
+    sa.a = sa.b = floatx16{0};
+#pragma unroll
+    for (int k = 0; k < NQK; ++k) {
+      if (k & 1) sa.b = Mat<E>::mfma32(kread(smem, k), qf[k >> 1], sa.b);
+      else sa.a = Mat<E>::mfma32(kread(smem, k), qf[k >> 1], sa.a);
     }
+#pragma unroll
+    for (int st = 0; st < 4; ++st) wa.w[st] = wb.w[st] = shortx8{0};
+    phase_barrier();                                    // K(0) has been read
+    using Even = std::integral_constant<int, 0>;
+    using Odd = std::integral_constant<int, 1>;
+    int j = 0;
+    for (; j + 1 < n; j += 2) {
+      step(Even{}, j, sa, wa, sb, wb);
+      step(Odd{}, j + 1, sb, wb, sa, wa);
+    }
+    if (j < n) {
+      step(Even{}, j, sa, wa, sb, wb);
+      wa = wb;
+    }
+    const lds_char* vlast = smem + (2 + ((n - 1) & 1)) * MAT;
+#pragma unroll
+    for (int k = 0; k < NPV; ++k) o[k % NO] = Mat<E>::mfma32(vread(vlast, k), wa.w[k / NO], o[k % NO]);
   }
 
   // A bad page seen by any wave spoils the tile.
@@ -931,6 +1025,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
                                           o[q >> 2][4 * (q & 3) + r] = add_nonfinite<E>(o[q >> 2][4 * (q & 3) + r], v, seen);
                                         });
   }
+  const float l_run = (l4[0] + l4[1]) + (l4[2] + l4[3]);
   float l = l_run + __shfl_xor(l_run, 32);
   if (bad_s) l = __builtin_nanf("");
   if (row < nrows) store_rows<D, E>(p, whole, slot, kPagedTile, row - r0, half, ref, o, m_run, l);
@@ -947,24 +1042,6 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
 
 // ──────────────────────────── prefill, tall tiles ──────────────────────────
 
-// Workgroup barrier that nothing crosses: the memory clobber orders LDS and
-// global accesses, the scheduling barriers keep a phase's arithmetic in it.
-__device__ __forceinline__ void phase_barrier() {
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_barrier" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-}
-// Materialise x here, so that the compiler does not sink its computation into
-// the phase that uses it.
-template <typename T>
-__device__ __forceinline__ void keep(T& x) {
-  asm volatile("" : "+v"(x));
-}
-template <int N>
-__device__ __forceinline__ void wait_copies() {
-  static_assert(N >= 0 && N < 16, "vmcnt immediate");
-  __builtin_amdgcn_s_waitcnt(0x0F70 | N);
-}
 // 4 bytes per lane, global -> LDS at `l` + 4 * lane (see copy16).
 __device__ __forceinline__ void copy4(const void* from, const lds_char* l) {
   const uint32_t la = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)l);
