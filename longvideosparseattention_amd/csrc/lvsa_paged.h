@@ -101,11 +101,10 @@ __host__ __device__ inline int page_of(const PagedView& c, int pos) {
   return (int)(((uint64_t)(uint32_t)pos * c.ps_mul) >> c.ps_shift);
 }
 
-// Sequence s.  Ranges and lengths outside what the caller allocated are cut to
-// it and flagged.
-__host__ __device__ inline PagedSeq paged_seq(const PagedView& c, int s) {
+// The sequence of rows [a, e) with `len` keys.  Ranges and lengths outside what
+// the caller allocated are cut to it and flagged.
+__host__ __device__ inline PagedSeq paged_seq(const PagedView& c, int a, int e, int len) {
   PagedSeq r;
-  const int a = c.cu[s], e = c.cu[s + 1], len = c.lens[s];
   const int64_t cap = (int64_t)c.max_pages * c.page_size;
   r.flags = 0;
   r.L = len;
@@ -119,6 +118,10 @@ __host__ __device__ inline PagedSeq paged_seq(const PagedView& c, int s) {
   const int64_t first = (int64_t)r.L - ((int64_t)e - lo);
   r.first = first < -(1 << 30) ? -(1 << 30) : first > INT32_MAX ? INT32_MAX : (int)first;
   return r;
+}
+
+__host__ __device__ inline PagedSeq paged_seq(const PagedView& c, int s) {
+  return paged_seq(c, c.cu[s], c.cu[s + 1], c.lens[s]);
 }
 
 // Key position that a kernel reads for `pos`: past the end the last key, whose
@@ -204,14 +207,23 @@ __device__ __forceinline__ void paged_flag(const PagedView& c, int bit) {
 }
 
 // The sequence that row t belongs to (the same for every lane of the wave; t
-// uniform), or -1.
-__device__ __forceinline__ int paged_seq_of_row(const PagedView& c, int t, int lane) {
+// uniform), or -1.  Every lane reads one sequence, so that a batch of up to 64
+// costs one trip to memory.
+__device__ __forceinline__ int paged_seq_of_row(const PagedView& c, int t, int lane, PagedSeq* q) {
   for (int s0 = 0; s0 < c.B; s0 += 64) {
     const int s = s0 + lane;
-    bool in = false;
-    if (s < c.B) in = c.cu[s] <= t && t < c.cu[s + 1];
-    const uint64_t m = __builtin_amdgcn_ballot_w64(in);
-    if (m) return s0 + __builtin_ctzll(m);
+    int a = 0, e = 0, len = 0;
+    if (s < c.B) {
+      a = c.cu[s];
+      e = c.cu[s + 1];
+      len = c.lens[s];
+    }
+    const uint64_t m = __builtin_amdgcn_ballot_w64(a <= t && t < e);
+    if (m) {
+      const int i = __builtin_ctzll(m);
+      *q = paged_seq(c, __builtin_amdgcn_readlane(a, i), __builtin_amdgcn_readlane(e, i), __builtin_amdgcn_readlane(len, i));
+      return s0 + i;
+    }
   }
   return -1;
 }

@@ -98,7 +98,11 @@ struct AppendParams {
 // chunk's angles are read once and serve all of them.  A rotated element
 // needs its partner: in the same chunk with interleaved pairs, else rot / 2
 // elements away, which is a second 16-byte load of a line that the neighbours
-// fetch anyway.  Bound by memory.
+// fetch anyway.  Bound by memory, and for small calls by the trips to it one
+// after the other: the batch, the page with the angles, the row.  (Rows read
+// ahead of their slot cost more in registers than they save: 93 instead of 80 us
+// for 7868 tokens of 32 + 8 + 8 rows of 128 into a 4-bit cache and their reading
+// back.)
 //
 // 16-bit caches: turned in fp32, one rounding at the end.  4-bit caches: the
 // turned key is formed in 64 bits, where both products are exact and the sum
@@ -109,9 +113,15 @@ template <int D, typename E, int BITS>
 __device__ __forceinline__ void append_token(const AppendParams& p, int t) {
   constexpr int CH = D / 8, RPP = 256 / CH;
   const int lane = threadIdx.x & 63;
-  const int s = paged_seq_of_row(p.c, t, lane);
+  const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
+  const int half = p.rot / 2;
+  const bool turn = 8 * c < p.rot;
+  const bool second = !p.interleaved && 8 * c >= half;   // this chunk holds the second elements of its pairs
+  const int partner = p.interleaved ? 0 : second ? -half : half;
+  const int Hkv = p.c.Hkv, rows = r0 < RPP ? 2 * Hkv + (p.q ? p.H : 0) : 0;   // D = 96 and 192 leave a few threads over
+  PagedSeq sq;
+  const int s = paged_seq_of_row(p.c, t, lane, &sq);
   if (s < 0) return;                        // a row of no sequence: left alone
-  const PagedSeq sq = paged_seq(p.c, s);
   const int64_t pos = (int64_t)sq.first + (t - sq.t0);
   int flags = sq.flags;
   int64_t page = 0, slot = 0;
@@ -130,13 +140,7 @@ __device__ __forceinline__ void append_token(const AppendParams& p, int t) {
   const bool bad = flags != 0;
   if (bad && threadIdx.x == 0) paged_flag(p.c, flags);
 
-  const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
-  if (r0 >= RPP) return;                    // D = 96 and 192 leave a few threads over; whole groups of four
-  const int half = p.rot / 2;
-  const bool turn = 8 * c < p.rot;
   float cs[8], sn[8];
-  int partner = 0;
-  bool second = false;                      // this chunk holds the second elements of its pairs
   if (turn && !bad) {
     const int64_t base = angle * half;
     if (p.interleaved) {
@@ -146,9 +150,7 @@ __device__ __forceinline__ void append_token(const AppendParams& p, int t) {
         sn[i] = p.sin[base + 4 * c + i];
       }
     } else {
-      second = 8 * c >= half;
       const int i0 = second ? 8 * c - half : 8 * c;
-      partner = second ? -half : half;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         cs[i] = p.cos[base + i0 + i];
@@ -157,13 +159,9 @@ __device__ __forceinline__ void append_token(const AppendParams& p, int t) {
     }
   }
 
-  const int Hkv = p.c.Hkv, rows = 2 * Hkv + (p.q ? p.H : 0);
   for (int r = r0; r < rows; r += RPP) {
     const bool is_k = r < Hkv, is_q = r >= 2 * Hkv;
     const int h = is_k ? r : is_q ? r - 2 * Hkv : r - Hkv;
-    const char* src = is_k ? p.k + t * p.k_str[0] + h * p.k_str[1]
-                    : is_q ? p.q + t * p.q_str[0] + h * p.q_str[1]
-                           : p.v + t * p.v_str[0] + h * p.v_str[1];
     if (bad) {
       if (is_q) {
         const uint32_t n2 = Half<E>::kNaN * 0x10001u;
@@ -171,12 +169,14 @@ __device__ __forceinline__ void append_token(const AppendParams& p, int t) {
       }
       continue;
     }
+    const char* src = is_k ? p.k + t * p.k_str[0] + h * p.k_str[1]
+                    : is_q ? p.q + t * p.q_str[0] + h * p.q_str[1]
+                           : p.v + t * p.v_str[0] + h * p.v_str[1];
     const u32x4 raw = *reinterpret_cast<const u32x4*>(src + 16 * c);
     const bool turned = turn && (is_k || is_q);
-    float x[8];
+    float x[8], y[8];
     Half<E>::unpack(raw, x);
-    float y[8];
-    if (turned && !p.interleaved) Half<E>::unpack(*reinterpret_cast<const u32x4*>(src + 16 * c + 2 * partner), y);
+    if (turned && partner) Half<E>::unpack(*reinterpret_cast<const u32x4*>(src + 16 * c + 2 * partner), y);
     if (BITS == 16 || is_q) {
       u32x4 w = raw;
       if (turned) {
@@ -199,16 +199,24 @@ __device__ __forceinline__ void append_token(const AppendParams& p, int t) {
       *reinterpret_cast<u32x4*>(dst + 16 * c) = w;
     } else {
       if (turned) {
+        // The angles are widened here, row by row, and two elements are formed at
+        // a time: fewer registers, more waves, 73 instead of 80 us as above.
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(cs[i]), "+v"(sn[i]));
         if (p.interleaved) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const double a = x[2 * i], b = x[2 * i + 1], cc = cs[i], ss = sn[i];
             x[2 * i] = to_odd(__builtin_fma(a, cc, -(b * ss)));
             x[2 * i + 1] = to_odd(__builtin_fma(b, cc, a * ss));
+            __builtin_amdgcn_sched_barrier(0);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = to_odd(__builtin_fma((double)x[i], (double)cs[i], (double)y[i] * (double)sn[i]));
+          for (int i = 0; i < 8; ++i) {
+            x[i] = to_odd(__builtin_fma((double)x[i], (double)cs[i], (double)y[i] * (double)sn[i]));
+            if (i & 1) __builtin_amdgcn_sched_barrier(0);
+          }
         }
       }
       // the largest of the 32 values that four neighbouring threads hold; a
@@ -314,7 +322,8 @@ __device__ __forceinline__ void merge_row(const PagedAttnParams& p, int row, int
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   E* out = reinterpret_cast<E*>(p.o + t * p.o_str[0] + hq * p.o_str[1]);
   float* lse = p.lse ? p.lse + (int64_t)t * p.H + hq : nullptr;
-  const int s = paged_seq_of_row(p.c, t, lane);
+  PagedSeq sq;
+  const int s = paged_seq_of_row(p.c, t, lane, &sq);
   if (s < 0) {
     if (p.fill_tail) {
       for (int d = threadIdx.x; d < D; d += 256) out[d] = (E)0.f;
@@ -322,7 +331,6 @@ __device__ __forceinline__ void merge_row(const PagedAttnParams& p, int row, int
     }
     return;
   }
-  const PagedSeq sq = paged_seq(p.c, s);
   const int h = hq / p.group;
   const int r = (t - sq.t0) * p.group + hq % p.group;
   DecodeSlots parts = {0, 0, 0};
