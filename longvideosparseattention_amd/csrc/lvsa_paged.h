@@ -155,9 +155,14 @@ __host__ __device__ inline int unit_shares(int64_t U, int grid, int least = 1) {
   const int64_t n = U / least;
   return n < 1 ? 1 : n < grid ? (int)n : grid;
 }
+// a / b for a >= 0, b > 0: in 32 bits where both fit (64-bit division is 150
+// instructions on the device, and these are at the head of a latency chain).
+__host__ __device__ inline int64_t quotient(int64_t a, int64_t b) {
+  return ((uint64_t)a | (uint64_t)b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
 // First unit of share w of G over U units, and the share of unit u.
-__host__ __device__ inline int64_t unit_start(int64_t U, int G, int w) { return w * U / G; }
-__host__ __device__ inline int wg_of_unit(int64_t U, int G, int64_t u) { return (int)(((u + 1) * G - 1) / U); }
+__host__ __device__ inline int64_t unit_start(int64_t U, int G, int w) { return quotient(w * U, G); }
+__host__ __device__ inline int wg_of_unit(int64_t U, int G, int64_t u) { return (int)quotient((u + 1) * G - 1, U); }
 
 // Partials of the row tile whose key steps are units [u0, u0 + nb): none if one
 // work-group has them all, else one per work-group, in the first of its two
@@ -228,10 +233,20 @@ __device__ __forceinline__ int paged_seq_of_row(const PagedView& c, int t, int l
   return -1;
 }
 
-// Inclusive sum over the lanes of a wave.
-__device__ __forceinline__ int64_t wave_scan(int64_t x, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
+// The sequence that lane `from` holds, for every lane.
+__device__ __forceinline__ PagedSeq from_lane(const PagedSeq& s, int from) {
+  return PagedSeq{__builtin_amdgcn_readlane(s.t0, from), __builtin_amdgcn_readlane(s.n, from),
+                  __builtin_amdgcn_readlane(s.L, from), __builtin_amdgcn_readlane(s.first, from),
+                  __builtin_amdgcn_readlane(s.flags, from)};
+}
+__device__ __forceinline__ int64_t from_lane(int64_t x, int from) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), from) << 32 |
+                   (uint32_t)__builtin_amdgcn_readlane((int)x, from));
+}
+
+// Inclusive sum over the first `count` lanes of a wave.
+__device__ __forceinline__ int64_t wave_scan(int64_t x, int lane, int count = 64) {
+  for (int d = 1; d < 64 && d < count; d <<= 1) {
     const int64_t y = __shfl_up(x, d);
     if (lane >= d) x += y;
   }

@@ -311,19 +311,42 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(PagedView c, char* ko
 
 // One work-group per output row: finds the row's sequence, tile and the slots
 // that hold partials of it, and merges them: o = sum_i 2^(m_i - M) o_i / sum_i
-// 2^(m_i - M) l_i.  The four waves take the slots in turn and are summed in
-// their order, so results do not depend on timing.  Rows whose tile one
-// work-group of the decode kernel did whole are written already.  Rows without
-// keys and rows of no sequence are this kernel's too.
+// 2^(m_i - M) l_i.  The four waves take the slots in turn, each with a running
+// maximum as in the attention itself, and are joined in their order, so results
+// do not depend on timing.  Rows whose tile one work-group of the decode kernel
+// did whole are written already.  Rows without keys and rows of no sequence are
+// this kernel's too.  Latency: the batch, the partials (two slots of a wave at a
+// time, maxima and sums beside them), one exchange.
 template <typename E>
 __device__ __forceinline__ void merge_row(const PagedAttnParams& p, int row, int D, int rows, int keys,
                                           float (*acc_s)[256], float (*ml_s)[2]) {
-  const int t = row / p.H, hq = row % p.H;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = (uint32_t)row / (uint32_t)p.H, hq = row - t * p.H;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), B = p.c.B;
   E* out = reinterpret_cast<E*>(p.o + t * p.o_str[0] + hq * p.o_str[1]);
   float* lse = p.lse ? p.lse + (int64_t)t * p.H + hq : nullptr;
-  PagedSeq sq;
-  const int s = paged_seq_of_row(p.c, t, lane, &sq);
+  PagedSeq sq = {};
+  int s = -1;
+  int64_t U = 0, base = 0;
+  for (int s0 = 0; s0 < B; s0 += 64) {
+    PagedSeq q = {};
+    int64_t n = 0;
+    bool in = false;
+    if (s0 + lane < B) {
+      const int a = p.c.cu[s0 + lane], e = p.c.cu[s0 + lane + 1];
+      q = paged_seq(p.c, a, e, p.c.lens[s0 + lane]);
+      n = decode_units(p, q, rows, keys);
+      in = a <= t && t < e;
+    }
+    const int64_t incl = wave_scan(n, lane, B - s0);
+    const uint64_t m = __builtin_amdgcn_ballot_w64(in);
+    if (m && s < 0) {
+      const int at = __builtin_ctzll(m);
+      s = s0 + at;
+      sq = from_lane(q, at);
+      base = U + from_lane(incl - n, at);
+    }
+    U += from_lane(incl, B - s0 < 64 ? B - s0 - 1 : 63);
+  }
   if (s < 0) {
     if (p.fill_tail) {
       for (int d = threadIdx.x; d < D; d += 256) out[d] = (E)0.f;
@@ -331,18 +354,9 @@ __device__ __forceinline__ void merge_row(const PagedAttnParams& p, int row, int
     }
     return;
   }
-  const int h = hq / p.group;
-  const int r = (t - sq.t0) * p.group + hq % p.group;
+  const int h = (uint32_t)hq / (uint32_t)p.group;
+  const int r = (t - sq.t0) * p.group + (hq - h * p.group);
   DecodeSlots parts = {0, 0, 0};
-  int64_t U = 0, base = 0;
-  for (int s0 = 0; s0 < p.c.B; s0 += 64) {
-    const int i = s0 + lane;
-    int64_t n = 0;
-    if (i < p.c.B) n = decode_units(p, paged_seq(p.c, i), rows, keys);
-    const int64_t incl = wave_scan(n, lane);
-    if (s >= s0 && s < s0 + 64) base = U + __shfl(incl - n, s - s0);
-    U += __shfl(incl, 63);
-  }
   const int nb = (int)(((int64_t)sq.L + keys - 1) / keys);
   if (nb > 0) {
     parts = decode_slots(U, unit_shares(U, p.grid), base + ((int64_t)(r / rows) * p.c.Hkv + h) * nb, nb);
@@ -352,34 +366,44 @@ __device__ __forceinline__ void merge_row(const PagedAttnParams& p, int row, int
   const int rr = r % rows;
   auto slot_of = [&](int i) { return i == 0 ? parts.first : parts.rest + 2 * i; };
 
-  float M = kNoKeys;
-  for (int i = wave; i < count; i += 4) {
-    const float m = p.ws_ml[2 * (slot_of(i) * rows + rr)];
-    M = __builtin_fmaxf(M, m);
-  }
-  if (lane == 0) ml_s[wave][0] = M;
-  __syncthreads();
-  M = __builtin_fmaxf(__builtin_fmaxf(ml_s[0][0], ml_s[1][0]), __builtin_fmaxf(ml_s[2][0], ml_s[3][0]));
-  float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = wave; i < count; i += 4) {
-    const int64_t at = slot_of(i) * rows + rr;
-    const float w = __builtin_amdgcn_exp2f(p.ws_ml[2 * at] - M);
-    l = __builtin_fmaf(w, p.ws_ml[2 * at + 1], l);
+  float M = kNoKeys, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = wave; i < count; i += 8) {
+    float m[2], ls[2], x[2][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int d = lane + 64 * k;
-      if (d < D) acc[k] = __builtin_fmaf(w, p.ws_o[at * D + d], acc[k]);
+    for (int j = 0; j < 2; ++j) {          // past the last one: the first again, with no weight
+      const bool real = i + 4 * j < count;
+      const int64_t at = slot_of(real ? i + 4 * j : i) * rows + rr;
+      m[j] = real ? p.ws_ml[2 * at] : kNoKeys;
+      ls[j] = real ? p.ws_ml[2 * at + 1] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[j][k] = real && 64 * k < D && lane + 64 * k < D ? p.ws_o[at * D + lane + 64 * k] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float top = __builtin_fmaxf(M, m[j]);
+      const float a = __builtin_amdgcn_exp2f(M - top), b = __builtin_amdgcn_exp2f(m[j] - top);
+      l = l * a + ls[j] * b;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] = acc[k] * a + x[j][k] * b;
+      M = top;
     }
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) acc_s[wave][lane + 64 * k] = acc[k];
-  if (lane == 0) ml_s[wave][1] = l;
+  if (lane == 0) {
+    ml_s[wave][0] = M;
+    ml_s[wave][1] = l;
+  }
   __syncthreads();
-  l = (ml_s[0][1] + ml_s[1][1]) + (ml_s[2][1] + ml_s[3][1]);
+  M = __builtin_fmaxf(__builtin_fmaxf(ml_s[0][0], ml_s[1][0]), __builtin_fmaxf(ml_s[2][0], ml_s[3][0]));
+  float w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = __builtin_amdgcn_exp2f(ml_s[k][0] - M);
+  l = (ml_s[0][1] * w[0] + ml_s[1][1] * w[1]) + (ml_s[2][1] * w[2] + ml_s[3][1] * w[3]);
   if (sq.flags & LVSA_PAGED_BAD_LENGTH) l = __builtin_nanf("");
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   for (int d = threadIdx.x; d < D; d += 256)
-    out[d] = (E)(((acc_s[0][d] + acc_s[1][d]) + (acc_s[2][d] + acc_s[3][d])) * inv);
+    out[d] = (E)(((acc_s[0][d] * w[0] + acc_s[1][d] * w[1]) + (acc_s[2][d] * w[2] + acc_s[3][d] * w[3])) * inv);
   if (lse && threadIdx.x == 0) *lse = l == 0.f ? -__builtin_inff() : (M + __log2f(l)) * 0.69314718055994530942f;
 }
 

@@ -234,17 +234,25 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 192 && NT == 2)) ? 1 : 2) v
   lds_char* vbuf = (lds_char*)smem_raw + wave * (T * TB);
   float* obuf = reinterpret_cast<float*>(smem_raw);
 
-  // The share [u, u_end) and the sequence it starts in.
+  // The share [u, u_end) and the sequence it starts in.  A lane holds one
+  // sequence, so that a batch of up to 64 is read once.
+  const int B = p.c.B;
+  PagedSeq mine = {};
+  int64_t n_mine = 0, upto = 0;                // units of the lane's sequence; with those before it
   int64_t U = 0;
   int flags = 0;
-  for (int s0 = 0; s0 < p.c.B; s0 += 64) {
-    int64_t n = 0;
-    if (s0 + lane < p.c.B) {
-      const PagedSeq q = paged_seq(p.c, s0 + lane);
-      n = decode_units(p, q, ROWS, KEYS);
-      flags |= q.flags;
+  auto read_batch = [&](int s0) __attribute__((always_inline)) {
+    n_mine = 0;
+    if (s0 + lane < B) {
+      mine = paged_seq(p.c, s0 + lane);
+      n_mine = decode_units(p, mine, ROWS, KEYS);
+      flags |= mine.flags;
     }
-    U += __shfl(wave_scan(n, lane), 63);
+    upto = wave_scan(n_mine, lane, B - s0);
+  };
+  for (int s0 = 0; s0 < B; s0 += 64) {
+    read_batch(s0);
+    U += from_lane(upto, B - s0 < 64 ? B - s0 - 1 : 63);
   }
   if (blockIdx.x == 0 && wave == 0 && flags) paged_flag(p.c, flags);
   if (U == 0) return;
@@ -252,25 +260,25 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 192 && NT == 2)) ? 1 : 2) v
   if ((int)blockIdx.x >= shares) return;
   int64_t u = unit_start(U, shares, blockIdx.x);
   const int64_t u_end = unit_start(U, shares, blockIdx.x + 1);
-  int seq = 0;
+  int seq = 0, held = 0;                       // lanes hold sequences [held, held + 64)
   int64_t base = 0;                            // units before sequence `seq`
-  for (int s0 = 0; s0 < p.c.B; s0 += 64) {
-    int64_t n = 0;
-    if (s0 + lane < p.c.B) n = decode_units(p, paged_seq(p.c, s0 + lane), ROWS, KEYS);
-    const int64_t incl = wave_scan(n, lane);
-    const uint64_t above = __builtin_amdgcn_ballot_w64(base + incl > u);
+  for (int s0 = 0; s0 < B; s0 += 64) {
+    if (B > 64) read_batch(s0);
+    held = s0;
+    const uint64_t above = __builtin_amdgcn_ballot_w64(s0 + lane < B && base + upto > u);
     if (above) {
       const int at = __builtin_ctzll(above);
       seq = s0 + at;
-      base += __shfl(incl - n, at);
+      base += from_lane(upto - n_mine, at);
       break;
     }
-    base += __shfl(incl, 63);
+    base += from_lane(upto, 63);
   }
 
   const int64_t u_first = u;
-  while (u < u_end && seq < p.c.B) {
-    const PagedSeq sq = uniform(paged_seq(p.c, seq));
+  while (u < u_end && seq < B) {
+    if (seq >= held + 64) read_batch(held += 64);
+    const PagedSeq sq = from_lane(mine, seq - held);
     const int64_t units = decode_units(p, sq, ROWS, KEYS);
     if (u >= base + units) {
       base += units;
@@ -278,11 +286,11 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 192 && NT == 2)) ? 1 : 2) v
       continue;
     }
     const int nb = (int)(((int64_t)sq.L + KEYS - 1) / KEYS);
-    const int64_t run = (u - base) / nb;
+    const int64_t run = quotient(u - base, nb);
     const int blk0 = (int)((u - base) - run * nb);
     const int64_t left = u_end - u;
     const int blk1 = left < nb - blk0 ? blk0 + (int)left : nb;
-    const int rt = (int)(run / p.c.Hkv), h = (int)(run - (int64_t)rt * p.c.Hkv);
+    const int rt = (int)quotient(run, p.c.Hkv), h = (int)(run - (int64_t)rt * p.c.Hkv);
     const int nrows = sq.n * p.group;
     const int r0 = rt * ROWS;
 
