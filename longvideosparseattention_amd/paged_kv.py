@@ -48,6 +48,7 @@ from . import hip_ops
 
 __all__ = ["PagedKVCache", "paged_kv_append", "paged_kv_gather", "paged_attention"]
 
+_INT32 = torch.int32
 _DTYPES = {torch.bfloat16: capi.LVSA_BF16, torch.float16: capi.LVSA_FP16}
 _STATUS = {
     capi.PAGED_BAD_PAGE: "a page number outside the cache",
@@ -178,13 +179,15 @@ class PagedKVCache:
 
 
 def _int32(t: torch.Tensor, name: str, dims: int, device: torch.device) -> None:
+    if isinstance(t, torch.Tensor) and t.dtype is _INT32 and t.dim() == dims and t.device == device and t.stride(-1) == 1:
+        return
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         hip_ops._require_device(t, name)
     if t.dtype != torch.int32 or t.dim() != dims:
         raise TypeError(f"{name} must be a {dims}-D int32 tensor, got {t.dim()}-D {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the cache on {device}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.shape[-1] > 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
 
 
@@ -213,9 +216,10 @@ def _tokens(t: torch.Tensor, name: str, heads: Optional[int], cache: PagedKVCach
     repacked on the device), its address and its first two strides."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         hip_ops._require_device(t, name)
-    if t.dim() != 3 or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be [N, {'H' if heads is None else heads}, {cache.head_dim}], got {tuple(t.shape)}")
-    if t.dtype != dtype:
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} must be [N, {'H' if heads is None else heads}, {cache.head_dim}], got {tuple(shape)}")
+    if t.dtype is not dtype:
         raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
     if t.device != cache.device:
         raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
@@ -234,17 +238,18 @@ def _result(out: Optional[torch.Tensor], like: torch.Tensor, name: str):
     """The tensor a call writes (``out``, or a new one) with its address and strides."""
     if out is None:
         out = torch.empty_like(like, memory_format=torch.contiguous_format)
-    else:
-        if not isinstance(out, torch.Tensor) or out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
-            raise ValueError(f"{name} must be {tuple(like.shape)} of {like.dtype} on {like.device}")
-        if out.stride(2) != 1 or (out.data_ptr() | ((out.stride(0) | out.stride(1)) * 2)) & 15:
-            raise ValueError(f"{name} needs a contiguous last dimension and rows at multiples of 16 bytes")
-        if out.numel() and _span(out)[0] < _span(like)[1] and _span(like)[0] < _span(out)[1]:
-            raise ValueError(f"{name} must not share memory with the input")
-        N, H, D = out.shape
-        a, b = sorted(((N, out.stride(0)), (H, out.stride(1))), key=lambda x: x[1])
-        if (a[0] > 1 and a[1] < D) or (b[0] > 1 and b[1] < (a[1] * (a[0] - 1) if a[0] > 1 else 0) + D):
-            raise ValueError(f"{name} has overlapping rows")
+        _, H, D = like.shape
+        return out, out.data_ptr(), H * D, D
+    if not isinstance(out, torch.Tensor) or out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+        raise ValueError(f"{name} must be {tuple(like.shape)} of {like.dtype} on {like.device}")
+    if out.stride(2) != 1 or (out.data_ptr() | ((out.stride(0) | out.stride(1)) * 2)) & 15:
+        raise ValueError(f"{name} needs a contiguous last dimension and rows at multiples of 16 bytes")
+    if out.numel() and _span(out)[0] < _span(like)[1] and _span(like)[0] < _span(out)[1]:
+        raise ValueError(f"{name} must not share memory with the input")
+    N, H, D = out.shape
+    a, b = sorted(((N, out.stride(0)), (H, out.stride(1))), key=lambda x: x[1])
+    if (a[0] > 1 and a[1] < D) or (b[0] > 1 and b[1] < (a[1] * (a[0] - 1) if a[0] > 1 else 0) + D):
+        raise ValueError(f"{name} has overlapping rows")
     return out, out.data_ptr(), out.stride(0), out.stride(1)
 
 
@@ -303,12 +308,14 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, cu_se
         raise ValueError("cos and sin go together")
     if cos is not None:
         for t, name in ((cos, "cos"), (sin, "sin")):
-            hip_ops._require_device(t, name)
-            if t.dtype != torch.float32 or t.dim() != 2 or not t.is_contiguous() or t.shape != cos.shape:
+            if not isinstance(t, torch.Tensor) or not t.is_cuda:
+                hip_ops._require_device(t, name)
+            if t.dtype is not torch.float32 or t.dim() != 2 or not t.is_contiguous() or t.shape != cos.shape:
                 raise TypeError(f"{name} must be a contiguous fp32 [positions, rot / 2] tensor like its partner")
             if t.device != cache.device:
                 raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
-        angles, rot = cos.shape[0], 2 * cos.shape[1]
+        angles, rot = cos.shape
+        rot *= 2
         if rot % 16 or not 0 < rot <= cache.head_dim:
             raise ValueError(f"cos and sin turn {rot} dimensions: a multiple of 16 up to {cache.head_dim}")
         cos_ptr, sin_ptr = cos.data_ptr(), sin.data_ptr()
@@ -411,7 +418,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, cu_seqlens: torch.Tens
         head = (q_ptr, o_ptr, 0 if lse is None else lse.data_ptr(), *q_str, *o_str, scale, H, int(bool(causal)),
                 int(fresh), min(mq, 0x7fffffff), min(mk, 0x7fffffff))
         _ATTN.pack_into(a, _ATTN_AT, *head, 0, 0)
-        need = _workspace_bytes(a, (cache.device, cache.bits, D, cache.num_kv_heads, cache.page_size, N, H, *page_table.shape,
+        need = _workspace_bytes(a, (cache.device.index, cache.bits, D, cache.num_kv_heads, cache.page_size, N, H, *page_table.shape,
                                     mq, mk), cache.device)
         if need:
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
