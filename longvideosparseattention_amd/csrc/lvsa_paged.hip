@@ -119,6 +119,15 @@ __device__ __forceinline__ void append_token(const AppendParams& p, int t) {
   const bool second = !p.interleaved && 8 * c >= half;   // this chunk holds the second elements of its pairs
   const int partner = p.interleaved ? 0 : second ? -half : half;
   const int Hkv = p.c.Hkv, rows = r0 < RPP ? 2 * Hkv + (p.q ? p.H : 0) : 0;   // D = 96 and 192 leave a few threads over
+  u32x4 raw = {}, other = {};
+  auto load = [&](int r) __attribute__((always_inline)) {
+    const char* src = r < Hkv ? p.k + t * p.k_str[0] + r * p.k_str[1]
+                    : r >= 2 * Hkv ? p.q + t * p.q_str[0] + (r - 2 * Hkv) * p.q_str[1]
+                                   : p.v + t * p.v_str[0] + (r - Hkv) * p.v_str[1];
+    raw = *reinterpret_cast<const u32x4*>(src + 16 * c);
+    if (turn && partner && (r < Hkv || r >= 2 * Hkv)) other = *reinterpret_cast<const u32x4*>(src + 16 * c + 2 * partner);
+  };
+
   PagedSeq sq;
   const int s = paged_seq_of_row(p.c, t, lane, &sq);
   if (s < 0) return;                        // a row of no sequence: left alone
@@ -169,16 +178,13 @@ __device__ __forceinline__ void append_token(const AppendParams& p, int t) {
       }
       continue;
     }
-    const char* src = is_k ? p.k + t * p.k_str[0] + h * p.k_str[1]
-                    : is_q ? p.q + t * p.q_str[0] + h * p.q_str[1]
-                           : p.v + t * p.v_str[0] + h * p.v_str[1];
-    const u32x4 raw = *reinterpret_cast<const u32x4*>(src + 16 * c);
+    load(r);
     const bool turned = turn && (is_k || is_q);
     float x[8], y[8];
+    u32x4 w = raw;
     Half<E>::unpack(raw, x);
-    if (turned && partner) Half<E>::unpack(*reinterpret_cast<const u32x4*>(src + 16 * c + 2 * partner), y);
+    Half<E>::unpack(other, y);
     if (BITS == 16 || is_q) {
-      u32x4 w = raw;
       if (turned) {
         float z[8];
         if (p.interleaved) {
