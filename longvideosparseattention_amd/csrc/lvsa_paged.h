@@ -86,6 +86,17 @@ int paged_attn_d256(const PagedAttnParams& p, int bits, int rows, bool bf16, hip
 
 // Keys that the four waves of a decode work-group take per step.
 __host__ __device__ constexpr int paged_decode_keys(int D) { return 4 * (D >= 192 ? 16 : 32); }
+// Decode work-groups that a compute unit holds at once: what the registers
+// allow (the kernels are compiled for it), and what a launch starts of them, so
+// that equal shares end together.  16-bit caches are read at 5.7 TB/s by one
+// group as by four (40 sequences of 12000 keys, 8 heads of 128: 341, 342, 342,
+// 346 us with 1 to 4), 4-bit ones need waves to decode behind the loads (180,
+// 122, 111, 128 us; of 64: 123, 85, 75, 72).
+__host__ __device__ constexpr int paged_decode_groups(int D, int bits, int rows) {
+  if (bits == 16) return D == 64 || (D <= 128 && rows == 16) ? 2 : 1;
+  if (rows == 16) return D == 64 ? 4 : D <= 128 ? 3 : 2;
+  return D == 64 ? 3 : D <= 192 ? 2 : 1;
+}
 constexpr int kPagedTile = 128;        // rows of a prefill tile
 constexpr int kPagedTall = 256;        // rows of a tall one (head sizes up to 128)
 constexpr int kPagedBlock = 64;        // its keys per step

@@ -716,7 +716,7 @@ AttnShape attn_shape(const lvsa_paged_attn_args* a) {
   if (tile_rows <= 32) {
     s.rows = tile_rows <= 16 ? 16 : 32;
     const int64_t kv = a->max_kv_len > 0 && a->max_kv_len < cap ? a->max_kv_len : cap;
-    const int64_t units = ceil_div(kv, paged_decode_keys(D)) * a->cache.Hkv * B, slots = 2 * cus;
+    const int64_t units = ceil_div(kv, paged_decode_keys(D)) * a->cache.Hkv * B, slots = cus * paged_decode_groups(D, a->cache.bits, s.rows);
     s.grid = (int)(units < slots ? (units > 0 ? units : 1) : slots);
   } else {
     s.rows = D <= 128 && tile_rows > kPagedTile ? kPagedTall : kPagedTile;
