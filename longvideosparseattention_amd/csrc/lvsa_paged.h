@@ -100,7 +100,10 @@ __host__ __device__ constexpr int paged_decode_groups(int D, int bits, int rows)
 constexpr int kPagedTile = 128;        // rows of a prefill tile
 constexpr int kPagedTall = 256;        // rows of a tall one (head sizes up to 128)
 constexpr int kPagedBlock = 64;        // its keys per step
-constexpr int kPagedLeast = 4;         // fewest steps of a share that is worth its partials
+// Fewest steps of a prefill share that is worth its partials (two sequences of 256
+// rows, 16 heads of 128, over 600 keys: 63, 50, 76 us with 1, 4, 16; over 1200: 64,
+// 54, 65; over 300: 43, 50, 92).
+constexpr int kPagedLeast = 4;
 
 // The running maximum of a row that has seen no key: below every finite score,
 // and still finite, so that differences to it are never NaN.

@@ -713,6 +713,14 @@ AttnShape attn_shape(const lvsa_paged_attn_args* a) {
   const int64_t cap = (int64_t)a->batch.max_pages * a->cache.page_size;
   const int64_t q = a->max_q_len > 0 && a->max_q_len < N ? a->max_q_len : N;
   const int64_t tile_rows = q * group;
+  // Rows of the tiles, from sequences of n rows over 8000 keys, 16 heads of 128
+  // (us):                16 bits: n = 16   24   32   40     4 bits: 16   24   32   40
+  //   decode, 16 rows           107  140  143                      43   62   66
+  //   decode, 32 rows           106  110  114  143                 51   55   60   90
+  //   prefill, 128 rows         124  124  124  127                 96   97   97   98
+  // (head sizes 64 and 256 cross at the same places).  Above 128 rows, where a
+  // tall tile's rows share twice the keys' copies: 160 rows 110 -> 98, 256 rows
+  // 124 -> 106, 400 rows 180 -> 158 us; 96 rows 94 -> 94, of 64 56 -> 61 us.
   if (tile_rows <= 32) {
     s.rows = tile_rows <= 16 ? 16 : 32;
     const int64_t kv = a->max_kv_len > 0 && a->max_kv_len < cap ? a->max_kv_len : cap;
@@ -722,7 +730,12 @@ AttnShape attn_shape(const lvsa_paged_attn_args* a) {
     s.rows = D <= 128 && tile_rows > kPagedTile ? kPagedTall : kPagedTile;
     s.tiles = (int)(ceil_div(N * group, s.rows) + B);
     const int64_t units = s.tiles * ceil_div(cap > 0 ? cap : 1, kPagedBlock) * a->cache.Hkv;
-    const int64_t slots = cus * (D >= 192 || s.rows == kPagedTall ? 1 : 2);
+    // Two work-groups of 128 rows on a unit hide each other's waits, but where
+    // there are fewer tiles than units most of a share's work is its partial: 4
+    // sequences of 128 rows, 16 heads of 128, 8000 keys 98 -> 81 us with one, 16
+    // of them 219 -> 241 (of 64: 58 -> 52 and 133 -> 161).
+    const bool two = D <= 128 && s.rows == kPagedTile && (int64_t)s.tiles * a->cache.Hkv > cus;
+    const int64_t slots = two ? 2 * cus : cus;
     // a multiple of the XCDs: see share_of
     s.grid = (int)(8 * ceil_div(units < slots ? units : slots, 8));
     s.plan_bytes = plan_offset(s, 5);

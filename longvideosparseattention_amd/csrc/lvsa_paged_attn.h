@@ -742,8 +742,8 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   // starts at its tile's first key block and the one it starts with ends at the
   // last, so that the work-groups of an XCD walk a head's keys at about the
   // same place at the same time, and its L2 serves them.
-  const int64_t per_head = hd.per_head, U = per_head * p.c.Hkv, u_first = unit_start(U, shares, share);
-  int left = uniform((int)(unit_start(U, shares, share + 1) - u_first));
+  const int64_t U = hd.per_head * p.c.Hkv;
+  int left = uniform((int)(unit_start(U, shares, share + 1) - unit_start(U, shares, share)));
   int h = uniform(p.ends[share].h), ti = uniform(p.ends[share].tile), blk_end = uniform(p.ends[share].blk);
   for (;;) {
   const PlanTile tile = p.plan_tiles[ti];
@@ -751,7 +751,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   const PagedSeq sq = uniform(tile.sq);
   const int blk0 = left < blk_end ? blk_end - left : 0;
   const bool whole = blk0 == 0 && blk_end == units;
-  const int64_t slot = 2 * (int64_t)share + (u_first < h * per_head + p.before[ti] ? 1 : 0);   // see decode_slots
+  const int64_t slot = 2 * (int64_t)share + (left > blk_end ? 1 : 0);   // the share comes from another tile: see decode_slots
   const int blk1 = blk_end < nb ? blk_end : nb;
   const int nrows = sq.n * p.group;
   const int r_last = r0 + kPagedTile < nrows ? r0 + kPagedTile - 1 : nrows - 1;
@@ -1113,8 +1113,8 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
   // starts at its tile's first key block and the one it starts with ends at the
   // last, so that the work-groups of an XCD walk a head's keys at about the
   // same place at the same time, and its L2 serves them.
-  const int64_t per_head = hd.per_head, U = per_head * p.c.Hkv, u_first = unit_start(U, shares, share);
-  int left = uniform((int)(unit_start(U, shares, share + 1) - u_first));
+  const int64_t U = hd.per_head * p.c.Hkv;
+  int left = uniform((int)(unit_start(U, shares, share + 1) - unit_start(U, shares, share)));
   int h = uniform(p.ends[share].h), ti = uniform(p.ends[share].tile), blk_end = uniform(p.ends[share].blk);
   for (;;) {
   const PlanTile tile = p.plan_tiles[ti];
@@ -1122,7 +1122,7 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
   const PagedSeq sq = uniform(tile.sq);
   const int blk0 = left < blk_end ? blk_end - left : 0;
   const bool whole = blk0 == 0 && blk_end == units;
-  const int64_t slot = 2 * (int64_t)share + (u_first < h * per_head + p.before[ti] ? 1 : 0);   // see decode_slots
+  const int64_t slot = 2 * (int64_t)share + (left > blk_end ? 1 : 0);   // the share comes from another tile: see decode_slots
   const int blk1 = blk_end < nb ? blk_end : nb;
   const int nrows = sq.n * p.group;
   const int r_last = r0 + kPagedTall < nrows ? r0 + kPagedTall - 1 : nrows - 1;
