@@ -14,6 +14,7 @@ namespace {
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxGrid = 1 << 20;      // work-groups of a launch that walks its rows
+constexpr int kMaxGridY = 1 << 15;     // sequences of a gather's launch
 
 template <typename E> struct Half;
 template <> struct Half<__bf16> {
@@ -259,18 +260,18 @@ __device__ __forceinline__ void append_token(const AppendParams& p, int t) {
 
 template <int D, typename E, int BITS>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
-  for (int t = blockIdx.x; t < p.c.N; t += gridDim.x) append_token<D, E, BITS>(p, t);
+  for (int64_t t = blockIdx.x; t < p.c.N; t += gridDim.x) append_token<D, E, BITS>(p, (int)t);
 }
 
 // ──────────────────────────────── gather ───────────────────────────────────
 
-// Work-groups of grid.x walk (position, head, chunk) of sequence blockIdx.y in
-// the order of the output, so that the writes, two thirds or more of the
+// Work-groups of grid.x walk (position, head, chunk) of sequence b0 + blockIdx.y
+// in the order of the output, so that the writes, two thirds or more of the
 // traffic, are contiguous; blockIdx.z: keys, values.  Bound by memory.
 template <int D, typename E, int BITS>
-__global__ __launch_bounds__(256) void paged_gather_kernel(PagedView c, char* ko, char* vo, int max_len) {
+__global__ __launch_bounds__(256) void paged_gather_kernel(PagedView c, char* ko, char* vo, int max_len, int b0) {
   constexpr int CH = D / 8;
-  const int b = blockIdx.y;
+  const int b = b0 + blockIdx.y;
   const bool is_v = blockIdx.z;
   int L = c.lens[b];
   const int64_t cap = (int64_t)c.max_pages * c.page_size;
@@ -417,8 +418,8 @@ template <typename E>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnParams p, int D, int rows, int keys) {
   __shared__ float acc_s[4][256];
   __shared__ float ml_s[4][2];
-  for (int row = blockIdx.x; row < p.c.N * p.H; row += gridDim.x) {
-    merge_row<E>(p, row, D, rows, keys, acc_s, ml_s);
+  for (int64_t row = blockIdx.x; row < (int64_t)p.c.N * p.H; row += gridDim.x) {
+    merge_row<E>(p, (int)row, D, rows, keys, acc_s, ml_s);
     __syncthreads();             // the next row writes the same LDS
   }
 }
@@ -684,8 +685,9 @@ template <int D, typename E, int BITS> struct Gather {
     const int64_t chunks = (int64_t)max_len * c.Hkv * (D / 8);
     const int64_t want = ceil_div(chunks, 256);
     const unsigned gx = (unsigned)(want < 4096 ? want : 4096);
-    hipLaunchKernelGGL((paged_gather_kernel<D, E, BITS>), dim3(gx, (unsigned)c.B, 2), dim3(256), 0, stream, c, (char*)ko,
-                       (char*)vo, max_len);
+    for (int64_t b0 = 0; b0 < c.B; b0 += kMaxGridY)
+      hipLaunchKernelGGL((paged_gather_kernel<D, E, BITS>), dim3(gx, (unsigned)(c.B - b0 < kMaxGridY ? c.B - b0 : kMaxGridY), 2),
+                         dim3(256), 0, stream, c, (char*)ko, (char*)vo, max_len, (int)b0);
     return launch_status("lvsa_paged_gather");
   }
 };
@@ -818,8 +820,7 @@ int lvsa_paged_gather(const lvsa_paged_cache* cache, const lvsa_paged_batch* bat
   PagedView c{};
   const int rc = paged_view(what, cache, batch, false, &c);
   if (rc) return rc;
-  LVSA_REQUIRE(max_len >= 0 && batch->B <= 65535, LVSA_ERR_INVALID_ARG, "%s: %d sequences of %d tokens", what, batch->B,
-               max_len);
+  LVSA_REQUIRE(max_len >= 0, LVSA_ERR_INVALID_ARG, "%s: %d tokens", what, max_len);
   if (batch->B == 0 || max_len == 0) return LVSA_OK;
   LVSA_REQUIRE(k_out && v_out && aligned16((int64_t)(uintptr_t)k_out) && aligned16((int64_t)(uintptr_t)v_out),
                LVSA_ERR_INVALID_ARG, "%s: outputs must be non-null and 16-byte aligned", what);

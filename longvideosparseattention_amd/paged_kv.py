@@ -130,6 +130,8 @@ class PagedKVCache:
         for t in (v, k_scale, v_scale):
             if t is not None and t.device != self.device:
                 raise ValueError(f"cache tensors on {self.device} and {t.device}")
+        if k.data_ptr() == v.data_ptr() or (k_scale is not None and k_scale.data_ptr() == v_scale.data_ptr()):
+            raise ValueError("cache keys and values must not share memory")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         ptrs = [0 if t is None else t.data_ptr() for t in (k, v, k_scale, v_scale)]
@@ -234,8 +236,8 @@ def _tokens(t: torch.Tensor, name: str, heads: Optional[int], cache: PagedKVCach
     return t, ptr, s0, s1
 
 
-def _result(out: Optional[torch.Tensor], like: torch.Tensor, name: str):
-    """The tensor a call writes (``out``, or a new one) with its address and strides."""
+def _result(out: Optional[torch.Tensor], like: torch.Tensor, name: str, *inputs: torch.Tensor):
+    """The tensor a call writes (``out``, or a new one) with its address and strides; ``inputs``: what else it reads."""
     if out is None:
         out = torch.empty_like(like, memory_format=torch.contiguous_format)
         _, H, D = like.shape
@@ -244,8 +246,9 @@ def _result(out: Optional[torch.Tensor], like: torch.Tensor, name: str):
         raise ValueError(f"{name} must be {tuple(like.shape)} of {like.dtype} on {like.device}")
     if out.stride(2) != 1 or (out.data_ptr() | ((out.stride(0) | out.stride(1)) * 2)) & 15:
         raise ValueError(f"{name} needs a contiguous last dimension and rows at multiples of 16 bytes")
-    if out.numel() and _span(out)[0] < _span(like)[1] and _span(like)[0] < _span(out)[1]:
-        raise ValueError(f"{name} must not share memory with the input")
+    for t in (like, *inputs):
+        if t.numel() and _span(out)[0] < _span(t)[1] and _span(t)[0] < _span(out)[1]:
+            raise ValueError(f"{name} must not share memory with the input")
     N, H, D = out.shape
     a, b = sorted(((N, out.stride(0)), (H, out.stride(1))), key=lambda x: x[1])
     if (a[0] > 1 and a[1] < D) or (b[0] > 1 and b[1] < (a[1] * (a[0] - 1) if a[0] > 1 else 0) + D):
@@ -300,7 +303,7 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, cu_se
         H = q.shape[1]
         if q.shape[0] != N or H < 1:
             raise ValueError(f"k has {N} tokens, q {tuple(q.shape)}")
-        q_out, qo_ptr, *qo_str = _result(q_out, q, "q_out")
+        q_out, qo_ptr, *qo_str = _result(q_out, q, "q_out", k, v)
     elif q_out is not None:
         raise ValueError("q_out without q")
     rot = angles = cos_ptr = sin_ptr = pos_ptr = 0

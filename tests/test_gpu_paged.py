@@ -184,6 +184,22 @@ def test_gather(gpu, D, Hkv, page, layout, dtype, bits):
     assert k.shape == v.shape == (4, 0, Hkv, D)
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+def test_gather_of_more_sequences_than_a_grid_has_rows(gpu, bits):
+    B = 70000
+    cache = lv.PagedKVCache.allocate(3, 4, 1, 64, bits=bits, device=gpu)
+    one = torch.randn(3, 1, 64, generator=torch.Generator().manual_seed(1)).to(BF).to(gpu)
+    table = torch.arange(3, dtype=torch.int32, device=gpu)[:, None]
+    first = torch.arange(4, dtype=torch.int32, device=gpu)
+    lv.paged_kv_append(cache, one, one, first, torch.ones(3, dtype=torch.int32, device=gpu), table)
+    of = torch.arange(B, device=gpu) % 3
+    k, v = lv.paged_kv_gather(cache, (of != 1).int(), of.int()[:, None].contiguous(), 2)
+    few, _ = lv.paged_kv_gather(cache, torch.ones(3, dtype=torch.int32, device=gpu), table, 1)
+    want = torch.where((of != 1)[:, None, None], few[of, 0], 0)
+    assert torch.equal(k[:, 0], want) and torch.equal(v[:, 0], want) and (k[:, 1] == 0).all() and (v[:, 1] == 0).all()
+    cache.check()
+
+
 # ── attention: single tokens and few rows ────────────────────────────────────
 
 DECODE = [  # sequences, D, H, Hkv, page, layout
@@ -266,6 +282,23 @@ def test_hints_change_no_result_beyond_rounding(gpu, bits):
                {"max_kv_len": 1}, {"max_q_len": 10 ** 10, "max_kv_len": 10 ** 10}):
         _attend(b, q, True, what=str(kw), **kw)
         _attend(b, q, False, what=str(kw), **kw)
+
+
+@pytest.mark.parametrize("B", [65, 128, 1100, 4300])
+def test_many_sequences(gpu, B):
+    """More sequences than a wave holds, than the plan takes at a time, and more row tiles than it keeps in LDS."""
+    seqs = [(0 if s % 7 == 3 else 1 + (s % 11 == 0), s % 5 + (s * s) % 13) for s in range(B)]
+    seqs = [(min(n, L), L) for n, L in seqs]
+    b = Batch(gpu, seqs, 64, 2, 1, 8, BF, seed=6, tail=2)
+    q, k, v = b.randn(b.N, 2, 64), b.randn(b.N, 1, 64), b.randn(b.N, 1, 64)
+    lv.paged_kv_append(b.cache, k, v, *b.call())
+    for s, (n, L) in enumerate(seqs):
+        b.K[s][L - n:], b.V[s][L - n:] = k[b.ends[s]:b.ends[s + 1]].double().cpu(), v[b.ends[s]:b.ends[s + 1]].double().cpu()
+    for hint in (2, 0):
+        o, lse = _attend(b, q, max_q_len=hint)
+        assert (o[b.n_rows:] == 0).all() and (lse[b.n_rows:] == float("-inf")).all()
+    got, _ = lv.paged_kv_gather(b.cache, b.lens, b.table_dev, 17)
+    assert all(torch.equal(got[s, :L].double().cpu(), b.K[s]) for s, (_, L) in enumerate(seqs))
 
 
 @pytest.mark.parametrize("scale", [1e-6, 0.3, 40.0])
@@ -669,6 +702,9 @@ def test_refusals(gpu):
         app(positions=torch.zeros(2, dtype=torch.int32, device=gpu))
     with pytest.raises(ValueError, match="share memory"):
         app(q=q, q_out=q)
+    with pytest.raises(ValueError, match="share memory"):         # the keys' memory
+        both = b.randn(2, 8, 128)
+        lv.paged_kv_append(b.cache, both[:, 3:5], k, cu, lens, table, q=q, q_out=both[:, :4])
     with pytest.raises(ValueError, match="tokens"):
         lv.paged_kv_append(b.cache, k, k[:1], cu, lens, table)
     with pytest.raises(ValueError, match="max_len"):
@@ -687,4 +723,6 @@ def test_refusals(gpu):
         lv.PagedKVCache(t, t)
     with pytest.raises(ValueError, match="differ"):
         lv.PagedKVCache(b.cache.k, b.cache.v[:1])
+    with pytest.raises(ValueError, match="share memory"):
+        lv.PagedKVCache(b.cache.k, b.cache.k)
     b.cache.check()
