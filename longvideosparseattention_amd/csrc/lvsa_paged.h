@@ -100,6 +100,19 @@ __host__ __device__ constexpr int paged_decode_groups(int D, int bits, int rows)
 constexpr int kPagedTile = 128;        // rows of a prefill tile
 constexpr int kPagedTall = 256;        // rows of a tall one (head sizes up to 128)
 constexpr int kPagedBlock = 64;        // its keys per step
+// Chunks run on the decode kernel, too, where their rows (of all heads) and twice
+// its steps come to no more than this per compute unit: latency counts there, and
+// it needs no plan.  Prefill and decode kernel, us, head size 128, causal:
+//   tokens, heads / key heads, keys   rows + 2 steps per unit    16 bits     4 bits
+//   20, 16 / 4, 2000                        1.3 +  2             33   17     32   17
+//   256, 16 / 4, 300                       16   +  3             43   30     40   30
+//   256, 16 / 4, 1000                      16   +  8             51   34     49   33
+//   512, 16 / 4, 512                       32   +  8             57   40     54   45
+//   384, 16 / 16, 600                      24   +  8             45   47     43   42
+//   512, 16 / 16, 1000                     32   + 17             44   47     41   50
+//   4 times 256, 16 / 4, 256               64   +  8             47   66     45   55
+// and with D = 256 and 2000 tokens of 2 heads over themselves, 16 + 32: 65, 80 us.
+constexpr int kPagedShort = 40;
 // Fewest steps of a prefill share that is worth its partials (two sequences of 256
 // rows, 16 heads of 128, over 600 keys: 63, 50, 76 us with 1, 4, 16; over 1200: 64,
 // 54, 65; over 300: 43, 50, 92).

@@ -503,7 +503,10 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int
   }
   const int tiles = (int)done;
   const int64_t U = units * p.c.Hkv;
-  const int shares = U > 0 ? unit_shares(U, p.grid, kPagedLeast) : 0;
+  // a share for every tile, whatever its keys, where there are work-groups for it
+  const int64_t whole = (int64_t)tiles * p.c.Hkv;
+  const int least = U > 0 ? unit_shares(U, p.grid, kPagedLeast) : 0;
+  const int shares = whole <= least ? least : whole < p.grid ? (int)whole : p.grid;
   if (threadIdx.x == 0) *p.head = PlanHead{units, tiles, shares};
   const bool in_lds = tiles <= kPlanLds;
   for (int w = threadIdx.x; w < shares; w += 1024) {
@@ -723,10 +726,13 @@ AttnShape attn_shape(const lvsa_paged_attn_args* a) {
   // (head sizes 64 and 256 cross at the same places).  Above 128 rows, where a
   // tall tile's rows share twice the keys' copies: 160 rows 110 -> 98, 256 rows
   // 124 -> 106, 400 rows 180 -> 158 us; 96 rows 94 -> 94, of 64 56 -> 61 us.
-  if (tile_rows <= 32) {
+  const int64_t kv = a->max_kv_len > 0 && a->max_kv_len < cap ? a->max_kv_len : cap;
+  const int64_t steps = ceil_div(kv, paged_decode_keys(D)) * a->cache.Hkv;     // of a row tile
+  const int64_t short_units = steps * (ceil_div(N * group, 32) + B);
+  if (tile_rows <= 32 || N * a->H + 2 * short_units <= kPagedShort * cus) {
     s.rows = tile_rows <= 16 ? 16 : 32;
-    const int64_t kv = a->max_kv_len > 0 && a->max_kv_len < cap ? a->max_kv_len : cap;
-    const int64_t units = ceil_div(kv, paged_decode_keys(D)) * a->cache.Hkv * B, slots = cus * paged_decode_groups(D, a->cache.bits, s.rows);
+    const int64_t units = tile_rows <= 32 ? steps * B : short_units;
+    const int64_t slots = cus * paged_decode_groups(D, a->cache.bits, s.rows);
     s.grid = (int)(units < slots ? (units > 0 ? units : 1) : slots);
   } else {
     s.rows = D <= 128 && tile_rows > kPagedTile ? kPagedTall : kPagedTile;

@@ -559,11 +559,16 @@ def test_frames_chunk_by_chunk_against_the_dense_call(gpu):
 @pytest.mark.parametrize("n", [1, 60])
 def test_a_captured_step_serves_later_steps(gpu, n, bits):
     """Append and attention captured once, replayed with new tokens, lengths and tables, eager work in between."""
+    _captured_step(gpu, n, bits, 20)
+
+
+def _captured_step(gpu, n, bits, columns):
     D, H, Hkv, ps, B = 128, 4, 2, 16, 3
     g = torch.Generator().manual_seed(5)
     make = lambda: lv.PagedKVCache.allocate(64, ps, Hkv, D, bits=bits, device=gpu)  # noqa: E731
     cache, other = make(), make()
-    table = torch.randperm(64, generator=g)[:B * 20].view(B, 20).to(torch.int32).to(gpu)
+    table = torch.full((B, columns), -1, dtype=torch.int32, device=gpu)
+    table[:, :20] = torch.randperm(64, generator=g)[:B * 20].view(B, 20).to(gpu)
     cos, sin = _angles(400, D, gpu)
     cu = (torch.arange(B + 1, dtype=torch.int32) * n).to(gpu)
     lens = torch.zeros(B, dtype=torch.int32, device=gpu)
@@ -653,6 +658,85 @@ def test_offsets_beyond_32_bits(gpu, bits):
         assert torch.equal(lv.paged_attention(q[:1], c, one, lens, t, max_q_len=1),
                            lv.paged_attention(q[:1], small, one, lens, near, max_q_len=1))
     cache.check()
+
+
+# ── chunks with room for long caches ─────────────────────────────────────────
+
+# Where the page table leaves room for them, chunks run on the kernels of long caches whatever the lengths are: the
+# chunks' tests again with such tables.
+ROOM = 700000
+ROOMY = ([(test_attention_of_chunks, dict(i=i, dtype=dtype, bits=bits, causal=causal)) for i in range(len(CHUNKS))
+          for dtype in (BF, HF) for bits in (16, 4) for causal in (True, False)] +
+         [(test_few_tiles_over_long_caches_run_in_parts, dict(bits=bits, D=D, n=n, L=L)) for bits, D in ((16, 128), (4, 64), (16, 256))
+          for n, L in ((40, 9000), (300, 5000))] +
+         [(test_hints_change_no_result_beyond_rounding, dict(bits=bits)) for bits in (16, 4)] +
+         [(test_scales, dict(scale=scale, n=150)) for scale in (1e-6, 0.3, 40.0)] +
+         [(test_scores_far_from_zero, dict(n=n)) for n in (40, 150)] +
+         [(test_rows_without_keys, dict(hint=0))] +
+         [(test_nothing_of_an_unattended_key_reaches_a_row, dict(n=n, D=D, bits=bits)) for bits in (16, 4)
+          for n, D in ((20, 64), (20, 256), (40, 128), (60, 96), (150, 128), (150, 96), (150, 64), (150, 192))] +
+         [(test_an_infinite_score, dict(n=n)) for n in (40, 150)] +
+         [(test_bad_pages_spoil_their_sequence_only, dict(page=page, n=n, bits=bits)) for page in (-1, "past", 2 ** 31 - 1)
+          for n in (30, 120) for bits in (16, 4)] +
+         [(test_many_sequences, dict(B=B)) for B in (65, 1100)])
+
+
+@pytest.mark.parametrize("i", range(len(ROOMY)), ids=lambda i: ROOMY[i][0].__name__[5:] + "-" + "-".join(
+    str(v).replace("torch.", "") for v in ROOMY[i][1].values()))
+def test_with_room(gpu, monkeypatch, i):
+    class Roomy(Batch):
+        def __init__(self, dev, seqs, D, H, Hkv, page, *a, **kw):
+            super().__init__(dev, seqs, D, H, Hkv, page, *a, extra_columns=-(-(ROOM if len(seqs) < 10 else 20000) // page), **kw)
+
+    monkeypatch.setitem(globals(), "Batch", Roomy)
+    test, kw = ROOMY[i]
+    test(gpu, **kw)
+
+
+@pytest.mark.parametrize("n", [40, 100])
+def test_bad_lengths_and_row_ranges_with_room(gpu, n):
+    b = Batch(gpu, [(n, 150), (n, 140), (n, 133)], 128, 4, 2, 16, BF, extra_columns=ROOM // 16)
+    q = b.randn(b.N, 4, 128)
+    want, _, tol, _ = ref.attention(b, q)
+    for bad in (-1, -2 ** 31, 2 ** 31 - 1, ROOM + 161):
+        lens = b.lens.clone()
+        lens[1] = bad
+        o = lv.paged_attention(q, b.cache, b.cu, lens, b.table_dev, max_kv_len=ROOM) if bad < 0 else None
+        if bad > 0:                                       # cut to the table's room, whose further pages are no pages
+            lens[0] = lens[2] = 0
+            q1 = q[:2 * n]
+            o = lv.paged_attention(q1, b.cache, torch.tensor([0, n, n + 1, n + 1], dtype=torch.int32, device=gpu), lens, b.table_dev)
+            assert torch.isnan(o[n]).all()
+        else:
+            assert torch.isnan(o[n:2 * n]).all()
+            for r in (slice(0, n), slice(2 * n, 3 * n)):
+                ref.check_close(o[r], want[r], tol[r], f"beside length {bad}")
+        with pytest.raises(ValueError, match="kv_lens"):
+            b.cache.check()
+    for cu in ([0, n, 2 * n, 3 * n + 50], [0, 2 * n, n, 3 * n], [-5, n, 2 * n, 3 * n], [0, n, 2 ** 31 - 1, 3 * n]):
+        cu = torch.tensor(cu, dtype=torch.int32, device=gpu)
+        lv.paged_attention(q, b.cache, cu, b.lens, b.table_dev)
+        with pytest.raises(ValueError, match="cu_seqlens"):
+            b.cache.check()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_captured_chunk_with_room(gpu, bits):
+    _captured_step(gpu, 60, bits, ROOM // 16)
+
+
+def test_chunks_on_two_streams(gpu):
+    b = Batch(gpu, [(70, 900), (1, 50), (200, 200)], 128, 8, 2, 16, BF, extra_columns=ROOM // 16)
+    q = b.randn(b.N, 8, 128)
+    first, _ = _attend(b, q)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(6):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(lv.paged_attention(q, b.cache, *b.call()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, first) for x in got)
 
 
 # ── refusals ─────────────────────────────────────────────────────────────────
