@@ -203,7 +203,9 @@ __device__ __forceinline__ void append_token(const AppendParams& p, int t) {
       char* dst = is_q ? p.qo + t * p.qo_str[0] + h * p.qo_str[1]
                        : (is_k ? p.c.k + page * p.c.k_str[0] + slot * p.c.k_str[1] + h * p.c.k_str[2]
                                : p.c.v + page * p.c.v_str[0] + slot * p.c.v_str[1] + h * p.c.v_str[2]);
-      *reinterpret_cast<u32x4*>(dst + 16 * c) = w;
+      // turned queries pass the L2 by (another kernel reads them): 74.7 -> 72.5 us as above
+      if (is_q) __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(dst + 16 * c));
+      else *reinterpret_cast<u32x4*>(dst + 16 * c) = w;
     } else {
       if (turned) {
         // The angles are widened here, row by row, and two elements are formed at
@@ -267,7 +269,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 
 // Work-groups of grid.x walk (position, head, chunk) of sequence b0 + blockIdx.y
 // in the order of the output, so that the writes, two thirds or more of the
-// traffic, are contiguous; blockIdx.z: keys, values.  Bound by memory.
+// traffic, are contiguous; blockIdx.z: keys, values.  Bound by memory.  The
+// output passes the L2 by, which is too small for it and serves the table and the
+// cache's lines: 12 sequences of up to 2500 tokens, 16 heads of 64 in 4 bits, 38.5
+// -> 24.9 us; 15600 tokens of 12 heads of 128 in 16 bits 36.5 -> 33.2 us.
 template <int D, typename E, int BITS>
 __global__ __launch_bounds__(256) void paged_gather_kernel(PagedView c, char* ko, char* vo, int max_len, int b0) {
   constexpr int CH = D / 8;
@@ -310,7 +315,7 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(PagedView c, char* ko
         }
       }
     }
-    out[i] = w;
+    __builtin_nontemporal_store(w, out + i);
   }
 }
 
@@ -445,8 +450,8 @@ __device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* lds, int64_t* 
 
 // One work-group: lists the row tiles with their key blocks, where the shares
 // end and what is to be joined there.  Latency only: two dependent reads of
-// memory, scans and searches in LDS (searches in memory past kPlanLds tiles); 4
-// us beside launches of 30 us and more.  With it every work-group of those
+// memory, scans and searches in LDS (searches in memory past kPlanLds tiles); 7 to
+// 9 us beside launches of 30 us and more.  With it every work-group of those
 // gets the same number of key blocks, whatever the lengths, where tiles as units
 // leave the last round to a few (516 tiles on 256 CUs: three rounds for two
 // rounds' work).
@@ -538,7 +543,8 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int
 // plan says so.  blockIdx.y: 32 rows of the tile.  A lane has four elements of
 // a row and a wave R rows at a time, so that every partial is one 16-byte load
 // per lane with the next ones in flight behind it: what bounds it is the bytes,
-// 67 MB for a launch whose 256 shares all end inside a tile of 256 rows of 128.
+// 67 MB for a launch whose 256 shares all end inside a tile of 256 rows of 128 (16
+// us; 9 us of head size 64).
 template <int D, typename E>
 __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(PagedAttnParams p, int rows) {
   typedef float f4 __attribute__((ext_vector_type(4)));

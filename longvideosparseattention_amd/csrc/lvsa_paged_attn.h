@@ -6,14 +6,17 @@
 // pair is token r / group, head r % group of the group, so that a tile of rows
 // reads each key and value once for all of them.
 //
-//   paged_decode_kernel   few rows (tiles of 16 or 32): bound by the bytes of
-//                         the cache.  Matrix instructions of 16 rows, each
-//                         wave on keys of its own.
+//   paged_decode_kernel   few rows (tiles of 16 or 32) and short chunks: bound by
+//                         the bytes of the cache, or by latency.  Matrix
+//                         instructions of 16 rows, each wave on keys of its own.
 //   paged_prefill_kernel  tiles of 128 rows: bound by the matrix cores and the
 //                         softmax.  Four waves of 32 rows share key blocks of
 //                         64 in LDS.
+//   paged_tall_kernel     tiles of 256 rows (head sizes up to 128): the same
+//                         bound, eight waves on the same blocks.
+// Which one runs follows from the sizes (attn_shape, lvsa_paged.hip).
 //
-// Both form S^T = K Q^T, so that a lane owns one row's scores, and O^T += V^T
+// All form S^T = K Q^T, so that a lane owns one row's scores, and O^T += V^T
 // P^T with P straight from S^T's registers: the order of the keys within a
 // step is permuted alike on both operands.  V^T comes out of LDS by
 // transposing reads.
@@ -24,9 +27,9 @@
 //   prefill   8 keys (tile t of the matrix): 128 (c ^ (t & 1)) + 16 (r ^ 4 ((c >>
 //             1) & 1)).  One copy instruction brings 128 bytes of each of 8
 //             keys (16 keys x 64 bytes, as in decode, cost the L1 twice the
-//             lookups and 100 of frames_chunk's 800 us).  Head size 96, whose 12
-//             chunks do not divide by 8, keeps 16 keys x 64 bytes with 4 (c & 3)
-//             in the place of 8 (c & 1).
+//             lookups and 100 of 800 us for 4680 tokens over 32760 keys).  Head
+//             size 96, whose 12 chunks do not divide by 8, keeps 16 keys x 64
+//             bytes with 4 (c & 3) in the place of 8 (c & 1).
 // In each, what 16 lanes of a 16-byte read, or 32 of a transposing read (8 keys
 // of two chunks in decode, 4 keys of four in prefill), take in one cycle covers
 // the 64 banks once.
@@ -205,7 +208,11 @@ struct Step<D, 4, T> {
   uint32_t ks[T][2], vs[T][2];
 };
 
-// Two work-groups per CU (up to 256 registers) where the operands allow it.
+// Bound by the bytes: 45 sequences of up to 16000 keys, 32 heads over 8 of 128, in
+// 16 bits at 5.7 TB/s (329 us), 40 of up to 32000 in 4 bits at 4.9 TB/s (154 us;
+// there the decoding of codes on the vector units takes as long as the bytes).  A
+// single sequence of 1001 keys takes 8 us, all of it trips to memory one after
+// the other, and its merge 5 us.
 //
 // The launch's work, sum over sequences of row tiles x key heads x key steps,
 // is cut into `grid` equal shares, so that ragged batches keep every
@@ -214,6 +221,7 @@ struct Step<D, 4, T> {
 // of two slots of the work-group and paged_merge_kernel joins them.  The
 // share's bounds follow from the lengths alone, so the merge finds the slots
 // without a word from this kernel.
+//
 // Launch bounds: the registers of the work-groups that are to be on a unit at
 // once; of the large heads those fit without being asked for, and asking spoils
 // the schedule (D = 256, 4 bits: 275 instead of 215 us for 40 sequences of 12000).
@@ -720,6 +728,10 @@ __device__ __forceinline__ void wait_copies() {
 // 16-bit pages are copied without passing registers; of 4-bit pages the codes
 // are loaded a step ahead and written to LDS as 16-bit values, so every row is
 // decoded once for 128 query rows.
+//
+// 780 tokens of 12 heads over 4 of 256, over 31980 keys in 4 bits: 382 us with
+// plan and joining, 780 TFLOP/s (500 us with a phase of products after a phase of
+// softmax).  4 sequences of 128 tokens, 16 heads of 128, over 16384 keys: 141 us.
 template <int D, typename E, int BITS>
 __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(PagedAttnParams p) {
   constexpr int ND = D / 32, NK = D / 16, NO = D / 32;
@@ -1075,6 +1087,14 @@ __device__ __forceinline__ void copy4(const void* from, const lds_char* l) {
 //   M(j)  S(j) = K(j) Q^T and O += V(j-1) P(j-1) as one stream of matrix
 //         instructions whose LDS operands are read LA instructions ahead
 //   S(j)  masks, maximum, P(j), row sums
+//
+// The products get the higher priority of the two waves on a SIMD (3%).  4680
+// tokens of 12 heads of 128 over 32760 keys: 764 us with plan and joining, 1.06
+// PFLOP/s (950 us with tiles of 128 rows and two independent work-groups; 840 us
+// with products and exponentials of one wave interleaved, which the issue of the
+// vector instructions beside the matrix ones holds up; 660 us without the copies,
+// which is what the data's way costs).  Causal prompts of head size 64: 184 us,
+// 680 TFLOP/s, bound by the exponentials: half the products per weight.
 //
 // Group 0 runs M(j) in phase 2 j and S(j) in phase 2 j + 1, group 1 one phase
 // later.  LDS holds four blocks of 64 keys of K and of V; group 0 brings K,
