@@ -15,6 +15,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxGrid = 1 << 20;      // work-groups of a launch that walks its rows
 constexpr int kMaxGridY = 1 << 15;     // sequences of a gather's launch
+constexpr int kFewTokens = 10;         // of an append, per compute unit
 
 template <typename E> struct Half;
 template <> struct Half<__bf16> {
@@ -110,9 +111,15 @@ struct AppendParams {
 // rounds once, and goes to odd-rounded fp32 for the converter: a key next to
 // the border of two codes or of two scales comes out as the exact value's
 // would, on every device and in every order of evaluation.
-template <int D, typename E, int BITS>
+//
+// 256 threads for few tokens, where the row after row of one wave would be waited
+// for, 64 where there are many: each wave looks the token up for itself (the same
+// 7868 tokens 72 us with 256, 64 with 128, 61 with 64; on 256 units, 256 and 64
+// threads: 32 tokens 5.8, 10.3 us, 2048 16.0, 16.6, 4096 27.7, 22.1; into 16 bits
+// 4.5, 7.6, 13.0, 14.7, 26.8, 26.7).
+template <int D, typename E, int BITS, int THREADS>
 __device__ __forceinline__ void append_token(const AppendParams& p, int t) {
-  constexpr int CH = D / 8, RPP = 256 / CH;
+  constexpr int CH = D / 8, RPP = THREADS / CH;
   const int lane = threadIdx.x & 63;
   const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
   const int half = p.rot / 2;
@@ -260,9 +267,9 @@ __device__ __forceinline__ void append_token(const AppendParams& p, int t) {
   }
 }
 
-template <int D, typename E, int BITS>
-__global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
-  for (int64_t t = blockIdx.x; t < p.c.N; t += gridDim.x) append_token<D, E, BITS>(p, (int)t);
+template <int D, typename E, int BITS, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendParams p) {
+  for (int64_t t = blockIdx.x; t < p.c.N; t += gridDim.x) append_token<D, E, BITS, THREADS>(p, (int)t);
 }
 
 // ──────────────────────────────── gather ───────────────────────────────────
@@ -684,8 +691,11 @@ int by_type(int D, int dtype, int bits, A&&... a) {
 
 template <int D, typename E, int BITS> struct Append {
   static int go(const AppendParams& p, hipStream_t stream) {
-    hipLaunchKernelGGL((paged_append_kernel<D, E, BITS>), dim3((unsigned)(p.c.N < kMaxGrid ? p.c.N : kMaxGrid)), dim3(256), 0,
-                       stream, p);
+    const dim3 grid((unsigned)(p.c.N < kMaxGrid ? p.c.N : kMaxGrid));
+    if (p.c.N <= kFewTokens * cu_count())
+      hipLaunchKernelGGL((paged_append_kernel<D, E, BITS, 256>), grid, dim3(256), 0, stream, p);
+    else
+      hipLaunchKernelGGL((paged_append_kernel<D, E, BITS, 64>), grid, dim3(64), 0, stream, p);
     return launch_status("lvsa_paged_append");
   }
 };

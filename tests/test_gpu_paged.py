@@ -125,6 +125,31 @@ def test_append_4_bits_gives_the_exact_values_codes(gpu, i, dtype):
         assert torch.equal(g, w), f"{name}: {(g != w).sum().item()} of {g.numel()} bytes differ"
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("D,H,Hkv,rot,inter", [(64, 3, 1, 64, False), (96, 2, 2, 96, True), (128, 5, 1, 128, False),
+                                               (192, 2, 1, 64, False), (256, 2, 1, 256, True)])
+def test_many_tokens_equal_few_at_a_time(gpu, D, H, Hkv, rot, inter, bits):
+    """Thousands of tokens in one call (a wave each) leave the bits that calls of a few hundred (four waves each) leave."""
+    N, ps = 5000, 64
+    g = torch.Generator().manual_seed(8)
+    k, v, q = (torch.randn(N, h, D, generator=g).to(BF).to(gpu) for h in (Hkv, Hkv, H))
+    cos, sin = _angles(N, rot, gpu)
+    table = torch.randperm(80, generator=g)[None, :79].to(torch.int32).to(gpu)
+    caches = [lv.PagedKVCache.allocate(80, ps, Hkv, D, bits=bits, device=gpu) for _ in range(2)]
+    of = lambda *x: torch.tensor(x, dtype=torch.int32, device=gpu)  # noqa: E731
+    whole = lv.paged_kv_append(caches[0], k, v, of(0, N), of(N), table, q=q, cos=cos, sin=sin, interleaved=inter)
+    for a in range(0, N, 700):
+        e = min(a + 700, N)
+        part = lv.paged_kv_append(caches[1], k[a:e], v[a:e], of(0, e - a), of(e), table, q=q[a:e], cos=cos, sin=sin,
+                                  interleaved=inter)
+        assert torch.equal(part, whole[a:e])
+    for x in ("k", "v", "k_scale", "v_scale"):
+        if getattr(caches[0], x) is not None:
+            assert torch.equal(getattr(caches[0], x), getattr(caches[1], x))
+    for c in caches:
+        c.check()
+
+
 def test_codes_of_ties_and_borders(gpu):
     """Every tie and its neighbours, at the smallest and the largest scale, both signs."""
     mids = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
