@@ -1089,8 +1089,8 @@ __device__ __forceinline__ void copy4(const void* from, const lds_char* l) {
 //   S(j)  masks, maximum, P(j), row sums
 //
 // The products get the higher priority of the two waves on a SIMD (3%).  4680
-// tokens of 12 heads of 128 over 32760 keys: 764 us with plan and joining, 1.06
-// PFLOP/s (950 us with tiles of 128 rows and two independent work-groups; 840 us
+// tokens of 12 heads of 128 over 32760 keys: 750 to 780 us with plan and joining,
+// by the card's clock, 1.03 to 1.07 PFLOP/s (950 us with tiles of 128 rows and two independent work-groups; 840 us
 // with products and exponentials of one wave interleaved, which the issue of the
 // vector instructions beside the matrix ones holds up; 660 us without the copies,
 // which is what the data's way costs).  Causal prompts of head size 64: 184 us,
