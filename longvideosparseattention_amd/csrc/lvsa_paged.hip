@@ -732,7 +732,8 @@ AttnShape attn_shape(const lvsa_paged_attn_args* a) {
   const int group = a->H / a->cache.Hkv, D = a->cache.D;
   const int64_t N = a->batch.N, cus = cu_count(), B = a->batch.B < N ? a->batch.B : N;
   const int64_t cap = (int64_t)a->batch.max_pages * a->cache.page_size;
-  const int64_t q = a->max_q_len > 0 && a->max_q_len < N ? a->max_q_len : N;
+  // unknown: single tokens where there are no more rows than sequences, else one sequence of all rows
+  const int64_t q = a->max_q_len > 0 ? (a->max_q_len < N ? a->max_q_len : N) : N <= a->batch.B ? 1 : N;
   const int64_t tile_rows = q * group;
   // Rows of the tiles, from sequences of n rows over 8000 keys, 16 heads of 128
   // (us):                16 bits: n = 16   24   32   40     4 bits: 16   24   32   40
@@ -786,7 +787,7 @@ int attn_check(const lvsa_paged_attn_args* a, PagedView* v) {
                a->cache.Hkv);
   LVSA_REQUIRE((int64_t)a->batch.N * a->H < (1LL << 31) - 4096, LVSA_ERR_UNSUPPORTED, "%s: %d rows of %d heads", what,
                a->batch.N, a->H);
-  LVSA_REQUIRE(a->scale > 0.f && a->scale <= 3.4028235e38f, LVSA_ERR_INVALID_ARG, "%s: scale %g must be positive and finite",
+  LVSA_REQUIRE(a->scale > 0.f && a->scale <= 2.0e38f, LVSA_ERR_INVALID_ARG, "%s: scale %g must be positive and at most 2e38",
                what, (double)a->scale);
   return LVSA_OK;
 }

@@ -394,8 +394,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, cu_seqlens: torch.Tens
 
     ``max_q_len`` (the most rows of a sequence) and ``max_kv_len`` (the longest
     cache) only choose a kernel and its split: results are right whatever they
-    say, but without ``max_q_len`` a batch of single tokens is taken for one long
-    sequence and runs slower.  ``out`` must not share memory with ``q``; rows of no
+    say.  Without ``max_q_len`` more rows than sequences are taken for one long
+    sequence, which runs slower for a few rows of each.  ``out`` must not share memory with ``q``; rows of no
     sequence are left as they were in ``out`` and are 0 in a new tensor (``lse``:
     ``-inf``).  Scores, softmax and sums are fp32; weights enter the second product
     in ``q``'s type."""
@@ -406,8 +406,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, cu_seqlens: torch.Tens
     if H < 1 or H % cache.num_kv_heads:
         raise ValueError(f"num heads {H} must be a multiple of kv heads {cache.num_kv_heads}")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0.0 < scale <= 3.4e38:
-        raise ValueError(f"scale {scale} must be positive and finite")
+    if not 0.0 < scale <= 2e38:              # times log2(e) within fp32
+        raise ValueError(f"scale {scale} must be positive and at most 2e38")
     batch = _batch(cache, cu_seqlens, kv_lens, page_table, N)
     fresh = out is None
     out, o_ptr, *o_str = _result(out, q, "out")

@@ -309,6 +309,17 @@ def test_hints_change_no_result_beyond_rounding(gpu, bits):
         _attend(b, q, False, what=str(kw), **kw)
 
 
+def test_single_tokens_need_no_hint(gpu):
+    """As many rows as sequences: taken for single tokens, whoever's they are."""
+    b = Batch(gpu, [(1, 900), (1, 5), (0, 30), (1, 300)], 128, 8, 2, 16, BF, tail=1)
+    q = b.randn(b.N, 8, 128)
+    o, lse = _attend(b, q)
+    hint = lv.paged_attention(q, b.cache, *b.call(), max_q_len=1, return_lse=True)
+    assert torch.equal(o, hint[0]) and torch.equal(lse, hint[1])
+    b = Batch(gpu, [(0, 7), (4, 700), (0, 0), (0, 30)], 128, 8, 2, 16, BF)      # all of one sequence
+    _attend(b, b.randn(b.N, 8, 128))
+
+
 @pytest.mark.parametrize("B", [65, 128, 1100, 4300])
 def test_many_sequences(gpu, B):
     """More sequences than a wave holds, than the plan takes at a time, and more row tiles than it keeps in LDS."""
@@ -788,7 +799,7 @@ def test_refusals(gpu):
         att(q, b.cache, cu[:1], lens, table)
     with pytest.raises(ValueError, match="kv_lens"):
         att(q, b.cache, cu, lens.repeat(2), table)
-    for scale in (0.0, -1.0, float("nan"), float("inf")):
+    for scale in (0.0, -1.0, 3e38, float("nan"), float("inf")):
         with pytest.raises(ValueError, match="scale"):
             att(q, b.cache, cu, lens, table, scale=scale)
     with pytest.raises(ValueError, match="share memory"):
