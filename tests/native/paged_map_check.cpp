@@ -5,7 +5,8 @@
 //   - no row, page-table entry or page outside what the caller allocated is
 //     named, whatever the device arrays hold;
 //   - the work-groups' shares cover every unit once, partial sums go to slots
-//     of their own, and decode_slots finds exactly those of a row tile.
+//     of their own, and decode_slots finds exactly those of a row tile;
+//   - quotient is the quotient.
 // Prints "paged map ok" and exits 0, or names the first failure.
 #include "lvsa_paged.h"
 
@@ -126,6 +127,15 @@ int main() {
       }
     }
   }
+  // quotients in 32 bits where both operands fit, in 64 elsewhere
+  int trial = 0;
+  for (; trial < 200000; ++trial) {
+    const int64_t x = upto((INT64_MAX >> 1) >> upto(61)), y = 1 + upto((INT64_MAX >> 1) >> upto(61));
+    CHECK(quotient(x, y) == x / y, "%lld / %lld", (long long)x, (long long)y);
+  }
+  for (int64_t x : {0xffffffffLL, 0x100000000LL, 0x100000001LL})
+    for (int64_t y : {1LL, 2LL, 0xffffffffLL, 0x100000000LL, 0x100000001LL})
+      CHECK(quotient(x, y) == x / y, "%lld / %lld", (long long)x, (long long)y);
   printf("paged map ok\n");
   return 0;
 }
