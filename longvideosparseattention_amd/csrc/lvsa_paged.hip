@@ -439,12 +439,17 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnParams p, int
 // ───────────────────────── plan of a prefill launch ────────────────────────
 
 // Sum over the work-group's 1024 threads before this one, and the total.
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* lds, int64_t* total) {
+// `count`: threads that may hold anything but 0.
+__device__ __forceinline__ int64_t block_scan(int64_t x, int count, int64_t* lds, int64_t* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t incl = wave_scan(x, lane);
+  const int64_t incl = wave_scan(x, lane, count);
   __syncthreads();
-  if (lane == 63) lds[wave] = incl;
+  if (lane == (count < 64 ? count - 1 : 63)) lds[wave] = incl;
   __syncthreads();
+  if (count <= 64) {                       // the first wave's
+    *total = lds[0];
+    return incl - x;
+  }
   int64_t before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < 16; ++w) {
@@ -457,8 +462,8 @@ __device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* lds, int64_t* 
 
 // One work-group: lists the row tiles with their key blocks, where the shares
 // end and what is to be joined there.  Latency only: two dependent reads of
-// memory, scans and searches in LDS (searches in memory past kPlanLds tiles); 7 to
-// 9 us beside launches of 30 us and more.  With it every work-group of those
+// memory, scans and searches in LDS (searches in memory past kPlanLds tiles); 6 to
+// 8 us beside launches of 25 us and more.  With it every work-group of those
 // gets the same number of key blocks, whatever the lengths, where tiles as units
 // leave the last round to a few (516 tiles on 256 CUs: three rounds for two
 // rounds' work).
@@ -468,6 +473,7 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int
   __shared__ int64_t before_s[kPlanLds];
   __shared__ PagedSeq seq_s[1024];
   __shared__ int64_t first_s[1024];                    // tiles before a sequence of the chunk
+  __shared__ PlanTile tile_s[1024];                    // the first tiles
   int64_t done = 0, units = 0;                          // tiles and units before this chunk of sequences
   for (int s0 = 0; s0 < p.c.B; s0 += 1024) {
     const int s = s0 + threadIdx.x, ns = p.c.B - s0 < 1024 ? p.c.B - s0 : 1024;
@@ -479,7 +485,7 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int
       nt = ((int64_t)q.n * p.group + rows - 1) / rows;
     }
     int64_t all;
-    const int64_t at = block_scan(nt, lds, &all);
+    const int64_t at = block_scan(nt, ns, lds, &all);
     first_s[threadIdx.x] = at;
     seq_s[threadIdx.x] = q;
     __syncthreads();
@@ -502,11 +508,12 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int
         w.units = w.blocks > 0 ? w.blocks : 1;
       }
       int64_t sum;
-      const int64_t u = units + block_scan(w.units, lds, &sum);
+      const int64_t u = units + block_scan(w.units, all - t0 < 1024 ? (int)(all - t0) : 1024, lds, &sum);
       if (t < all) {
         p.plan_tiles[done + t] = w;
         p.before[done + t] = u;
         if (done + t < kPlanLds) before_s[done + t] = u;
+        if (done + t < 1024) tile_s[done + t] = w;
       }
       units += sum;
     }
@@ -523,7 +530,7 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int
   const bool in_lds = tiles <= kPlanLds;
   for (int w = threadIdx.x; w < shares; w += 1024) {
     const int64_t u = unit_start(U, shares, w + 1) - 1;
-    const int64_t h = u / units, rest = u - h * units;
+    const int64_t h = quotient(u, units), rest = u - h * units;
     int lo = 0, hi = tiles - 1;  // last tile with before <= rest
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -531,7 +538,7 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int
       else hi = mid - 1;
     }
     const int64_t b = in_lds ? before_s[lo] : p.before[lo];
-    const PlanTile tile = p.plan_tiles[lo];
+    const PlanTile tile = lo < 1024 ? tile_s[lo] : p.plan_tiles[lo];
     const int blk = (int)(rest - b) + 1;
     p.ends[w] = PlanEnd{(int)h, lo, blk, 0};
     // a tile that shares divide is joined by the one it starts in
