@@ -362,8 +362,8 @@ LVSA_API int lvsa_paged_gather(const lvsa_paged_cache* cache, const lvsa_paged_b
  * [N, H], contiguous) its natural log-sum-exp; a row without keys gets 0 and
  * -inf, a row of a sequence with a bad page or length NaN.  Keys
  * that a row does not attend have no effect on it, infinities and NaN
- * included.  Rows of no sequence are zeroed (lse -inf) if `fill_tail`, else
- * left as they are.  `max_q_len` and `max_kv_len` (0: unknown) only choose a kernel and its
+ * included.  Rows of no sequence: `fill_tail` 1 zeroes them (lse -inf), 2 writes
+ * their lse alone, 0 leaves both as they are.  `max_q_len` and `max_kv_len` (0: unknown) only choose a kernel and its
  * split; results hold whatever they say.  Workspace: device memory of
  * lvsa_paged_attn_workspace_query bytes, 16-byte aligned, any contents,
  * not shared by calls that overlap.                                          */

@@ -368,7 +368,8 @@ __device__ __forceinline__ void merge_row(const PagedAttnParams& p, int row, int
   }
   if (s < 0) {
     if (p.fill_tail) {
-      for (int d = threadIdx.x; d < D; d += 256) out[d] = (E)0.f;
+      if (p.fill_tail == 1)
+        for (int d = threadIdx.x; d < D; d += 256) out[d] = (E)0.f;
       if (lse && threadIdx.x == 0) *lse = -__builtin_inff();
     }
     return;

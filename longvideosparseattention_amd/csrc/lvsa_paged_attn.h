@@ -597,7 +597,7 @@ __global__ __launch_bounds__(256, D == 256 || (D == 192 && NT == 2) ? 1 : paged_
 
 // ─────────────────────────────── prefill ───────────────────────────────────
 
-// Rows before the first and behind the last sequence: 0 and -inf.
+// Rows before the first and behind the last sequence: 0 (fill_tail 1) and -inf.
 __device__ __forceinline__ void fill_tail_rows(const PagedAttnParams& p, int D, int lane, int wave, int waves) {
   const int head = p.c.cu[0] < 0 ? 0 : p.c.cu[0] > p.c.N ? p.c.N : p.c.cu[0];
   const int tail = p.c.cu[p.c.B] < head ? head : p.c.cu[p.c.B] > p.c.N ? p.c.N : p.c.cu[p.c.B];
@@ -605,7 +605,8 @@ __device__ __forceinline__ void fill_tail_rows(const PagedAttnParams& p, int D, 
   const int64_t wg = blockIdx.x, wgs = gridDim.x;
   for (int64_t i = wg * waves + wave; i < n; i += waves * wgs) {
     const int64_t r = i / p.H, hq = i - r * p.H, t = r < head ? r : tail + (r - head);
-    for (int d = lane; d < D; d += 64) reinterpret_cast<uint16_t*>(p.o + t * p.o_str[0] + hq * p.o_str[1])[d] = 0;
+    if (p.fill_tail == 1)
+      for (int d = lane; d < D; d += 64) reinterpret_cast<uint16_t*>(p.o + t * p.o_str[0] + hq * p.o_str[1])[d] = 0;
     if (p.lse && lane == 0) p.lse[t * p.H + hq] = -__builtin_inff();
   }
 }

@@ -397,7 +397,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, cu_seqlens: torch.Tens
     say.  Without ``max_q_len`` more rows than sequences are taken for one long
     sequence, which runs slower for a few rows of each.  ``out`` must not share memory with ``q``; rows of no
     sequence are left as they were in ``out`` and are 0 in a new tensor (``lse``:
-    ``-inf``).  Scores, softmax and sums are fp32; weights enter the second product
+    ``-inf`` in both cases).  Scores, softmax and sums are fp32; weights enter the second product
     in ``q``'s type."""
     dtype = q.dtype if isinstance(q, torch.Tensor) else None
     packed = cache._pack(dtype)
@@ -419,7 +419,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, cu_seqlens: torch.Tens
         a = capi.PagedAttnArgs()
         C.memmove(C.addressof(a), packed + batch, _ATTN_AT)
         head = (q_ptr, o_ptr, 0 if lse is None else lse.data_ptr(), *q_str, *o_str, scale, H, int(bool(causal)),
-                int(fresh), min(mq, 0x7fffffff), min(mk, 0x7fffffff))
+                1 if fresh else 2, min(mq, 0x7fffffff), min(mk, 0x7fffffff))
         _ATTN.pack_into(a, _ATTN_AT, *head, 0, 0)
         need = _workspace_bytes(a, (cache.device.index, cache.bits, D, cache.num_kv_heads, cache.page_size, N, H, *page_table.shape,
                                     mq, mk), cache.device)
