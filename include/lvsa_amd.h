@@ -335,7 +335,8 @@ typedef struct lvsa_paged_batch {
  * cache) names another row.  The first `rot` dimensions turn (a multiple of 16):
  * (a, b) -> (a cos - b sin, b cos + a sin) with pairs (2i, 2i + 1) if
  * `interleaved`, else (i, i + rot / 2).  Tokens with a bad page, length, row range or
- * position are not written, and their q_out is NaN.  Two tokens of a call must
+ * position are not written, and their q_out is NaN (a row that several ranges
+ * hold is the first one's).  Two tokens of a call must
  * not share a slot.  The reference has neither cache nor rotation here: its
  * adapters rotate Q and K before the attention call (lvsa/rope.py:10-27).     */
 typedef struct lvsa_paged_append_args {
@@ -360,7 +361,8 @@ LVSA_API int lvsa_paged_gather(const lvsa_paged_cache* cache, const lvsa_paged_b
  * of Hkv), row at position p attends its sequence's keys below kv_lens and, if
  * `causal`, up to p.  o = sum_j softmax_j(scale q.k_j) v_j, lse (optional,
  * [N, H], contiguous) its natural log-sum-exp; a row without keys gets 0 and
- * -inf, a row of a sequence with a bad page or length NaN.  Keys
+ * -inf, a row of a sequence with a bad page or length NaN, and so is every row
+ * of o and lse where cu_seqlens does not ascend within [0, N].  Keys
  * that a row does not attend have no effect on it, infinities and NaN
  * included.  Rows of no sequence: `fill_tail` 1 zeroes them (lse -inf), 2 writes
  * their lse alone, 0 leaves both as they are.  `max_q_len` and `max_kv_len` (0: unknown) only choose a kernel and its

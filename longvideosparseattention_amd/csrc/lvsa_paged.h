@@ -42,6 +42,7 @@ struct PagedSeq {
 struct PlanHead {
   int64_t per_head;              // units of one key head
   int32_t tiles, shares;
+  int32_t bad_cu, pad;           // the row ranges do not ascend within the rows: the whole result is NaN
 };
 struct PlanTile {
   int32_t seq, r0, units, blocks;
@@ -238,8 +239,8 @@ __device__ __forceinline__ void paged_flag(const PagedView& c, int bit) {
   if (c.status) atomicOr(c.status, bit);
 }
 
-// The sequence that row t belongs to (the same for every lane of the wave; t
-// uniform), or -1.  Every lane reads one sequence, so that a batch of up to 64
+// The first sequence whose row range holds row t (the same for every lane of the
+// wave; t uniform), or -1.  Every lane reads one sequence, so that a batch of up to 64
 // costs one trip to memory.
 __device__ __forceinline__ int paged_seq_of_row(const PagedView& c, int t, int lane, PagedSeq* q) {
   for (int s0 = 0; s0 < c.B; s0 += 64) {

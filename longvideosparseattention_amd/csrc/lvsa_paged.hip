@@ -267,8 +267,16 @@ __device__ __forceinline__ void append_token(const AppendParams& p, int t) {
   }
 }
 
+// Reports row ranges that do not ascend within the rows, whether or not a row is
+// in them (a work-group beside the tokens', so that none of those waits for it).
+__device__ __forceinline__ void flag_row_ranges(const PagedView& c) {
+  for (int s = threadIdx.x; s < c.B; s += blockDim.x)
+    if (const int bad = paged_seq(c, s).flags & LVSA_PAGED_BAD_CU) paged_flag(c, bad);
+}
+
 template <int D, typename E, int BITS, int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendParams p) {
+  if (blockIdx.x == gridDim.x - 1) flag_row_ranges(p.c);
   for (int64_t t = blockIdx.x; t < p.c.N; t += gridDim.x) append_token<D, E, BITS, THREADS>(p, (int)t);
 }
 
@@ -333,8 +341,8 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(PagedView c, char* ko
 // 2^(m_i - M) l_i.  The four waves take the slots in turn, each with a running
 // maximum as in the attention itself, and are joined in their order, so results
 // do not depend on timing.  Rows whose tile one work-group of the decode kernel
-// did whole are written already.  Rows without keys and rows of no sequence are
-// this kernel's too.  Latency: the batch, the partials (two slots of a wave at a
+// did whole are written already.  Rows without keys, rows of no sequence and, as
+// NaN, all rows of a batch whose row ranges are bad are this kernel's too.  Latency: the batch, the partials (two slots of a wave at a
 // time, maxima and sums beside them), one exchange.
 template <typename E>
 __device__ __forceinline__ void merge_row(const PagedAttnParams& p, int row, int D, int rows, int keys,
@@ -346,6 +354,7 @@ __device__ __forceinline__ void merge_row(const PagedAttnParams& p, int row, int
   PagedSeq sq = {};
   int s = -1;
   int64_t U = 0, base = 0;
+  int flags = 0;
   for (int s0 = 0; s0 < B; s0 += 64) {
     PagedSeq q = {};
     int64_t n = 0;
@@ -355,6 +364,7 @@ __device__ __forceinline__ void merge_row(const PagedAttnParams& p, int row, int
       q = paged_seq(p.c, a, e, p.c.lens[s0 + lane]);
       n = decode_units(p, q, rows, keys);
       in = a <= t && t < e;
+      flags |= q.flags;
     }
     const int64_t incl = wave_scan(n, lane, B - s0);
     const uint64_t m = __builtin_amdgcn_ballot_w64(in);
@@ -365,6 +375,11 @@ __device__ __forceinline__ void merge_row(const PagedAttnParams& p, int row, int
       base = U + from_lane(incl - n, at);
     }
     U += from_lane(incl, B - s0 < 64 ? B - s0 - 1 : 63);
+  }
+  if (__builtin_amdgcn_ballot_w64(flags & LVSA_PAGED_BAD_CU)) {
+    for (int d = threadIdx.x; d < D; d += 256) out[d] = (E)__builtin_nanf("");
+    if (lse && threadIdx.x == 0) *lse = __builtin_nanf("");
+    return;
   }
   if (s < 0) {
     if (p.fill_tail) {
@@ -475,6 +490,9 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int
   __shared__ PagedSeq seq_s[1024];
   __shared__ int64_t first_s[1024];                    // tiles before a sequence of the chunk
   __shared__ PlanTile tile_s[1024];                    // the first tiles
+  __shared__ int bad_cu;
+  if (threadIdx.x == 0) bad_cu = 0;
+  __syncthreads();
   int64_t done = 0, units = 0;                          // tiles and units before this chunk of sequences
   for (int s0 = 0; s0 < p.c.B; s0 += 1024) {
     const int s = s0 + threadIdx.x, ns = p.c.B - s0 < 1024 ? p.c.B - s0 : 1024;
@@ -483,6 +501,7 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int
     if (s < p.c.B) {
       q = paged_seq(p.c, s);
       if (q.flags) paged_flag(p.c, q.flags);
+      if (q.flags & LVSA_PAGED_BAD_CU) bad_cu = 1;
       nt = ((int64_t)q.n * p.group + rows - 1) / rows;
     }
     int64_t all;
@@ -490,7 +509,7 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int
     first_s[threadIdx.x] = at;
     seq_s[threadIdx.x] = q;
     __syncthreads();
-    // row ranges that overlap give more tiles than the bound: the rest is dropped
+    // row ranges that overlap (bad ones) give more tiles than the bound: the rest is dropped
     if (done + all > p.tiles) all = p.tiles - done;
     for (int64_t t0 = 0; t0 < all; t0 += 1024) {
       const int64_t t = t0 + threadIdx.x;
@@ -526,8 +545,9 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int
   // a share for every tile, whatever its keys, where there are work-groups for it
   const int64_t whole = (int64_t)tiles * p.c.Hkv;
   const int least = U > 0 ? unit_shares(U, p.grid, kPagedLeast) : 0;
-  const int shares = whole <= least ? least : whole < p.grid ? (int)whole : p.grid;
-  if (threadIdx.x == 0) *p.head = PlanHead{units, tiles, shares};
+  // (none where the row ranges are bad: the launch then only spoils the result)
+  const int shares = bad_cu ? 0 : whole <= least ? least : whole < p.grid ? (int)whole : p.grid;
+  if (threadIdx.x == 0) *p.head = PlanHead{units, tiles, shares, bad_cu, 0};
   const bool in_lds = tiles <= kPlanLds;
   for (int w = threadIdx.x; w < shares; w += 1024) {
     const int64_t u = unit_start(U, shares, w + 1) - 1;
@@ -699,7 +719,7 @@ int by_type(int D, int dtype, int bits, A&&... a) {
 
 template <int D, typename E, int BITS> struct Append {
   static int go(const AppendParams& p, hipStream_t stream) {
-    const dim3 grid((unsigned)(p.c.N < kMaxGrid ? p.c.N : kMaxGrid));
+    const dim3 grid((unsigned)(p.c.N < kMaxGrid ? p.c.N : kMaxGrid) + 1);
     if (p.c.N <= kFewTokens * cu_count())
       hipLaunchKernelGGL((paged_append_kernel<D, E, BITS, 256>), grid, dim3(256), 0, stream, p);
     else

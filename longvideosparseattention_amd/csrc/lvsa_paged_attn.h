@@ -266,7 +266,7 @@ __global__ __launch_bounds__(256, D == 256 || (D == 192 && NT == 2) ? 1 : paged_
     U += from_lane(upto, B - s0 < 64 ? B - s0 - 1 : 63);
   }
   if (blockIdx.x == 0 && wave == 0 && flags) paged_flag(p.c, flags);
-  if (U == 0) return;
+  if (U == 0 || __builtin_amdgcn_ballot_w64(flags & LVSA_PAGED_BAD_CU)) return;   // bad row ranges: the merge spoils all rows
   const int shares = unit_shares(U, p.grid);
   if ((int)blockIdx.x >= shares) return;
   int64_t u = unit_start(U, shares, blockIdx.x);
@@ -611,6 +611,17 @@ __device__ __forceinline__ void fill_tail_rows(const PagedAttnParams& p, int D, 
   }
 }
 
+// All rows of a batch whose row ranges are bad: NaN.
+template <typename E>
+__device__ __forceinline__ void spoil_rows(const PagedAttnParams& p, int D, int lane, int wave, int waves) {
+  const int64_t n = (int64_t)p.c.N * p.H;
+  for (int64_t i = (int64_t)blockIdx.x * waves + wave; i < n; i += (int64_t)waves * gridDim.x) {
+    const int64_t t = i / p.H, hq = i - t * p.H;
+    for (int d = lane; d < D; d += 64) reinterpret_cast<E*>(p.o + t * p.o_str[0] + hq * p.o_str[1])[d] = (E)__builtin_nanf("");
+    if (p.lse && lane == 0) p.lse[i] = __builtin_nanf("");
+  }
+}
+
 // Share of a work-group.  Consecutive work-groups go to the eight XCDs in turn:
 // an XCD gets consecutive shares, few key heads' tiles, whose keys its L2 then
 // serves to all of them.
@@ -747,8 +758,12 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   const int half = lane >> 5, i32 = lane & 31;       // S^T: column (row of the tile) i32
   const int g = lane >> 4, x = lane & 15;
 
-  if (p.fill_tail) fill_tail_rows(p, D, lane, wave, 4);
   const PlanHead hd = *p.head;
+  if (uniform(hd.bad_cu)) {
+    spoil_rows<E>(p, D, lane, wave, 4);
+    return;
+  }
+  if (p.fill_tail) fill_tail_rows(p, D, lane, wave, 4);
   const int shares = uniform(hd.shares), share = share_of(blockIdx.x, shares);
   if (share < 0) return;
   // The share's tiles from the last to the first: the part that it ends with
@@ -1126,8 +1141,12 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
   const int half = lane >> 5, i32 = lane & 31;
   const int g = lane >> 4, x = lane & 15;
 
-  if (p.fill_tail) fill_tail_rows(p, D, lane, wave, 8);
   const PlanHead hd = *p.head;
+  if (uniform(hd.bad_cu)) {
+    spoil_rows<E>(p, D, lane, wave, 8);
+    return;
+  }
+  if (p.fill_tail) fill_tail_rows(p, D, lane, wave, 8);
   const int shares = uniform(hd.shares), share = share_of(blockIdx.x, shares);
   if (share < 0) return;
   // The share's tiles from the last to the first: the part that it ends with

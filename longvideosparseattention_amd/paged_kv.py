@@ -27,7 +27,10 @@ What the host cannot see is checked on the device: page numbers outside the
 cache, lengths beyond the table, row ranges outside the batch and positions
 outside the angle table never leave the caller's memory.  They spoil the rows
 they concern (NaN; an append leaves such tokens out) and set the cache's status,
-which :meth:`PagedKVCache.check` turns into an error.
+which :meth:`PagedKVCache.check` turns into an error.  Where ``cu_seqlens`` does
+not ascend within the packed rows, nobody knows whose rows are whose: attention
+returns NaN in every row, an append takes a row for the first sequence whose
+range holds it.
 
 The reference has no cache: it attends over whole tensors
 (``lvsa/sparse_attention.py:643-706``) that its adapters have rotated before

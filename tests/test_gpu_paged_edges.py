@@ -31,3 +31,68 @@ def test_lse_of_rows_of_no_sequence_beside_out(gpu, n, room):
     lv.paged_attention(q, b.cache, *b.call(), max_q_len=n, out=out.fill_(3.0))
     assert (out[b.n_rows:] == 3.0).all() and torch.equal(out[:b.n_rows], want[0][:b.n_rows])
     b.cache.check()
+
+
+# ── row ranges that do not ascend within the rows ────────────────────────────
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("D,n,room", [(128, 1, 0), (128, 20, 0), (64, 60, ROOM), (128, 150, ROOM), (256, 60, ROOM)])
+def test_bad_row_ranges_spoil_the_whole_result(gpu, D, n, room, bits):
+    """Which rows are whose is unknown: every row is NaN, none is left unwritten, with the caller's result or a new one."""
+    b = Batch(gpu, [(n, 150), (n, 160), (n, 153)], D, 4, 2, 16, BF, bits=bits, extra_columns=room // 16)
+    q = b.randn(b.N, 4, D)
+    good = lv.paged_attention(q, b.cache, *b.call(), max_q_len=n, return_lse=True)
+    big = 2 ** 31 - 1
+    for cu in ([0, n, 2 * n, 3 * n + 50], [0, 2 * n, n, 3 * n], [-5, n, 2 * n, 3 * n], [0, n, big, 3 * n], [0, 3 * n, 0, 3 * n],
+               [3 * n, 0, 3 * n, 0], [2 * n, n, -1, 0], [-2 ** 31, big, -2 ** 31, big], [big, big, big, big], [0, 3 * n, n, n]):
+        cu_dev = torch.tensor(cu, dtype=torch.int32, device=gpu)
+        for out in (None, torch.zeros_like(q)):
+            o, lse = lv.paged_attention(q, b.cache, cu_dev, b.lens, b.table_dev, max_q_len=n, out=out, return_lse=True)
+            assert torch.isnan(o).all() and torch.isnan(lse).all(), cu
+            with pytest.raises(ValueError, match="cu_seqlens"):
+                b.cache.check()
+    o, lse = lv.paged_attention(q, b.cache, *b.call(), max_q_len=n, return_lse=True)
+    assert torch.equal(o, good[0]) and torch.equal(lse, good[1])
+    b.cache.check()
+
+
+@pytest.mark.parametrize("where", [3, 70, 199])
+@pytest.mark.parametrize("room", [0, ROOM])
+def test_a_bad_row_range_among_many_sequences(gpu, room, where):
+    """Of 200 sequences one range descends, in whichever 64 of them: the same."""
+    B = 200
+    b = Batch(gpu, [(1, 5 + i % 9) for i in range(B)], 64, 2, 1, 8, BF, extra_columns=min(room, 20000) // 8)
+    q = b.randn(b.N, 2, 64)
+    kw = {"max_q_len": 100} if room else {"max_q_len": 1}
+    cu = b.cu.clone()
+    cu[where + 1] = cu[where] - 1 if where < B - 1 else b.N + 1
+    o, lse = lv.paged_attention(q, b.cache, cu, b.lens, b.table_dev, return_lse=True, **kw)
+    assert torch.isnan(o).all() and torch.isnan(lse).all()
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        b.cache.check()
+
+
+@pytest.mark.parametrize("B,where", [(3, 1), (150, 10), (150, 100), (150, 149)])
+def test_an_append_reports_every_bad_row_range(gpu, B, where):
+    """A descending range without rows of its own is reported too; rows are the first sequence's that holds them."""
+    b = Batch(gpu, [(2, 8)] * B, 64, 1, 1, 8, BF)
+    k, v, q = b.randn(b.N, 1, 64), b.randn(b.N, 1, 64), b.randn(b.N, 1, 64)
+    cu = b.cu.clone()
+    cu[where + 1] = cu[where] - 1 if where < B - 1 else 2 ** 31 - 1
+    before = b.cache.k.clone()
+    qo = lv.paged_kv_append(b.cache, k, v, cu, b.lens, b.table_dev, q=q)
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        b.cache.check()
+    host = cu.tolist()
+    for t in range(b.N):
+        s = next((s for s in range(B) if host[s] <= t < host[s + 1]), None)
+        if s is None:
+            continue
+        if host[s + 1] > b.N:                             # its own range is bad: left out
+            assert torch.isnan(qo[t]).all()
+            page = b.pages[s][0]
+            assert torch.equal(b.cache.k[page].nan_to_num(3.0), before[page].nan_to_num(3.0))
+        else:
+            slot = 8 - (host[s + 1] - host[s]) + t - host[s]
+            assert torch.equal(b.cache.k[b.pages[s][0], slot], k[t]) and torch.equal(qo[t], q[t])
