@@ -55,7 +55,8 @@ template <>
 struct Mat<__bf16> {
   typedef __bf16 v8 __attribute__((ext_vector_type(8)));
   typedef __bf16 v2 __attribute__((ext_vector_type(2)));
-  static constexpr uint32_t kExp = 0x7f80u, kOne = 0x3f80u;
+  static constexpr uint32_t kExp = 0x7f80u;
+  static constexpr uint32_t kFinite = 252;    // largest scale byte that leaves every 4-bit value finite: 6 * 2^125
   __device__ static floatx4 mfma16(shortx8 a, shortx8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
   }
@@ -75,7 +76,8 @@ struct Mat<_Float16> {
   typedef _Float16 v8 __attribute__((ext_vector_type(8)));
   typedef _Float16 v4 __attribute__((ext_vector_type(4)));
   typedef _Float16 v2 __attribute__((ext_vector_type(2)));
-  static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u;
+  static constexpr uint32_t kExp = 0x7c00u;
+  static constexpr uint32_t kFinite = 140;    // 6 * 2^13
   __device__ static floatx4 mfma16(shortx8 a, shortx8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
   }
@@ -141,7 +143,9 @@ __device__ __forceinline__ bool any_nonfinite(shortx8 x) {
 // their way into LDS, and the matrix product runs on zeros in their place
 // (finite8).  Where any were found, they are added at the end, from memory, to
 // the rows that attend them (add_nonfinite): no sum of finite terms changes an
-// infinity or a NaN, so the order does not matter.
+// infinity or a NaN, so the order does not matter.  4-bit values count as the
+// 16-bit numbers they are decoded to: infinities too where a caller's scale
+// takes them past the type's range.
 template <typename E>
 __device__ __forceinline__ shortx8 finite8(shortx8 x) {
 #pragma unroll
@@ -172,8 +176,10 @@ __device__ __forceinline__ void add_nonfinite_keys(const PagedView& c, const int
       if constexpr (BITS == 16) {
         v = *reinterpret_cast<const u32x2*>(row + 2 * d);
       } else {
-        const bool nan = c.vs[at.page * c.vs_str[0] + at.slot * c.vs_str[1] + h * c.vs_str[2] + d / 32] == 255;
-        v = nan ? u32x2{0x7fff7fffu, 0x7fff7fffu} : u32x2{0u, 0u};
+        const uint32_t codes = *reinterpret_cast<const uint16_t*>(row + d / 2);
+        const uint32_t sb = c.vs[at.page * c.vs_str[0] + at.slot * c.vs_str[1] + h * c.vs_str[2] + d / 32];
+        const float s = __builtin_bit_cast(float, sb << 23);
+        v = u32x2{Mat<E>::template decode<0>(codes, s), Mat<E>::template decode<1>(codes, s)};
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) o(q, r, (v[r >> 1] >> (16 * (r & 1))) & 0xffffu, seen);
@@ -858,8 +864,8 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
       const bool up = kTwoScales && ((D / 4) * g + 8 * i) / 32 != (D / 4) * g / 32;
       const uint32_t sb = up ? c.s[1] : c.s[0];
       shortx8 w = decode8<E>(c.w[i], sb);
-      if (masked && sb == 255) {                        // NaN: see finite8
-        w = shortx8{0};
+      if (masked && sb > Mat<E>::kFinite && any_nonfinite<E>(w)) {
+        w = finite8<E>(w);
         odd_s = 1;
       }
       *reinterpret_cast<lds8*>(to + prefill_chunk<D>(x, ND * g + i)) = w;
@@ -1258,8 +1264,8 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
       const bool up = kTwoScales && ((D / 4) * g + 8 * i) / 32 != (D / 4) * g / 32;
       const uint32_t sb = up ? c.s[1] : c.s[0];
       shortx8 w = decode8<E>(c.w[i], sb);
-      if (masked && sb == 255) {                        // NaN: see finite8
-        w = shortx8{0};
+      if (masked && sb > Mat<E>::kFinite && any_nonfinite<E>(w)) {
+        w = finite8<E>(w);
         odd_s = 1;
       }
       *reinterpret_cast<lds8*>(ring + stage * MAT + prefill_chunk<D>(x, ND * g + i)) = w;

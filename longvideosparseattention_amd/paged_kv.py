@@ -96,7 +96,9 @@ class PagedKVCache:
     4 bits: ``uint8 [pages, page_size, H_kv, D / 2]`` codes (element ``d`` in byte
     ``d // 2``, the low four bits for even ``d``) and ``k_scale`` / ``v_scale``,
     ``uint8 [pages, page_size, H_kv, D / 32]``: a value is its E2M1 number times
-    ``2^(scale - 127)``.  Strides are free as long as rows start at multiples of
+    ``2^(scale - 127)`` (scale 255: NaN) as the caller's 16-bit type holds it, which
+    is exactly, for every scale that an append writes, and as an infinity beyond
+    its range.  Strides are free as long as rows start at multiples of
     16 bytes; :meth:`allocate` lays the rows of a head within a page next to each
     other, which reads fastest.  Two caches may share pages of one allocation.
     """

@@ -96,3 +96,41 @@ def test_an_append_reports_every_bad_row_range(gpu, B, where):
         else:
             slot = 8 - (host[s + 1] - host[s]) + t - host[s]
             assert torch.equal(b.cache.k[b.pages[s][0], slot], k[t]) and torch.equal(qo[t], q[t])
+
+
+# ── 4-bit values beyond the range of 16 bits ─────────────────────────────────
+
+
+@pytest.mark.parametrize("dtype,byte", [(HF, 141), (HF, 143), (HF, 254), (BF, 253), (BF, 254)])
+@pytest.mark.parametrize("n,D,room", [(4, 128, 0), (20, 192, 0), (60, 64, ROOM), (60, 256, ROOM), (150, 96, ROOM), (150, 64, ROOM),
+                                      (150, 128, ROOM), (150, 192, ROOM)])
+def test_4_bit_values_beyond_the_types_range(gpu, n, D, room, dtype, byte):
+    """Scales whose larger values the queries' type holds as infinities (as the gather returns them): without effect on
+    rows that do not attend the key, in the result of those that do."""
+    L = n + 60
+    b = Batch(gpu, [(n, L)], D, 2, 1, 16, dtype, bits=4, extra_columns=room // 16)
+    q = b.randn(n, 2, D)
+    b.V[0] *= 0.25                                        # no sums of its own beyond the type's range
+    b.cache.v_scale.copy_(torch.where(b.cache.v_scale == 255, 255, b.cache.v_scale - 2))
+    clean, _ = lv.paged_attention(q, b.cache, *b.call(), max_q_len=n, return_lse=True)
+    where = L - n + n // 2                                # attended from row n / 2 on
+    page, slot = b.pages[0][where // 16], where % 16
+    b.cache.v_scale[page, slot, 0, 1] = byte
+    codes = b.cache.v[page, slot, 0, 16:32].cpu()
+    codes[0], codes[1], codes[2] = 0x7F, 0x10, 0x02        # -6 and 6, 0 and 0.5, 1 and 0
+    b.cache.v[page, slot, 0, 16:32] = codes.to(gpu)
+    held = ref.dequantize(codes, torch.tensor([byte], dtype=torch.uint8)).to(dtype).double()
+    assert held[:2].isinf().all() and held[2] == 0
+    b.V[0][where, 0, 32:64] = held
+    kept, _ = lv.paged_kv_gather(b.cache, b.lens, b.table_dev, L, dtype=dtype)[::-1]
+    assert torch.equal(kept[0, where, 0, 32:64].double().cpu(), held)
+    o = lv.paged_attention(q, b.cache, *b.call(), max_q_len=n)
+    assert torch.equal(o[:n // 2], clean[:n // 2])
+    want, _, tol, _ = ref.attention(b, q)
+    inf = held.isinf()
+    got = o[n // 2:].double().cpu()
+    assert torch.equal(got[..., 32:64][..., inf], want[n // 2:, :, 32:64][..., inf])
+    rest = torch.ones(D, dtype=torch.bool)
+    rest[32:64] = held == 0                               # finite values of that scale: sums may leave the type's range
+    ref.check_close(got[..., rest], want[n // 2:][..., rest], tol[n // 2:][..., rest], "beside the infinities")
+    b.cache.check()
