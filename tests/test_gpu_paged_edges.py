@@ -134,3 +134,39 @@ def test_4_bit_values_beyond_the_types_range(gpu, n, D, room, dtype, byte):
     rest[32:64] = held == 0                               # finite values of that scale: sums may leave the type's range
     ref.check_close(got[..., rest], want[n // 2:][..., rest], tol[n // 2:][..., rest], "beside the infinities")
     b.cache.check()
+
+
+# ── weights far below their row's largest ────────────────────────────────────
+
+
+@pytest.mark.parametrize("dtype", [HF, BF])
+@pytest.mark.parametrize("gap", [8.0, 14.0, 16.0])
+@pytest.mark.parametrize("seqs,D,H,room", [([(1, 600)] * 40, 128, 8, 0), ([(2, 600)] * 40, 256, 8, 0), ([(20, 600)] * 30, 64, 8, 0),
+                                           ([(140, 900)] * 16, 64, 8, ROOM), ([(100, 900)] * 16, 128, 8, ROOM),
+                                           ([(100, 900)] * 12, 256, 8, ROOM)])
+def test_small_weights_beside_keys_far_above_them(gpu, seqs, D, H, room, gap, dtype):
+    """The keys that take nearly all the weight have values of 0, so the rest is the whole result.  Weights down to 2^-23 =
+    e^-15.94 of their row's largest keep half a step in both types; the smallest here, e^-16, are off by 1.06 of it, which
+    the reference's 2 * 664 fp32 roundings of the sums (0.16 of it) leave room for."""
+    L = seqs[0][1]
+    b = Batch(gpu, seqs, D, H, H, 64, dtype, extra_columns=room // 64)
+    g = torch.Generator().manual_seed(1)
+    K, V = torch.zeros(L, H, D), torch.randn(L, H, D, generator=g) + 1
+    K[:, :, 0] = 0.5 * torch.rand(L, H, generator=g)      # the others' weights: e^(0 .. 0.5 - gap)
+    tops = [7, 39, 71, 103]                               # one for each wave of a step
+    K[tops, :, 0], V[tops] = gap, 0.0
+    for t, x, mine in ((b.cache.k, K, b.K), (b.cache.v, V, b.V)):
+        host = torch.zeros(t.shape, dtype=dtype)
+        for s in range(len(seqs)):
+            b._put(host, s, x.to(dtype))
+            mine[s] = x.to(dtype).double()
+        t.copy_(host)
+    q = torch.zeros(b.N, H, D, dtype=dtype, device=gpu)
+    q[:, :, 0] = 1
+    o, lse = lv.paged_attention(q, b.cache, *b.call(), scale=1.0, max_q_len=seqs[0][0], return_lse=True)
+    wo, wl, tol, ltol = ref.attention(b, q, True, 1.0)
+    # The results are down to 2e-5.  fp16 has normal numbers from 2^-14 = 6e-5 on; below, they are multiples of 2^-24, and
+    # rounding to them is off by up to 2^-25, which the reference's relative half step (2^-11 of the value) is less than.
+    ref.check_close(o, wo, tol + (2.0 ** -25 if dtype == HF else 0.0), "attention")
+    ref.check_close(lse, wl, ltol, "lse")
+    b.cache.check()
