@@ -361,12 +361,13 @@ LVSA_API int lvsa_paged_gather(const lvsa_paged_cache* cache, const lvsa_paged_b
  * of Hkv), row at position p attends its sequence's keys below kv_lens and, if
  * `causal`, up to p.  o = sum_j softmax_j(scale q.k_j) v_j, lse (optional,
  * [N, H], contiguous) its natural log-sum-exp; a row without keys gets 0 and
- * -inf, a row of a sequence with a bad page or length NaN, and so is every row
- * of o and lse where cu_seqlens does not ascend within [0, N].  Keys
- * that a row does not attend have no effect on it, infinities and NaN
- * included.  Rows of no sequence: `fill_tail` 1 zeroes them (lse -inf), 2 writes
- * their lse alone, 0 leaves both as they are.  `max_q_len` and `max_kv_len` (0: unknown) only choose a kernel and its
- * split; results hold whatever they say.  Workspace: device memory of
+ * -inf.  NaN: all rows of a sequence with a bad length, or a bad page among its
+ * kv_lens tokens' (attended by the row or not), and every row of o and lse where
+ * cu_seqlens does not ascend within [0, N].  Keys that a row does not attend have
+ * no effect on it, infinities and NaN included.  Rows of no sequence: `fill_tail`
+ * 1 zeroes them (lse -inf), 2 writes their lse alone, 0 leaves both as they are.
+ * `max_q_len` and `max_kv_len` (0: unknown) only choose a kernel and its split;
+ * results hold whatever they say.  Workspace: device memory of
  * lvsa_paged_attn_workspace_query bytes, 16-byte aligned, any contents,
  * not shared by calls that overlap.                                          */
 typedef struct lvsa_paged_attn_args {

@@ -483,6 +483,10 @@ __device__ __forceinline__ int64_t block_scan(int64_t x, int count, int64_t* lds
 // gets the same number of key blocks, whatever the lengths, where tiles as units
 // leave the last round to a few (516 tiles on 256 CUs: three rounds for two
 // rounds' work).
+//
+// A bad page spoils its whole sequence, but a causal tile does not look behind its
+// last row's key: the plan looks through the pages of the rows of every tile but a
+// sequence's first (8 threads each) and marks the tiles before one with a bad page.
 constexpr int kPlanLds = 4096;
 __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int rows) {
   __shared__ int64_t lds[16];
@@ -571,6 +575,18 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int
       j = PlanJoin{d.first, d.rest, d.count, (int)h, tile.r0, left < rows ? left : rows, tile.sq.t0, {0, 0, 0}};
     }
     p.joins[w] = j;
+  }
+  for (int i = (1023 - threadIdx.x) >> 3; p.causal && i < tiles; i += 128) {   // from the threads without shares on
+    const PlanTile w = i < 1024 ? tile_s[i] : p.plan_tiles[i];
+    const int left = w.sq.n * p.group - w.r0, r1 = w.r0 + (left < rows ? left : rows) - 1;
+    const int k0 = key_limit(p, w.sq, w.r0), k1 = key_limit(p, w.sq, r1);
+    if (w.r0 == 0 || k1 == 0) continue;
+    const int32_t* table = p.c.table + w.seq * p.c.table_str;
+    bool bad = false;
+    for (int e = page_of(p.c, k0 > 0 ? k0 - 1 : 0) + (threadIdx.x & 7); e <= page_of(p.c, k1 - 1); e += 8)
+      bad |= (uint32_t)table[e] >= (uint32_t)p.c.n_pages;
+    for (int k = i - 1; bad && k >= 0 && p.plan_tiles[k].seq == w.seq; --k)
+      p.plan_tiles[k].sq.flags = w.sq.flags | LVSA_PAGED_BAD_PAGE;
   }
 }
 

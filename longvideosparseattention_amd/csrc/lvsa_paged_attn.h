@@ -819,7 +819,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   auto key_pos = [&](int b, int key) __attribute__((always_inline)) {
     return key_within(b * kPagedBlock + 16 * wave + key, sq.L);
   };
-  bool bad = (sq.flags & LVSA_PAGED_BAD_LENGTH) != 0;
+  bool bad = (sq.flags & (LVSA_PAGED_BAD_LENGTH | LVSA_PAGED_BAD_PAGE)) != 0;
   auto row_of = [&](int b, int key, int page, int64_t& pg, int64_t& slot) __attribute__((always_inline)) {
     const PagedRow at = paged_row(p.c, key_pos(b, key), page);
     bad |= !at.ok;
@@ -1199,7 +1199,7 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
   auto key_pos = [&](int j, int key) __attribute__((always_inline)) {
     return key_within((blk0 + j) * kPagedBlock + 16 * dw + key, sq.L);
   };
-  bool bad = (sq.flags & LVSA_PAGED_BAD_LENGTH) != 0;
+  bool bad = (sq.flags & (LVSA_PAGED_BAD_LENGTH | LVSA_PAGED_BAD_PAGE)) != 0;
   auto row_at = [&](int j, int key, int page, int64_t& sc) __attribute__((always_inline)) {
     const PagedRow at = paged_row(p.c, key_pos(j, key), page);
     bad |= !at.ok;

@@ -25,9 +25,10 @@ batch).  Every call only enqueues work on the current stream.
 
 What the host cannot see is checked on the device: page numbers outside the
 cache, lengths beyond the table, row ranges outside the batch and positions
-outside the angle table never leave the caller's memory.  They spoil the rows
-they concern (NaN; an append leaves such tokens out) and set the cache's status,
-which :meth:`PagedKVCache.check` turns into an error.  Where ``cu_seqlens`` does
+outside the angle table never leave the caller's memory.  They spoil what they
+concern — attention's rows of that sequence, gathered tokens (NaN), an append's
+tokens (left out) — and set the cache's status, which
+:meth:`PagedKVCache.check` turns into an error.  Where ``cu_seqlens`` does
 not ascend within the packed rows, nobody knows whose rows are whose: attention
 returns NaN in every row, an append takes a row for the first sequence whose
 range holds it.

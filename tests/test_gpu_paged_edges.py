@@ -170,3 +170,41 @@ def test_small_weights_beside_keys_far_above_them(gpu, seqs, D, H, room, gap, dt
     ref.check_close(o, wo, tol + (2.0 ** -25 if dtype == HF else 0.0), "attention")
     ref.check_close(lse, wl, ltol, "lse")
     b.cache.check()
+
+
+# ── pages of keys that some rows do not attend ───────────────────────────────
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("D,n,room", [(64, 700, ROOM), (128, 700, ROOM), (128, 100, ROOM), (192, 700, ROOM), (256, 400, ROOM),
+                                      (64, 300, 0)])
+@pytest.mark.parametrize("at", ["near", "far", "last"])
+def test_a_bad_page_spoils_all_rows_of_its_sequence(gpu, at, D, n, room, bits):
+    """Also those of a causal chunk that come before the page's keys, however far before."""
+    ps = 16
+    b = Batch(gpu, [(70, 90), (n, n + 5), (40, 333)], D, 2, 1, ps, BF, bits=bits, extra_columns=room // ps)
+    q = b.randn(b.N, 2, D)
+    good, glse = lv.paged_attention(q, b.cache, *b.call(), return_lse=True)
+    assert not torch.isnan(good).any()
+    key = {"near": 5 + (130 if n > 200 else 70), "far": n - 40, "last": n + 4}[at]
+    b.table_dev[1, key // ps] = b.cache.num_pages
+    o, lse = lv.paged_attention(q, b.cache, *b.call(), return_lse=True)
+    assert torch.isnan(o[70:70 + n]).all() and torch.isnan(lse[70:70 + n]).all()
+    assert torch.equal(o[:70], good[:70]) and torch.equal(o[70 + n:], good[70 + n:])
+    assert torch.equal(lse[:70], glse[:70]) and torch.equal(lse[70 + n:], glse[70 + n:])
+    with pytest.raises(ValueError, match="page number"):
+        b.cache.check()
+
+
+@pytest.mark.parametrize("room", [0, ROOM])
+def test_a_bad_page_behind_rows_without_keys(gpu, room):
+    """More rows than cached keys: rows before the first cached position are spoiled like the rest of their sequence."""
+    b = Batch(gpu, [(300, 40), (90, 90)], 128, 1, 1, 8, BF, extra_columns=room // 8)
+    q = b.randn(b.N, 1, 128)
+    o = lv.paged_attention(q, b.cache, *b.call())
+    assert (o[:260] == 0).all() and not torch.isnan(o).any()
+    b.table_dev[0, 4] = -1
+    o = lv.paged_attention(q, b.cache, *b.call())
+    assert torch.isnan(o[:300]).all() and not torch.isnan(o[300:]).any()
+    with pytest.raises(ValueError, match="page number"):
+        b.cache.check()
