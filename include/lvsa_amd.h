@@ -294,8 +294,8 @@ LVSA_API int lvsa_gather_frames(const void* src, const int64_t src_str[3], void*
  * d; strides in bytes) and, at k_scale with ks_str, one byte for every 32
  * elements: the scale 2^(byte - 127), 255 for a group of NaN.  Row addresses
  * are multiples of 16 bytes (the scales' of one).
- * `status` (optional, one int32, never cleared by a call): calls set
- * LVSA_PAGED_* bits in it for what they find on the device.                  */
+ * `status` (optional, one int32): calls set LVSA_PAGED_* bits in it for what they
+ * find on the device; lvsa_paged_take_status alone clears it.                */
 typedef struct lvsa_paged_cache {
   void* k; void* v;
   void* k_scale; void* v_scale;          /* 4 bits only                         */
@@ -349,6 +349,10 @@ typedef struct lvsa_paged_append_args {
   int32_t H, rot, interleaved, n_angles;
 } lvsa_paged_append_args;
 LVSA_API int lvsa_paged_append(const lvsa_paged_append_args* a, hipStream_t stream);
+
+/* Moves a cache's status word to `found` (one int32 of device memory) and leaves
+ * 0, in one step: bits that calls on other streams set meanwhile are not lost. */
+LVSA_API int lvsa_paged_take_status(int32_t* status, int32_t* found, hipStream_t stream);
 
 /* Reads every sequence's cached keys and values into k_out / v_out
  * [B, max_len, Hkv, D] (contiguous, in `dtype` of the cache struct); zeros

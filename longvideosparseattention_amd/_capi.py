@@ -165,6 +165,7 @@ SIGNATURES = {
                                      C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                      C.c_int32, C.c_void_p]),
     "lvsa_paged_append": (C.c_int, [C.POINTER(PagedAppendArgs), C.c_void_p]),
+    "lvsa_paged_take_status": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "lvsa_paged_gather": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedBatch), C.c_void_p, C.c_void_p, C.c_int32,
                                     C.c_void_p]),
     "lvsa_paged_attn_fwd": (C.c_int, [C.POINTER(PagedAttnArgs), C.c_void_p]),

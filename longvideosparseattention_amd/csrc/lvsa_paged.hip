@@ -650,6 +650,10 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(PagedAttnParams 
   }
 }
 
+// The status word, and 0 in its place: in one step, so that what a call of another
+// stream finds meanwhile stays for the next taker.
+__global__ void paged_take_status_kernel(int32_t* status, int32_t* found) { *found = atomicExch(status, 0); }
+
 // ─────────────────────────────── host side ─────────────────────────────────
 
 int cu_count() {
@@ -877,6 +881,14 @@ int lvsa_paged_append(const lvsa_paged_append_args* a, hipStream_t stream) {
   p.interleaved = a->interleaved;
   p.n_angles = a->n_angles;
   return by_type<Append>(a->cache.D, a->cache.dtype, a->cache.bits, p, stream);
+}
+
+int lvsa_paged_take_status(int32_t* status, int32_t* found, hipStream_t stream) {
+  clear_error();
+  const char* what = "lvsa_paged_take_status";
+  LVSA_REQUIRE(status && found, LVSA_ERR_INVALID_ARG, "%s: null pointer", what);
+  hipLaunchKernelGGL(paged_take_status_kernel, dim3(1), dim3(1), 0, stream, status, found);
+  return launch_status(what);
 }
 
 int lvsa_paged_gather(const lvsa_paged_cache* cache, const lvsa_paged_batch* batch, void* k_out, void* v_out,

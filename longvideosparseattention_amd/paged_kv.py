@@ -171,10 +171,13 @@ class PagedKVCache:
 
     def check(self) -> None:
         """Raise ``ValueError`` for what earlier calls found wrong on the device,
-        and forget it.  Waits for the device."""
-        found = int(self.status.item())
+        on whatever stream, and forget it.  Waits for the device; what calls
+        enqueued meanwhile find is the next check's."""
+        torch.cuda.synchronize(self.device)
+        taken = torch.empty_like(self.status)
+        hip_ops._call(self.device, "lvsa_paged_take_status", self.status.data_ptr(), taken.data_ptr())
+        found = int(taken.item())
         if found:
-            self.status.zero_()
             raise ValueError("paged cache: " + "; ".join(text for bit, text in _STATUS.items() if found & bit))
 
     def _pack(self, dtype: torch.dtype) -> bytes:

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import longvideosparseattention_amd as lv
+from longvideosparseattention_amd import _capi, hip_ops
 
 import paged_ref as ref
 from paged_ref import Batch
@@ -208,3 +209,39 @@ def test_a_bad_page_behind_rows_without_keys(gpu, room):
     assert torch.isnan(o[:300]).all() and not torch.isnan(o[300:]).any()
     with pytest.raises(ValueError, match="page number"):
         b.cache.check()
+
+
+# ── the cache's status ───────────────────────────────────────────────────────
+
+
+def test_check_waits_for_every_stream(gpu):
+    """A call that runs late on another stream is in the answer, and the answer is given once."""
+    b = Batch(gpu, [(1, 100)], 128, 4, 2, 16, BF)
+    q = b.randn(1, 4, 128)
+    bad = torch.full_like(b.table_dev, -1)
+    x = torch.randn(8192, 8192, device=gpu, dtype=BF)
+    torch.mm(x, x)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(40):                               # some 40 ms
+            torch.mm(x, x)
+        lv.paged_attention(q, b.cache, b.cu, b.lens, bad, max_q_len=1)
+    with pytest.raises(ValueError, match="page number"):
+        b.cache.check()
+    torch.cuda.synchronize()
+    b.cache.check()
+
+
+def test_check_takes_what_it_reports(gpu):
+    """What is found between the read and the end of a check is the next one's."""
+    b = Batch(gpu, [(1, 100)], 128, 4, 2, 16, BF)
+    b.cache.status.fill_(_capi.PAGED_BAD_PAGE | _capi.PAGED_BAD_POSITION)
+    found = torch.zeros(1, dtype=torch.int32, device=gpu)
+    hip_ops._call(gpu, "lvsa_paged_take_status", b.cache.status.data_ptr(), found.data_ptr())
+    b.cache.status.fill_(_capi.PAGED_BAD_LENGTH)
+    assert found.item() == _capi.PAGED_BAD_PAGE | _capi.PAGED_BAD_POSITION
+    with pytest.raises(ValueError) as e:
+        b.cache.check()
+    assert "kv_lens" in str(e.value) and "page number" not in str(e.value)
+    b.cache.check()
