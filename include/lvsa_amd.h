@@ -337,7 +337,8 @@ typedef struct lvsa_paged_batch {
  * `interleaved`, else (i, i + rot / 2).  Tokens with a bad page, length, row range or
  * position are not written, and their q_out is NaN (a row that several ranges
  * hold is the first one's).  Two tokens of a call must
- * not share a slot.  The reference has neither cache nor rotation here: its
+ * not share a slot.  q_out shares no memory with k, v and q (refused), and none of
+ * the four with the pages that the call writes.  The reference has neither cache nor rotation here: its
  * adapters rotate Q and K before the attention call (lvsa/rope.py:10-27).     */
 typedef struct lvsa_paged_append_args {
   lvsa_paged_cache cache;
@@ -371,7 +372,8 @@ LVSA_API int lvsa_paged_gather(const lvsa_paged_cache* cache, const lvsa_paged_b
  * no effect on it, infinities and NaN included.  Rows of no sequence: `fill_tail`
  * 1 zeroes them (lse -inf), 2 writes their lse alone, 0 leaves both as they are.
  * `max_q_len` and `max_kv_len` (0: unknown) only choose a kernel and its split;
- * results hold whatever they say.  Workspace: device memory of
+ * results hold whatever they say.  o shares no memory with q (refused), nor with
+ * the cache.  Workspace: device memory of
  * lvsa_paged_attn_workspace_query bytes, 16-byte aligned, any contents,
  * not shared by calls that overlap.                                          */
 typedef struct lvsa_paged_attn_args {

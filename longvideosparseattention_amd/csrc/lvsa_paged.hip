@@ -674,6 +674,18 @@ int cu_count() {
 
 bool aligned16(int64_t x) { return (x & 15) == 0; }
 
+// Whether two [N, heads, D] tensors of 16-bit elements (strides in bytes) lie within
+// each other's bounds.
+bool share_memory(const void* a, const int64_t* as, int ah, const void* b, const int64_t* bs, int bh, int N, int D) {
+  auto bound = [&](const void* at, const int64_t* str, int heads, bool high) {
+    int64_t x = (int64_t)(uintptr_t)at + (high ? 2 * (int64_t)D : 0);
+    const int64_t far[2] = {(N - 1) * str[0], (heads - 1) * str[1]};
+    for (int64_t f : far) x += high == (f > 0) ? f : 0;
+    return x;
+  };
+  return bound(a, as, ah, false) < bound(b, bs, bh, true) && bound(b, bs, bh, false) < bound(a, as, ah, true);
+}
+
 // Checks a cache and a batch and forms the device's view of them.
 int paged_view(const char* what, const lvsa_paged_cache* c, const lvsa_paged_batch* b, bool rows, PagedView* v) {
   LVSA_REQUIRE(c->D == 64 || c->D == 96 || c->D == 128 || c->D == 192 || c->D == 256, LVSA_ERR_UNSUPPORTED,
@@ -869,6 +881,11 @@ int lvsa_paged_append(const lvsa_paged_append_args* a, hipStream_t stream) {
                  LVSA_ERR_INVALID_ARG, "%s: rows must start at multiples of 16 bytes", what);
   }
   if (a->batch.N == 0 || a->batch.B == 0) return LVSA_OK;
+  // a half-split row's partners are read after other threads have written theirs
+  const int heads[3] = {a->cache.Hkv, a->cache.Hkv, a->H};
+  for (int i = 0; i < 3; ++i)
+    LVSA_REQUIRE(!a->q || !share_memory(a->q_out, p.qo_str, a->H, ptrs[i], outs[i], heads[i], a->batch.N, a->cache.D),
+                 LVSA_ERR_INVALID_ARG, "%s: q_out must not share memory with k, v and q", what);
   p.k = (const char*)a->k;
   p.v = (const char*)a->v;
   p.q = (const char*)a->q;
@@ -938,6 +955,8 @@ int lvsa_paged_attn_fwd(const lvsa_paged_attn_args* a, hipStream_t stream) {
                "%s: %lld bytes of 16-byte aligned workspace needed", what, (long long)need);
   LVSA_REQUIRE(need == 0 || a->workspace_bytes >= need, LVSA_ERR_CAPACITY, "%s: workspace of %lld bytes < %lld", what,
                (long long)a->workspace_bytes, (long long)need);
+  LVSA_REQUIRE(!share_memory(a->o, p.o_str, a->H, a->q, p.q_str, a->H, a->batch.N, a->cache.D), LVSA_ERR_INVALID_ARG,
+               "%s: o must not share memory with q", what);
   p.q = (const char*)a->q;
   p.o = (char*)a->o;
   p.lse = a->lse;

@@ -62,7 +62,7 @@ _STATUS = {
     capi.PAGED_BAD_POSITION: "a position outside the rows of cos and sin",
 }
 
-# The C structs as they are packed (see include/lvsa_amd.h): one pack_into per
+# The C structs as they are packed (see include/lvsa_amd.h): one copy per
 # call instead of a ctypes assignment per field.
 _CACHE = struct.Struct("@4P12q4i2iP")
 _BATCH = struct.Struct("@3Pq3i4x")
@@ -139,6 +139,8 @@ class PagedKVCache:
         if k.data_ptr() == v.data_ptr() or (k_scale is not None and k_scale.data_ptr() == v_scale.data_ptr()):
             raise ValueError("cache keys and values must not share memory")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._spans = [_span(t) for t in (k, v, k_scale, v_scale) if t is not None]
+        self._low, self._high = min(a for a, _ in self._spans), max(e for _, e in self._spans)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         ptrs = [0 if t is None else t.data_ptr() for t in (k, v, k_scale, v_scale)]
         self._packed = {
@@ -169,6 +171,11 @@ class PagedKVCache:
         return cls(rows(head_dim // 2, torch.uint8), rows(head_dim // 2, torch.uint8),
                    rows(head_dim // 32, torch.uint8), rows(head_dim // 32, torch.uint8))
 
+    def _holds(self, t: torch.Tensor) -> bool:
+        """Whether ``t`` lies within the bounds of the cache's tensors."""
+        lo, hi = _span(t)
+        return t.numel() > 0 and any(lo < e and a < hi for a, e in self._spans)
+
     def check(self) -> None:
         """Raise ``ValueError`` for what earlier calls found wrong on the device,
         on whatever stream, and forget it.  Waits for the device; what calls
@@ -190,7 +197,7 @@ class PagedKVCache:
 
 
 def _int32(t: torch.Tensor, name: str, dims: int, device: torch.device) -> None:
-    if isinstance(t, torch.Tensor) and t.dtype is _INT32 and t.dim() == dims and t.device == device and t.stride(-1) == 1:
+    if isinstance(t, torch.Tensor) and t.dtype is _INT32 and t.dim() == dims and t.get_device() == device.index and t.stride(-1) == 1:
         return
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         hip_ops._require_device(t, name)
@@ -232,7 +239,7 @@ def _tokens(t: torch.Tensor, name: str, heads: Optional[int], cache: PagedKVCach
         raise ValueError(f"{name} must be [N, {'H' if heads is None else heads}, {cache.head_dim}], got {tuple(shape)}")
     if t.dtype is not dtype:
         raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
-    if t.device != cache.device:
+    if t.get_device() != cache.device.index:
         raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient: the paged cache has no backward pass (detach it or use no_grad)")
@@ -245,7 +252,7 @@ def _tokens(t: torch.Tensor, name: str, heads: Optional[int], cache: PagedKVCach
     return t, ptr, s0, s1
 
 
-def _result(out: Optional[torch.Tensor], like: torch.Tensor, name: str, *inputs: torch.Tensor):
+def _result(out: Optional[torch.Tensor], like: torch.Tensor, name: str, cache: PagedKVCache, *inputs: torch.Tensor):
     """The tensor a call writes (``out``, or a new one) with its address and strides; ``inputs``: what else it reads."""
     if out is None:
         out = torch.empty_like(like, memory_format=torch.contiguous_format)
@@ -258,6 +265,8 @@ def _result(out: Optional[torch.Tensor], like: torch.Tensor, name: str, *inputs:
     for t in (like, *inputs):
         if t.numel() and _span(out)[0] < _span(t)[1] and _span(t)[0] < _span(out)[1]:
             raise ValueError(f"{name} must not share memory with the input")
+    if cache._holds(out):
+        raise ValueError(f"{name} must not share memory with the cache")
     N, H, D = out.shape
     a, b = sorted(((N, out.stride(0)), (H, out.stride(1))), key=lambda x: x[1])
     if (a[0] > 1 and a[1] < D) or (b[0] > 1 and b[1] < (a[1] * (a[0] - 1) if a[0] > 1 else 0) + D):
@@ -293,7 +302,9 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, cu_se
     ties to even; 32 values with an infinity or a NaN among them become NaN.
 
     Rows of no sequence are left alone, in the cache and in ``q_out`` (undefined
-    in a new tensor).  No two tokens of a call may have the same slot.  A token
+    in a new tensor).  No two tokens of a call may have the same slot.  ``k`` and
+    ``v`` may be views of the cache itself (they are copied first); ``q_out`` must
+    not share memory with the inputs or the cache.  A token
     with a bad page, length, row range or position is left out, its row of
     ``q_out`` NaN."""
     dtype = k.dtype if isinstance(k, torch.Tensor) else None
@@ -304,6 +315,11 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, cu_se
     N = k.shape[0]
     if v.shape[0] != N:
         raise ValueError(f"k has {N} tokens, v {v.shape[0]}")
+    # tokens that are the cache's own, whose slots the call may write: read before it
+    if k_ptr < cache._high and k_ptr + 2 * (N * k_str[0] + Hkv * k_str[1]) > cache._low and cache._holds(k):
+        k, k_ptr, *k_str = _tokens(k.clone(memory_format=torch.contiguous_format), "k", Hkv, cache, dtype)
+    if v_ptr < cache._high and v_ptr + 2 * (N * v_str[0] + Hkv * v_str[1]) > cache._low and cache._holds(v):
+        v, v_ptr, *v_str = _tokens(v.clone(memory_format=torch.contiguous_format), "v", Hkv, cache, dtype)
     batch = _batch(cache, cu_seqlens, kv_lens, page_table, N)
     H = q_ptr = qo_ptr = 0
     q_str = qo_str = (0, 0)
@@ -312,7 +328,7 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, cu_se
         H = q.shape[1]
         if q.shape[0] != N or H < 1:
             raise ValueError(f"k has {N} tokens, q {tuple(q.shape)}")
-        q_out, qo_ptr, *qo_str = _result(q_out, q, "q_out", k, v)
+        q_out, qo_ptr, *qo_str = _result(q_out, q, "q_out", cache, k, v)
     elif q_out is not None:
         raise ValueError("q_out without q")
     rot = angles = cos_ptr = sin_ptr = pos_ptr = 0
@@ -322,9 +338,9 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, cu_se
         for t, name in ((cos, "cos"), (sin, "sin")):
             if not isinstance(t, torch.Tensor) or not t.is_cuda:
                 hip_ops._require_device(t, name)
-            if t.dtype is not torch.float32 or t.dim() != 2 or not t.is_contiguous() or t.shape != cos.shape:
+            if t.dtype is not torch.float32 or t.dim() != 2 or not t.is_contiguous() or (t is not cos and t.shape != cos.shape):
                 raise TypeError(f"{name} must be a contiguous fp32 [positions, rot / 2] tensor like its partner")
-            if t.device != cache.device:
+            if t.get_device() != cache.device.index:
                 raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
         angles, rot = cos.shape
         rot *= 2
@@ -338,12 +354,11 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, cu_se
         if positions.shape[0] != N:
             raise ValueError(f"k has {N} tokens, positions {positions.shape[0]}")
         pos_ptr = positions.data_ptr()
-    a = capi.PagedAppendArgs()
-    C.memmove(C.addressof(a), packed + batch, _ATTN_AT)
     if N == 0:
         return q_out
-    _APPEND.pack_into(a, _ATTN_AT, k_ptr, v_ptr, q_ptr, qo_ptr, *k_str, *v_str, *q_str, *qo_str, cos_ptr, sin_ptr,
-                      pos_ptr, H, rot, int(bool(interleaved)), angles)
+    a = capi.PagedAppendArgs.from_buffer_copy(packed + batch + _APPEND.pack(
+        k_ptr, v_ptr, q_ptr, qo_ptr, *k_str, *v_str, *q_str, *qo_str, cos_ptr, sin_ptr, pos_ptr, H, rot,
+        int(bool(interleaved)), angles))
     hip_ops._call(cache.device, "lvsa_paged_append", C.byref(a))
     return q_out
 
@@ -404,7 +419,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, cu_seqlens: torch.Tens
     ``max_q_len`` (the most rows of a sequence) and ``max_kv_len`` (the longest
     cache) only choose a kernel and its split: results are right whatever they
     say.  Without ``max_q_len`` more rows than sequences are taken for one long
-    sequence, which runs slower for a few rows of each.  ``out`` must not share memory with ``q``; rows of no
+    sequence, which runs slower for a few rows of each.  ``out`` must not share memory with ``q`` or the cache; rows of no
     sequence are left as they were in ``out`` and are 0 in a new tensor (``lse``:
     ``-inf`` in both cases).  Scores, softmax and sums are fp32; weights enter the second product
     in ``q``'s type."""
@@ -419,17 +434,15 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, cu_seqlens: torch.Tens
         raise ValueError(f"scale {scale} must be positive and at most 2e38")
     batch = _batch(cache, cu_seqlens, kv_lens, page_table, N)
     fresh = out is None
-    out, o_ptr, *o_str = _result(out, q, "out")
+    out, o_ptr, *o_str = _result(out, q, "out", cache)
     lse = torch.empty(N, H, dtype=torch.float32, device=q.device) if return_lse else None
     if N:
         mq, mk = int(max_q_len or 0), int(max_kv_len or 0)
         if mq < 0 or mk < 0:
             raise ValueError(f"max_q_len {max_q_len} and max_kv_len {max_kv_len} must not be negative")
-        a = capi.PagedAttnArgs()
-        C.memmove(C.addressof(a), packed + batch, _ATTN_AT)
         head = (q_ptr, o_ptr, 0 if lse is None else lse.data_ptr(), *q_str, *o_str, scale, H, int(bool(causal)),
                 1 if fresh else 2, min(mq, 0x7fffffff), min(mk, 0x7fffffff))
-        _ATTN.pack_into(a, _ATTN_AT, *head, 0, 0)
+        a = capi.PagedAttnArgs.from_buffer_copy(packed + batch + _ATTN.pack(*head, 0, 0))
         need = _workspace_bytes(a, (cache.device.index, cache.bits, D, cache.num_kv_heads, cache.page_size, N, H, *page_table.shape,
                                     mq, mk), cache.device)
         if need:

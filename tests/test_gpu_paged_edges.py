@@ -245,3 +245,37 @@ def test_check_takes_what_it_reports(gpu):
         b.cache.check()
     assert "kv_lens" in str(e.value) and "page number" not in str(e.value)
     b.cache.check()
+
+
+# ── tensors that share memory ────────────────────────────────────────────────
+
+
+@pytest.mark.parametrize("layout", ["heads", "tokens"])
+@pytest.mark.parametrize("rot,inter", [(0, False), (128, False), (64, True)])
+def test_new_tokens_that_are_the_caches_own(gpu, rot, inter, layout):
+    """Keys and values taken from the pages that the call writes, each shifted by some slots: as from a copy of them."""
+    ps, Hkv, D, n = 64, 2, 128, 40
+    b = Batch(gpu, [(n, 70), (20, 30)], D, 4, Hkv, ps, BF, layout=layout)
+    cos, sin = (torch.rand(70, rot // 2, device=gpu) for _ in range(2))
+    kw = {"cos": cos, "sin": sin, "interleaved": inter} if rot else {}
+    page = b.pages[0][0]
+    b.cache.k.nan_to_num_(0.25)
+    b.cache.v.nan_to_num_(0.5)
+    k, v = b.cache.k[page, 2:62], b.cache.v[page, 1:61]                   # [60, Hkv, D] of the first page
+    want = [lv.PagedKVCache(b.cache.k.clone(), b.cache.v.clone())]
+    lv.paged_kv_append(want[0], k.clone(), v.clone(), *b.call(), **kw)
+    lv.paged_kv_append(b.cache, k, v, *b.call(), **kw)
+    assert torch.equal(b.cache.k, want[0].k) and torch.equal(b.cache.v, want[0].v)
+    b.cache.check()
+
+
+def test_results_in_the_caches_memory_are_refused(gpu):
+    b = Batch(gpu, [(4, 20)], 128, 2, 2, 16, BF)
+    q, k = b.randn(4, 2, 128), b.randn(4, 2, 128)
+    for t in (b.cache.k, b.cache.v):
+        inside = t[0, 3:7]
+        with pytest.raises(ValueError, match="share memory with the cache"):
+            lv.paged_attention(q, b.cache, *b.call(), out=inside)
+        with pytest.raises(ValueError, match="share memory with the cache"):
+            lv.paged_kv_append(b.cache, k, k, *b.call(), q=q, q_out=inside)
+    b.cache.check()
