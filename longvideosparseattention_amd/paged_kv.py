@@ -76,6 +76,7 @@ assert _ATTN_AT + _APPEND.size == C.sizeof(capi.PagedAppendArgs)
 
 def _cache_rows(t: torch.Tensor, name: str, dtype: torch.dtype, width: int, align: int) -> Tuple[int, int, int]:
     hip_ops._require_device(t, name)
+    _no_gradient(t, name)
     if t.dim() != 4 or t.shape[3] != width or t.dtype != dtype:
         raise ValueError(f"{name} must be [pages, page_size, H_kv, {width}] of {dtype}, got {tuple(t.shape)} of {t.dtype}")
     es = t.element_size()
@@ -88,6 +89,11 @@ def _cache_rows(t: torch.Tensor, name: str, dtype: torch.dtype, width: int, alig
             raise ValueError(f"{name} has overlapping rows (shape {tuple(t.shape)}, strides {t.stride()})")
         at = stride * (size - 1) + at
     return t.stride(0), t.stride(1), t.stride(2)
+
+
+def _no_gradient(t: torch.Tensor, name: str) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient: the paged cache has no backward pass (detach it or use no_grad)")
 
 
 class PagedKVCache:
@@ -241,8 +247,8 @@ def _tokens(t: torch.Tensor, name: str, heads: Optional[int], cache: PagedKVCach
         raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
     if t.get_device() != cache.device.index:
         raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{name} requires a gradient: the paged cache has no backward pass (detach it or use no_grad)")
+    if t.requires_grad:
+        _no_gradient(t, name)
     s0, s1, s2 = t.stride()
     ptr = t.data_ptr()
     if s2 != 1 or (ptr | ((s0 | s1) * 2)) & 15:
@@ -342,6 +348,8 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, cu_se
                 raise TypeError(f"{name} must be a contiguous fp32 [positions, rot / 2] tensor like its partner")
             if t.get_device() != cache.device.index:
                 raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
+            if t.requires_grad:
+                _no_gradient(t, name)
         angles, rot = cos.shape
         rot *= 2
         if rot % 16 or not 0 < rot <= cache.head_dim:

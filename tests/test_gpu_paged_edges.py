@@ -279,3 +279,19 @@ def test_results_in_the_caches_memory_are_refused(gpu):
         with pytest.raises(ValueError, match="share memory with the cache"):
             lv.paged_kv_append(b.cache, k, k, *b.call(), q=q, q_out=inside)
     b.cache.check()
+
+
+def test_gradients_of_angles_and_pages_are_refused(gpu):
+    b = Batch(gpu, [(4, 20)], 128, 2, 2, 16, BF)
+    k = b.randn(4, 2, 128)
+    cos, sin = (torch.rand(20, 64, device=gpu) for _ in range(2))
+    for kw in ({"cos": cos.clone().requires_grad_(), "sin": sin}, {"cos": cos, "sin": sin.clone().requires_grad_()}):
+        with pytest.raises(RuntimeError, match="gradient"):
+            lv.paged_kv_append(b.cache, k, k, *b.call(), **kw)
+        with torch.no_grad():
+            lv.paged_kv_append(b.cache, k, k, *b.call(), **kw)
+    with pytest.raises(RuntimeError, match="gradient"):
+        lv.PagedKVCache(b.cache.k.clone().requires_grad_(), b.cache.v)
+    with pytest.raises(RuntimeError, match="gradient"):
+        lv.PagedKVCache(b.cache.k, b.cache.v.clone().requires_grad_())
+    b.cache.check()
