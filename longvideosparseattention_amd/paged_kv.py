@@ -33,6 +33,8 @@ not ascend within the packed rows, nobody knows whose rows are whose: attention
 returns NaN in every row, an append takes a row for the first sequence whose
 range holds it.
 
+Inside ``torch.compile`` the calls break the graph and run as they are.
+
 The reference has no cache: it attends over whole tensors
 (``lvsa/sparse_attention.py:643-706``) that its adapters have rotated before
 (``lvsa/rope.py:10-27``).
@@ -46,6 +48,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.compiler import is_compiling
 
 from . import _capi as capi
 from . import hip_ops
@@ -182,6 +185,7 @@ class PagedKVCache:
         lo, hi = _span(t)
         return t.numel() > 0 and any(lo < e and a < hi for a, e in self._spans)
 
+    @torch.compiler.disable
     def check(self) -> None:
         """Raise ``ValueError`` for what earlier calls found wrong on the device,
         on whatever stream, and forget it.  Waits for the device; what calls
@@ -313,6 +317,9 @@ def paged_kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, cu_se
     not share memory with the inputs or the cache.  A token
     with a bad page, length, row range or position is left out, its row of
     ``q_out`` NaN."""
+    if is_compiling():
+        return _outside["append"](cache, k, v, cu_seqlens, kv_lens, page_table, q=q, cos=cos, sin=sin, positions=positions,
+                                  interleaved=interleaved, q_out=q_out)
     dtype = k.dtype if isinstance(k, torch.Tensor) else None
     packed = cache._pack(dtype)
     Hkv = cache.num_kv_heads
@@ -379,6 +386,8 @@ def paged_kv_gather(cache: PagedKVCache, kv_lens: torch.Tensor, page_table: torc
     ``dtype``: the cache's for 16 bits; bf16 (the default) or fp16 for 4, both of
     which hold every 4-bit value exactly.  A bad page gives NaN for its tokens, a
     bad length for the whole sequence."""
+    if is_compiling():
+        return _outside["gather"](cache, kv_lens, page_table, max_len, dtype=dtype)
     if dtype is None:
         dtype = cache.dtype or torch.bfloat16
     packed = cache._pack(dtype)
@@ -431,6 +440,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, cu_seqlens: torch.Tens
     sequence are left as they were in ``out`` and are 0 in a new tensor (``lse``:
     ``-inf`` in both cases).  Scores, softmax and sums are fp32; weights enter the second product
     in ``q``'s type."""
+    if is_compiling():
+        return _outside["attention"](q, cache, cu_seqlens, kv_lens, page_table, causal=causal, scale=scale,
+                                     return_lse=return_lse, max_q_len=max_q_len, max_kv_len=max_kv_len, out=out)
     dtype = q.dtype if isinstance(q, torch.Tensor) else None
     packed = cache._pack(dtype)
     q, q_ptr, *q_str = _tokens(q, "q", None, cache, dtype)
@@ -458,3 +470,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, cu_seqlens: torch.Tens
             a.workspace, a.workspace_bytes = ws.data_ptr(), need
         hip_ops._call(cache.device, "lvsa_paged_attn_fwd", C.byref(a))
     return (out, lse) if return_lse else out
+
+
+# Within torch.compile the calls break the graph and run as they are: they take
+# addresses and call C.  (Called through these only there: a wrapper on every call
+# costs half a microsecond.)
+_outside = {name: torch.compiler.disable(fn) for name, fn in
+            (("append", paged_kv_append), ("gather", paged_kv_gather), ("attention", paged_attention))}

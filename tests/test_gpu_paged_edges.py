@@ -295,3 +295,26 @@ def test_gradients_of_angles_and_pages_are_refused(gpu):
     with pytest.raises(RuntimeError, match="gradient"):
         lv.PagedKVCache(b.cache.k, b.cache.v.clone().requires_grad_())
     b.cache.check()
+
+
+# ── inside torch.compile ─────────────────────────────────────────────────────
+
+
+def test_calls_inside_a_compiled_function(gpu):
+    """The calls break the graph and run as they are, with the same results, also for other lengths later."""
+    b = Batch(gpu, [(3, 40), (3, 20)], 128, 4, 2, 16, BF)
+    cos, sin = (torch.rand(64, 64, device=gpu) for _ in range(2))
+
+    def f(q, k, v, lens):
+        qr = lv.paged_kv_append(b.cache, k * 1.0, v * 1.0, b.cu, lens, b.table_dev, q=q * 1.0, cos=cos, sin=sin)
+        o, lse = lv.paged_attention(qr, b.cache, b.cu, lens, b.table_dev, max_q_len=3, return_lse=True)
+        kk, vv = lv.paged_kv_gather(b.cache, lens, b.table_dev, 40)
+        b.cache.check()
+        return o * 2.0, lse + 1.0, kk + 0, vv + 0
+
+    g = torch.compile(f, backend="eager")
+    for back in (0, 1, 2):
+        x = b.randn(6, 4, 128), b.randn(6, 2, 128), b.randn(6, 2, 128), b.lens - back
+        want, got = f(*x), g(*x)
+        assert all(torch.equal(a.nan_to_num(3.0), c.nan_to_num(3.0)) for a, c in zip(want, got))
+    b.cache.check()
