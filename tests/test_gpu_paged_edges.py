@@ -1,10 +1,12 @@
 """The paged cache where calls leave the usual path: padded batches with the caller's result, arguments that the
 device finds wrong, values that a type cannot hold, far larger and smaller weights, many sequences, other streams."""
+import ctypes
+
 import pytest
 import torch
 
 import longvideosparseattention_amd as lv
-from longvideosparseattention_amd import _capi, hip_ops
+from longvideosparseattention_amd import _capi, hip_ops, paged_kv
 
 import paged_ref as ref
 from paged_ref import Batch
@@ -318,3 +320,48 @@ def test_calls_inside_a_compiled_function(gpu):
         want, got = f(*x), g(*x)
         assert all(torch.equal(a.nan_to_num(3.0), c.nan_to_num(3.0)) for a, c in zip(want, got))
     b.cache.check()
+
+
+# ── many sequences and tiles on the kernels of long caches ───────────────────
+
+
+def _workspace(b, heads, hint, sequences):
+    """Bytes that a call of the batch, cut to its first sequences, asks for."""
+    a = _capi.PagedAttnArgs.from_buffer_copy(
+        b.cache._pack(b.dtype) + paged_kv._batch(b.cache, b.cu[:sequences + 1], b.lens[:sequences], b.table_dev[:sequences], b.N) +
+        bytes(paged_kv._ATTN.size))
+    a.q = a.o = 1 << 20
+    a.q_str = a.o_str = _capi._Str2(heads * b.D, b.D)
+    a.scale, a.H, a.max_q_len = 1.0, heads, hint
+    n = ctypes.c_int64()
+    assert _capi.lib().lvsa_paged_attn_workspace_query(ctypes.byref(a), ctypes.byref(n)) == 0
+    return n.value
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D,hint", [(64, 40), (64, 200), (256, 40)])
+@pytest.mark.parametrize("B", [65, 1100, 5200])
+def test_many_sequences_of_the_plan(gpu, B, D, hint, causal):
+    """More sequences than the plan takes at a time, more row tiles than it keeps whole (1024) or in LDS at all (4096),
+    shares that span many tiles: on the 128-row and 256-row kernels.  Then a bad page in a late sequence."""
+    seqs = [(0 if s % 7 == 3 else 1 + (s % 11 == 0), s % 5 + (s * s) % 13) for s in range(B)]
+    seqs = [(min(n, L), L) for n, L in seqs]
+    seqs[B // 2] = (300, 301)                             # several tiles of one sequence in between
+    if B > 5000:
+        seqs[-3] = (600, 600)
+    b = Batch(gpu, seqs, D, 2, 1, 8, BF, seed=6, tail=2, extra_columns=(20000 if B < 1000 else 2400) // 8)
+    # every tile takes 56 bytes of the plan; the decode kernel's workspace does not follow the sequences here
+    assert _workspace(b, 2, hint, B) - _workspace(b, 2, hint, B // 2) >= 56 * (B - B // 2) - 16
+    q = b.randn(b.N, 2, D)
+    o, lse = lv.paged_attention(q, b.cache, *b.call(), causal=causal, return_lse=True, max_q_len=hint)
+    wo, wl, tol, ltol = ref.attention(b, q, causal)
+    ref.check_close(o, wo, tol, "attention")
+    ref.check_close(lse, wl, ltol, "lse")
+    b.cache.check()
+    late = B - 3 if B > 5000 else B // 2
+    b.table_dev[late, 37] = -1                            # keys 296 .. 303: behind the first tile's
+    bad, _ = lv.paged_attention(q, b.cache, *b.call(), causal=causal, return_lse=True, max_q_len=hint)
+    lo, hi = b.ends[late], b.ends[late + 1]
+    assert torch.isnan(bad[lo:hi]).all() and torch.equal(bad[:lo], o[:lo]) and torch.equal(bad[hi:], o[hi:])
+    with pytest.raises(ValueError, match="page number"):
+        b.cache.check()
