@@ -192,6 +192,21 @@ __host__ __device__ inline int64_t quotient(int64_t a, int64_t b) {
 __host__ __device__ inline int64_t unit_start(int64_t U, int G, int w) { return quotient(w * U, G); }
 __host__ __device__ inline int wg_of_unit(int64_t U, int G, int64_t u) { return (int)quotient((u + 1) * G - 1, U); }
 
+// Shares of a prefill launch: one for every (tile, key head), whatever its keys,
+// where there are work-groups for it, else of kPagedLeast units at least.
+__host__ __device__ inline int plan_shares(int64_t U, int64_t pairs, int grid) {
+  if (U <= 0) return 0;
+  const int least = unit_shares(U, grid, kPagedLeast);
+  return pairs <= least ? least : pairs < grid ? (int)pairs : grid;
+}
+// Share of a work-group.  Consecutive work-groups go to the eight XCDs in turn:
+// an XCD gets consecutive shares, few key heads' tiles, whose keys its L2 then
+// serves to all of them.
+__host__ __device__ inline int share_of(int wg, int shares) {
+  const int per = (shares + 7) / 8, s = (wg & 7) * per + (wg >> 3);
+  return (wg >> 3) < per && s < shares ? s : -1;
+}
+
 // Partials of the row tile whose key steps are units [u0, u0 + nb): none if one
 // work-group has them all, else one per work-group, in the first of its two
 // slots but where it came to the tile from another one.

@@ -546,11 +546,8 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PagedAttnParams p, int
   }
   const int tiles = (int)done;
   const int64_t U = units * p.c.Hkv;
-  // a share for every tile, whatever its keys, where there are work-groups for it
-  const int64_t whole = (int64_t)tiles * p.c.Hkv;
-  const int least = U > 0 ? unit_shares(U, p.grid, kPagedLeast) : 0;
-  // (none where the row ranges are bad: the launch then only spoils the result)
-  const int shares = bad_cu ? 0 : whole <= least ? least : whole < p.grid ? (int)whole : p.grid;
+  // none where the row ranges are bad: the launch then only spoils the result
+  const int shares = bad_cu ? 0 : plan_shares(U, (int64_t)tiles * p.c.Hkv, p.grid);
   if (threadIdx.x == 0) *p.head = PlanHead{units, tiles, shares, bad_cu, 0};
   const bool in_lds = tiles <= kPlanLds;
   for (int w = threadIdx.x; w < shares; w += 1024) {

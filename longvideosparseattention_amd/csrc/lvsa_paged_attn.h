@@ -638,14 +638,6 @@ __device__ __forceinline__ void spoil_rows(const PagedAttnParams& p, int D, int 
   }
 }
 
-// Share of a work-group.  Consecutive work-groups go to the eight XCDs in turn:
-// an XCD gets consecutive shares, few key heads' tiles, whose keys its L2 then
-// serves to all of them.
-__device__ __forceinline__ int share_of(int wg, int shares) {
-  const int per = (shares + 7) / 8, s = (wg & 7) * per + (wg >> 3);
-  return (wg >> 3) < per && s < shares ? s : -1;
-}
-
 // A row's result, or its partial sums where shares divide its tile: O of
 // element 32 dt + 8 q + 4 half + i in o[dt][4 q + i].
 template <int D, typename E>
