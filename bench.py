@@ -94,19 +94,27 @@ def copy_calibration(mib: int) -> int:
 
 
 def source_hash() -> str:
-    """Hash of what is compiled (the HIP sources, headers, the generated key
-    loop and the build script): names the build a committed counters file was
-    measured on.  The loop generator itself is left out: its output, the
-    .inc, is hashed, so a comment in the generator does not rename the build."""
+    """Hash of what the benchmarked kernels are compiled from (the HIP sources,
+    headers, the generated key loop and the build script): names the build a
+    committed counters file was measured on.  The loop generator itself is left
+    out: its output, the .inc, is hashed, so a comment in the generator does not
+    rename the build.  So are the paged cache's units, their lines in the build
+    script and their section of the header: no call of this benchmark runs them."""
     import hashlib
+    import re
 
     h = hashlib.sha256()
     pkg = os.path.join(ROOT, "longvideosparseattention_amd")
     csrc = os.path.join(pkg, "csrc")
-    files = sorted(f for f in os.listdir(csrc) if f.endswith((".hip", ".h", ".inc")))
+    files = sorted(f for f in os.listdir(csrc) if f.endswith((".hip", ".h", ".inc")) and not f.startswith("lvsa_paged"))
     for name in files + ["../build_lib.py", "../../include/lvsa_amd.h"]:
         with open(os.path.join(csrc, name), "rb") as f:
-            h.update(name.encode() + b"\0" + f.read())
+            text = f.read()
+        if name.endswith("build_lib.py"):
+            text = re.sub(rb'    "lvsa_paged[^\n]*\n', b"", text)
+        if name.endswith("lvsa_amd.h"):
+            text = re.sub(r"/\* (?:─)+ paged key/value cache (?:─)+ \*/.*?(?=/\* Library identification)".encode(), b"", text, flags=re.S)
+        h.update(name.encode() + b"\0" + text)
     return h.hexdigest()[:16]
 
 
