@@ -49,16 +49,17 @@ typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
 
-// A row's weights are 2^(score - m), m its reference: the running maximum less
-// kLift, and moved only when a score exceeds it by kLift + kRise, so that the
-// usual step rescales nothing.  bf16 has fp32's range: no lift, weights up to 2^8.
+// A row's weights are 2^(score - m), m its reference: the running maximum less a
+// lift, and moved only when a score exceeds it by lift and rise, so that the usual
+// step rescales nothing.  bf16 has fp32's range: no lift, weights up to 2^8.
 // fp16's normal numbers reach from 2^-14 to 2^16: lifted by 9 with a rise of 6, a
 // row's largest weight is 2^9 to 2^15, and weights down to 2^-23 of it keep all
 // their bits (unlifted they were subnormal from 2^-14 of it on and 0 below 2^-25:
 // the rest of a row beside keys with nearly all its weight, but values of 0, came
 // out up to 20% off).  The rise costs rescaled steps: causal prompts of head size
 // 64 in fp16 185.6 us with 8 (and a lift of 7), 187.3 with 6, 188.7 with 5, 190.9
-// with 4.
+// with 4.  Scores from 2^20 on, which fp32 holds to an eighth and worse, have no
+// lift: half a step of theirs more would overflow from 2^24 on (2^27 without).
 template <typename E>
 struct Mat;
 template <>
@@ -66,7 +67,7 @@ struct Mat<__bf16> {
   typedef __bf16 v8 __attribute__((ext_vector_type(8)));
   typedef __bf16 v2 __attribute__((ext_vector_type(2)));
   static constexpr uint32_t kExp = 0x7f80u;
-  static constexpr float kLift = 0.f, kRise = 8.f;
+  static constexpr bool kLifted = false;
   static constexpr uint32_t kFinite = 252;    // largest scale byte that leaves every 4-bit value finite: 6 * 2^125
   __device__ static floatx4 mfma16(shortx8 a, shortx8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
@@ -88,7 +89,7 @@ struct Mat<_Float16> {
   typedef _Float16 v4 __attribute__((ext_vector_type(4)));
   typedef _Float16 v2 __attribute__((ext_vector_type(2)));
   static constexpr uint32_t kExp = 0x7c00u;
-  static constexpr float kLift = 9.f, kRise = 6.f;
+  static constexpr bool kLifted = true;
   static constexpr uint32_t kFinite = 140;    // 6 * 2^13
   __device__ static floatx4 mfma16(shortx8 a, shortx8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
@@ -102,6 +103,23 @@ struct Mat<_Float16> {
   template <int SEL>
   __device__ static uint32_t decode(uint32_t codes, float scale) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, SEL));
+  }
+};
+
+constexpr float kFarScore = 1048576.f;
+// A row's reference: m, and the score above which it moves.
+template <typename E>
+struct Reference {
+  float m = kNoKeys;
+  float above = kNoKeys;                  // kept in a register where the rise depends on the row
+  __device__ __forceinline__ bool exceeded(float top) const { return Mat<E>::kLifted ? top > above : top > m + 8.0f; }
+  // Moves to a block's largest score; returns the factor of what was summed so far.
+  __device__ __forceinline__ float move(float top) {
+    if constexpr (Mat<E>::kLifted) top -= __builtin_fabsf(top) < kFarScore ? 9.0f : 0.0f;
+    const float next = __builtin_fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - next);
+    m = next;
+    if constexpr (Mat<E>::kLifted) above = m + (__builtin_fabsf(m) < kFarScore ? 15.0f : 8.0f);
+    return alpha;
   }
 };
 
@@ -346,10 +364,10 @@ __global__ __launch_bounds__(256, D == 256 || (D == 192 && NT == 2) ? 1 : paged_
     }
 
     floatx4 o[NT][NO];
-    float m_run[NT], l_run[NT];
+    Reference<E> ref_run[NT];
+    float l_run[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      m_run[n] = kNoKeys;
       l_run[n] = 0.f;
 #pragma unroll
       for (int i = 0; i < NO; ++i) o[n][i] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -464,15 +482,13 @@ __global__ __launch_bounds__(256, D == 256 || (D == 192 && NT == 2) ? 1 : paged_
           top = __builtin_fmaxf(top, __builtin_fmaxf(__builtin_fmaxf(s[n][1][0], s[n][1][1]),
                                                      __builtin_fmaxf(s[n][1][2], s[n][1][3])));
         top *= p.scale_log2;
-        if (__builtin_amdgcn_ballot_w64(top > m_run[n] + (Mat<E>::kLift + Mat<E>::kRise))) {
+        if (__builtin_amdgcn_ballot_w64(ref_run[n].exceeded(top))) {
           top = __builtin_fmaxf(top, __shfl_xor(top, 16));
           top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-          const float m_new = __builtin_fmaxf(m_run[n], top - Mat<E>::kLift);
-          const float alpha = __builtin_amdgcn_exp2f(m_run[n] - m_new);
+          const float alpha = ref_run[n].move(top);
           l_run[n] *= alpha;
 #pragma unroll
           for (int i = 0; i < NO; ++i) o[n][i] *= alpha;
-          m_run[n] = m_new;
         }
         uint32_t w[2 * T];
 #pragma unroll
@@ -480,7 +496,7 @@ __global__ __launch_bounds__(256, D == 256 || (D == 192 && NT == 2) ? 1 : paged_
           float e[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j][r], p.scale_log2, -m_run[n]));
+            e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j][r], p.scale_log2, -ref_run[n].m));
             l_run[n] += e[r];
           }
           w[2 * j] = pack2<E>(e[0], e[1]);
@@ -562,11 +578,11 @@ __global__ __launch_bounds__(256, D == 256 || (D == 192 && NT == 2) ? 1 : paged_
       l += __shfl_xor(l, 16);
       l += __shfl_xor(l, 32);
       __syncthreads();                         // V tiles (and the last tile's exchange) have been read
-      if (g == 0) m_s[wave][x] = m_run[n];
+      if (g == 0) m_s[wave][x] = ref_run[n].m;
       if (n == 0 && __builtin_amdgcn_ballot_w64(bad) && lane == 0) bad_s = 1;
       __syncthreads();
       const float M = __builtin_fmaxf(__builtin_fmaxf(m_s[0][x], m_s[1][x]), __builtin_fmaxf(m_s[2][x], m_s[3][x]));
-      const float w = __builtin_amdgcn_exp2f(m_run[n] - M);
+      const float w = __builtin_amdgcn_exp2f(ref_run[n].m - M);
       if (g == 0) l_s[wave][x] = l * w;
 #pragma unroll
       for (int i = 0; i < NO; ++i)
@@ -885,7 +901,8 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   floatx16 o[NO];
 #pragma unroll
   for (int i = 0; i < NO; ++i) o[i] = floatx16{0};
-  float m_run = kNoKeys, l4[4] = {0.f, 0.f, 0.f, 0.f};
+  Reference<E> ref_run;
+  float l4[4] = {0.f, 0.f, 0.f, 0.f};
   struct Scores {
     floatx16 a, b;                                      // keys 0 .. 31 and 32 .. 63 of a block
   };
@@ -945,12 +962,11 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
       t[c] = vmax(vmax(m, s.b[4 * c + 2]), s.b[4 * c + 3]);
     }
     float top = vmax(vmax(t[0], t[1]), vmax(t[2], t[3])) * p.scale_log2;
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m_run + (Mat<E>::kLift + Mat<E>::kRise)) != 0, 0)) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(ref_run.exceeded(top)) != 0, 0)) {
       // The reference is kept a whole number, so that this factor is a power of two
       // and the weights of block j - 1, rounded already, scale exactly.
       top = __builtin_floorf(__builtin_fmaxf(top, __shfl_xor(top, 32)));
-      const float m_new = __builtin_fmaxf(m_run, top - Mat<E>::kLift);
-      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      const float alpha = ref_run.move(top);
 #pragma unroll
       for (int i = 0; i < 4; ++i) l4[i] *= alpha;
 #pragma unroll
@@ -963,7 +979,6 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
         for (int i = 0; i < 8; ++i) w[i] = (E)((float)w[i] * alpha);
         pv.w[st] = __builtin_bit_cast(shortx8, w);
       }
-      m_run = m_new;
     }
     __builtin_amdgcn_sched_barrier(0);
 
@@ -993,8 +1008,8 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
       for (; done < (i + 1) * NE / NM; ++done) {
         const int st = done / 4, q = done % 4;
         const floatx16& y = st < 2 ? s.a : s.b;
-        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(y[8 * (st & 1) + 2 * q], p.scale_log2, -m_run));
-        const float c = __builtin_amdgcn_exp2f(__builtin_fmaf(y[8 * (st & 1) + 2 * q + 1], p.scale_log2, -m_run));
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(y[8 * (st & 1) + 2 * q], p.scale_log2, -ref_run.m));
+        const float c = __builtin_amdgcn_exp2f(__builtin_fmaf(y[8 * (st & 1) + 2 * q + 1], p.scale_log2, -ref_run.m));
         l4[q] += a + c;
         u32x4 w = __builtin_bit_cast(u32x4, pn.w[st]);
         w[q] = pack2<E>(a, c);
@@ -1079,7 +1094,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   const float l_run = (l4[0] + l4[1]) + (l4[2] + l4[3]);
   float l = l_run + __shfl_xor(l_run, 32);
   if (bad_s) l = __builtin_nanf("");
-  if (row < nrows) store_rows<D, E>(p, whole, slot, kPagedTile, row - r0, half, ref, o, m_run, l);
+  if (row < nrows) store_rows<D, E>(p, whole, slot, kPagedTile, row - r0, half, ref, o, ref_run.m, l);
   left -= blk_end - blk0;
   if (left <= 0) break;
   if (--ti < 0) {
@@ -1286,7 +1301,8 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
   shortx8 pb[4];
 #pragma unroll
   for (int st = 0; st < 4; ++st) pb[st] = shortx8{0};
-  float m_run = kNoKeys, l4[4] = {0.f, 0.f, 0.f, 0.f};
+  Reference<E> ref_run;
+  float l4[4] = {0.f, 0.f, 0.f, 0.f};
 
   constexpr int LA = D == 128 ? 6 : 4;
   constexpr bool kEarly = D == 128;
@@ -1370,15 +1386,13 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
       t[c] = vmax(vmax(m, s1[4 * c + 2]), s1[4 * c + 3]);
     }
     float top = vmax(vmax(t[0], t[1]), vmax(t[2], t[3])) * p.scale_log2;
-    if (__builtin_amdgcn_ballot_w64(top > m_run + (Mat<E>::kLift + Mat<E>::kRise))) {
+    if (__builtin_amdgcn_ballot_w64(ref_run.exceeded(top))) {
       top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-      const float m_new = __builtin_fmaxf(m_run, top - Mat<E>::kLift);
-      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      const float alpha = ref_run.move(top);
 #pragma unroll
       for (int i = 0; i < 4; ++i) l4[i] *= alpha;
 #pragma unroll
       for (int i = 0; i < NO; ++i) o[i] *= alpha;
-      m_run = m_new;
     }
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
@@ -1386,8 +1400,8 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
       u32x4 w;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * (st & 1) + 2 * i], p.scale_log2, -m_run));
-        const float c = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * (st & 1) + 2 * i + 1], p.scale_log2, -m_run));
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * (st & 1) + 2 * i], p.scale_log2, -ref_run.m));
+        const float c = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * (st & 1) + 2 * i + 1], p.scale_log2, -ref_run.m));
         l4[i] += a + c;
         w[i] = pack2<E>(a, c);
       }
@@ -1403,7 +1417,7 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
     for (int st = 0; st < 4; ++st) keep(pb[st]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) keep(l4[i]);
-    keep(m_run);
+    keep(ref_run.m);
 #pragma unroll
     for (int dt = 0; dt < NO; ++dt) keep(o[dt]);
 #pragma unroll
@@ -1475,7 +1489,7 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
   const float l_run = (l4[0] + l4[1]) + (l4[2] + l4[3]);
   float l = l_run + __shfl_xor(l_run, 32);
   if (bad_s) l = __builtin_nanf("");
-  if (row < nrows) store_rows<D, E>(p, whole, slot, kPagedTall, row - r0, half, ref, o, m_run, l);
+  if (row < nrows) store_rows<D, E>(p, whole, slot, kPagedTall, row - r0, half, ref, o, ref_run.m, l);
   left -= blk_end - blk0;
   if (left <= 0) break;
   if (--ti < 0) {

@@ -175,6 +175,69 @@ def test_small_weights_beside_keys_far_above_them(gpu, seqs, D, H, room, gap, dt
     b.cache.check()
 
 
+@pytest.mark.parametrize("dtype,size", [(HF, 2.0 ** 19), (HF, 2.0 ** 21), (HF, 2.0 ** 23), (HF, 2.0 ** 25), (BF, 2.0 ** 25), (BF, 2.0 ** 29)])
+@pytest.mark.parametrize("n,D,room", [(1, 128, 0), (20, 64, 0), (150, 64, ROOM), (100, 128, ROOM), (60, 256, ROOM)])
+def test_scores_of_millions(gpu, n, D, room, dtype, size):
+    """Scores that rise, or fall, along the keys up to +-``size``, far more than a weight's range apart: a row's result is
+    the value of its largest score's key, its lse that score."""
+    L = 300
+    b = Batch(gpu, [(n, L)], D, 2, 1, 16, dtype, extra_columns=room // 16)
+    k = torch.zeros(L, 1, D)
+    k[:, 0, 0] = (torch.arange(1, L + 1) / 512.0).to(dtype).float()       # rising; in bf16 neighbours may be equal
+    host = torch.zeros(b.cache.k.shape, dtype=dtype)
+    b._put(host, 0, k.to(dtype))
+    b.cache.k.copy_(host)
+    for sign in (1.0, -1.0):
+        q = torch.zeros(n, 2, D, dtype=dtype, device=gpu)
+        q[:, :, 0] = sign * 2.0 ** 10
+        scale = size / 2.0 ** 9
+        o, lse = lv.paged_attention(q, b.cache, *b.call(), scale=scale, max_q_len=n, return_lse=True)
+        b.cache.check()
+        z = sign * 2.0 ** 10 * scale * k[:, 0, 0].double()
+        for i in range(n):
+            mine = z[:L - n + i + 1]
+            top = (mine == mine.max()).nonzero()[:, 0]    # several where bf16 rounds keys alike: their mean
+            want = b.V[0][top, 0].mean(0)
+            # equal weights of a few keys, a rounding of each and of the result
+            assert (o[i].double().cpu() - want).abs().max() <= 3 * ref.U[dtype] * b.V[0][top, 0].abs().amax()
+            # roundings of the score, the scale, its product with log2(e), the sum with the weights' logarithm and ln 2, and
+            # the logarithm of at most four equal weights
+            assert (lse[i].double().cpu() - mine.max() ).abs().max() <= 6 * ref.F32 * mine.abs().max() + 4
+
+
+@pytest.mark.parametrize("dtype", [HF, BF])
+@pytest.mark.parametrize("base,step", [(0, 4), (2 ** 13, 4), (2 ** 17, 4), (2 ** 23, 4), (2 ** 24, 6), (2 ** 25, 4)])
+@pytest.mark.parametrize("n,D,room", [(1, 128, 0), (20, 64, 0), (150, 64, ROOM), (100, 128, ROOM), (60, 256, ROOM)])
+def test_scores_a_few_units_apart_around_a_large_one(gpu, n, D, room, base, step, dtype):
+    """``base`` plus a small number that rises by one or two steps from keys to keys, scale 1: exact in fp32, so the weights are those
+    of the small numbers alone, each e^x with a relative error of 2^-24 |x| and its roundings."""
+    L = 700
+    b = Batch(gpu, [(n, L)], D, 2, 1, 16, dtype, extra_columns=room // 16)
+    j = torch.arange(L)
+    small = (step * (j // 50 + j // 130)).to(dtype)       # up to 18 steps
+    k = torch.zeros(L, 1, D, dtype=dtype)
+    k[:, 0, 0], k[:, 0, 1] = small, float(base) / 4096 if base > 4096 else float(base)
+    host = torch.zeros(b.cache.k.shape, dtype=dtype)
+    b._put(host, 0, k)
+    b.cache.k.copy_(host)
+    q = torch.zeros(n, 2, D, dtype=dtype, device=gpu)
+    q[:, :, 0], q[:, :, 1] = 1.0, 4096.0 if base > 4096 else 1.0
+    o, lse = lv.paged_attention(q, b.cache, *b.call(), scale=1.0, max_q_len=n, return_lse=True)
+    b.cache.check()
+    z = small.double()[None] + base
+    seen = j[None] <= torch.arange(L - n, L)[:, None]
+    w = torch.softmax(torch.where(seen, z, float("-inf")), -1)
+    V = b.V[0][:, 0]
+    want, A = w @ V, w @ V.abs()
+    # a weight's exponent is off by 110 * 2^-23, the weight by half a step of its type and the sums by 764 roundings
+    u, F = ref.U[dtype], ref.F32
+    tol = u * want.abs() + A * (u + 2 * 220 * F + 2 * 764 * F) + (2.0 ** -25 if dtype == HF else 0.0)
+    ref.check_close(o[:, 0], want, tol, "attention")
+    ref.check_close(o[:, 1], want, tol, "attention")
+    wl = torch.logsumexp(torch.where(seen, z, float("-inf")), -1)[:, None].expand(n, 2)
+    ref.check_close(lse, wl, 6 * F * wl.abs() + 764 * F + 220 * F, "lse")
+
+
 # ── pages of keys that some rows do not attend ───────────────────────────────
 
 
