@@ -372,8 +372,9 @@ LVSA_API int lvsa_paged_gather(const lvsa_paged_cache* cache, const lvsa_paged_b
  * no effect on it, infinities and NaN included.  Rows of no sequence: `fill_tail`
  * 1 zeroes them (lse -inf), 2 writes their lse alone, 0 leaves both as they are.
  * `max_q_len` and `max_kv_len` (0: unknown) only choose a kernel and its split;
- * results hold whatever they say.  o shares no memory with q (refused), nor with
- * the cache.  Workspace: device memory of
+ * results hold whatever they say, within rounding: the order of a row's sums
+ * follows from them and from the lengths of the whole batch (a call repeated gives
+ * the same bits).  o shares no memory with q (refused), nor with the cache.  Workspace: device memory of
  * lvsa_paged_attn_workspace_query bytes, 16-byte aligned, any contents,
  * not shared by calls that overlap.                                          */
 typedef struct lvsa_paged_attn_args {

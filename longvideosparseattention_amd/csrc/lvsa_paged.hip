@@ -343,7 +343,8 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(PagedView c, char* ko
 // do not depend on timing.  Rows whose tile one work-group of the decode kernel
 // did whole are written already.  Rows without keys, rows of no sequence and, as
 // NaN, all rows of a batch whose row ranges are bad are this kernel's too.  Latency: the batch, the partials (two slots of a wave at a
-// time, maxima and sums beside them), one exchange.
+// time, maxima and sums beside them), one exchange.  Every row goes through the
+// batch again, 64 sequences a trip.
 template <typename E>
 __device__ __forceinline__ void merge_row(const PagedAttnParams& p, int row, int D, int rows, int keys,
                                           float (*acc_s)[256], float (*ml_s)[2]) {

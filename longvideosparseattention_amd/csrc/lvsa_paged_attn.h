@@ -765,9 +765,11 @@ __device__ __forceinline__ void wait_copies() {
 // are loaded a step ahead and written to LDS as 16-bit values, so every row is
 // decoded once for 128 query rows.
 //
-// 780 tokens of 12 heads over 4 of 256, over 31980 keys in 4 bits: 382 us with
-// plan and joining, 780 TFLOP/s (500 us with a phase of products after a phase of
-// softmax).  4 sequences of 128 tokens, 16 heads of 128, over 16384 keys: 141 us.
+// 780 tokens of 12 heads over 4 of 256, over 31980 keys in 4 bits: 378 us with
+// plan and joining, 790 TFLOP/s (500 us with a phase of products after a phase of
+// softmax).  The decoding of K and V, their addresses, the mask and the maximum
+// stand before a step's first product, on the only wave of a SIMD: MFMA busy a
+// third of the time, vector instructions another.  4 sequences of 128 tokens, 16 heads of 128, over 16384 keys: 141 us.
 template <int D, typename E, int BITS>
 __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(PagedAttnParams p) {
   constexpr int ND = D / 32, NK = D / 16, NO = D / 32;
@@ -1131,8 +1133,10 @@ __device__ __forceinline__ void copy4(const void* from, const lds_char* l) {
 // by the card's clock, 1.03 to 1.07 PFLOP/s (950 us with tiles of 128 rows and two independent work-groups; 840 us
 // with products and exponentials of one wave interleaved, which the issue of the
 // vector instructions beside the matrix ones holds up; 660 us without the copies,
-// which is what the data's way costs).  Causal prompts of head size 64: 184 us,
-// 680 TFLOP/s, bound by the exponentials: half the products per weight.
+// which is what the data's way costs).  Causal prompts of head size 64: 189 us,
+// 660 TFLOP/s: half the products per weight, so the softmax is the longer phase, and
+// only one of a SIMD's two waves is in it at a time, which issues a vector
+// instruction every 8 cycles where two would every 4 (VALU issuing 50%, MFMA 32%).
 //
 // Group 0 runs M(j) in phase 2 j and S(j) in phase 2 j + 1, group 1 one phase
 // later.  LDS holds four blocks of 64 keys of K and of V; group 0 brings K,

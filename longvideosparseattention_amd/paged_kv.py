@@ -434,12 +434,20 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, cu_seqlens: torch.Tens
     without keys gives 0 and ``-inf``.  ``scale`` defaults to ``1 / sqrt(D)``.
 
     ``max_q_len`` (the most rows of a sequence) and ``max_kv_len`` (the longest
-    cache) only choose a kernel and its split: results are right whatever they
-    say.  Without ``max_q_len`` more rows than sequences are taken for one long
-    sequence, which runs slower for a few rows of each.  ``out`` must not share memory with ``q`` or the cache; rows of no
-    sequence are left as they were in ``out`` and are 0 in a new tensor (``lse``:
-    ``-inf`` in both cases).  Scores, softmax and sums are fp32; weights enter the second product
-    in ``q``'s type."""
+    cache) only choose a kernel and its split: results are right whatever they say.
+    Without ``max_q_len`` more rows than sequences are taken for one long sequence,
+    which runs slower for a few rows of each; without ``max_kv_len`` the table's
+    width counts, and where that has room for long caches a short chunk takes up to
+    twice the time (20 tokens over 2000 keys 33 instead of 17 us). ``out`` must not
+    share memory with ``q`` or the cache; rows of no sequence are left as they were
+    in ``out`` and are 0 in a new tensor (``lse``: ``-inf`` in both cases).
+
+    Scores, softmax and sums are fp32; weights enter the second product in ``q``'s
+    type (in fp16 with fewer bits below 2^-23 of their row's largest).  A run
+    repeated gives the same bits, but the order of a row's sums follows from the
+    lengths of the whole batch: beside other sequences a result may differ within
+    rounding.  A row whose scores are all ``-inf`` counts as one without keys;
+    scaled scores from 9e7 (fp16) or 1.4e9 (bf16) on may give NaN."""
     if is_compiling():
         return _outside["attention"](q, cache, cu_seqlens, kv_lens, page_table, causal=causal, scale=scale,
                                      return_lse=return_lse, max_q_len=max_q_len, max_kv_len=max_kv_len, out=out)
