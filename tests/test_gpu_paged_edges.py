@@ -428,3 +428,128 @@ def test_many_sequences_of_the_plan(gpu, B, D, hint, causal):
     assert torch.isnan(bad[lo:hi]).all() and torch.equal(bad[:lo], o[:lo]) and torch.equal(bad[hi:], o[hi:])
     with pytest.raises(ValueError, match="page number"):
         b.cache.check()
+
+
+# ── layouts and sizes ────────────────────────────────────────────────────────
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("n,D,room", [(1, 128, 0), (20, 96, 0), (60, 64, ROOM), (150, 128, ROOM), (60, 256, ROOM)])
+def test_strided_queries_results_and_pages(gpu, n, D, room, bits):
+    """Queries and results that are views of packed tensors, keys with their heads' rows apart, values with their tokens'."""
+    H, Hkv, ps = 4, 2, 16
+    b = Batch(gpu, [(n, 200), (n, 170)], D, H, Hkv, ps, BF, bits=bits, extra_columns=room // ps)
+    q = b.randn(b.N, H, D)
+    want, wl = lv.paged_attention(q, b.cache, *b.call(), max_q_len=n, return_lse=True)
+    c = b.cache
+
+    def tokens(t):                                        # one half of [pages, 2, page_size, heads, X]
+        wide = torch.full((t.shape[0], 2, *t.shape[1:]), 77, dtype=t.dtype, device=gpu)
+        wide[:, 1] = t
+        return wide[:, 1]
+
+    def heads(t):                                         # [heads, pages, page_size, X]
+        return torch.empty(t.shape[2], t.shape[0], t.shape[1], t.shape[3], dtype=t.dtype, device=gpu).permute(1, 2, 0, 3).copy_(t)
+
+    both = (c.k, c.v) if bits == 16 else (c.k, c.v, c.k_scale, c.v_scale)
+    other = lv.PagedKVCache(*[(heads if i % 2 == 0 else tokens)(t) for i, t in enumerate(both)])
+    packed = torch.full((b.N, 3 * H, D), float("nan"), dtype=BF, device=gpu)
+    packed[:, H:2 * H] = q
+    out = torch.full((H + 1, b.N + 2, D), 9.0, dtype=BF, device=gpu)
+    view = out[1:, 1:-1].transpose(0, 1)                  # [N, H, D], a head's rows next to each other
+    got, gl = lv.paged_attention(packed[:, H:2 * H], other, *b.call(), max_q_len=n, out=view, return_lse=True)
+    assert torch.equal(got, want) and torch.equal(gl, wl)
+    assert (out[0] == 9.0).all() and (out[:, 0] == 9.0).all() and (out[:, -1] == 9.0).all()
+    k, v = lv.paged_kv_gather(other, b.lens, b.table_dev, 200)
+    wk, wv = lv.paged_kv_gather(c, b.lens, b.table_dev, 200)
+    assert torch.equal(k, wk) and torch.equal(v, wv)
+    new = b.randn(b.N, 3 * Hkv, D)
+    for x in (c, other):
+        lv.paged_kv_append(x, new[:, :Hkv], new[:, Hkv:2 * Hkv], *b.call())
+    for t, u in zip(both, (other.k, other.v) if bits == 16 else (other.k, other.v, other.k_scale, other.v_scale)):
+        assert torch.equal(t.nan_to_num(3.0) if bits == 16 else t, u.nan_to_num(3.0) if bits == 16 else u)
+    c.check()
+    other.check()
+
+
+def test_more_tokens_and_rows_than_a_launch_has_work_groups(gpu):
+    """1.2 million tokens appended, and 1.1 million output rows over a few keys on the decode kernel's merge."""
+    N, ps, D = 1_200_000, 4096, 64
+    cache = lv.PagedKVCache.allocate(300, ps, 1, D, device=gpu)
+    g = torch.Generator(device=gpu).manual_seed(1)
+    k, v = (torch.randn(N, 1, D, generator=g, device=gpu).to(BF) for _ in range(2))
+    of = lambda *x: torch.tensor(x, dtype=torch.int32, device=gpu)  # noqa: E731
+    table = torch.randperm(300, generator=g, device=gpu)[None, :293].to(torch.int32)
+    lv.paged_kv_append(cache, k, v, of(0, N), of(N), table)
+    got = lv.paged_kv_gather(cache, of(N), table, N)
+    assert torch.equal(got[0][0], k) and torch.equal(got[1][0], v)
+    n, H, L = 70_000, 16, 10
+    q = torch.randn(n, H, D, generator=g, device=gpu).to(BF)
+    o = lv.paged_attention(q, cache, of(0, n), of(L), table, causal=False, max_q_len=1)
+    w = torch.softmax(q.float().flatten(0, 1) @ k[:L, 0].float().T / 8.0, -1)
+    want, A = w @ v[:L, 0].float(), w @ v[:L, 0].float().abs()
+    # weights and results rounded to bf16, scores of 64 products and the sums in fp32 on both sides
+    err = (o.float().flatten(0, 1) - want).abs() - (ref.U[BF] * want.abs() + A * (ref.U[BF] + 2.0 ** -14))
+    assert err.max().item() <= 0
+    cache.check()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_seventeen_million_keys(gpu, bits):
+    """Positions past 2^24: keys of 0 weigh alike, so a result is the mean of the values, here 1 for the first half of the
+    keys and 3 for the rest, and the lse the logarithm of their number."""
+    L, ps, D, n = 17_000_000, 50_000, 64, 300
+    pages = L // ps
+    one, three = (0x22, 0x55) if bits == 4 else (1.0, 3.0)               # E2M1: 2 is 1.0, 5 is 3.0
+    shape = (pages, ps, 1, D // 2 if bits == 4 else D)
+    dt = torch.uint8 if bits == 4 else BF
+    k, v = (torch.zeros(shape, dtype=dt, device=gpu) for _ in range(2))
+    table = torch.randperm(pages, generator=torch.Generator().manual_seed(3)).to(torch.int32).to(gpu)[None]
+    v[table[0, :pages // 2].long()], v[table[0, pages // 2:].long()] = one, three
+    scales = [torch.full((pages, ps, 1, D // 32), 127, dtype=torch.uint8, device=gpu) for _ in range(2)] if bits == 4 else []
+    cache = lv.PagedKVCache(k, v, *scales)
+    cu, lens = (torch.tensor(x, dtype=torch.int32, device=gpu) for x in ([0, n], [L]))
+    q = torch.ones(n, 1, D, dtype=BF, device=gpu)
+    o, lse = lv.paged_attention(q, cache, cu, lens, table, return_lse=True)
+    o1, lse1 = lv.paged_attention(q[:1], cache, cu.clamp(max=1), lens, table, return_lse=True)
+    seen = torch.arange(L - n + 1, L + 1, dtype=torch.float64)
+    half = pages // 2 * ps
+    want = (half + 3.0 * (seen - half)) / seen
+    # counts of equal weights and of their values, each summed in fp32: under 2^17 terms to a partial sum of a lane
+    tol = ref.U[BF] * want + want * (2.0 ** 17 * ref.F32)
+    assert ((o[:, 0].double().cpu() - want[:, None]).abs() <= tol[:, None]).all()
+    assert ((o1[:, 0].double().cpu() - want[-1]).abs() <= tol[-1]).all()
+    for got, w in ((lse[:, 0], seen.log()), (lse1[:, 0], seen[-1:].log())):
+        assert ((got.double().cpu() - w).abs() <= 2.0 ** 17 * ref.F32 + 8 * ref.F32 * w).all()
+    cache.check()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_two_captured_graphs_of_one_pool(gpu, bits):
+    """A step of single tokens and a chunk, captured into one memory pool (their workspaces may be the same memory) and
+    replayed in turn with eager calls in between: each as its eager result."""
+    one = Batch(gpu, [(1, 4000), (1, 50), (1, 2500)], 128, 8, 2, 16, BF, bits=bits, tail=1)
+    many = Batch(gpu, [(70, 900), (150, 150)], 128, 8, 2, 16, BF, bits=bits, extra_columns=ROOM // 16)
+    runs = []
+    for b, hint in ((one, 1), (many, 150)):
+        q, out = b.randn(b.N, 8, 128), torch.zeros(b.N, 8, 128, dtype=BF, device=gpu)
+        call = lambda b=b, q=q, hint=hint, out=out: lv.paged_attention(q, b.cache, *b.call(), max_q_len=hint, out=out,  # noqa: E731
+                                                                       return_lse=True)
+        want = [x.clone() for x in call()]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=runs[0][1].pool() if runs else None):
+            got = call()
+        runs.append((call, graph, got, want))
+    for i in range(4):
+        for call, graph, got, want in runs if i % 2 else runs[::-1]:
+            for x in got:
+                x.fill_(7.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x[:-1], w[:-1]) for x, w in zip(got, want)), i
+            assert (got[0][-1] == 7.0).all() if call is runs[0][0] else torch.equal(got[0][-1], want[0][-1])
+            assert torch.equal(got[1], want[1])
+            assert all(torch.equal(x[:-1], w[:-1]) for x, w in zip(call(), want))
+    one.cache.check()
+    many.cache.check()
