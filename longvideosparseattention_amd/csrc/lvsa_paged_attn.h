@@ -191,12 +191,12 @@ __device__ __forceinline__ float add_nonfinite(float o, uint32_t bits, bool seen
 // Adds what keys [k0, k1) hold besides finite numbers to a row that attends
 // keys below `lim`: quad q of the row's elements, d0 + q * step .. + 3, in
 // o(q).  Rare, and slow: a key at a time.
-template <typename E, int BITS, int NQ, typename O>
-__device__ __forceinline__ void add_nonfinite_keys(const PagedView& c, const int32_t* table, int h, int k0, int k1,
+template <typename E, int BITS, int NQ, typename Keys, typename O>
+__device__ __forceinline__ void add_nonfinite_keys(const PagedView& c, const Keys& keys, int h, int k0, int k1,
                                                    int lim, int d0, int step, O o) {
 #pragma unroll 1
   for (int k = k0; k < k1; ++k) {
-    const PagedRow at = paged_row(c, k, table[page_of(c, k)]);
+    const PagedRow at = keys.row(k, keys.page(k));
     const char* row = c.v + at.page * c.v_str[0] + at.slot * c.v_str[1] + h * c.v_str[2];
     const bool seen = k < lim;
 #pragma unroll
@@ -216,6 +216,22 @@ __device__ __forceinline__ void add_nonfinite_keys(const PagedView& c, const int
     }
   }
 }
+
+// The keys that a tile of rows walks, numbered from 0 to L - 1: all of a
+// sequence's by position, each looked up in the page table ...
+struct PagedKeys {
+  const PagedView& c;
+  const int32_t* table;
+  int L;
+  __device__ __forceinline__ int page(int k) const { return table[page_of(c, k)]; }
+  __device__ __forceinline__ PagedRow row(int k, int page) const { return paged_row(c, k, page); }
+  // Whether `n` keys from k on lie in slots one after the other, from `slot`.
+  __device__ __forceinline__ bool together(int k, int n, int* slot) const {
+    *slot = k - page_of(c, k) * c.page_size;
+    return k + n <= L && *slot + n <= c.page_size;
+  }
+  __device__ __forceinline__ int limit(int lim) const { return lim; }       // keys below position `lim`
+};
 
 // Row r of a (sequence, key head) pair: its token and query head.
 struct RowRef {
@@ -244,6 +260,322 @@ struct Step<D, 4, T> {
   uint32_t ks[T][2], vs[T][2];
 };
 
+// What a work-group does next: key steps [blk0, blk1) of the rows [r0, r0 + ROWS)
+// before row nrows of sequence sq and key head h; into the result where that is the
+// rows' whole work, else to partial `slot`.  bad: the rows come out as NaN.
+struct DecodePart {
+  PagedSeq sq;
+  int h, r0, nrows, blk0, blk1;
+  int64_t slot;
+  bool whole, bad;
+};
+
+// A part, with the keys that `keys` names; behind it the work-group may go on to another one.
+template <int D, typename E, int BITS, int NT, typename Keys>
+__device__ __forceinline__ void decode_part(const PagedAttnParams& p, const DecodePart& part, const Keys& keys) {
+  constexpr int T = D >= 192 ? 1 : 2;          // 16-key tiles per wave and step
+  constexpr int KW = 16 * T, KEYS = 4 * KW;    // keys per wave, per work-group
+  static_assert(KEYS == paged_decode_keys(D), "merge and kernel count key steps alike");
+  constexpr int ND = D / 32, NO = D / 16, ROWS = 16 * NT;
+  constexpr int TB = 32 * D;                   // bytes of a 16-key tile
+  constexpr int OP = D + 4;                    // row pitch of the exchanged O
+  constexpr bool kTwoScales = D == 96 || D >= 192;
+  constexpr int kVBytes = 4 * T * TB, kOBytes = 4 * 16 * OP * 4;
+  __shared__ __attribute__((aligned(1024))) char smem_raw[kVBytes > kOBytes ? kVBytes : kOBytes];
+  __shared__ float m_s[4][16], l_s[4][16];
+  __shared__ int bad_s;
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, x = lane & 15;
+  lds_char* vbuf = (lds_char*)smem_raw + wave * (T * TB);
+  float* obuf = reinterpret_cast<float*>(smem_raw);
+  const PagedSeq& sq = part.sq;
+  const int h = part.h, r0 = part.r0, nrows = part.nrows, blk0 = part.blk0, blk1 = part.blk1;
+  const int64_t slot = part.slot;
+  const bool whole = part.whole;
+
+  // Q of the tile, in the order of the keys' elements; rows past the end
+  // repeat the last one.
+  shortx8 qf[NT][ND];
+  int lim[NT];
+  int lim_min = keys.L;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = r0 + 16 * n + x < nrows ? r0 + 16 * n + x : nrows - 1;
+    const RowRef ref = row_ref(p, sq, h, r);
+    const char* qp = p.q + ref.tok * p.q_str[0] + ref.head * p.q_str[1];
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      const int d = BITS == 16 ? 32 * i + 8 * g : (D / 4) * g + 8 * i;
+      qf[n][i] = *reinterpret_cast<const shortx8*>(qp + 2 * d);
+    }
+    lim[n] = keys.limit(key_limit(p, sq, r));
+  }
+  {
+    const int first = keys.limit(key_limit(p, sq, r0));
+    lim_min = first < lim_min ? first : lim_min;
+  }
+
+  floatx4 o[NT][NO];
+  Reference<E> ref_run[NT];
+  float l_run[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    l_run[n] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NO; ++i) o[n][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  bool bad = part.bad, odd_keys = false;
+
+  const char* kbase = p.c.k + h * p.c.k_str[2];
+  const char* vbase = p.c.v + h * p.c.v_str[2];
+  const uint8_t* ksbase = BITS == 4 ? p.c.ks + h * p.c.ks_str[2] : nullptr;
+  const uint8_t* vsbase = BITS == 4 ? p.c.vs + h * p.c.vs_str[2] : nullptr;
+
+  // Key x of tile j of step b (past the end: the last key).
+  auto key_pos = [&](int b, int j) __attribute__((always_inline)) {
+    return key_within(b * KEYS + wave * KW + 16 * j + x, keys.L);
+  };
+  auto load_pages = [&](int b, int* page) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < T; ++j) page[j] = keys.page(key_pos(b, j));
+  };
+  auto load = [&](int b, const int* page, Step<D, BITS, T>& st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+      const PagedRow at = keys.row(key_pos(b, j), page[j]);
+      bad |= !at.ok;
+      const char* kr = kbase + at.page * p.c.k_str[0] + at.slot * p.c.k_str[1];
+      const char* vr = vbase + at.page * p.c.v_str[0] + at.slot * p.c.v_str[1];
+      if constexpr (BITS == 16) {
+#pragma unroll
+        for (int i = 0; i < ND; ++i) st.k[j][i] = *reinterpret_cast<const u32x4*>(kr + 64 * i + 16 * g);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) st.v[j][i] = *reinterpret_cast<const u32x4*>(vr + 64 * i + 16 * g);
+      } else {
+        const uint32_t* kw = reinterpret_cast<const uint32_t*>(kr + (D / 8) * g);
+        const uint32_t* vw = reinterpret_cast<const uint32_t*>(vr + (D / 8) * g);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) st.k[j][i] = kw[i];
+#pragma unroll
+        for (int i = 0; i < ND; ++i) st.v[j][i] = vw[i];
+        const uint8_t* ksr = ksbase + at.page * p.c.ks_str[0] + at.slot * p.c.ks_str[1];
+        const uint8_t* vsr = vsbase + at.page * p.c.vs_str[0] + at.slot * p.c.vs_str[1];
+        const int lo = (D / 4) * g / 32, hi = ((D / 4) * g + D / 4 - 1) / 32;
+        st.ks[j][0] = ksr[lo];
+        st.vs[j][0] = vsr[lo];
+        st.ks[j][1] = kTwoScales ? ksr[hi] : 0;
+        st.vs[j][1] = kTwoScales ? vsr[hi] : 0;
+      }
+    }
+  };
+  // Elements of step i of a lane's piece, in the scale that covers them.
+  auto scale_of = [&](const uint32_t* s, int i) __attribute__((always_inline)) {
+    if constexpr (!kTwoScales) return s[0];
+    return ((D / 4) * g + 8 * i) / 32 == (D / 4) * g / 32 ? s[0] : s[1];
+  };
+
+  auto compute = [&](int b, Step<D, BITS, T>& st) __attribute__((always_inline)) {
+    const int key0 = b * KEYS + wave * KW;
+    if (key0 >= keys.L) return;                // the last step's waves past the end
+    // V to LDS, chunk by chunk
+    const bool masked = key0 + KW > lim_min;
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < T; ++j)
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        shortx8 w;
+        int c;
+        if constexpr (BITS == 16) {
+          w = __builtin_bit_cast(shortx8, st.v[j][i]);
+          c = 4 * i + g;
+        } else {
+          w = decode8<E>(st.v[j][i], scale_of(st.vs[j], i));
+          c = ND * g + i;
+        }
+        if (masked) {
+          odd |= any_nonfinite<E>(w);
+          w = finite8<E>(w);
+        }
+        *reinterpret_cast<__attribute__((address_space(3))) shortx8*>(vbuf + decode_chunk(D, 16 * j + x, c)) = w;
+      }
+    if (masked) odd_keys |= odd;
+    // S^T: row 4 g + r of tile j, column x
+    floatx4 s[NT][T];
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        shortx8 kf;
+        if constexpr (BITS == 16) kf = __builtin_bit_cast(shortx8, st.k[j][i]);
+        else kf = decode8<E>(st.k[j][i], scale_of(st.ks[j], i));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][j] = Mat<E>::mfma16(kf, qf[n][i], s[n][j]);
+      }
+    }
+    typedef short vp __attribute__((ext_vector_type(4 * T)));
+    vp pb[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < T; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool seen = key0 + 16 * j + 4 * g + r < lim[n];
+            s[n][j][r] = seen ? s[n][j][r] : -__builtin_inff();
+          }
+      }
+      float top = __builtin_fmaxf(__builtin_fmaxf(s[n][0][0], s[n][0][1]), __builtin_fmaxf(s[n][0][2], s[n][0][3]));
+      if constexpr (T == 2)
+        top = __builtin_fmaxf(top, __builtin_fmaxf(__builtin_fmaxf(s[n][1][0], s[n][1][1]),
+                                                   __builtin_fmaxf(s[n][1][2], s[n][1][3])));
+      top *= p.scale_log2;
+      if (__builtin_amdgcn_ballot_w64(ref_run[n].exceeded(top))) {
+        top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+        const float alpha = ref_run[n].move(top);
+        l_run[n] *= alpha;
+#pragma unroll
+        for (int i = 0; i < NO; ++i) o[n][i] *= alpha;
+      }
+      uint32_t w[2 * T];
+#pragma unroll
+      for (int j = 0; j < T; ++j) {
+        float e[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j][r], p.scale_log2, -ref_run[n].m));
+          l_run[n] += e[r];
+        }
+        w[2 * j] = pack2<E>(e[0], e[1]);
+        w[2 * j + 1] = pack2<E>(e[2], e[3]);
+      }
+      if constexpr (T == 2) pb[n] = __builtin_bit_cast(vp, u32x4{w[0], w[1], w[2], w[3]});
+      else pb[n] = __builtin_bit_cast(vp, u32x2{w[0], w[1]});
+    }
+    // O^T: row (element) 16 i + 4 g + r, column (query row) x
+    const int half = x & 3, row = 4 * g + (x >> 2);
+    auto vfrag = [&](int i) __attribute__((always_inline)) {
+      const int c = 2 * i + (half >> 1);
+      vp a;
+      const shortx4 a0 = read_tr(vbuf + decode_chunk(D, row, c) + 8 * (half & 1));
+      if constexpr (T == 2) {
+        const shortx4 a1 = read_tr(vbuf + decode_chunk(D, 16 + row, c) + 8 * (half & 1));
+        a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+      } else {
+        a = a0;
+      }
+      return a;
+    };
+#pragma unroll
+    for (int i = 0; i < NO; ++i) {
+      const vp a = vfrag(i);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) o[n][i] = Mat<E>::mfma16(a, pb[n], o[n][i]);
+    }
+  };
+
+  // Two steps in flight: while one is computed the next one's rows are on
+  // their way, and the page numbers of the one after that.
+  {
+    Step<D, BITS, T> sa, sb;
+    int page[T];
+    load_pages(blk0, page);
+    load(blk0, page, sa);
+    load_pages(blk0 + 1, page);
+    for (int b = blk0; b < blk1; b += 2) {
+      if (b + 1 < blk1) {
+        load(b + 1, page, sb);
+        load_pages(b + 2, page);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      compute(b, sa);
+      if (b + 1 < blk1) {
+        if (b + 2 < blk1) {
+          load(b + 2, page, sa);
+          load_pages(b + 3, page);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        compute(b + 1, sb);
+      }
+    }
+  }
+
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd_keys) != 0, 0)) {
+    const int from = lim_min / KEYS > blk0 ? lim_min / KEYS : blk0;
+    for (int b = from; b < blk1; ++b) {
+      const int k0 = b * KEYS + wave * KW, k1 = k0 + KW < keys.L ? k0 + KW : keys.L;
+      if (k0 + KW <= lim_min) continue;             // not masked: its values are in the sums already
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        add_nonfinite_keys<E, BITS, NO>(p.c, keys, h, k0, k1, lim[n], 4 * g, 16,
+                                        [&](int q, int r, uint32_t v, bool seen) __attribute__((always_inline)) {
+                                          o[n][q][r] = add_nonfinite<E>(o[n][q][r], v, seen);
+                                        });
+    }
+  }
+
+  // Join the four waves: rows' sums over the lanes, then maxima, sums and O
+  // through LDS, in the order of the waves.
+  if (threadIdx.x == 0) bad_s = 0;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float l = l_run[n];
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    __syncthreads();                         // V tiles (and the last tile's exchange) have been read
+    if (g == 0) m_s[wave][x] = ref_run[n].m;
+    if (n == 0 && __builtin_amdgcn_ballot_w64(bad) && lane == 0) bad_s = 1;
+    __syncthreads();
+    const float M = __builtin_fmaxf(__builtin_fmaxf(m_s[0][x], m_s[1][x]), __builtin_fmaxf(m_s[2][x], m_s[3][x]));
+    const float w = __builtin_amdgcn_exp2f(ref_run[n].m - M);
+    if (g == 0) l_s[wave][x] = l * w;
+#pragma unroll
+    for (int i = 0; i < NO; ++i)
+      *reinterpret_cast<floatx4*>(obuf + (wave * 16 + x) * OP + 16 * i + 4 * g) = o[n][i] * w;
+    __syncthreads();
+    // thread: row tr, elements of every 16th quad
+    const int tr = threadIdx.x >> 4, td = threadIdx.x & 15;
+    const int r = r0 + 16 * n + tr;
+    const float Mr = __builtin_fmaxf(__builtin_fmaxf(m_s[0][tr], m_s[1][tr]), __builtin_fmaxf(m_s[2][tr], m_s[3][tr]));
+    float lr = (l_s[0][tr] + l_s[1][tr]) + (l_s[2][tr] + l_s[3][tr]);
+    if (bad_s) lr = __builtin_nanf("");
+    if (r < nrows) {
+      const float inv = lr == 0.f ? 0.f : 1.0f / lr;
+      const RowRef ref = row_ref(p, sq, h, r);
+      char* op = p.o + ref.tok * p.o_str[0] + ref.head * p.o_str[1];
+      float* wo = whole ? nullptr : p.ws_o + (slot * ROWS + 16 * n + tr) * D;
+      for (int d = 4 * td; d < D; d += 64) {
+        floatx4 a = *reinterpret_cast<const floatx4*>(obuf + tr * OP + d);
+#pragma unroll
+        for (int k = 1; k < 4; ++k) a += *reinterpret_cast<const floatx4*>(obuf + (k * 16 + tr) * OP + d);
+        if (whole) {
+          *reinterpret_cast<u32x2*>(op + 2 * d) = u32x2{pack2<E>(a[0] * inv, a[1] * inv), pack2<E>(a[2] * inv, a[3] * inv)};
+        } else {
+          *reinterpret_cast<floatx4*>(wo + d) = a;
+        }
+      }
+      if (td == 0) {
+        if (!whole) {
+          float* ml = p.ws_ml + 2 * (slot * ROWS + 16 * n + tr);
+          ml[0] = Mr;
+          ml[1] = lr;
+        } else if (p.lse) {
+          p.lse[ref.tok * p.H + ref.head] =
+              lr == 0.f ? -__builtin_inff() : (Mr + __log2f(lr)) * 0.69314718055994530942f;
+        }
+      }
+    }
+  }
+  if (bad_s && threadIdx.x == 0 && !(sq.flags & LVSA_PAGED_BAD_LENGTH)) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
+  __syncthreads();                           // the exchange has been read: V tiles and bad_s may be written
+}
+
 // Bound by the bytes: 45 sequences of up to 16000 keys, 32 heads over 8 of 128, in
 // 16 bits at 5.7 TB/s (329 us), 40 of up to 32000 in 4 bits at 4.9 TB/s (154 us;
 // there the decoding of codes on the vector units takes as long as the bytes).  A
@@ -263,23 +595,8 @@ struct Step<D, 4, T> {
 // the schedule (D = 256, 4 bits: 275 instead of 215 us for 40 sequences of 12000).
 template <int D, typename E, int BITS, int NT>
 __global__ __launch_bounds__(256, D == 256 || (D == 192 && NT == 2) ? 1 : paged_decode_groups(D, BITS, 16 * NT)) void paged_decode_kernel(PagedAttnParams p) {
-  constexpr int T = D >= 192 ? 1 : 2;          // 16-key tiles per wave and step
-  constexpr int KW = 16 * T, KEYS = 4 * KW;    // keys per wave, per work-group
-  static_assert(KEYS == paged_decode_keys(D), "merge and kernel count key steps alike");
-  constexpr int ND = D / 32, NO = D / 16, ROWS = 16 * NT;
-  constexpr int TB = 32 * D;                   // bytes of a 16-key tile
-  constexpr int OP = D + 4;                    // row pitch of the exchanged O
-  constexpr bool kTwoScales = D == 96 || D >= 192;
-  constexpr int kVBytes = 4 * T * TB, kOBytes = 4 * 16 * OP * 4;
-  __shared__ __attribute__((aligned(1024))) char smem_raw[kVBytes > kOBytes ? kVBytes : kOBytes];
-  __shared__ float m_s[4][16], l_s[4][16];
-  __shared__ int bad_s;
-
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = lane >> 4, x = lane & 15;
-  lds_char* vbuf = (lds_char*)smem_raw + wave * (T * TB);
-  float* obuf = reinterpret_cast<float*>(smem_raw);
+  constexpr int ROWS = 16 * NT, KEYS = paged_decode_keys(D);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
 
   // The share [u, u_end) and the sequence it starts in.  A lane holds one
   // sequence, so that a batch of up to 64 is read once.
@@ -338,291 +655,10 @@ __global__ __launch_bounds__(256, D == 256 || (D == 192 && NT == 2) ? 1 : paged_
     const int64_t left = u_end - u;
     const int blk1 = left < nb - blk0 ? blk0 + (int)left : nb;
     const int rt = (int)quotient(run, p.c.Hkv), h = (int)(run - (int64_t)rt * p.c.Hkv);
-    const int nrows = sq.n * p.group;
-    const int r0 = rt * ROWS;
-
-    // Q of the tile, in the order of the keys' elements; rows past the end
-    // repeat the last one.
-    shortx8 qf[NT][ND];
-    int lim[NT];
-    int lim_min = sq.L;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int r = r0 + 16 * n + x < nrows ? r0 + 16 * n + x : nrows - 1;
-      const RowRef ref = row_ref(p, sq, h, r);
-      const char* qp = p.q + ref.tok * p.q_str[0] + ref.head * p.q_str[1];
-#pragma unroll
-      for (int i = 0; i < ND; ++i) {
-        const int d = BITS == 16 ? 32 * i + 8 * g : (D / 4) * g + 8 * i;
-        qf[n][i] = *reinterpret_cast<const shortx8*>(qp + 2 * d);
-      }
-      lim[n] = key_limit(p, sq, r);
-    }
-    {
-      const int first = key_limit(p, sq, r0);
-      lim_min = first < lim_min ? first : lim_min;
-    }
-
-    floatx4 o[NT][NO];
-    Reference<E> ref_run[NT];
-    float l_run[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      l_run[n] = 0.f;
-#pragma unroll
-      for (int i = 0; i < NO; ++i) o[n][i] = floatx4{0.f, 0.f, 0.f, 0.f};
-    }
-    bool bad = (sq.flags & LVSA_PAGED_BAD_LENGTH) != 0, odd_keys = false;
-
-    const char* kbase = p.c.k + h * p.c.k_str[2];
-    const char* vbase = p.c.v + h * p.c.v_str[2];
-    const uint8_t* ksbase = BITS == 4 ? p.c.ks + h * p.c.ks_str[2] : nullptr;
-    const uint8_t* vsbase = BITS == 4 ? p.c.vs + h * p.c.vs_str[2] : nullptr;
-    const int32_t* table = p.c.table + seq * p.c.table_str;
-
-    // Key x of tile j of step b (past the end: the last key).
-    auto key_pos = [&](int b, int j) __attribute__((always_inline)) {
-      return key_within(b * KEYS + wave * KW + 16 * j + x, sq.L);
-    };
-    auto load_pages = [&](int b, int* page) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < T; ++j) page[j] = table[page_of(p.c, key_pos(b, j))];
-    };
-    auto load = [&](int b, const int* page, Step<D, BITS, T>& st) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < T; ++j) {
-        const PagedRow at = paged_row(p.c, key_pos(b, j), page[j]);
-        bad |= !at.ok;
-        const char* kr = kbase + at.page * p.c.k_str[0] + at.slot * p.c.k_str[1];
-        const char* vr = vbase + at.page * p.c.v_str[0] + at.slot * p.c.v_str[1];
-        if constexpr (BITS == 16) {
-#pragma unroll
-          for (int i = 0; i < ND; ++i) st.k[j][i] = *reinterpret_cast<const u32x4*>(kr + 64 * i + 16 * g);
-#pragma unroll
-          for (int i = 0; i < ND; ++i) st.v[j][i] = *reinterpret_cast<const u32x4*>(vr + 64 * i + 16 * g);
-        } else {
-          const uint32_t* kw = reinterpret_cast<const uint32_t*>(kr + (D / 8) * g);
-          const uint32_t* vw = reinterpret_cast<const uint32_t*>(vr + (D / 8) * g);
-#pragma unroll
-          for (int i = 0; i < ND; ++i) st.k[j][i] = kw[i];
-#pragma unroll
-          for (int i = 0; i < ND; ++i) st.v[j][i] = vw[i];
-          const uint8_t* ksr = ksbase + at.page * p.c.ks_str[0] + at.slot * p.c.ks_str[1];
-          const uint8_t* vsr = vsbase + at.page * p.c.vs_str[0] + at.slot * p.c.vs_str[1];
-          const int lo = (D / 4) * g / 32, hi = ((D / 4) * g + D / 4 - 1) / 32;
-          st.ks[j][0] = ksr[lo];
-          st.vs[j][0] = vsr[lo];
-          st.ks[j][1] = kTwoScales ? ksr[hi] : 0;
-          st.vs[j][1] = kTwoScales ? vsr[hi] : 0;
-        }
-      }
-    };
-    // Elements of step i of a lane's piece, in the scale that covers them.
-    auto scale_of = [&](const uint32_t* s, int i) __attribute__((always_inline)) {
-      if constexpr (!kTwoScales) return s[0];
-      return ((D / 4) * g + 8 * i) / 32 == (D / 4) * g / 32 ? s[0] : s[1];
-    };
-
-    auto compute = [&](int b, Step<D, BITS, T>& st) __attribute__((always_inline)) {
-      const int key0 = b * KEYS + wave * KW;
-      if (key0 >= sq.L) return;                // the last step's waves past the end
-      // V to LDS, chunk by chunk
-      const bool masked = key0 + KW > lim_min;
-      bool odd = false;
-#pragma unroll
-      for (int j = 0; j < T; ++j)
-#pragma unroll
-        for (int i = 0; i < ND; ++i) {
-          shortx8 w;
-          int c;
-          if constexpr (BITS == 16) {
-            w = __builtin_bit_cast(shortx8, st.v[j][i]);
-            c = 4 * i + g;
-          } else {
-            w = decode8<E>(st.v[j][i], scale_of(st.vs[j], i));
-            c = ND * g + i;
-          }
-          if (masked) {
-            odd |= any_nonfinite<E>(w);
-            w = finite8<E>(w);
-          }
-          *reinterpret_cast<__attribute__((address_space(3))) shortx8*>(vbuf + decode_chunk(D, 16 * j + x, c)) = w;
-        }
-      if (masked) odd_keys |= odd;
-      // S^T: row 4 g + r of tile j, column x
-      floatx4 s[NT][T];
-#pragma unroll
-      for (int j = 0; j < T; ++j) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < ND; ++i) {
-          shortx8 kf;
-          if constexpr (BITS == 16) kf = __builtin_bit_cast(shortx8, st.k[j][i]);
-          else kf = decode8<E>(st.k[j][i], scale_of(st.ks[j], i));
-#pragma unroll
-          for (int n = 0; n < NT; ++n) s[n][j] = Mat<E>::mfma16(kf, qf[n][i], s[n][j]);
-        }
-      }
-      typedef short vp __attribute__((ext_vector_type(4 * T)));
-      vp pb[NT];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if (masked) {
-#pragma unroll
-          for (int j = 0; j < T; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const bool seen = key0 + 16 * j + 4 * g + r < lim[n];
-              s[n][j][r] = seen ? s[n][j][r] : -__builtin_inff();
-            }
-        }
-        float top = __builtin_fmaxf(__builtin_fmaxf(s[n][0][0], s[n][0][1]), __builtin_fmaxf(s[n][0][2], s[n][0][3]));
-        if constexpr (T == 2)
-          top = __builtin_fmaxf(top, __builtin_fmaxf(__builtin_fmaxf(s[n][1][0], s[n][1][1]),
-                                                     __builtin_fmaxf(s[n][1][2], s[n][1][3])));
-        top *= p.scale_log2;
-        if (__builtin_amdgcn_ballot_w64(ref_run[n].exceeded(top))) {
-          top = __builtin_fmaxf(top, __shfl_xor(top, 16));
-          top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-          const float alpha = ref_run[n].move(top);
-          l_run[n] *= alpha;
-#pragma unroll
-          for (int i = 0; i < NO; ++i) o[n][i] *= alpha;
-        }
-        uint32_t w[2 * T];
-#pragma unroll
-        for (int j = 0; j < T; ++j) {
-          float e[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j][r], p.scale_log2, -ref_run[n].m));
-            l_run[n] += e[r];
-          }
-          w[2 * j] = pack2<E>(e[0], e[1]);
-          w[2 * j + 1] = pack2<E>(e[2], e[3]);
-        }
-        if constexpr (T == 2) pb[n] = __builtin_bit_cast(vp, u32x4{w[0], w[1], w[2], w[3]});
-        else pb[n] = __builtin_bit_cast(vp, u32x2{w[0], w[1]});
-      }
-      // O^T: row (element) 16 i + 4 g + r, column (query row) x
-      const int half = x & 3, row = 4 * g + (x >> 2);
-      auto vfrag = [&](int i) __attribute__((always_inline)) {
-        const int c = 2 * i + (half >> 1);
-        vp a;
-        const shortx4 a0 = read_tr(vbuf + decode_chunk(D, row, c) + 8 * (half & 1));
-        if constexpr (T == 2) {
-          const shortx4 a1 = read_tr(vbuf + decode_chunk(D, 16 + row, c) + 8 * (half & 1));
-          a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-        } else {
-          a = a0;
-        }
-        return a;
-      };
-#pragma unroll
-      for (int i = 0; i < NO; ++i) {
-        const vp a = vfrag(i);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) o[n][i] = Mat<E>::mfma16(a, pb[n], o[n][i]);
-      }
-    };
-
-    // Two steps in flight: while one is computed the next one's rows are on
-    // their way, and the page numbers of the one after that.
-    {
-      Step<D, BITS, T> sa, sb;
-      int page[T];
-      load_pages(blk0, page);
-      load(blk0, page, sa);
-      load_pages(blk0 + 1, page);
-      for (int b = blk0; b < blk1; b += 2) {
-        if (b + 1 < blk1) {
-          load(b + 1, page, sb);
-          load_pages(b + 2, page);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        compute(b, sa);
-        if (b + 1 < blk1) {
-          if (b + 2 < blk1) {
-            load(b + 2, page, sa);
-            load_pages(b + 3, page);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-          compute(b + 1, sb);
-        }
-      }
-    }
-
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd_keys) != 0, 0)) {
-      const int from = lim_min / KEYS > blk0 ? lim_min / KEYS : blk0;
-      for (int b = from; b < blk1; ++b) {
-        const int k0 = b * KEYS + wave * KW, k1 = k0 + KW < sq.L ? k0 + KW : sq.L;
-        if (k0 + KW <= lim_min) continue;             // not masked: its values are in the sums already
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          add_nonfinite_keys<E, BITS, NO>(p.c, table, h, k0, k1, lim[n], 4 * g, 16,
-                                          [&](int q, int r, uint32_t v, bool seen) __attribute__((always_inline)) {
-                                            o[n][q][r] = add_nonfinite<E>(o[n][q][r], v, seen);
-                                          });
-      }
-    }
-
-    // Join the four waves: rows' sums over the lanes, then maxima, sums and O
-    // through LDS, in the order of the waves.
-    const bool whole = blk0 == 0 && blk1 == nb;
-    const int64_t slot = 2 * (int64_t)blockIdx.x + (u_first < u - blk0 ? 1 : 0);   // see decode_slots
-    if (threadIdx.x == 0) bad_s = 0;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float l = l_run[n];
-      l += __shfl_xor(l, 16);
-      l += __shfl_xor(l, 32);
-      __syncthreads();                         // V tiles (and the last tile's exchange) have been read
-      if (g == 0) m_s[wave][x] = ref_run[n].m;
-      if (n == 0 && __builtin_amdgcn_ballot_w64(bad) && lane == 0) bad_s = 1;
-      __syncthreads();
-      const float M = __builtin_fmaxf(__builtin_fmaxf(m_s[0][x], m_s[1][x]), __builtin_fmaxf(m_s[2][x], m_s[3][x]));
-      const float w = __builtin_amdgcn_exp2f(ref_run[n].m - M);
-      if (g == 0) l_s[wave][x] = l * w;
-#pragma unroll
-      for (int i = 0; i < NO; ++i)
-        *reinterpret_cast<floatx4*>(obuf + (wave * 16 + x) * OP + 16 * i + 4 * g) = o[n][i] * w;
-      __syncthreads();
-      // thread: row tr, elements of every 16th quad
-      const int tr = threadIdx.x >> 4, td = threadIdx.x & 15;
-      const int r = r0 + 16 * n + tr;
-      const float Mr = __builtin_fmaxf(__builtin_fmaxf(m_s[0][tr], m_s[1][tr]), __builtin_fmaxf(m_s[2][tr], m_s[3][tr]));
-      float lr = (l_s[0][tr] + l_s[1][tr]) + (l_s[2][tr] + l_s[3][tr]);
-      if (bad_s) lr = __builtin_nanf("");
-      if (r < nrows) {
-        const float inv = lr == 0.f ? 0.f : 1.0f / lr;
-        const RowRef ref = row_ref(p, sq, h, r);
-        char* op = p.o + ref.tok * p.o_str[0] + ref.head * p.o_str[1];
-        float* wo = whole ? nullptr : p.ws_o + (slot * ROWS + 16 * n + tr) * D;
-        for (int d = 4 * td; d < D; d += 64) {
-          floatx4 a = *reinterpret_cast<const floatx4*>(obuf + tr * OP + d);
-#pragma unroll
-          for (int k = 1; k < 4; ++k) a += *reinterpret_cast<const floatx4*>(obuf + (k * 16 + tr) * OP + d);
-          if (whole) {
-            *reinterpret_cast<u32x2*>(op + 2 * d) = u32x2{pack2<E>(a[0] * inv, a[1] * inv), pack2<E>(a[2] * inv, a[3] * inv)};
-          } else {
-            *reinterpret_cast<floatx4*>(wo + d) = a;
-          }
-        }
-        if (td == 0) {
-          if (!whole) {
-            float* ml = p.ws_ml + 2 * (slot * ROWS + 16 * n + tr);
-            ml[0] = Mr;
-            ml[1] = lr;
-          } else if (p.lse) {
-            p.lse[ref.tok * p.H + ref.head] =
-                lr == 0.f ? -__builtin_inff() : (Mr + __log2f(lr)) * 0.69314718055994530942f;
-          }
-        }
-      }
-    }
-    if (bad_s && threadIdx.x == 0 && !(sq.flags & LVSA_PAGED_BAD_LENGTH)) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
-    __syncthreads();                           // the exchange has been read: V tiles and bad_s may be written
+    const DecodePart part = {sq, h, rt * ROWS, sq.n * p.group, blk0, blk1,
+                             2 * (int64_t)blockIdx.x + (u_first < u - blk0 ? 1 : 0),   // see decode_slots
+                             blk0 == 0 && blk1 == nb, (sq.flags & LVSA_PAGED_BAD_LENGTH) != 0};
+    decode_part<D, E, BITS, NT>(p, part, PagedKeys{p.c, p.c.table + seq * p.c.table_str, sq.L});
     u += blk1 - blk0;
   }
 }
@@ -757,21 +793,10 @@ __device__ __forceinline__ void wait_copies() {
   static_assert(N >= 0 && N < 16, "vmcnt immediate");
   __builtin_amdgcn_s_waitcnt(0x0F70 | N);
 }
-// Four waves of 32 rows, the matrix core of each SIMD with one or two of them:
-// a wave feeds it by itself, with the products of the blocks before and after
-// while it forms the weights of its own block between them.  Two LDS places
-// each for K and V of a block of 64 keys; wave w brings tile w (16 keys).
-// 16-bit pages are copied without passing registers; of 4-bit pages the codes
-// are loaded a step ahead and written to LDS as 16-bit values, so every row is
-// decoded once for 128 query rows.
-//
-// 780 tokens of 12 heads over 4 of 256, over 31980 keys in 4 bits: 378 us with
-// plan and joining, 790 TFLOP/s (500 us with a phase of products after a phase of
-// softmax).  The decoding of K and V, their addresses, the mask and the maximum
-// stand before a step's first product, on the only wave of a SIMD: MFMA busy a
-// third of the time, vector instructions another.  4 sequences of 128 tokens, 16 heads of 128, over 16384 keys: 141 us.
-template <int D, typename E, int BITS>
-__global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(PagedAttnParams p) {
+// Rows [r0, r0 + 128) before row nrows of sequence sq and key head h over key blocks
+// [blk0, blk1), with the keys that `keys` names; see DecodePart.
+template <int D, typename E, int BITS, typename Keys>
+__device__ __forceinline__ void prefill_part(const PagedAttnParams& p, const DecodePart& part, const Keys& keys) {
   constexpr int ND = D / 32, NK = D / 16, NO = D / 32;
   constexpr int TB = 32 * D, MAT = 4 * TB;           // 16-key tile, 64-key matrix
   constexpr bool kTwoScales = D == 96 || D >= 192;
@@ -784,37 +809,17 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   const int half = lane >> 5, i32 = lane & 31;       // S^T: column (row of the tile) i32
   const int g = lane >> 4, x = lane & 15;
 
-  const PlanHead hd = *p.head;
-  if (uniform(hd.bad_cu)) {
-    spoil_rows<E>(p, D, lane, wave, 4);
-    return;
-  }
-  if (p.fill_tail) fill_tail_rows(p, D, lane, wave, 4);
-  const int shares = uniform(hd.shares), share = share_of(blockIdx.x, shares);
-  if (share < 0) return;
-  // The share's tiles from the last to the first: the part that it ends with
-  // starts at its tile's first key block and the one it starts with ends at the
-  // last, so that the work-groups of an XCD walk a head's keys at about the
-  // same place at the same time, and its L2 serves them.
-  const int64_t U = hd.per_head * p.c.Hkv;
-  int left = uniform((int)(unit_start(U, shares, share + 1) - unit_start(U, shares, share)));
-  int h = uniform(p.ends[share].h), ti = uniform(p.ends[share].tile), blk_end = uniform(p.ends[share].blk);
-  for (;;) {
-  const PlanTile tile = p.plan_tiles[ti];
-  const int seq = uniform(tile.seq), r0 = uniform(tile.r0), units = uniform(tile.units), nb = uniform(tile.blocks);
-  const PagedSeq sq = uniform(tile.sq);
-  const int blk0 = left < blk_end ? blk_end - left : 0;
-  const bool whole = blk0 == 0 && blk_end == units;
-  const int64_t slot = 2 * (int64_t)share + (left > blk_end ? 1 : 0);   // the share comes from another tile: see decode_slots
-  const int blk1 = blk_end < nb ? blk_end : nb;
-  const int nrows = sq.n * p.group;
+  const PagedSeq& sq = part.sq;
+  const int h = part.h, r0 = part.r0, nrows = part.nrows, blk0 = part.blk0, blk1 = part.blk1;
+  const int64_t slot = part.slot;
+  const bool whole = part.whole;
   const int r_last = r0 + kPagedTile < nrows ? r0 + kPagedTile - 1 : nrows - 1;
-  const int lim_min = key_limit(p, sq, r0), lim_max = key_limit(p, sq, r_last);
+  const int lim_min = keys.limit(key_limit(p, sq, r0)), lim_max = keys.limit(key_limit(p, sq, r_last));
 
   const int row = r0 + 32 * wave + i32;             // this lane's row of the pair
   const int rc = row < nrows ? row : nrows - 1;
   const RowRef ref = row_ref(p, sq, h, rc);
-  const int lim = key_limit(p, sq, rc);
+  const int lim = keys.limit(key_limit(p, sq, rc));
   shortx8 qf[NK];
   {
     const char* qp = p.q + ref.tok * p.q_str[0] + ref.head * p.q_str[1] + 16 * half;
@@ -824,14 +829,13 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
 
   const char* kbase = p.c.k + h * p.c.k_str[2];
   const char* vbase = p.c.v + h * p.c.v_str[2];
-  const int32_t* table = p.c.table + seq * p.c.table_str;
   // Wave w brings keys 16 w .. 16 w + 15 of a block (past the end: the last key).
   auto key_pos = [&](int b, int key) __attribute__((always_inline)) {
-    return key_within(b * kPagedBlock + 16 * wave + key, sq.L);
+    return key_within(b * kPagedBlock + 16 * wave + key, keys.L);
   };
-  bool bad = (sq.flags & (LVSA_PAGED_BAD_LENGTH | LVSA_PAGED_BAD_PAGE)) != 0;
+  bool bad = part.bad;
   auto row_of = [&](int b, int key, int page, int64_t& pg, int64_t& slot) __attribute__((always_inline)) {
-    const PagedRow at = paged_row(p.c, key_pos(b, key), page);
+    const PagedRow at = keys.row(key_pos(b, key), page);
     bad |= !at.ok;
     pg = at.page;
     slot = at.slot;
@@ -846,8 +850,9 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   // Copies keys 16 w .. + 15 of block b of one matrix; `page`: key x's, per lane.
   auto bring16 = [&](int b, int page, const char* base, const int64_t* str, const uint32_t* offs, lds_char* to)
       __attribute__((always_inline)) {
-    const int key0 = b * kPagedBlock + 16 * wave, slot0 = key0 - page_of(p.c, key0) * p.c.page_size;
-    if (p.short_rows && key0 + 16 <= sq.L && slot0 + 16 <= p.c.page_size) {   // the 16 keys lie in one page
+    const int key0 = b * kPagedBlock + 16 * wave;
+    int slot0;
+    if (p.short_rows && keys.together(key0, 16, &slot0)) {   // the 16 keys lie in one page
       const int pg0 = uniform(page);
       const bool ok = (uint32_t)pg0 < (uint32_t)p.c.n_pages;
       bad |= !ok;
@@ -944,7 +949,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
     }
 #pragma unroll
     for (int i = 0; i < 3; ++i) page[i] = page[i + 1];
-    page[3] = table[page_of(p.c, key_pos(blk0 + j + 4, x))];
+    page[3] = keys.page(key_pos(blk0 + j + 4, x));
 
     if (is_masked(j)) {
       const int here = lim - (blk0 + j) * kPagedBlock - 4 * half;   // keys of this block that the row attends, from 4 half on
@@ -1038,7 +1043,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
     // K of blocks 0 and 1; V of the block before the first: zeros, with P = 0
     for (int at = 16 * (int)threadIdx.x; at < MAT; at += 4096) *reinterpret_cast<lds8*>(smem + 3 * MAT + at) = shortx8{0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) page[i] = table[page_of(p.c, key_pos(blk0 + i, x))];
+    for (int i = 0; i < 4; ++i) page[i] = keys.page(key_pos(blk0 + i, x));
     if constexpr (BITS == 16) {
       bring16(blk0, page[0], kbase, p.c.k_str, koffs, smem + wave * TB);
       bring16(blk0 + 1, page[1], kbase, p.c.k_str, koffs, smem + MAT + wave * TB);
@@ -1088,7 +1093,7 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   if (__builtin_expect(odd_s != 0, 0)) {
     const int from = lim_min / kPagedBlock > blk0 ? lim_min / kPagedBlock : blk0;
     const int k1 = blk1 * kPagedBlock < lim_max ? blk1 * kPagedBlock : lim_max;
-    add_nonfinite_keys<E, BITS, 4 * NO>(p.c, table, h, from * kPagedBlock, k1, lim, 4 * half, 8,
+    add_nonfinite_keys<E, BITS, 4 * NO>(p.c, keys, h, from * kPagedBlock, k1, lim, 4 * half, 8,
                                         [&](int q, int r, uint32_t v, bool seen) __attribute__((always_inline)) {
                                           o[q >> 2][4 * (q & 3) + r] = add_nonfinite<E>(o[q >> 2][4 * (q & 3) + r], v, seen);
                                         });
@@ -1097,6 +1102,50 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(Pa
   float l = l_run + __shfl_xor(l_run, 32);
   if (bad_s) l = __builtin_nanf("");
   if (row < nrows) store_rows<D, E>(p, whole, slot, kPagedTile, row - r0, half, ref, o, ref_run.m, l);
+}
+
+// Four waves of 32 rows, the matrix core of each SIMD with one or two of them:
+// a wave feeds it by itself, with the products of the blocks before and after
+// while it forms the weights of its own block between them.  Two LDS places
+// each for K and V of a block of 64 keys; wave w brings tile w (16 keys).
+// 16-bit pages are copied without passing registers; of 4-bit pages the codes
+// are loaded a step ahead and written to LDS as 16-bit values, so every row is
+// decoded once for 128 query rows.
+//
+// 780 tokens of 12 heads over 4 of 256, over 31980 keys in 4 bits: 378 us with
+// plan and joining, 790 TFLOP/s (500 us with a phase of products after a phase of
+// softmax).  The decoding of K and V, their addresses, the mask and the maximum
+// stand before a step's first product, on the only wave of a SIMD: MFMA busy a
+// third of the time, vector instructions another.  4 sequences of 128 tokens, 16 heads of 128, over 16384 keys: 141 us.
+template <int D, typename E, int BITS>
+__global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_prefill_kernel(PagedAttnParams p) {
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const PlanHead hd = *p.head;
+  if (uniform(hd.bad_cu)) {
+    spoil_rows<E>(p, D, lane, wave, 4);
+    return;
+  }
+  if (p.fill_tail) fill_tail_rows(p, D, lane, wave, 4);
+  const int shares = uniform(hd.shares), share = share_of(blockIdx.x, shares);
+  if (share < 0) return;
+  // The share's tiles from the last to the first: the part that it ends with
+  // starts at its tile's first key block and the one it starts with ends at the
+  // last, so that the work-groups of an XCD walk a head's keys at about the
+  // same place at the same time, and its L2 serves them.
+  const int64_t U = hd.per_head * p.c.Hkv;
+  int left = uniform((int)(unit_start(U, shares, share + 1) - unit_start(U, shares, share)));
+  int h = uniform(p.ends[share].h), ti = uniform(p.ends[share].tile), blk_end = uniform(p.ends[share].blk);
+  for (;;) {
+  const PlanTile tile = p.plan_tiles[ti];
+  const int seq = uniform(tile.seq), r0 = uniform(tile.r0), units = uniform(tile.units), nb = uniform(tile.blocks);
+  const PagedSeq sq = uniform(tile.sq);
+  const int blk0 = left < blk_end ? blk_end - left : 0;
+  const bool whole = blk0 == 0 && blk_end == units;
+  const int64_t slot = 2 * (int64_t)share + (left > blk_end ? 1 : 0);   // the share comes from another tile: see decode_slots
+  const int blk1 = blk_end < nb ? blk_end : nb;
+  const DecodePart part = {sq, h, r0, sq.n * p.group, blk0, blk1, slot, whole,
+                           (sq.flags & (LVSA_PAGED_BAD_LENGTH | LVSA_PAGED_BAD_PAGE)) != 0};
+  prefill_part<D, E, BITS>(p, part, PagedKeys{p.c, p.c.table + seq * p.c.table_str, sq.L});
   left -= blk_end - blk0;
   if (left <= 0) break;
   if (--ti < 0) {
@@ -1485,7 +1534,7 @@ __global__ __launch_bounds__(512, 1) void paged_tall_kernel(PagedAttnParams p) {
   if (__builtin_expect(odd_s != 0, 0)) {
     const int from = lim_min / kPagedBlock > blk0 ? lim_min / kPagedBlock : blk0;
     const int k1 = blk1 * kPagedBlock < lim_max ? blk1 * kPagedBlock : lim_max;
-    add_nonfinite_keys<E, BITS, 4 * NO>(p.c, table, h, from * kPagedBlock, k1, lim, 4 * half, 8,
+    add_nonfinite_keys<E, BITS, 4 * NO>(p.c, PagedKeys{p.c, table, sq.L}, h, from * kPagedBlock, k1, lim, 4 * half, 8,
                                         [&](int q, int r, uint32_t v, bool seen) __attribute__((always_inline)) {
                                           o[q >> 2][4 * (q & 3) + r] = add_nonfinite<E>(o[q >> 2][4 * (q & 3) + r], v, seen);
                                         });
