@@ -312,6 +312,8 @@ typedef struct lvsa_paged_cache {
 #define LVSA_PAGED_BAD_CU 4       /* cu_seqlens not ascending within [0, N]        */
 #define LVSA_PAGED_BAD_APPEND 8   /* more new tokens than kv_lens counts           */
 #define LVSA_PAGED_BAD_POSITION 16 /* a rotation position outside the angle table  */
+#define LVSA_PAGED_BAD_BLOCK 32   /* a list of blocks that does not ascend or names one
+                                     behind its sequence's end                     */
 
 /* A batch over a cache, all device memory.  Sequence b has kv_lens[b] cached
  * tokens, position p in slot p % page_size of page page_table[b * table_stride
@@ -392,6 +394,97 @@ LVSA_API int lvsa_paged_attn_fwd(const lvsa_paged_attn_args* a, hipStream_t stre
 /* Bytes of workspace lvsa_paged_attn_fwd needs for `a` on the current device
  * (a->workspace and workspace_bytes are not read); host only.                 */
 LVSA_API int lvsa_paged_attn_workspace_query(const lvsa_paged_attn_args* a, int64_t* bytes);
+
+/* Parts of a cache instead of all of it.  A page holds page_size / block blocks
+ * of `block` slots (a divisor of the page size); block j of a sequence is its
+ * positions j * block .. (j + 1) * block - 1.
+ *
+ * Writes the mean key (of the tokens there are, in fp32) of
+ * every block that holds one of the newest tokens, or of every block of every
+ * sequence where the batch has no cu_seqlens.  means: part i, head h of page p at
+ * means + p * m_str[0] + i * m_str[1] + h * m_str[2] floats, D of them, rows at
+ * multiples of 16 bytes.  Blocks of a bad page, length or row range are left out.
+ * Sequences that share a page and count different numbers of tokens in one of its
+ * blocks leave the mean of either.  The reference has no counterpart.         */
+LVSA_API int lvsa_paged_block_means(const lvsa_paged_cache* cache, const lvsa_paged_batch* batch, float* means,
+                                    const int64_t m_str[3], int32_t block, hipStream_t stream);
+
+/* Selects blocks by their means.  Rows of a sequence are taken in tiles of `tile`;
+ * tile i of sequence b is list cu_seqlens[b] / tile + b + i of N / tile + B lists,
+ * with tile = 1 list cu_seqlens[b] + i of N.  For every list and key head the `top`
+ * blocks among those that a row of the tile may attend (with `causal` up to its last
+ * row's): blocks below `first`, those of the rows' own positions with `last` - 1
+ * before them (`last` 0: none of these), then the highest sums of q.mean over the
+ * tile's rows and the head's query heads, in 64 bits; equal ones by the lower
+ * number, NaN last.  blocks [lists, Hkv, top]: ascending, -1 behind; -1 throughout
+ * for lists of no tile and for bad lengths and row ranges; a block whose page is bad
+ * counts as NaN.  What is always selected has to fit: first, and for last > 0 last -
+ * 1 and the blocks that a tile's rows may lie in, (tile - 2) / block + 2 (1 for a tile
+ * of one), are at most `top` together, and top at most 1024.                    */
+typedef struct lvsa_paged_select_args {
+  lvsa_paged_cache cache;
+  lvsa_paged_batch batch;
+  const void* q;                         /* [N, H, D]                           */
+  const float* means;
+  int32_t* blocks;
+  int64_t q_str[2], m_str[3];
+  int32_t H, block, top, tile, first, last, causal;
+} lvsa_paged_select_args;
+LVSA_API int lvsa_paged_select(const lvsa_paged_select_args* a, hipStream_t stream);
+
+/* lvsa_paged_attn_fwd over lists of blocks: a row attends, of the keys that it would
+ * attend there, those of its tile's list (see lvsa_paged_select).  A list ends at its
+ * first negative number; before it blocks ascend and start below kv_lens.  NaN: rows
+ * whose list does not, or names a block on a bad page, rows of a sequence with a bad
+ * length, and all rows where cu_seqlens does not ascend.  max_q_len and max_kv_len
+ * of `attn` are not read.                                                     */
+typedef struct lvsa_paged_block_attn_args {
+  lvsa_paged_attn_args attn;
+  const int32_t* blocks;
+  int32_t block, top, tile;
+} lvsa_paged_block_attn_args;
+LVSA_API int lvsa_paged_block_attn_fwd(const lvsa_paged_block_attn_args* a, hipStream_t stream);
+LVSA_API int lvsa_paged_block_attn_workspace_query(const lvsa_paged_block_attn_args* a, int64_t* bytes);
+
+/* What the newest rows give to every cached token of their sequence: weights at
+ * page p, slot t, head h (weights + p * w_str[0] + t * w_str[1] + h * w_str[2]) +=
+ * sum over the sequence's rows that attend the token and the head's query heads of
+ * exp(scale q.k - lse), with lse [N, H] as lvsa_paged_attn_fwd gives it.  The newest
+ * tokens' own weights start from 0, with `accumulate` 0 all of the sequence's do.
+ * Rows whose lse is not finite give nothing; sequences without new rows, with a bad
+ * length or row range and tokens on a bad page are left alone.  `max_q_len` (0:
+ * unknown) only chooses a kernel.                                             */
+typedef struct lvsa_paged_weights_args {
+  lvsa_paged_cache cache;
+  lvsa_paged_batch batch;
+  const void* q; const float* lse; float* weights;
+  int64_t q_str[2], w_str[3];
+  float scale;
+  int32_t H, causal, accumulate, max_q_len;
+} lvsa_paged_weights_args;
+LVSA_API int lvsa_paged_weights(const lvsa_paged_weights_args* a, hipStream_t stream);
+
+/* Cuts every sequence to `keep` tokens a head: the first `first`, the newest `last`
+ * and of the others those of the largest weights (equal ones by the lower position,
+ * NaN last); shorter sequences keep all.  The kept ones' keys, values, scales and
+ * weights move, in their order, to positions 0 .. keep - 1 on the pages of
+ * new_table [B] (rows of new_pages, new_stride apart), or, without it, on the
+ * sequence's own first pages.  kept [B, Hkv, keep]: their old positions, -1 behind;
+ * new_lens [B]: how many.  A sequence with a bad length or a bad page (a new one
+ * that is one of its old ones among them) is not moved: -1, and a length of 0 with
+ * new_table, kv_lens' without.  No page of new_table may be another sequence's, in
+ * either table, and pages that sequences share are not cut in place.  cu_seqlens
+ * and N of the batch are not used.                                            */
+typedef struct lvsa_paged_evict_args {
+  lvsa_paged_cache cache;
+  lvsa_paged_batch batch;
+  float* weights;
+  const int32_t* new_table;
+  int32_t* kept; int32_t* new_lens;
+  int64_t w_str[3], new_stride;
+  int32_t new_pages, keep, first, last;
+} lvsa_paged_evict_args;
+LVSA_API int lvsa_paged_evict(const lvsa_paged_evict_args* a, hipStream_t stream);
 
 /* Library identification and error reporting. */
 LVSA_API const char* lvsa_version(void);

@@ -22,6 +22,7 @@ _BLOCK = ("BlockSparseAttentionWrapper", "single_prefill_with_kv_cache", "HipDua
           "get_shared_runner")
 
 _PAGED = ("PagedKVCache", "paged_kv_append", "paged_kv_gather", "paged_attention")
+_PARTS = ("paged_kv_block_means", "paged_kv_select", "paged_block_attention", "paged_kv_weights", "paged_kv_evict")
 
 
 def __getattr__(name):
@@ -31,6 +32,8 @@ def __getattr__(name):
         from . import block_sparse as m
     elif name in _PAGED:
         from . import paged_kv as m
+    elif name in _PARTS:
+        from . import paged_parts as m
     elif name == "build_global_kv":
         from . import global_kv as m
     elif name == "DistributedLVSAProcessor":
@@ -44,4 +47,4 @@ def __getattr__(name):
     return value
 
 
-__all__ = list(_SPARSE) + list(_BLOCK) + list(_PAGED) + ["build_global_kv", "DistributedLVSAProcessor", "step_attention"]
+__all__ = list(_SPARSE) + list(_BLOCK) + list(_PAGED) + list(_PARTS) + ["build_global_kv", "DistributedLVSAProcessor", "step_attention"]

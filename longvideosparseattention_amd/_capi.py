@@ -107,6 +107,7 @@ class AttnArgs(C.Structure):
 
 # Bits of a paged cache's status word (LVSA_PAGED_*).
 PAGED_BAD_PAGE, PAGED_BAD_LENGTH, PAGED_BAD_CU, PAGED_BAD_APPEND, PAGED_BAD_POSITION = 1, 2, 4, 8, 16
+PAGED_BAD_BLOCK = 32
 
 _Str2 = C.c_int64 * 2
 
@@ -147,6 +148,38 @@ class PagedAttnArgs(C.Structure):
     ]
 
 
+class PagedSelectArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("batch", PagedBatch),
+        ("q", C.c_void_p), ("means", C.c_void_p), ("blocks", C.c_void_p), ("q_str", _Str2), ("m_str", _Str3),
+        ("H", C.c_int32), ("block", C.c_int32), ("top", C.c_int32), ("tile", C.c_int32), ("first", C.c_int32),
+        ("last", C.c_int32), ("causal", C.c_int32),
+    ]
+
+
+class PagedBlockAttnArgs(C.Structure):
+    _fields_ = [
+        ("attn", PagedAttnArgs), ("blocks", C.c_void_p), ("block", C.c_int32), ("top", C.c_int32), ("tile", C.c_int32),
+    ]
+
+
+class PagedWeightsArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("batch", PagedBatch),
+        ("q", C.c_void_p), ("lse", C.c_void_p), ("weights", C.c_void_p), ("q_str", _Str2), ("w_str", _Str3),
+        ("scale", C.c_float), ("H", C.c_int32), ("causal", C.c_int32), ("accumulate", C.c_int32), ("max_q_len", C.c_int32),
+    ]
+
+
+class PagedEvictArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("batch", PagedBatch),
+        ("weights", C.c_void_p), ("new_table", C.c_void_p), ("kept", C.c_void_p), ("new_lens", C.c_void_p),
+        ("w_str", _Str3), ("new_stride", C.c_int64),
+        ("new_pages", C.c_int32), ("keep", C.c_int32), ("first", C.c_int32), ("last", C.c_int32),
+    ]
+
+
 # Every symbol the header declares, with its ctypes signature.
 SIGNATURES = {
     "lvsa_mask_sizes_query": (C.c_int, [C.POINTER(MaskParams), C.POINTER(MaskSizes)]),
@@ -170,6 +203,13 @@ SIGNATURES = {
                                     C.c_void_p]),
     "lvsa_paged_attn_fwd": (C.c_int, [C.POINTER(PagedAttnArgs), C.c_void_p]),
     "lvsa_paged_attn_workspace_query": (C.c_int, [C.POINTER(PagedAttnArgs), C.POINTER(C.c_int64)]),
+    "lvsa_paged_block_means": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedBatch), C.c_void_p, C.POINTER(C.c_int64),
+                                         C.c_int32, C.c_void_p]),
+    "lvsa_paged_select": (C.c_int, [C.POINTER(PagedSelectArgs), C.c_void_p]),
+    "lvsa_paged_block_attn_fwd": (C.c_int, [C.POINTER(PagedBlockAttnArgs), C.c_void_p]),
+    "lvsa_paged_block_attn_workspace_query": (C.c_int, [C.POINTER(PagedBlockAttnArgs), C.POINTER(C.c_int64)]),
+    "lvsa_paged_weights": (C.c_int, [C.POINTER(PagedWeightsArgs), C.c_void_p]),
+    "lvsa_paged_evict": (C.c_int, [C.POINTER(PagedEvictArgs), C.c_void_p]),
     "lvsa_version": (C.c_char_p, []),
     "lvsa_last_error": (C.c_char_p, []),
 }

@@ -45,6 +45,13 @@ SOURCES = {
     "lvsa_paged_d128.hip": [],
     "lvsa_paged_d192.hip": [],
     "lvsa_paged_d256.hip": [],
+    "lvsa_paged_blocks.hip": [],
+    "lvsa_paged_evict.hip": [],
+    "lvsa_paged_list_d64.hip": [],
+    "lvsa_paged_list_d96.hip": [],
+    "lvsa_paged_list_d128.hip": [],
+    "lvsa_paged_list_d192.hip": [],
+    "lvsa_paged_list_d256.hip": [],
 }
 
 HIPCC_FLAGS = [

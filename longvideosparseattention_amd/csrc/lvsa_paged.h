@@ -222,13 +222,64 @@ __host__ __device__ inline DecodeSlots decode_slots(int64_t U, int G, int64_t u0
 
 // p / d as (p * mul) >> shift, exact for 0 <= p < 2^31: with 2^l >= d and mul =
 // floor(2^(31 + l) / d) + 1, mul * d exceeds 2^(31 + l) by at most 2^l.
-inline void set_page_size(PagedView* v, int page_size) {
+struct Divisor {
+  uint32_t mul, shift;
+  int32_t by;
+};
+inline Divisor divisor(int d) {
   int l = 0;
-  while ((1LL << l) < page_size) ++l;
-  v->page_size = page_size;
-  v->ps_mul = (uint32_t)((1ULL << (31 + l)) / (uint64_t)page_size + 1);
-  v->ps_shift = (uint32_t)(31 + l);
+  while ((1LL << l) < d) ++l;
+  return Divisor{(uint32_t)((1ULL << (31 + l)) / (uint64_t)d + 1), (uint32_t)(31 + l), d};
 }
+__host__ __device__ inline int operator/(int p, const Divisor& d) { return (int)(((uint64_t)(uint32_t)p * d.mul) >> d.shift); }
+
+inline void set_page_size(PagedView* v, int page_size) {
+  const Divisor d = divisor(page_size);
+  v->page_size = page_size;
+  v->ps_mul = d.mul;
+  v->ps_shift = d.shift;
+}
+
+// ── tiles of rows and blocks of keys (lvsa_paged_list.h) ─────────────────────
+
+// Blocks of `block` slots, `parts` to a page; rows of a sequence in tiles of `tile`,
+// `lists` of which the batch may have, each with up to `top` blocks a key head.
+struct ListView {
+  Divisor block, parts, tile;
+  int32_t lists, top;
+};
+constexpr int kListMax = 1024;         // blocks of a list: what a work-group keeps of it is 12 KB of LDS
+
+// Tiles of sequence `s`: from where on, and how many.
+__host__ __device__ inline int64_t first_list(const ListView& v, int s, const PagedSeq& q) {
+  return v.tile.by == 1 ? q.t0 : (int64_t)(q.t0 / v.tile) + s;
+}
+__host__ __device__ inline int list_count(const ListView& v, const PagedSeq& q) { return (int)(((int64_t)q.n + v.tile.by - 1) / v.tile.by); }
+
+struct BlockAttnParams {
+  ListView v;
+  const int32_t* blocks;               // [lists][Hkv][top]
+  int32_t subs, splits;                // row tiles of a list, work-groups that share its keys
+  int64_t units;                       // lists x subs x key heads
+};
+int paged_block_attn_d64(const PagedAttnParams& p, const BlockAttnParams& l, int bits, int rows, bool bf16, hipStream_t stream);
+int paged_block_attn_d96(const PagedAttnParams& p, const BlockAttnParams& l, int bits, int rows, bool bf16, hipStream_t stream);
+int paged_block_attn_d128(const PagedAttnParams& p, const BlockAttnParams& l, int bits, int rows, bool bf16, hipStream_t stream);
+int paged_block_attn_d192(const PagedAttnParams& p, const BlockAttnParams& l, int bits, int rows, bool bf16, hipStream_t stream);
+int paged_block_attn_d256(const PagedAttnParams& p, const BlockAttnParams& l, int bits, int rows, bool bf16, hipStream_t stream);
+
+// Accumulated weights (lvsa_paged_weights.h).
+struct WeightsParams {
+  const float* lse;
+  char* w;
+  int64_t w_str[3];                    // bytes
+  int32_t accumulate;
+};
+int paged_weights_d64(const PagedAttnParams& p, const WeightsParams& w, int bits, bool bf16, hipStream_t stream);
+int paged_weights_d96(const PagedAttnParams& p, const WeightsParams& w, int bits, bool bf16, hipStream_t stream);
+int paged_weights_d128(const PagedAttnParams& p, const WeightsParams& w, int bits, bool bf16, hipStream_t stream);
+int paged_weights_d192(const PagedAttnParams& p, const WeightsParams& w, int bits, bool bf16, hipStream_t stream);
+int paged_weights_d256(const PagedAttnParams& p, const WeightsParams& w, int bits, bool bf16, hipStream_t stream);
 
 // End of the keys that row r attends, and the key blocks of the tile of rows
 // [r0, r1].
@@ -294,6 +345,31 @@ __device__ __forceinline__ int64_t wave_scan(int64_t x, int lane, int count = 64
     if (lane >= d) x += y;
   }
   return x;
+}
+
+// Work-groups take the units of all sequences in turn: `count` says how many a
+// sequence has, `work` does unit i of sequence s.
+template <typename Count, typename Work>
+__device__ __forceinline__ void walk_units(const PagedView& c, Count count, Work work) {
+  const int lane = threadIdx.x & 63;
+  int64_t base = 0, u = blockIdx.x;            // units before these sequences, the next one of this work-group
+  int flags = 0;
+  for (int s0 = 0; s0 < c.B; s0 += 64) {
+    PagedSeq mine = {};
+    int64_t n = 0;
+    if (s0 + lane < c.B) {
+      mine = c.cu ? paged_seq(c, s0 + lane) : paged_seq(c, 0, 0, c.lens[s0 + lane]);
+      flags |= mine.flags;
+      if (!mine.flags) n = count(mine);
+    }
+    const int64_t upto = wave_scan(n, lane), end = base + from_lane(upto, 63);
+    for (; u < end; u += gridDim.x) {
+      const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(base + upto > u));
+      work(s0 + at, from_lane(mine, at), u - base - from_lane(upto - n, at));
+    }
+    base = end;
+  }
+  if (blockIdx.x == 0 && threadIdx.x < 64 && flags) paged_flag(c, flags);
 }
 
 }  // namespace

@@ -2,72 +2,17 @@
 // and 4-bit quantisation on the way), reading a cache back, the merge of
 // attention partials, and the C ABI.  The attention kernels are in
 // lvsa_paged_attn.h.
-#include "lvsa_paged.h"
-
-#include <mutex>
+#include "lvsa_paged_host.h"
+#include "lvsa_paged_rows.h"
 
 using namespace lvsa;
 
 namespace lvsa {
 namespace {
 
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-
 constexpr int kMaxGrid = 1 << 20;      // work-groups of a launch that walks its rows
 constexpr int kMaxGridY = 1 << 15;     // sequences of a gather's launch
 constexpr int kFewTokens = 10;         // of an append, per compute unit
-
-template <typename E> struct Half;
-template <> struct Half<__bf16> {
-  static constexpr uint32_t kNaN = 0x7fc0u;
-  __device__ static void unpack(u32x4 u, float* x) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __builtin_bit_cast(float, u[i] << 16);
-      x[2 * i + 1] = __builtin_bit_cast(float, u[i] & 0xffff0000u);
-    }
-  }
-};
-template <> struct Half<_Float16> {
-  static constexpr uint32_t kNaN = 0x7e00u;
-  __device__ static void unpack(u32x4 u, float* x) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)u[i]);
-      x[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(u[i] >> 16));
-    }
-  }
-};
-template <typename E>
-__device__ __forceinline__ u32x4 pack8(const float* x) {
-  u32x4 u;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    typedef E v2 __attribute__((ext_vector_type(2)));
-    u[i] = __builtin_bit_cast(uint32_t, v2{(E)x[2 * i], (E)x[2 * i + 1]});
-  }
-  return u;
-}
-
-// Eight 4-bit values at byte scale `s` (2^(s - 127), 255: NaN).  Exact in both
-// types for the scales that the append writes.
-template <typename E>
-__device__ __forceinline__ u32x4 unpack_e2m1(uint32_t codes, uint32_t s) {
-  const float f = __builtin_bit_cast(float, s << 23);
-  u32x4 u;
-  if constexpr (__is_same(E, __bf16)) {
-    u[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, f, 0));
-    u[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, f, 1));
-    u[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, f, 2));
-    u[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, f, 3));
-  } else {
-    u[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, f, 0));
-    u[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, f, 1));
-    u[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, f, 2));
-    u[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, f, 3));
-  }
-  return u;
-}
 
 // x in 32 bits, rounded to odd: the two neighbours' sticky bit is kept, so that
 // a later rounding to few bits (and a comparison with a number of few bits)
@@ -653,99 +598,6 @@ __global__ __launch_bounds__(256) void paged_merge_tiles_kernel(PagedAttnParams 
 __global__ void paged_take_status_kernel(int32_t* status, int32_t* found) { *found = atomicExch(status, 0); }
 
 // ─────────────────────────────── host side ─────────────────────────────────
-
-int cu_count() {
-  static std::mutex mu;
-  static int cached[64] = {0};
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) {
-    (void)hipGetLastError();       // no device: sizes are still answered
-    return 256;
-  }
-  std::lock_guard<std::mutex> lock(mu);
-  if (cached[dev] == 0) {
-    int n = 0;
-    cached[dev] = hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && n > 0 ? n : 256;
-  }
-  return cached[dev];
-}
-
-bool aligned16(int64_t x) { return (x & 15) == 0; }
-
-// Whether two [N, heads, D] tensors of 16-bit elements (strides in bytes) lie within
-// each other's bounds.
-bool share_memory(const void* a, const int64_t* as, int ah, const void* b, const int64_t* bs, int bh, int N, int D) {
-  auto bound = [&](const void* at, const int64_t* str, int heads, bool high) {
-    int64_t x = (int64_t)(uintptr_t)at + (high ? 2 * (int64_t)D : 0);
-    const int64_t far[2] = {(N - 1) * str[0], (heads - 1) * str[1]};
-    for (int64_t f : far) x += high == (f > 0) ? f : 0;
-    return x;
-  };
-  return bound(a, as, ah, false) < bound(b, bs, bh, true) && bound(b, bs, bh, false) < bound(a, as, ah, true);
-}
-
-// Checks a cache and a batch and forms the device's view of them.
-int paged_view(const char* what, const lvsa_paged_cache* c, const lvsa_paged_batch* b, bool rows, PagedView* v) {
-  LVSA_REQUIRE(c->D == 64 || c->D == 96 || c->D == 128 || c->D == 192 || c->D == 256, LVSA_ERR_UNSUPPORTED,
-               "%s: head_dim %d not supported (64, 96, 128, 192, 256)", what, c->D);
-  LVSA_REQUIRE(c->bits == 16 || c->bits == 4, LVSA_ERR_UNSUPPORTED, "%s: caches hold 16 or 4 bits, not %d", what, c->bits);
-  LVSA_REQUIRE(c->dtype == LVSA_BF16 || c->dtype == LVSA_FP16, LVSA_ERR_UNSUPPORTED, "%s: dtype %d: bf16 or fp16", what,
-               c->dtype);
-  LVSA_REQUIRE(c->n_pages >= 1 && c->page_size >= 1 && c->Hkv >= 1, LVSA_ERR_INVALID_ARG,
-               "%s: %d pages of %d slots, %d heads", what, c->n_pages, c->page_size, c->Hkv);
-  LVSA_REQUIRE(c->k && c->v && (c->bits == 16 || (c->k_scale && c->v_scale)), LVSA_ERR_INVALID_ARG,
-               "%s: null cache pointer", what);
-  LVSA_REQUIRE(b->B >= 0 && b->max_pages >= 0 && b->N >= 0 && b->table_stride >= b->max_pages, LVSA_ERR_INVALID_ARG,
-               "%s: batch of %d sequences, %d pages (rows %lld apart), %d rows", what, b->B, b->max_pages,
-               (long long)b->table_stride, b->N);
-  LVSA_REQUIRE(b->B == 0 || (b->kv_lens && (b->page_table || b->max_pages == 0) && (!rows || b->cu_seqlens)),
-               LVSA_ERR_INVALID_ARG, "%s: null batch pointer", what);
-  LVSA_REQUIRE((int64_t)b->max_pages * c->page_size < (1LL << 31) - 4096, LVSA_ERR_UNSUPPORTED,
-               "%s: %d pages of %d slots: positions must stay below 2^31 - 4096", what, b->max_pages, c->page_size);
-  const int64_t unit = c->bits == 16 ? 2 : 1;
-  v->k = (char*)c->k;
-  v->v = (char*)c->v;
-  v->ks = (uint8_t*)c->k_scale;
-  v->vs = (uint8_t*)c->v_scale;
-  bool ok = aligned16((int64_t)(uintptr_t)c->k) && aligned16((int64_t)(uintptr_t)c->v);
-  for (int i = 0; i < 3; ++i) {
-    v->k_str[i] = c->k_str[i] * unit;
-    v->v_str[i] = c->v_str[i] * unit;
-    v->ks_str[i] = c->ks_str[i];
-    v->vs_str[i] = c->vs_str[i];
-    ok = ok && aligned16(v->k_str[i]) && aligned16(v->v_str[i]);
-  }
-  LVSA_REQUIRE(ok, LVSA_ERR_INVALID_ARG, "%s: cache rows must start at multiples of 16 bytes", what);
-  v->n_pages = c->n_pages;
-  v->Hkv = c->Hkv;
-  set_page_size(v, c->page_size);
-  v->status = c->status;
-  v->cu = b->cu_seqlens;
-  v->lens = b->kv_lens;
-  v->table = b->page_table;
-  v->table_str = b->table_stride;
-  v->B = b->B;
-  v->max_pages = b->max_pages;
-  v->N = b->N;
-  return LVSA_OK;
-}
-
-template <template <int, typename, int> class L, typename... A>
-int by_type(int D, int dtype, int bits, A&&... a) {
-#define LVSA_PAGED_CASE(d)                                                             \
-  case d:                                                                              \
-    if (dtype == LVSA_BF16) return bits == 16 ? L<d, __bf16, 16>::go(a...) : L<d, __bf16, 4>::go(a...); \
-    return bits == 16 ? L<d, _Float16, 16>::go(a...) : L<d, _Float16, 4>::go(a...);
-  switch (D) {
-    LVSA_PAGED_CASE(64)
-    LVSA_PAGED_CASE(96)
-    LVSA_PAGED_CASE(128)
-    LVSA_PAGED_CASE(192)
-    LVSA_PAGED_CASE(256)
-  }
-#undef LVSA_PAGED_CASE
-  return LVSA_ERR_UNSUPPORTED;
-}
 
 template <int D, typename E, int BITS> struct Append {
   static int go(const AppendParams& p, hipStream_t stream) {

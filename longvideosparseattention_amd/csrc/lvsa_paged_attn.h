@@ -220,6 +220,7 @@ __device__ __forceinline__ void add_nonfinite_keys(const PagedView& c, const Key
 // The keys that a tile of rows walks, numbered from 0 to L - 1: all of a
 // sequence's by position, each looked up in the page table ...
 struct PagedKeys {
+  static constexpr bool kStaged = false;      // looked up and checked before; there may be none
   const PagedView& c;
   const int32_t* table;
   int L;
@@ -482,7 +483,7 @@ __device__ __forceinline__ void decode_part(const PagedAttnParams& p, const Deco
 
   // Two steps in flight: while one is computed the next one's rows are on
   // their way, and the page numbers of the one after that.
-  {
+  if (!Keys::kStaged || blk0 < blk1) {
     Step<D, BITS, T> sa, sb;
     int page[T];
     load_pages(blk0, page);
@@ -572,7 +573,7 @@ __device__ __forceinline__ void decode_part(const PagedAttnParams& p, const Deco
       }
     }
   }
-  if (bad_s && threadIdx.x == 0 && !(sq.flags & LVSA_PAGED_BAD_LENGTH)) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
+  if (!Keys::kStaged && bad_s && threadIdx.x == 0 && !(sq.flags & LVSA_PAGED_BAD_LENGTH)) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
   __syncthreads();                           // the exchange has been read: V tiles and bad_s may be written
 }
 
@@ -1088,7 +1089,7 @@ __device__ __forceinline__ void prefill_part(const PagedAttnParams& p, const Dec
   // A bad page seen by any wave spoils the tile.
   if (__builtin_amdgcn_ballot_w64(bad) && lane == 0) bad_s = 1;
   __syncthreads();
-  if (bad_s && threadIdx.x == 0 && !(sq.flags & LVSA_PAGED_BAD_LENGTH)) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
+  if (!Keys::kStaged && bad_s && threadIdx.x == 0 && !(sq.flags & LVSA_PAGED_BAD_LENGTH)) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
 
   if (__builtin_expect(odd_s != 0, 0)) {
     const int from = lim_min / kPagedBlock > blk0 ? lim_min / kPagedBlock : blk0;

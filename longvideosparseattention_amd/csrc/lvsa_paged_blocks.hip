@@ -1,0 +1,559 @@
+// Blocks of the paged key/value cache on gfx950: their mean keys, the selection of
+// blocks by them, and the C ABI of what works on parts of a cache.  The attention
+// over selected blocks is in lvsa_paged_list.h, the accumulated weights in
+// lvsa_paged_weights.h, eviction in lvsa_paged_evict.hip.
+#include "lvsa_paged_host.h"
+#include "lvsa_paged_list.h"
+#include "lvsa_paged_rows.h"
+
+using namespace lvsa;
+
+namespace lvsa {
+namespace {
+
+struct MeansParams {
+  PagedView c;
+  char* means;
+  int64_t m_str[3];                      // bytes
+  Divisor block, parts;
+};
+
+// ────────────────────────────── mean keys ──────────────────────────────────
+
+// One work-group per block and head: a thread sums 8 elements of every RPP-th key,
+// the sums are joined in LDS.  fp32 within a thread (at most block / RPP keys), 64
+// bits across them, one rounding at the end.  Bound by the keys' bytes.
+template <int D, typename E, int BITS>
+__global__ __launch_bounds__(256) void paged_means_kernel(MeansParams p) {
+  constexpr int CH = D / 8, RPP = 256 / CH;
+  __shared__ float sum_s[RPP][D];
+  const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
+  // the blocks that hold new tokens, or all
+  auto first_block = [&](const PagedSeq& s) __attribute__((always_inline)) { return p.c.cu && s.first > 0 ? s.first / p.block : 0; };
+  auto count = [&](const PagedSeq& s) __attribute__((always_inline)) {
+    if (s.L == 0 || (p.c.cu && s.n == 0)) return (int64_t)0;
+    return ((int64_t)((s.L - 1) / p.block) + 1 - first_block(s)) * p.c.Hkv;
+  };
+  walk_units(p.c, count, [&](int seq, const PagedSeq& sq, int64_t u) __attribute__((always_inline)) {
+    const int i = (int)quotient(u, p.c.Hkv), h = (int)(u - (int64_t)i * p.c.Hkv);
+    const int b = first_block(sq) + i, entry = b / p.parts, part = b - entry * p.parts.by;
+    const int page = p.c.table[seq * p.c.table_str + entry];
+    if ((uint32_t)page >= (uint32_t)p.c.n_pages) {
+      if (threadIdx.x == 0) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
+      return;
+    }
+    const int left = sq.L - b * p.block.by, keys = left < p.block.by ? left : p.block.by;
+    const int64_t slot0 = (int64_t)part * p.block.by;
+    const char* kb = p.c.k + page * p.c.k_str[0] + slot0 * p.c.k_str[1] + h * p.c.k_str[2];
+    const uint8_t* sb = BITS == 4 ? p.c.ks + page * p.c.ks_str[0] + slot0 * p.c.ks_str[1] + h * p.c.ks_str[2] : nullptr;
+    float acc[8] = {};
+    if (r0 < RPP)
+      for (int r = r0; r < keys; r += RPP) {
+        float x[8];
+        if constexpr (BITS == 16) {
+          Half<E>::unpack(*reinterpret_cast<const u32x4*>(kb + r * p.c.k_str[1] + 16 * c), x);
+        } else {
+          const uint32_t codes = *reinterpret_cast<const uint32_t*>(kb + r * p.c.k_str[1] + 4 * c);
+          Half<__bf16>::unpack(unpack_e2m1<__bf16>(codes, sb[r * p.c.ks_str[1] + (c >> 2)]), x);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] += x[j];
+      }
+    if (r0 < RPP)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum_s[r0][8 * c + j] = acc[j];
+    __syncthreads();
+    if (threadIdx.x < D) {
+      double s = 0.0;
+      const int n = keys < RPP ? keys : RPP;
+      for (int r = 0; r < n; ++r) s += (double)sum_s[r][threadIdx.x];
+      float* m = reinterpret_cast<float*>(p.means + page * p.m_str[0] + part * p.m_str[1] + h * p.m_str[2]);
+      m[threadIdx.x] = (float)(s / (double)keys);
+    }
+    __syncthreads();
+  });
+}
+
+// ────────────────────────────── selection ──────────────────────────────────
+
+struct SelectParams {
+  PagedView c;
+  ListView v;
+  const char* q;
+  const char* means;
+  int32_t* blocks;
+  int64_t q_str[2], m_str[3];            // bytes
+  int32_t H, group, first, last, causal;
+};
+
+constexpr int kSelectKeys = 4096;        // blocks ranked at a time
+
+// A score as a number that sorts like it: NaN below -inf, 0 and -0 alike.
+__device__ __forceinline__ uint64_t rank_of(double s) {
+  if (s != s) return 0;
+  const uint64_t b = __builtin_bit_cast(uint64_t, s + 0.0);
+  return b >> 63 ? ~b : b | 1ull << 63;
+}
+
+// LDS of a selection: ranks and numbers of candidate blocks, in ascending order.
+struct Ranks {
+  uint64_t key[kSelectKeys];
+  int id[kSelectKeys];
+  int sum[2][4];
+  uint64_t bound[2][4];
+};
+
+// Leaves the `top` highest of n ranks, equal ones from the front, in their order.
+// The work-group (256) finds the top-th highest rank by halving the range between
+// the lowest and the highest, and stops where a bound cuts off exactly `top`.
+__device__ __forceinline__ void keep_highest(Ranks& r, int n, int top) {
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  constexpr uint64_t kAlways = ~0ull;
+  uint64_t lo = kAlways, hi = 0;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const uint64_t k = r.key[i];
+    if (k < lo) lo = k;
+    if (k > hi && k != kAlways) hi = k;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint64_t a = __shfl_xor((unsigned long long)lo, d), b = __shfl_xor((unsigned long long)hi, d);
+    if (a < lo) lo = a;
+    if (b > hi) hi = b;
+  }
+  if (lane == 0) {
+    r.bound[0][wave] = lo;
+    r.bound[1][wave] = hi;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (r.bound[0][w] < lo) lo = r.bound[0][w];
+    if (r.bound[1][w] > hi) hi = r.bound[1][w];
+  }
+  // at least `top` ranks are >= lo, and fewer are > hi
+  int above = -1, parity = 0;            // ranks >= lo where that is exactly `top`
+  while (lo < hi) {
+    const uint64_t mid = lo + (hi - lo) / 2 + 1;
+    int count = 0;
+    for (int i = threadIdx.x - lane; i < n; i += 256)
+      count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i + lane < n && r.key[i + lane < n ? i + lane : 0] >= mid));
+    if (lane == 0) r.sum[parity][wave] = count;
+    __syncthreads();
+    count = r.sum[parity][0] + r.sum[parity][1] + r.sum[parity][2] + r.sum[parity][3];
+    parity ^= 1;
+    if (count >= top) lo = mid;
+    else hi = mid - 1;
+    if (count == top) {
+      above = top;
+      break;
+    }
+  }
+  // all above lo, and of those equal to it the first ones
+  int equal = kSelectKeys;
+  if (above < 0) {
+    int count = 0;
+    for (int i = threadIdx.x - lane; i < n; i += 256)
+      count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i + lane < n && r.key[i + lane < n ? i + lane : 0] > lo));
+    if (lane == 0) r.sum[parity][wave] = count;
+    __syncthreads();
+    equal = top - (r.sum[parity][0] + r.sum[parity][1] + r.sum[parity][2] + r.sum[parity][3]);
+    parity ^= 1;
+  }
+  __syncthreads();                       // r.sum has been read
+  int put = 0, seen = 0;                 // kept so far, equal ones so far
+  const uint64_t before = (1ull << lane) - 1;
+  for (int i0 = 0; i0 < n; i0 += 256) {
+    const int i = i0 + (int)threadIdx.x;
+    const uint64_t k = i < n ? r.key[i] : 0;
+    const int id = i < n ? r.id[i] : 0;
+    const uint64_t gt = __builtin_amdgcn_ballot_w64(i < n && k > lo), eq = __builtin_amdgcn_ballot_w64(i < n && k == lo);
+    if (lane == 0) {
+      r.sum[0][wave] = __builtin_popcountll(gt);
+      r.sum[1][wave] = __builtin_popcountll(eq);
+    }
+    __syncthreads();                     // the ranks of these 256 have been read, too
+    int g0 = 0, e0 = 0, gs = 0, es = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      g0 += w < wave ? r.sum[0][w] : 0;
+      e0 += w < wave ? r.sum[1][w] : 0;
+      gs += r.sum[0][w];
+      es += r.sum[1][w];
+    }
+    const int g = g0 + __builtin_popcountll(gt & before), e = e0 + __builtin_popcountll(eq & before);
+    const int e_left = equal - seen;     // equal ones that still find room
+    const bool mine = gt >> lane & 1, also = (eq >> lane & 1) && e < e_left;
+    if (mine || also) {
+      const int at = put + g + (e < e_left ? e : e_left);
+      r.key[at] = k;
+      r.id[at] = id;
+    }
+    put += gs + (es < e_left ? es : e_left);
+    seen += es < e_left ? es : e_left;
+    __syncthreads();
+  }
+}
+
+// One work-group per list and key head: sums the tile's queries, scores every block
+// with it, eight lanes a block, and keeps the highest.  64-bit sums, so that which of
+// two blocks is the higher does not depend on the order they were summed in (short of
+// differences of 1e-15): a list is the same on every device and beside every batch.
+template <int D, typename E>
+__global__ __launch_bounds__(256) void paged_select_kernel(SelectParams p) {
+  constexpr int CH = D / 8, RPP = 256 / CH;
+  __shared__ Ranks ranks;
+  __shared__ double q_s[D];
+  double* part_s = reinterpret_cast<double*>(ranks.key);     // [RPP][D]: before any rank is there
+  static_assert(RPP * D <= kSelectKeys, "sums of the queries");
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  if (blockIdx.x == 0 && wave == 0) {
+    int flags = 0;
+    for (int s = lane; s < p.c.B; s += 64) flags |= paged_seq(p.c, s).flags;
+    if (flags) paged_flag(p.c, flags);
+  }
+  const int64_t total = (int64_t)p.v.lists * p.c.Hkv;
+  for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
+    const int64_t li = quotient(w, p.c.Hkv);
+    const int h = (int)(w - li * p.c.Hkv);
+    int32_t* out = p.blocks + w * p.v.top;
+    PagedSeq sq;
+    int i0, seq = paged_seq_of_list(p.c, p.v, li, lane, &sq, &i0);
+    if (seq >= 0 && sq.flags) seq = -1;
+    int n = 0, i1 = 0, near0 = 0, near1 = -1;
+    if (seq >= 0) {
+      i1 = i0 + p.v.tile.by < sq.n ? i0 + p.v.tile.by : sq.n;
+      const int p0 = sq.first + i0 > 0 ? sq.first + i0 : 0, end = sq.first + i1;    // the tile's positions [p0, end)
+      const int lim = !p.causal ? sq.L : end < 0 ? 0 : end;
+      n = lim > 0 ? (lim - 1) / p.v.block + 1 : 0;
+      if (p.last > 0 && end > 0) {
+        near0 = p0 / p.v.block - (p.last - 1);
+        near1 = (end - 1) / p.v.block;
+      }
+    }
+    const int top = p.v.top < n ? p.v.top : n;
+    if (n <= p.v.top) {                    // all of them
+      for (int i = threadIdx.x; i < p.v.top; i += 256) out[i] = i < n ? i : -1;
+      continue;
+    }
+    __syncthreads();                       // the ranks of the list before have been read
+    {
+      const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
+      double acc[8] = {};
+      const int rows = (i1 - i0) * p.group;
+      if (r0 < RPP) {
+        for (int r = r0; r < rows; r += RPP) {
+          const int i = r / p.group;
+          const char* src = p.q + (int64_t)(sq.t0 + i0 + i) * p.q_str[0] + (h * p.group + r - i * p.group) * p.q_str[1];
+          float x[8];
+          Half<E>::unpack(*reinterpret_cast<const u32x4*>(src + 16 * c), x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[j] += (double)x[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) part_s[r0 * D + 8 * c + j] = acc[j];
+      }
+      __syncthreads();
+      if (threadIdx.x < D) {
+        double s = 0.0;
+        for (int r = 0; r < RPP; ++r) s += part_s[r * D + threadIdx.x];
+        q_s[threadIdx.x] = s;
+      }
+      __syncthreads();
+    }
+    // lane l of eight: elements 4 l + 32 i .. + 3
+    const int l8 = lane & 7;
+    double q[D / 8];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[4 * i + j] = q_s[32 * i + 4 * l8 + j];
+    const int32_t* table = p.c.table + seq * p.c.table_str;
+    int kept = 0;
+    bool bad = false;
+    for (int b0 = 0; b0 < n;) {
+      const int room = kSelectKeys - kept, here = n - b0 < room ? n - b0 : room;
+      for (int i = threadIdx.x >> 3; i < here; i += 32) {
+        const int b = b0 + i, e = b / p.v.parts;
+        const int page = table[e];
+        const bool ok = (uint32_t)page < (uint32_t)p.c.n_pages;
+        bad |= !ok;
+        const char* m = p.means + (int64_t)(ok ? page : 0) * p.m_str[0] + (int64_t)(b - e * p.v.parts.by) * p.m_str[1] + h * p.m_str[2];
+        double s = 0.0;
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+          const floatx4 x = *reinterpret_cast<const floatx4*>(m + 128 * k + 16 * l8);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s = __builtin_fma((double)x[j], q[4 * k + j], s);
+        }
+        s += __shfl_xor(s, 1);
+        s += __shfl_xor(s, 2);
+        s += __shfl_xor(s, 4);
+        if (l8 == 0) {
+          ranks.key[kept + i] = b < p.first || (b >= near0 && b <= near1) ? ~0ull : ok ? rank_of(s) : 0;
+          ranks.id[kept + i] = b;
+        }
+      }
+      b0 += here;
+      kept += here;
+      __syncthreads();
+      if (kept > top) {
+        keep_highest(ranks, kept, top);
+        kept = top;
+      }
+    }
+    for (int i = threadIdx.x; i < p.v.top; i += 256) out[i] = i < kept ? ranks.id[i] : -1;
+    if (bad) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
+  }
+}
+
+// ─────────────────────────────── host side ─────────────────────────────────
+
+constexpr int64_t kMostGroups = 1 << 20;
+
+template <int D, typename E, int BITS> struct Means {
+  static int go(const MeansParams& p, unsigned grid, hipStream_t stream) {
+    hipLaunchKernelGGL((paged_means_kernel<D, E, BITS>), dim3(grid), dim3(256), 0, stream, p);
+    return launch_status("lvsa_paged_block_means");
+  }
+};
+template <int D, typename E, int BITS> struct Select {
+  static int go(const SelectParams& p, unsigned grid, hipStream_t stream) {
+    hipLaunchKernelGGL((paged_select_kernel<D, E>), dim3(grid), dim3(256), 0, stream, p);
+    return launch_status("lvsa_paged_select");
+  }
+};
+
+// Means beside a cache: their strides in bytes.
+int means_view(const char* what, const lvsa_paged_cache* c, const void* means, const int64_t* str, int block, int64_t* out,
+               Divisor* by_block, Divisor* by_parts) {
+  LVSA_REQUIRE(block >= 1 && c->page_size % block == 0, LVSA_ERR_INVALID_ARG, "%s: blocks of %d slots do not divide pages of %d",
+               what, block, c->page_size);
+  LVSA_REQUIRE((int64_t)c->n_pages * (c->page_size / block) < (1LL << 31), LVSA_ERR_UNSUPPORTED,
+               "%s: %d pages of %d blocks", what, c->n_pages, c->page_size / block);
+  bool ok = means && aligned16((int64_t)(uintptr_t)means);
+  for (int i = 0; i < 3 && str; ++i) {
+    out[i] = 4 * str[i];
+    ok = ok && aligned16(out[i]);
+  }
+  LVSA_REQUIRE(ok && str, LVSA_ERR_INVALID_ARG, "%s: means must be non-null and their rows start at multiples of 16 bytes", what);
+  *by_block = divisor(block);
+  *by_parts = divisor(c->page_size / block);
+  return LVSA_OK;
+}
+
+// Tiles of rows and lists of blocks.
+int list_view(const char* what, const lvsa_paged_cache* c, const lvsa_paged_batch* b, int block, int top, int tile, ListView* v) {
+  LVSA_REQUIRE(block >= 1 && c->page_size % block == 0, LVSA_ERR_INVALID_ARG, "%s: blocks of %d slots do not divide pages of %d",
+               what, block, c->page_size);
+  LVSA_REQUIRE(top >= 1 && top <= kListMax, LVSA_ERR_INVALID_ARG, "%s: lists of %d blocks (1 to %d)", what, top, kListMax);
+  LVSA_REQUIRE(tile >= 1, LVSA_ERR_INVALID_ARG, "%s: tiles of %d rows", what, tile);
+  const int64_t lists = tile == 1 ? b->N : (int64_t)(b->N / tile) + b->B;
+  LVSA_REQUIRE(lists < (1LL << 31), LVSA_ERR_UNSUPPORTED, "%s: %lld lists", what, (long long)lists);
+  v->block = divisor(block);
+  v->parts = divisor(c->page_size / block);
+  v->tile = divisor(tile);
+  v->lists = (int32_t)lists;
+  v->top = top;
+  return LVSA_OK;
+}
+
+// Queries: their strides in bytes.
+int query_view(const char* what, const lvsa_paged_cache* c, const lvsa_paged_batch* b, const void* q, const int64_t* str, int H,
+               int64_t* out) {
+  LVSA_REQUIRE(H >= 1 && H % c->Hkv == 0, LVSA_ERR_INVALID_ARG, "%s: %d heads over %d key heads", what, H, c->Hkv);
+  LVSA_REQUIRE((int64_t)b->N * H < (1LL << 31) - 4096, LVSA_ERR_UNSUPPORTED, "%s: %d rows of %d heads", what, b->N, H);
+  LVSA_REQUIRE(b->N == 0 || q, LVSA_ERR_INVALID_ARG, "%s: null q", what);
+  out[0] = 2 * str[0];
+  out[1] = 2 * str[1];
+  LVSA_REQUIRE(aligned16((int64_t)(uintptr_t)q) && aligned16(out[0]) && aligned16(out[1]), LVSA_ERR_INVALID_ARG,
+               "%s: rows must start at multiples of 16 bytes", what);
+  return LVSA_OK;
+}
+
+int scale_check(const char* what, float scale) {
+  LVSA_REQUIRE(scale > 0.f && scale <= 2.0e38f, LVSA_ERR_INVALID_ARG, "%s: scale %g must be positive and at most 2e38", what,
+               (double)scale);
+  return LVSA_OK;
+}
+
+// How an attention over lists runs: rows of a tile, row tiles of a list and
+// work-groups that share its keys.
+struct BlockShape {
+  int rows, subs, splits;
+  int64_t units, bytes;
+};
+BlockShape block_shape(const lvsa_paged_block_attn_args* a, const ListView& v) {
+  BlockShape s{};
+  const lvsa_paged_attn_args& t = a->attn;
+  const int64_t group = t.H / t.cache.Hkv, D = t.cache.D, N = t.batch.N, cus = cu_count();
+  const int64_t rows = (v.tile.by < N ? v.tile.by : N) * group;
+  s.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kPagedTile;
+  s.subs = (int)ceil_div(rows, s.rows);
+  s.units = (int64_t)v.lists * s.subs * t.cache.Hkv;
+  const int64_t cap = (int64_t)t.batch.max_pages * t.cache.page_size;
+  const int64_t keys = (int64_t)v.top * v.block.by < cap ? (int64_t)v.top * v.block.by : cap;
+  const int64_t steps = ceil_div(keys, s.rows == kPagedTile ? kPagedBlock : paged_decode_keys((int)D));
+  const int64_t want = ceil_div(2 * cus, s.units > 0 ? s.units : 1);
+  s.splits = (int)(want < steps ? want : steps);
+  if (s.splits < 1) s.splits = 1;
+  s.bytes = s.splits == 1 ? 0 : 4 * s.units * s.splits * s.rows * (D + 2);
+  return s;
+}
+
+int block_attn_check(const lvsa_paged_block_attn_args* a, PagedAttnParams* p, ListView* v) {
+  const char* what = "lvsa_paged_block_attn_fwd";
+  LVSA_REQUIRE(a != nullptr, LVSA_ERR_INVALID_ARG, "%s: null args", what);
+  const lvsa_paged_attn_args& t = a->attn;
+  int rc = paged_view(what, &t.cache, &t.batch, true, &p->c);
+  if (!rc) rc = query_view(what, &t.cache, &t.batch, t.q, t.q_str, t.H, p->q_str);
+  if (!rc) rc = scale_check(what, t.scale);
+  if (!rc) rc = list_view(what, &t.cache, &t.batch, a->block, a->top, a->tile, v);
+  return rc;
+}
+
+}  // namespace
+}  // namespace lvsa
+
+extern "C" {
+
+int lvsa_paged_block_means(const lvsa_paged_cache* cache, const lvsa_paged_batch* batch, float* means, const int64_t m_str[3],
+                           int32_t block, hipStream_t stream) {
+  clear_error();
+  const char* what = "lvsa_paged_block_means";
+  LVSA_REQUIRE(cache && batch, LVSA_ERR_INVALID_ARG, "%s: null args", what);
+  MeansParams p{};
+  int rc = paged_view(what, cache, batch, false, &p.c);
+  if (!rc) rc = means_view(what, cache, means, m_str, block, p.m_str, &p.block, &p.parts);
+  if (rc) return rc;
+  if (batch->B == 0 || (batch->cu_seqlens && batch->N == 0)) return LVSA_OK;
+  p.means = (char*)means;
+  const int64_t blocks = batch->cu_seqlens ? (int64_t)batch->N / block + 2LL * batch->B
+                                           : (int64_t)batch->B * batch->max_pages * p.parts.by;
+  const int64_t want = blocks * cache->Hkv, most = 16LL * cu_count();
+  return by_type<Means>(cache->D, cache->dtype, cache->bits, p, (unsigned)(want < 1 ? 1 : want < most ? want : most), stream);
+}
+
+int lvsa_paged_select(const lvsa_paged_select_args* a, hipStream_t stream) {
+  clear_error();
+  const char* what = "lvsa_paged_select";
+  LVSA_REQUIRE(a != nullptr, LVSA_ERR_INVALID_ARG, "%s: null args", what);
+  SelectParams p{};
+  Divisor block, parts;
+  int rc = paged_view(what, &a->cache, &a->batch, true, &p.c);
+  if (!rc) rc = query_view(what, &a->cache, &a->batch, a->q, a->q_str, a->H, p.q_str);
+  if (!rc) rc = means_view(what, &a->cache, a->means, a->m_str, a->block, p.m_str, &block, &parts);
+  if (!rc) rc = list_view(what, &a->cache, &a->batch, a->block, a->top, a->tile, &p.v);
+  if (rc) return rc;
+  const int64_t span = a->tile == 1 ? 1 : (int64_t)(a->tile - 2) / a->block + 2;
+  LVSA_REQUIRE(a->first >= 0 && a->last >= 0 && a->first + (a->last ? a->last - 1 + span : 0) <= a->top, LVSA_ERR_INVALID_ARG,
+               "%s: the first %d blocks, and the last %d of tiles of %d rows, do not fit into %d", what, a->first, a->last,
+               a->tile, a->top);
+  if (p.v.lists == 0 || a->batch.B == 0) return LVSA_OK;
+  LVSA_REQUIRE(a->blocks, LVSA_ERR_INVALID_ARG, "%s: null blocks", what);
+  p.q = (const char*)a->q;
+  p.means = (const char*)a->means;
+  p.blocks = a->blocks;
+  p.H = a->H;
+  p.group = a->H / a->cache.Hkv;
+  p.first = a->first;
+  p.last = a->last;
+  p.causal = a->causal;
+  const int64_t want = (int64_t)p.v.lists * a->cache.Hkv;
+  return by_type<Select>(a->cache.D, a->cache.dtype, 16, p, (unsigned)(want < kMostGroups ? want : kMostGroups), stream);
+}
+
+int lvsa_paged_block_attn_workspace_query(const lvsa_paged_block_attn_args* a, int64_t* bytes) {
+  clear_error();
+  LVSA_REQUIRE(bytes != nullptr, LVSA_ERR_INVALID_ARG, "lvsa_paged_block_attn_workspace_query: null output");
+  PagedAttnParams p{};
+  ListView v{};
+  const int rc = block_attn_check(a, &p, &v);
+  if (rc) return rc;
+  *bytes = a->attn.batch.N == 0 || a->attn.batch.B == 0 ? 0 : block_shape(a, v).bytes;
+  return LVSA_OK;
+}
+
+int lvsa_paged_block_attn_fwd(const lvsa_paged_block_attn_args* a, hipStream_t stream) {
+  clear_error();
+  const char* what = "lvsa_paged_block_attn_fwd";
+  PagedAttnParams p{};
+  BlockAttnParams l{};
+  int rc = block_attn_check(a, &p, &l.v);
+  if (rc) return rc;
+  const lvsa_paged_attn_args& t = a->attn;
+  if (t.batch.N == 0) return LVSA_OK;
+  LVSA_REQUIRE(t.o && a->blocks, LVSA_ERR_INVALID_ARG, "%s: null o or blocks", what);
+  p.o_str[0] = 2 * t.o_str[0];
+  p.o_str[1] = 2 * t.o_str[1];
+  LVSA_REQUIRE(aligned16((int64_t)(uintptr_t)t.o) && aligned16(p.o_str[0]) && aligned16(p.o_str[1]), LVSA_ERR_INVALID_ARG,
+               "%s: rows must start at multiples of 16 bytes", what);
+  LVSA_REQUIRE(!share_memory(t.o, p.o_str, t.H, t.q, p.q_str, t.H, t.batch.N, t.cache.D), LVSA_ERR_INVALID_ARG,
+               "%s: o must not share memory with q", what);
+  LVSA_REQUIRE(t.batch.B > 0, LVSA_ERR_INVALID_ARG, "%s: rows of no sequence", what);
+  const BlockShape s = block_shape(a, l.v);
+  LVSA_REQUIRE(s.bytes == 0 || (t.workspace && aligned16((int64_t)(uintptr_t)t.workspace)), LVSA_ERR_INVALID_ARG,
+               "%s: %lld bytes of 16-byte aligned workspace needed", what, (long long)s.bytes);
+  LVSA_REQUIRE(s.bytes == 0 || t.workspace_bytes >= s.bytes, LVSA_ERR_CAPACITY, "%s: workspace of %lld bytes < %lld", what,
+               (long long)t.workspace_bytes, (long long)s.bytes);
+  p.q = (const char*)t.q;
+  p.o = (char*)t.o;
+  p.lse = t.lse;
+  p.scale_log2 = t.scale * 1.4426950408889634f;
+  p.H = t.H;
+  p.group = t.H / t.cache.Hkv;
+  p.causal = t.causal;
+  p.fill_tail = t.fill_tail;
+  p.short_rows = p.c.k_str[1] >= 0 && p.c.k_str[1] < (1 << 26) && p.c.v_str[1] >= 0 && p.c.v_str[1] < (1 << 26);
+  p.ws_o = (float*)t.workspace;
+  p.ws_ml = p.ws_o + s.units * s.splits * s.rows * t.cache.D;
+  l.blocks = a->blocks;
+  l.subs = s.subs;
+  l.splits = s.splits;
+  l.units = s.units;
+  const bool bf16 = t.cache.dtype == LVSA_BF16;
+  switch (t.cache.D) {
+    case 64: return paged_block_attn_d64(p, l, t.cache.bits, s.rows, bf16, stream);
+    case 96: return paged_block_attn_d96(p, l, t.cache.bits, s.rows, bf16, stream);
+    case 128: return paged_block_attn_d128(p, l, t.cache.bits, s.rows, bf16, stream);
+    case 192: return paged_block_attn_d192(p, l, t.cache.bits, s.rows, bf16, stream);
+    default: return paged_block_attn_d256(p, l, t.cache.bits, s.rows, bf16, stream);
+  }
+}
+
+int lvsa_paged_weights(const lvsa_paged_weights_args* a, hipStream_t stream) {
+  clear_error();
+  const char* what = "lvsa_paged_weights";
+  LVSA_REQUIRE(a != nullptr, LVSA_ERR_INVALID_ARG, "%s: null args", what);
+  PagedAttnParams p{};
+  WeightsParams w{};
+  int rc = paged_view(what, &a->cache, &a->batch, true, &p.c);
+  if (!rc) rc = query_view(what, &a->cache, &a->batch, a->q, a->q_str, a->H, p.q_str);
+  if (!rc) rc = scale_check(what, a->scale);
+  if (rc) return rc;
+  bool ok = a->weights && ((uintptr_t)a->weights & 3) == 0;
+  LVSA_REQUIRE(ok && (a->lse || a->batch.N == 0), LVSA_ERR_INVALID_ARG, "%s: weights and lse must be non-null, fp32", what);
+  if (a->batch.N == 0 || a->batch.B == 0) return LVSA_OK;
+  p.q = (const char*)a->q;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.H = a->H;
+  p.group = a->H / a->cache.Hkv;
+  p.causal = a->causal;
+  w.lse = a->lse;
+  w.w = (char*)a->weights;
+  for (int i = 0; i < 3; ++i) w.w_str[i] = 4 * a->w_str[i];
+  w.accumulate = a->accumulate;
+  const int64_t want = (int64_t)a->batch.B * ceil_div((int64_t)a->batch.max_pages * a->cache.page_size, 128) * a->cache.Hkv;
+  const int64_t most = 8LL * cu_count();
+  p.grid = (int)(want < 1 ? 1 : want < most ? want : most);
+  const bool bf16 = a->cache.dtype == LVSA_BF16;
+  switch (a->cache.D) {
+    case 64: return paged_weights_d64(p, w, a->cache.bits, bf16, stream);
+    case 96: return paged_weights_d96(p, w, a->cache.bits, bf16, stream);
+    case 128: return paged_weights_d128(p, w, a->cache.bits, bf16, stream);
+    case 192: return paged_weights_d192(p, w, a->cache.bits, bf16, stream);
+    default: return paged_weights_d256(p, w, a->cache.bits, bf16, stream);
+  }
+}
+
+}  // extern "C"

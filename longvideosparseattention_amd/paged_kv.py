@@ -33,6 +33,9 @@ not ascend within the packed rows, nobody knows whose rows are whose: attention
 returns NaN in every row, an append takes a row for the first sequence whose
 range holds it.
 
+What works on parts of a cache (blocks selected by a score, tokens that are worth
+keeping) is in :mod:`paged_parts`.
+
 Inside ``torch.compile`` the calls break the graph and run as they are.
 
 The reference has no cache: it attends over whole tensors
@@ -63,6 +66,7 @@ _STATUS = {
     capi.PAGED_BAD_CU: "cu_seqlens that do not ascend within the packed rows",
     capi.PAGED_BAD_APPEND: "more new tokens than kv_lens counts",
     capi.PAGED_BAD_POSITION: "a position outside the rows of cos and sin",
+    capi.PAGED_BAD_BLOCK: "a list of blocks that does not ascend or names one behind its sequence's end",
 }
 
 # The C structs as they are packed (see include/lvsa_amd.h): one copy per
@@ -179,6 +183,19 @@ class PagedKVCache:
             return cls(rows(head_dim, dtype), rows(head_dim, dtype))
         return cls(rows(head_dim // 2, torch.uint8), rows(head_dim // 2, torch.uint8),
                    rows(head_dim // 32, torch.uint8), rows(head_dim // 32, torch.uint8))
+
+    def allocate_means(self, block_size: int) -> torch.Tensor:
+        """Zeroed means of all blocks of ``block_size`` slots, a divisor of the page
+        size: fp32 ``[pages, page_size / block_size, H_kv, D]`` (see
+        :func:`paged_kv_block_means`)."""
+        if block_size < 1 or self.page_size % block_size:
+            raise ValueError(f"blocks of {block_size} slots do not divide pages of {self.page_size}")
+        return torch.zeros(self.num_pages, self.num_kv_heads, self.page_size // block_size, self.head_dim, dtype=torch.float32,
+                           device=self.device).transpose(1, 2)
+
+    def allocate_weights(self) -> torch.Tensor:
+        """Zeroed weights of all slots: fp32 ``[pages, page_size, H_kv]`` (see :func:`paged_kv_weights`)."""
+        return torch.zeros(self.num_pages, self.num_kv_heads, self.page_size, dtype=torch.float32, device=self.device).transpose(1, 2)
 
     def _holds(self, t: torch.Tensor) -> bool:
         """Whether ``t`` lies within the bounds of the cache's tensors."""
