@@ -417,8 +417,8 @@ LVSA_API int lvsa_paged_block_means(const lvsa_paged_cache* cache, const lvsa_pa
  * before them (`last` 0: none of these), then the highest sums of q.mean over the
  * tile's rows and the head's query heads, in 64 bits; equal ones by the lower
  * number, NaN last.  blocks [lists, Hkv, top]: ascending, -1 behind; -1 throughout
- * for lists of no tile and for bad lengths and row ranges; a block whose page is bad
- * counts as NaN.  What is always selected has to fit: first, and for last > 0 last -
+ * for lists of no tile and of sequences with a bad length, and for all where
+ * cu_seqlens does not ascend; a block whose page is bad counts as NaN.  What is always selected has to fit: first, and for last > 0 last -
  * 1 and the blocks that a tile's rows may lie in, (tile - 2) / block + 2 (1 for a tile
  * of one), are at most `top` together, and top at most 1024.                    */
 typedef struct lvsa_paged_select_args {

@@ -87,12 +87,174 @@ struct SelectParams {
 };
 
 constexpr int kSelectKeys = 4096;        // blocks ranked at a time
+constexpr int kWaveKeys = 1024;          // by one wave
+constexpr int kGroup = 16;               // lists of a work-group that scores on the matrix cores
+constexpr int kGroupWaves = 4;
+constexpr uint64_t kAlways = ~0ull;      // the rank of what is always selected
 
 // A score as a number that sorts like it: NaN below -inf, 0 and -0 alike.
 __device__ __forceinline__ uint64_t rank_of(double s) {
   if (s != s) return 0;
   const uint64_t b = __builtin_bit_cast(uint64_t, s + 0.0);
   return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double score_of(uint64_t r) {
+  return __builtin_bit_cast(double, r >> 63 ? r & ~(1ull << 63) : ~r);
+}
+
+// A bound between lo and hi (lo < bound <= hi): half way between the scores, which
+// finds the border of scores that are spread in a dozen steps (half way between the
+// ranks, the exponents' halves, takes 20), or between the ranks where scores do not
+// say (infinities, NaN, neighbours) or have not led there in 24 steps.
+__device__ __forceinline__ uint64_t bound_between(uint64_t lo, uint64_t hi, int step) {
+  const uint64_t mid = step < 24 ? rank_of(0.5 * score_of(lo) + 0.5 * score_of(hi)) : 0;
+  return mid > lo && mid <= hi ? mid : lo + (hi - lo) / 2 + 1;
+}
+
+struct Span {
+  uint64_t lo, hi;
+};
+__device__ __forceinline__ Span wave_span(Span s) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint64_t a = __shfl_xor((unsigned long long)s.lo, d), b = __shfl_xor((unsigned long long)s.hi, d);
+    s.lo = a < s.lo ? a : s.lo;
+    s.hi = b > s.hi ? b : s.hi;
+  }
+  return s;
+}
+
+// One wave writes the `top` highest of n <= 64 K ranks (top < n), equal ones from the
+// front, to `out` in their order.  It holds the ranks, and the scores rounded to fp32,
+// which keeps their order, and halves the range between the lowest and the highest of
+// those that are not always selected until a bound cuts off exactly `top`: an fp32
+// comparison and a count per 64 of them, a dozen steps.  Where that does not come out
+// (the border runs between scores that fp32 does not tell apart, infinities, NaN), the
+// ranks themselves are halved.
+template <int K>
+__device__ __forceinline__ void wave_select(const uint64_t* ranks, int n, int top, int lane, int32_t* out) {
+  uint32_t up[K], low[K];
+  float x[K];
+  float lof = __builtin_inff(), hif = -__builtin_inff();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const bool in = 64 * k + lane < n;
+    const uint64_t r = ranks[in ? 64 * k + lane : n - 1];
+    x[k] = r == kAlways ? __builtin_inff() : r == 0 ? -__builtin_inff() : (float)score_of(r);
+    lof = __builtin_fminf(lof, x[k]);
+    hif = r != kAlways ? __builtin_fmaxf(hif, x[k]) : hif;
+    if (!in) x[k] = -__builtin_inff();     // below what any bound keeps
+    up[k] = in ? (uint32_t)(r >> 32) : 0;
+    low[k] = in ? (uint32_t)r : 0;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    lof = __builtin_fminf(lof, __shfl_xor(lof, d));
+    hif = __builtin_fmaxf(hif, __shfl_xor(hif, d));
+  }
+  int count = n;
+  uint64_t bound = 0;                      // at least `top` ranks from it on
+  {
+    float cut = 0.f;
+    for (;;) {
+      const float mid = 0.5f * lof + 0.5f * hif;
+      if (!(mid > lof && mid <= hif)) break;
+      int c = 0;
+#pragma unroll
+      for (int k = 0; k < K; ++k) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[k] >= mid));
+      if (c >= top) lof = mid;
+      else hif = mid;
+      if (c == top) {
+        count = c;
+        cut = mid;
+        break;
+      }
+      if (c < top && mid == hif && !(0.5f * lof + 0.5f * hif < hif)) break;
+    }
+    if (count == top) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {        // those below the cut drop out
+        if (!(x[k] >= cut)) up[k] = low[k] = 0;
+      }
+      bound = 1;
+    }
+  }
+  if (count != top) {
+    uint64_t high = kAlways;
+    while (bound < high && count != top) {
+      const uint64_t mid = bound + (high - bound) / 2 + 1;
+      int c = 0;
+#pragma unroll
+      for (int k = 0; k < K; ++k) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(((uint64_t)up[k] << 32 | low[k]) >= mid));
+      if (c >= top) {
+        bound = mid;
+        count = c;
+      } else {
+        high = mid - 1;
+      }
+    }
+  }
+  // all above the bound, and of those equal to it the first
+  int equal = n;
+  if (count != top) {
+    int above = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(((uint64_t)up[k] << 32 | low[k]) > bound));
+    equal = top - above;
+  }
+  const uint64_t before = (1ull << lane) - 1;
+  int put = 0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const bool in = 64 * k + lane < n;
+    const uint64_t r = (uint64_t)up[k] << 32 | low[k];
+    uint64_t take = __builtin_amdgcn_ballot_w64(in && r >= bound);
+    if (count != top) {
+      const uint64_t eq = __builtin_amdgcn_ballot_w64(in && r == bound);
+      const int e = __builtin_popcountll(eq & before);
+      take = __builtin_amdgcn_ballot_w64((take >> lane & 1) && (!(eq >> lane & 1) || e < equal));
+      equal -= __builtin_popcountll(eq & take);
+    }
+    if (take >> lane & 1) out[put + __builtin_popcountll(take & before)] = 64 * k + lane;
+    put += __builtin_popcountll(take);
+  }
+}
+__device__ __forceinline__ void wave_select(const uint64_t* ranks, int n, int top, int lane, int32_t* out) {
+  if (n <= 256) wave_select<4>(ranks, n, top, lane, out);
+  else if (n <= 384) wave_select<6>(ranks, n, top, lane, out);
+  else if (n <= 512) wave_select<8>(ranks, n, top, lane, out);
+  else wave_select<kWaveKeys / 64>(ranks, n, top, lane, out);
+}
+
+// What a list may name, and always does.
+struct ListRange {
+  int n, near0, near1;                     // blocks [0, n), of them [near0, near1] and below `first` always
+  __device__ __forceinline__ uint64_t rank(const SelectParams& p, int b, bool ok, double s) const {
+    return b < p.first || (b >= near0 && b <= near1) ? kAlways : ok ? rank_of(s) : 0;
+  }
+};
+__device__ __forceinline__ ListRange list_range(const SelectParams& p, const PagedSeq& sq, int i0, int i1) {
+  ListRange r = {0, 0, -1};
+  const int p0 = sq.first + i0 > 0 ? sq.first + i0 : 0, end = sq.first + i1;    // the tile's positions [p0, end)
+  const int lim = !p.causal ? sq.L : end < 0 ? 0 : end;
+  r.n = lim > 0 ? (lim - 1) / p.v.block + 1 : 0;
+  if (p.last > 0 && end > 0) {
+    r.near0 = p0 / p.v.block - (p.last - 1);
+    r.near1 = (end - 1) / p.v.block;
+  }
+  return r;
+}
+// Reports what is wrong with a batch; whether its row ranges are, and then every list
+// is empty.
+__device__ __forceinline__ bool refuse_batch(const SelectParams& p) {
+  const int lane = threadIdx.x & 63;
+  int flags = 0;
+  for (int s = lane; s < p.c.B; s += 64) flags |= paged_seq(p.c, s).flags;
+  if (blockIdx.x == 0 && threadIdx.x < 64 && flags) paged_flag(p.c, flags);
+  if (!__builtin_amdgcn_ballot_w64(flags & LVSA_PAGED_BAD_CU)) return false;
+  const int64_t n = (int64_t)p.v.lists * p.c.Hkv * p.v.top;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)blockDim.x * gridDim.x) p.blocks[i] = -1;
+  return true;
 }
 
 // LDS of a selection: ranks and numbers of candidate blocks, in ascending order.
@@ -103,65 +265,50 @@ struct Ranks {
   uint64_t bound[2][4];
 };
 
-// Leaves the `top` highest of n ranks, equal ones from the front, in their order.
-// The work-group (256) finds the top-th highest rank by halving the range between
-// the lowest and the highest, and stops where a bound cuts off exactly `top`.
+// Leaves the `top` highest of n ranks in their order, like wave_select, with the whole
+// work-group of 256.
 __device__ __forceinline__ void keep_highest(Ranks& r, int n, int top) {
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  constexpr uint64_t kAlways = ~0ull;
-  uint64_t lo = kAlways, hi = 0;
+  Span s = {kAlways, 0};
   for (int i = threadIdx.x; i < n; i += 256) {
     const uint64_t k = r.key[i];
-    if (k < lo) lo = k;
-    if (k > hi && k != kAlways) hi = k;
+    s.lo = k < s.lo ? k : s.lo;
+    s.hi = k != kAlways && k > s.hi ? k : s.hi;
   }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t a = __shfl_xor((unsigned long long)lo, d), b = __shfl_xor((unsigned long long)hi, d);
-    if (a < lo) lo = a;
-    if (b > hi) hi = b;
-  }
+  s = wave_span(s);
   if (lane == 0) {
-    r.bound[0][wave] = lo;
-    r.bound[1][wave] = hi;
+    r.bound[0][wave] = s.lo;
+    r.bound[1][wave] = s.hi;
   }
   __syncthreads();
+  uint64_t lo = s.lo, hi = s.hi;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    if (r.bound[0][w] < lo) lo = r.bound[0][w];
-    if (r.bound[1][w] > hi) hi = r.bound[1][w];
+    lo = r.bound[0][w] < lo ? r.bound[0][w] : lo;
+    hi = r.bound[1][w] > hi ? r.bound[1][w] : hi;
   }
-  // at least `top` ranks are >= lo, and fewer are > hi
-  int above = -1, parity = 0;            // ranks >= lo where that is exactly `top`
-  while (lo < hi) {
-    const uint64_t mid = lo + (hi - lo) / 2 + 1;
+  int parity = 0;
+  auto total = [&](auto test) __attribute__((always_inline)) {
     int count = 0;
-    for (int i = threadIdx.x - lane; i < n; i += 256)
-      count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i + lane < n && r.key[i + lane < n ? i + lane : 0] >= mid));
+    for (int i = (int)threadIdx.x - lane; i < n; i += 256)
+      count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i + lane < n && test(r.key[i + lane < n ? i + lane : 0])));
     if (lane == 0) r.sum[parity][wave] = count;
     __syncthreads();
     count = r.sum[parity][0] + r.sum[parity][1] + r.sum[parity][2] + r.sum[parity][3];
     parity ^= 1;
+    return count;
+  };
+  // at least `top` ranks are >= lo, and fewer are > hi
+  for (int step = 0; lo < hi; ++step) {
+    const uint64_t mid = bound_between(lo, hi, step);
+    const int count = total([&](uint64_t k) __attribute__((always_inline)) { return k >= mid; });
     if (count >= top) lo = mid;
     else hi = mid - 1;
-    if (count == top) {
-      above = top;
-      break;
-    }
+    if (count == top) break;
   }
-  // all above lo, and of those equal to it the first ones
-  int equal = kSelectKeys;
-  if (above < 0) {
-    int count = 0;
-    for (int i = threadIdx.x - lane; i < n; i += 256)
-      count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i + lane < n && r.key[i + lane < n ? i + lane : 0] > lo));
-    if (lane == 0) r.sum[parity][wave] = count;
-    __syncthreads();
-    equal = top - (r.sum[parity][0] + r.sum[parity][1] + r.sum[parity][2] + r.sum[parity][3]);
-    parity ^= 1;
-  }
+  int equal = top - total([&](uint64_t k) __attribute__((always_inline)) { return k > lo; });
   __syncthreads();                       // r.sum has been read
-  int put = 0, seen = 0;                 // kept so far, equal ones so far
+  int put = 0;
   const uint64_t before = (1ull << lane) - 1;
   for (int i0 = 0; i0 < n; i0 += 256) {
     const int i = i0 + (int)threadIdx.x;
@@ -173,24 +320,24 @@ __device__ __forceinline__ void keep_highest(Ranks& r, int n, int top) {
       r.sum[1][wave] = __builtin_popcountll(eq);
     }
     __syncthreads();                     // the ranks of these 256 have been read, too
-    int g0 = 0, e0 = 0, gs = 0, es = 0;
+    int g = 0, e = 0, gs = 0, es = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      g0 += w < wave ? r.sum[0][w] : 0;
-      e0 += w < wave ? r.sum[1][w] : 0;
+      g += w < wave ? r.sum[0][w] : 0;
+      e += w < wave ? r.sum[1][w] : 0;
       gs += r.sum[0][w];
       es += r.sum[1][w];
     }
-    const int g = g0 + __builtin_popcountll(gt & before), e = e0 + __builtin_popcountll(eq & before);
-    const int e_left = equal - seen;     // equal ones that still find room
-    const bool mine = gt >> lane & 1, also = (eq >> lane & 1) && e < e_left;
-    if (mine || also) {
-      const int at = put + g + (e < e_left ? e : e_left);
+    g += __builtin_popcountll(gt & before);
+    e += __builtin_popcountll(eq & before);
+    if ((gt >> lane & 1) || ((eq >> lane & 1) && e < equal)) {
+      const int at = put + g + (e < equal ? e : equal);
       r.key[at] = k;
       r.id[at] = id;
     }
-    put += gs + (es < e_left ? es : e_left);
-    seen += es < e_left ? es : e_left;
+    const int taken = es < equal ? es : equal;
+    put += gs + taken;
+    equal -= taken;
     __syncthreads();
   }
 }
@@ -201,17 +348,13 @@ __device__ __forceinline__ void keep_highest(Ranks& r, int n, int top) {
 // differences of 1e-15): a list is the same on every device and beside every batch.
 template <int D, typename E>
 __global__ __launch_bounds__(256) void paged_select_kernel(SelectParams p) {
-  constexpr int CH = D / 8, RPP = 256 / CH;
+  constexpr int CH = D / 8, RPP = 256 / CH, U = D <= 128 ? 4 : 2;    // U: blocks of eight lanes on their way
   __shared__ Ranks ranks;
   __shared__ double q_s[D];
   double* part_s = reinterpret_cast<double*>(ranks.key);     // [RPP][D]: before any rank is there
   static_assert(RPP * D <= kSelectKeys, "sums of the queries");
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  if (blockIdx.x == 0 && wave == 0) {
-    int flags = 0;
-    for (int s = lane; s < p.c.B; s += 64) flags |= paged_seq(p.c, s).flags;
-    if (flags) paged_flag(p.c, flags);
-  }
+  if (refuse_batch(p)) return;
   const int64_t total = (int64_t)p.v.lists * p.c.Hkv;
   for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
     const int64_t li = quotient(w, p.c.Hkv);
@@ -220,30 +363,25 @@ __global__ __launch_bounds__(256) void paged_select_kernel(SelectParams p) {
     PagedSeq sq;
     int i0, seq = paged_seq_of_list(p.c, p.v, li, lane, &sq, &i0);
     if (seq >= 0 && sq.flags) seq = -1;
-    int n = 0, i1 = 0, near0 = 0, near1 = -1;
+    ListRange range = {0, 0, -1};
+    int i1 = 0;
     if (seq >= 0) {
       i1 = i0 + p.v.tile.by < sq.n ? i0 + p.v.tile.by : sq.n;
-      const int p0 = sq.first + i0 > 0 ? sq.first + i0 : 0, end = sq.first + i1;    // the tile's positions [p0, end)
-      const int lim = !p.causal ? sq.L : end < 0 ? 0 : end;
-      n = lim > 0 ? (lim - 1) / p.v.block + 1 : 0;
-      if (p.last > 0 && end > 0) {
-        near0 = p0 / p.v.block - (p.last - 1);
-        near1 = (end - 1) / p.v.block;
-      }
+      range = list_range(p, sq, i0, i1);
     }
-    const int top = p.v.top < n ? p.v.top : n;
-    if (n <= p.v.top) {                    // all of them
-      for (int i = threadIdx.x; i < p.v.top; i += 256) out[i] = i < n ? i : -1;
+    const int n = range.n, top = p.v.top;
+    if (n <= top) {                        // all of them
+      for (int i = threadIdx.x; i < top; i += 256) out[i] = i < n ? i : -1;
       continue;
     }
     __syncthreads();                       // the ranks of the list before have been read
     {
       const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
       double acc[8] = {};
-      const int rows = (i1 - i0) * p.group;
-      if (r0 < RPP) {
+      const int rows = (i1 - i0) * p.group, used = rows < RPP ? rows : RPP;
+      if (r0 < used) {
         for (int r = r0; r < rows; r += RPP) {
-          const int i = r / p.group;
+          const int i = (uint32_t)r / (uint32_t)p.group;
           const char* src = p.q + (int64_t)(sq.t0 + i0 + i) * p.q_str[0] + (h * p.group + r - i * p.group) * p.q_str[1];
           float x[8];
           Half<E>::unpack(*reinterpret_cast<const u32x4*>(src + 16 * c), x);
@@ -256,7 +394,7 @@ __global__ __launch_bounds__(256) void paged_select_kernel(SelectParams p) {
       __syncthreads();
       if (threadIdx.x < D) {
         double s = 0.0;
-        for (int r = 0; r < RPP; ++r) s += part_s[r * D + threadIdx.x];
+        for (int r = 0; r < used; ++r) s += part_s[r * D + threadIdx.x];
         q_s[threadIdx.x] = s;
       }
       __syncthreads();
@@ -273,37 +411,156 @@ __global__ __launch_bounds__(256) void paged_select_kernel(SelectParams p) {
     bool bad = false;
     for (int b0 = 0; b0 < n;) {
       const int room = kSelectKeys - kept, here = n - b0 < room ? n - b0 : room;
-      for (int i = threadIdx.x >> 3; i < here; i += 32) {
-        const int b = b0 + i, e = b / p.v.parts;
-        const int page = table[e];
-        const bool ok = (uint32_t)page < (uint32_t)p.c.n_pages;
-        bad |= !ok;
-        const char* m = p.means + (int64_t)(ok ? page : 0) * p.m_str[0] + (int64_t)(b - e * p.v.parts.by) * p.m_str[1] + h * p.m_str[2];
-        double s = 0.0;
+      for (int i0 = threadIdx.x >> 3; i0 < here; i0 += 32 * U) {
+        floatx4 x[U][D / 32];
+        bool ok[U];
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-          const floatx4 x = *reinterpret_cast<const floatx4*>(m + 128 * k + 16 * l8);
+        for (int k = 0; k < U; ++k) {      // past the end: the last one again
+          const int i = i0 + 32 * k < here ? i0 + 32 * k : here - 1, e = (b0 + i) / p.v.parts;
+          const int page = table[e];
+          ok[k] = (uint32_t)page < (uint32_t)p.c.n_pages;
+          const char* m = p.means + (int64_t)(ok[k] ? page : 0) * p.m_str[0] + (int64_t)(b0 + i - e * p.v.parts.by) * p.m_str[1] + h * p.m_str[2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s = __builtin_fma((double)x[j], q[4 * k + j], s);
+          for (int j = 0; j < D / 32; ++j) x[k][j] = *reinterpret_cast<const floatx4*>(m + 128 * j + 16 * l8);
         }
-        s += __shfl_xor(s, 1);
-        s += __shfl_xor(s, 2);
-        s += __shfl_xor(s, 4);
-        if (l8 == 0) {
-          ranks.key[kept + i] = b < p.first || (b >= near0 && b <= near1) ? ~0ull : ok ? rank_of(s) : 0;
-          ranks.id[kept + i] = b;
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const int i = i0 + 32 * k;
+          double s = 0.0;
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) s = __builtin_fma((double)x[k][j][d], q[4 * j + d], s);
+          s += __shfl_xor(s, 1);
+          s += __shfl_xor(s, 2);
+          s += __shfl_xor(s, 4);
+          bad |= !ok[k];
+          if (l8 == 0 && i < here) {
+            ranks.key[kept + i] = range.rank(p, b0 + i, ok[k], s);
+            ranks.id[kept + i] = b0 + i;
+          }
         }
       }
       b0 += here;
       kept += here;
       __syncthreads();
-      if (kept > top) {
+      if (n <= kWaveKeys) {
+        if (wave == 0) wave_select(ranks.key, n, top, lane, out);
+      } else if (kept > top) {
         keep_highest(ranks, kept, top);
         kept = top;
       }
     }
-    for (int i = threadIdx.x; i < p.v.top; i += 256) out[i] = i < kept ? ranks.id[i] : -1;
+    if (n > kWaveKeys)
+      for (int i = threadIdx.x; i < top; i += 256) out[i] = ranks.id[i];
     if (bad) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
+  }
+}
+
+// One work-group per 16 lists of a sequence and key head, for lists of few rows: the
+// scores of 16 blocks for 16 lists on the matrix cores, in 64 bits; a wave then selects
+// for two lists.  A lane of group g = lane / 16 holds elements 16 i + 4 g .. + 3 of
+// block (of list) lane % 16.
+template <int D, typename E>
+__global__ __launch_bounds__(64 * kGroupWaves) void paged_select_group_kernel(SelectParams p, ListView groups, int pitch) {
+  extern __shared__ uint64_t group_ranks[];    // [16][pitch]
+  typedef double doublex4 __attribute__((ext_vector_type(4)));
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int g = lane >> 4, x = lane & 15, top = p.v.top;
+  if (refuse_batch(p)) return;
+  {                                        // lists of no tile: before, between and behind the sequences'
+    const int64_t per = (int64_t)p.c.Hkv * top;
+    for (int64_t s = (int64_t)blockIdx.x * kGroupWaves + wave; s < p.c.B; s += kGroupWaves * (int64_t)gridDim.x) {
+      const PagedSeq q = paged_seq(p.c, (int)s);
+      const int64_t from = first_list(p.v, (int)s, q) + list_count(p.v, q);
+      const int64_t to = s + 1 < p.c.B ? first_list(p.v, (int)s + 1, paged_seq(p.c, (int)s + 1)) : p.v.lists;
+      for (int64_t i = from * per + lane; i < to * per; i += 64) p.blocks[i] = -1;
+      if (s == 0)
+        for (int64_t i = lane; i < first_list(p.v, 0, q) * per; i += 64) p.blocks[i] = -1;
+    }
+  }
+  const int64_t total = (int64_t)groups.lists * p.c.Hkv;
+  for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
+    const int64_t gi = quotient(w, p.c.Hkv);
+    const int h = (int)(w - gi * p.c.Hkv);
+    PagedSeq sq;
+    int r0;
+    const int seq = paged_seq_of_list(p.c, groups, gi, lane, &sq, &r0);
+    if (seq < 0) continue;
+    const int tile = p.v.tile.by, lists = list_count(p.v, sq), l0 = r0 / p.v.tile;
+    const int64_t list0 = first_list(p.v, seq, sq) + l0;
+    auto range_of = [&](int l) __attribute__((always_inline)) {
+      const int i0 = (l0 + l) * tile, i1 = i0 + tile < sq.n ? i0 + tile : sq.n;
+      return list_range(p, sq, i0, i1);
+    };
+    const int here = lists - l0 < kGroup ? lists - l0 : kGroup;
+    const int n = sq.flags ? 0 : range_of(here - 1).n;       // of the last list, which sees the most
+    bool bad = false;
+    __syncthreads();                       // the ranks before have been read
+    if (n > top) {
+      double q[D / 4] = {};
+      {
+        const int l = x < here ? x : here - 1, i0 = (l0 + l) * tile, i1 = i0 + tile < sq.n ? i0 + tile : sq.n;
+        for (int i = i0; i < i1; ++i)
+          for (int j = 0; j < p.group; ++j) {
+            const char* src = p.q + (int64_t)(sq.t0 + i) * p.q_str[0] + (h * p.group + j) * p.q_str[1] + 8 * g;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              typedef E e4 __attribute__((ext_vector_type(4)));
+              const e4 v = *reinterpret_cast<const e4*>(src + 32 * k);
+#pragma unroll
+              for (int d = 0; d < 4; ++d) q[4 * k + d] += (double)(float)v[d];
+            }
+          }
+      }
+      const ListRange mine = range_of(x < here ? x : here - 1);
+      const int32_t* table = p.c.table + seq * p.c.table_str;
+      // the next 16 blocks' means are on their way while these are multiplied, and the
+      // page numbers of those after them
+      auto block_at = [&](int b0) __attribute__((always_inline)) { return b0 + x < n ? b0 + x : n - 1; };
+      floatx4 next[D / 16];
+      bool ok_next = false;
+      auto load = [&](int b0, int page) __attribute__((always_inline)) {
+        const int b = block_at(b0), e = b / p.v.parts;
+        ok_next = (uint32_t)page < (uint32_t)p.c.n_pages;
+        bad |= !ok_next;
+        const char* m = p.means + (int64_t)(ok_next ? page : 0) * p.m_str[0] + (int64_t)(b - e * p.v.parts.by) * p.m_str[1] + h * p.m_str[2] + 16 * g;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) next[k] = *reinterpret_cast<const floatx4*>(m + 64 * k);
+      };
+      load(16 * wave, table[block_at(16 * wave) / p.v.parts]);
+      int page = table[block_at(16 * (wave + kGroupWaves)) / p.v.parts];
+      for (int b0 = 16 * wave; b0 < n; b0 += 16 * kGroupWaves) {
+        floatx4 a[D / 16];
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) a[k] = next[k];
+        const uint64_t fine = __builtin_amdgcn_ballot_w64(ok_next);
+        load(b0 + 16 * kGroupWaves, page);
+        page = table[block_at(b0 + 32 * kGroupWaves) / p.v.parts];
+        __builtin_amdgcn_sched_barrier(0);
+        doublex4 s[2] = {};
+#pragma unroll
+        for (int k = 0; k < D / 4; ++k)
+          s[k & 1] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)a[k >> 2][k & 3], q[k], s[k & 1], 0, 0, 0);
+        s[0] += s[1];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {      // block 4 k + g, list x
+          const int r = 4 * k + g;
+          if (b0 + r < n) group_ranks[x * pitch + b0 + r] = mine.rank(p, b0 + r, fine >> r & 1, s[0][k]);
+        }
+      }
+      if (bad) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
+    }
+    __syncthreads();
+    for (int l = wave; l < here; l += kGroupWaves) {
+      const int nl = sq.flags ? 0 : range_of(l).n;
+      int32_t* out = p.blocks + ((list0 + l) * p.c.Hkv + h) * top;
+      if (nl > top) {
+        wave_select(group_ranks + l * pitch, nl, top, lane, out);
+      } else {
+        for (int i = lane; i < top; i += 64) out[i] = i < nl ? i : -1;
+      }
+    }
   }
 }
 
@@ -318,8 +575,19 @@ template <int D, typename E, int BITS> struct Means {
   }
 };
 template <int D, typename E, int BITS> struct Select {
-  static int go(const SelectParams& p, unsigned grid, hipStream_t stream) {
-    hipLaunchKernelGGL((paged_select_kernel<D, E>), dim3(grid), dim3(256), 0, stream, p);
+  static int go(const SelectParams& p, bool grouped, hipStream_t stream) {
+    if (grouped) {
+      ListView groups = p.v;
+      groups.tile = divisor(p.v.tile.by * kGroup);
+      groups.lists = p.c.N / groups.tile.by + p.c.B;
+      const int pitch = (int)((int64_t)p.c.max_pages * p.v.parts.by) | 1;
+      const int64_t want = (int64_t)groups.lists * p.c.Hkv;
+      hipLaunchKernelGGL((paged_select_group_kernel<D, E>), dim3((unsigned)(want < kMostGroups ? want : kMostGroups)), dim3(64 * kGroupWaves),
+                         (unsigned)(8 * kGroup * pitch), stream, p, groups, pitch);
+    } else {
+      const int64_t want = (int64_t)p.v.lists * p.c.Hkv;
+      hipLaunchKernelGGL((paged_select_kernel<D, E>), dim3((unsigned)(want < kMostGroups ? want : kMostGroups)), dim3(256), 0, stream, p);
+    }
     return launch_status("lvsa_paged_select");
   }
 };
@@ -459,8 +727,10 @@ int lvsa_paged_select(const lvsa_paged_select_args* a, hipStream_t stream) {
   p.first = a->first;
   p.last = a->last;
   p.causal = a->causal;
-  const int64_t want = (int64_t)p.v.lists * a->cache.Hkv;
-  return by_type<Select>(a->cache.D, a->cache.dtype, 16, p, (unsigned)(want < kMostGroups ? want : kMostGroups), stream);
+  // Lists together where sequences have many and they are short
+  const int64_t cap = (int64_t)a->batch.max_pages * p.v.parts.by;
+  const bool grouped = (int64_t)a->tile * p.group <= 16 && p.v.lists >= 8LL * a->batch.B && cap <= kWaveKeys;
+  return by_type<Select>(a->cache.D, a->cache.dtype, 16, p, grouped, stream);
 }
 
 int lvsa_paged_block_attn_workspace_query(const lvsa_paged_block_attn_args* a, int64_t* bytes) {

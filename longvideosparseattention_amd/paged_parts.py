@@ -161,8 +161,8 @@ def paged_kv_select(q: torch.Tensor, cache: PagedKVCache, means: torch.Tensor, c
     the tile's queries over its rows and the query heads of the key head, equal ones
     by their number, NaN last; ascending, ``-1`` behind.  What is always in a list has
     to fit into it.  Sums are 64 bits: which blocks are taken depends on nothing but
-    the values.  Lists of no tile, and of sequences with a bad length or row range,
-    are ``-1``; a block on a bad page counts as NaN."""
+    the values.  Lists of no tile and of sequences with a bad length are ``-1``, and all
+    where ``cu_seqlens`` does not ascend; a block on a bad page counts as NaN."""
     if is_compiling():
         return _outside["select"](q, cache, means, cu_seqlens, kv_lens, page_table, top, tile=tile, first=first, last=last,
                                   causal=causal)

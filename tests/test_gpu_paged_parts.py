@@ -80,6 +80,11 @@ SELECT = [  # sequences, D, H, Hkv, page, block, top, tile, first, last, causal
     ([(20, 20), (1, 1513), (40, 800)], 256, 8, 4, 390, 15, 9, 7, 1, 0, True),
     ([(2, 9000)], 64, 1, 1, 8, 1, 1024, 1, 0, 0, False),        # more blocks than are ranked at a time
     ([(1, 30000), (3, 11000)], 64, 4, 2, 64, 2, 100, 2, 1, 2, True),
+    ([(300, 700), (100, 900), (0, 50), (17, 17), (65, 64)], 64, 4, 2, 8, 8, 12, 1, 2, 2, True),    # sixteen lists at a time
+    ([(300, 2000), (210, 250)], 128, 3, 3, 20, 2, 33, 5, 0, 3, False),
+    ([(200, 300), (180, 200)], 96, 4, 1, 3, 1, 7, 3, 1, 0, True),
+    ([(90, 130), (70, 75)], 192, 2, 2, 16, 4, 5, 2, 1, 1, True),
+    ([(64, 700)], 256, 8, 1, 32, 8, 40, 1, 1, 1, False),
 ]
 
 
