@@ -25,37 +25,21 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
   return b >> 31 ? ~b : b | 1u << 31;
 }
 
-// Sums over the work-group's 1024 threads before this one, and the total.
-__device__ __forceinline__ int group_scan(int x, int* lds, int* total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int incl = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(incl, d);
-    if (lane >= d) incl += y;
-  }
-  __syncthreads();
-  if (lane == 63) lds[wave] = incl;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) {
-    before += w < wave ? lds[w] : 0;
-    all += lds[w];
-  }
-  *total = all;
-  return before + incl - x;
-}
+constexpr int kEvictHeld = 32;             // ranks that a thread of the selection holds
 
-// One work-group per sequence and head: finds the keep-th highest weight, 11 bits of
-// it at a time by counting how often each value of them occurs, and lists the tokens
-// from it on.  The counts are whole numbers, so the order of the atomics in LDS does
-// not matter.
+// One work-group per sequence and head: finds the keep-th highest weight by halving the
+// range of the ranks, which its threads hold (R each, or read again in every step where
+// a sequence is longer), and lists the tokens from it on.  A wave has consecutive
+// tokens, so that one exchange of counts gives all their places.  Latency: the page
+// table, the weights, 15 to 32 counts.  (Counting the values of 11 bits at a time in
+// LDS: 53 us for 64 heads of 16000 tokens.)
+template <int R>
 __global__ __launch_bounds__(1024) void paged_evict_select_kernel(EvictParams p) {
-  __shared__ int hist[2048];
-  __shared__ int lds[16];
-  __shared__ int bad_s, bin_s, above_s;
-  const int Hkv = p.c.Hkv, tid = threadIdx.x;
+  __shared__ int count_s[2][16];
+  __shared__ int gt_s[16], eq_s[16];
+  __shared__ uint32_t lo_s[16], hi_s[16];
+  __shared__ int bad_s, new_s[1024];
+  const int Hkv = p.c.Hkv, tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   for (int64_t u = blockIdx.x; u < (int64_t)p.c.B * Hkv; u += gridDim.x) {
     const int b = (int)quotient(u, Hkv), h = (int)(u - (int64_t)b * Hkv);
     const PagedSeq sq = paged_seq(p.c, 0, 0, p.c.lens[b]);
@@ -63,18 +47,51 @@ __global__ __launch_bounds__(1024) void paged_evict_select_kernel(EvictParams p)
     const int32_t* table = p.c.table + b * p.c.table_str;
     const int32_t* to = p.to ? p.to + b * p.to_str : nullptr;
     int32_t* kept = p.kept + u * p.keep;
-    __syncthreads();
+    // A wave's tokens: `per` times 64 from wave * 64 * per on.
+    const int per = (L + 1023) / 1024, first = wave * 64 * per + lane;
+    auto rank_at = [&](int pos) __attribute__((always_inline)) {
+      if (pos < p.first || pos >= L - p.last) return ~0u;
+      const PagedRow at = paged_row(p.c, pos, table[page_of(p.c, pos)]);
+      return rank_of(*reinterpret_cast<const float*>(p.w + at.page * p.w_str[0] + at.slot * p.w_str[1] + h * p.w_str[2]));
+    };
+    uint32_t held[R ? R : 1];
+    if constexpr (R > 0) {
+      if (L > p.keep) {                    // pages, then weights, all on their way at once
+        int64_t at[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          const int pos = key_within(first + 64 * (k < per ? k : 0), L);
+          at[k] = table[page_of(p.c, pos)];
+        }
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          const int pos = key_within(first + 64 * (k < per ? k : 0), L);
+          const PagedRow row = paged_row(p.c, pos, (int)at[k]);
+          at[k] = row.page * p.w_str[0] + row.slot * p.w_str[1] + h * p.w_str[2];
+        }
+#pragma unroll
+        for (int k = 0; k < R; ++k) held[k] = __builtin_bit_cast(uint32_t, *reinterpret_cast<const float*>(p.w + at[k]));
+      }
+    }
+    __syncthreads();                       // LDS of the head before has been read
     if (tid == 0) bad_s = sq.flags;
     __syncthreads();
     const int pages = L > 0 ? page_of(p.c, L - 1) + 1 : 0, news = left > 0 ? page_of(p.c, left - 1) + 1 : 0;
-    for (int e = tid; e < pages; e += 1024) {
-      const int page = table[e];
-      bool bad = (uint32_t)page >= (uint32_t)p.c.n_pages;
-      for (int i = 0; to && i < news; ++i) bad |= to[i] == page;
-      if (bad) atomicOr(&bad_s, LVSA_PAGED_BAD_PAGE);
+    bool odd = false;
+    for (int e = tid; e < pages; e += 1024) odd |= (uint32_t)table[e] >= (uint32_t)p.c.n_pages;
+    for (int i0 = 0; to && i0 < news; i0 += 1024) {      // a new page that is an old one
+      const int here = news - i0 < 1024 ? news - i0 : 1024;
+      __syncthreads();
+      if (tid < here) new_s[tid] = to[i0 + tid];
+      __syncthreads();
+      odd |= tid < here && (uint32_t)new_s[tid] >= (uint32_t)p.c.n_pages;
+      for (int e = tid; e < pages; e += 1024) {
+        const int page = table[e];
+#pragma unroll 8
+        for (int i = 0; i < here; ++i) odd |= new_s[i] == page;
+      }
     }
-    for (int i = tid; to && i < news; i += 1024)
-      if ((uint32_t)to[i] >= (uint32_t)p.c.n_pages) atomicOr(&bad_s, LVSA_PAGED_BAD_PAGE);
+    if (odd) atomicOr(&bad_s, LVSA_PAGED_BAD_PAGE);
     __syncthreads();
     const int bad = bad_s;
     if (bad) {
@@ -91,56 +108,95 @@ __global__ __launch_bounds__(1024) void paged_evict_select_kernel(EvictParams p)
       for (int i = tid; i < L; i += 1024) kept[i] = i;
       continue;
     }
-    auto rank = [&](int pos) __attribute__((always_inline)) {
-      if (pos < p.first || pos >= L - p.last) return ~0u;
-      const PagedRow at = paged_row(p.c, pos, table[page_of(p.c, pos)]);
-      return rank_of(*reinterpret_cast<const float*>(p.w + at.page * p.w_str[0] + at.slot * p.w_str[1] + h * p.w_str[2]));
-    };
-    uint32_t bound = 0;                    // the bits found so far
-    int want = p.keep;                     // of the ranks with these bits
+    if constexpr (R > 0) {
+#pragma unroll
+      for (int k = 0; k < R; ++k) {        // past the end 0, which no bound keeps
+        const int pos = first + 64 * k;
+        held[k] = k >= per || pos >= L ? 0 : pos < p.first || pos >= L - p.last ? ~0u : rank_of(__builtin_bit_cast(float, held[k]));
+      }
+    }
+    // `test` of a wave's tokens, 64 at a time
+    auto each = [&](auto test) __attribute__((always_inline)) {
+      if constexpr (R > 0) {
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+          if (k < per) test(first + 64 * k, held[k]);
+      } else {
 #pragma unroll 1
-    for (int step = 0; step < 3; ++step) {
-      const int shift = step == 0 ? 21 : step == 1 ? 10 : 0, bits = step == 2 ? 10 : 11;
-      hist[tid] = hist[tid + 1024] = 0;
-      __syncthreads();
-      for (int pos = tid; pos < L; pos += 1024) {
-        const uint32_t r = rank(pos);
-        if (step == 0 || r >> (shift + bits) == bound) atomicAdd(&hist[r >> shift & ((1u << bits) - 1)], 1);
+        for (int k = 0; k < per; ++k) test(first + 64 * k, first + 64 * k < L ? rank_at(first + 64 * k) : 0);
       }
-      __syncthreads();
-      // bins from the highest down, two a thread: the one that reaches `want`
-      const int hi = hist[2047 - 2 * tid], lo = hist[2046 - 2 * tid];
-      int all;
-      const int before = group_scan(hi + lo, lds, &all);
-      if (before < want && before + hi >= want) {
-        bin_s = 2047 - 2 * tid;
-        above_s = before;
-      } else if (before + hi < want && before + hi + lo >= want) {
-        bin_s = 2046 - 2 * tid;
-        above_s = before + hi;
-      }
-      __syncthreads();
-      bound = bound << bits | (uint32_t)bin_s;
-      want -= above_s;
-      __syncthreads();
+    };
+    uint32_t lo = ~0u, hi = 0;
+    each([&](int pos, uint32_t r) __attribute__((always_inline)) {
+      if (pos < L && r < lo) lo = r;
+      if (r != ~0u && r > hi) hi = r;
+    });
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t a = __shfl_xor((int)lo, d), z = __shfl_xor((int)hi, d);
+      lo = a < lo ? a : lo;
+      hi = z > hi ? z : hi;
     }
-    // all above the bound, and the first `want` equal to it
-    int put = 0, seen = 0;
-    for (int p0 = 0; p0 < L; p0 += 1024) {
-      const int pos = p0 + tid;
-      const uint32_t r = pos < L ? rank(pos) : 0;
-      const bool gt = pos < L && r > bound, eq = pos < L && r == bound;
-      int all;
-      const int both = group_scan((gt ? 1 : 0) | (eq ? 1 << 16 : 0), lds, &all);
-      const int room = want - seen, e = both >> 16;
-      const int at = put + (both & 0xffff) + (e < room ? e : room);
-      if ((gt || (eq && e < room)) && at < p.keep) kept[at] = pos;
-      const int es = all >> 16;
-      put += (all & 0xffff) + (es < room ? es : room);
-      seen += es < room ? es : room;
+    if (lane == 0) {
+      lo_s[wave] = lo;
+      hi_s[wave] = hi;
     }
-    // weights that another stream changes meanwhile: still positions
-    for (int i = put + tid; i < p.keep; i += 1024) kept[i] = i;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      lo = lo_s[w] < lo ? lo_s[w] : lo;
+      hi = hi_s[w] > hi ? hi_s[w] : hi;
+    }
+    // at least `keep` ranks are >= lo, and fewer are > hi
+    int parity = 0;
+    for (bool found = false; lo < hi && !found; parity ^= 1) {
+      const uint32_t mid = lo + (hi - lo) / 2 + 1;
+      int c = 0;
+      each([&](int pos, uint32_t r) __attribute__((always_inline)) { c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(r >= mid)); });
+      if (lane == 0) count_s[parity][wave] = c;
+      __syncthreads();
+      c = 0;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) c += count_s[parity][w];
+      if (c >= p.keep) lo = mid;
+      else hi = mid - 1;
+      found = c == p.keep;
+    }
+    // all above the bound, and the first of those equal to it
+    int gt = 0, eq = 0;
+    each([&](int pos, uint32_t r) __attribute__((always_inline)) {
+      gt += __builtin_popcountll(__builtin_amdgcn_ballot_w64(r > lo));
+      eq += __builtin_popcountll(__builtin_amdgcn_ballot_w64(pos < L && r == lo));
+    });
+    if (lane == 0) {
+      gt_s[wave] = gt;
+      eq_s[wave] = eq;
+    }
+    __syncthreads();
+    int put = 0, equal = p.keep;           // places before this wave's, equal ones that still find room
+#pragma unroll
+    for (int w = 0; w < 16; ++w) equal -= gt_s[w];
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      if (w >= wave) continue;
+      const int e = eq_s[w] < equal ? eq_s[w] : equal;
+      put += gt_s[w] + e;
+      equal -= e;
+    }
+    const uint64_t before = (1ull << lane) - 1;
+    each([&](int pos, uint32_t r) __attribute__((always_inline)) {
+      const uint64_t g = __builtin_amdgcn_ballot_w64(r > lo), e = __builtin_amdgcn_ballot_w64(pos < L && r == lo);
+      const int mine = __builtin_popcountll(e & before), es = __builtin_popcountll(e), taken = es < equal ? es : equal;
+      const int at = put + __builtin_popcountll(g & before) + (mine < equal ? mine : equal);
+      // (weights that another stream changes between two readings may give other counts)
+      if (((g >> lane & 1) || ((e >> lane & 1) && mine < equal)) && (uint32_t)at < (uint32_t)p.keep) kept[at] = pos;
+      put += __builtin_popcountll(g) + taken;
+      equal -= taken;
+    });
+    if constexpr (R == 0) {
+      if (wave == 15)
+        for (int i = put + lane; i < p.keep; i += 64) kept[i] = i;
+    }
   }
 }
 
@@ -148,10 +204,9 @@ __global__ __launch_bounds__(1024) void paged_evict_select_kernel(EvictParams p)
 struct Move {
   PagedRow from, at;
 };
-__device__ __forceinline__ Move move_of(const EvictParams& p, int b, const int32_t* kept, int i) {
+__device__ __forceinline__ Move move_of(const EvictParams& p, int b, int old, int i) {
   const int32_t* table = p.c.table + b * p.c.table_str;
   const int32_t* to = p.to ? p.to + b * p.to_str : table;
-  const int old = kept[i];
   return Move{paged_row(p.c, old, table[page_of(p.c, old)]), paged_row(p.c, i, to[page_of(p.c, i)])};
 }
 
@@ -166,24 +221,40 @@ __global__ __launch_bounds__(256) void paged_evict_move_kernel(EvictParams p, in
     const int part = (int)(u - bh * per), b = (int)quotient(bh, p.c.Hkv), h = (int)(bh - (int64_t)b * p.c.Hkv);
     const int left = p.new_lens[b];
     const int32_t* kept = p.kept + bh * p.keep;
-    for (int64_t k = (int64_t)part * 256 + threadIdx.x; k < (int64_t)left * CH; k += (int64_t)per * 256) {
-      const int i = (int)(k / CH), c = (int)(k % CH);
-      const Move m = move_of(p, b, kept, i);
-      const int64_t kf = m.from.page * p.c.k_str[0] + m.from.slot * p.c.k_str[1], kt = m.at.page * p.c.k_str[0] + m.at.slot * p.c.k_str[1];
-      const int64_t vf = m.from.page * p.c.v_str[0] + m.from.slot * p.c.v_str[1], vt = m.at.page * p.c.v_str[0] + m.at.slot * p.c.v_str[1];
-      const u32x4 x = *reinterpret_cast<const u32x4*>(p.c.k + kf + h * p.c.k_str[2] + 16 * c);
-      const u32x4 y = *reinterpret_cast<const u32x4*>(p.c.v + vf + h * p.c.v_str[2] + 16 * c);
-      *reinterpret_cast<u32x4*>(p.c.k + kt + h * p.c.k_str[2] + 16 * c) = x;
-      *reinterpret_cast<u32x4*>(p.c.v + vt + h * p.c.v_str[2] + 16 * c) = y;
-      if constexpr (BITS == 4) {           // 16 bytes are 32 elements: their scale
-        const int64_t ksf = m.from.page * p.c.ks_str[0] + m.from.slot * p.c.ks_str[1], kst = m.at.page * p.c.ks_str[0] + m.at.slot * p.c.ks_str[1];
-        const int64_t vsf = m.from.page * p.c.vs_str[0] + m.from.slot * p.c.vs_str[1], vst = m.at.page * p.c.vs_str[0] + m.at.slot * p.c.vs_str[1];
-        p.c.ks[kst + h * p.c.ks_str[2] + c] = p.c.ks[ksf + h * p.c.ks_str[2] + c];
-        p.c.vs[vst + h * p.c.vs_str[2] + c] = p.c.vs[vsf + h * p.c.vs_str[2] + c];
+    constexpr int U = 4;                   // pieces on their way
+    const int64_t n = (int64_t)left * CH;
+    for (int64_t k0 = (int64_t)part * 256 * U + threadIdx.x; k0 < n; k0 += (int64_t)per * 256 * U) {
+      u32x4 x[U], y[U];
+      Move m[U];
+      int c[U], i[U], old[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int64_t k = k0 + 256 * j < n ? k0 + 256 * j : n - 1;
+        i[j] = (int)quotient(k, CH);
+        c[j] = (int)(k - (int64_t)i[j] * CH);
+        old[j] = kept[i[j]];
       }
-      if (c == 0) {
-        const int64_t wf = m.from.page * p.w_str[0] + m.from.slot * p.w_str[1], wt = m.at.page * p.w_str[0] + m.at.slot * p.w_str[1];
-        *reinterpret_cast<float*>(p.w + wt + h * p.w_str[2]) = *reinterpret_cast<const float*>(p.w + wf + h * p.w_str[2]);
+#pragma unroll
+      for (int j = 0; j < U; ++j) m[j] = move_of(p, b, old[j], i[j]);
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        x[j] = *reinterpret_cast<const u32x4*>(p.c.k + m[j].from.page * p.c.k_str[0] + m[j].from.slot * p.c.k_str[1] + h * p.c.k_str[2] + 16 * c[j]);
+        y[j] = *reinterpret_cast<const u32x4*>(p.c.v + m[j].from.page * p.c.v_str[0] + m[j].from.slot * p.c.v_str[1] + h * p.c.v_str[2] + 16 * c[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        if (k0 + 256 * j >= n) continue;
+        *reinterpret_cast<u32x4*>(p.c.k + m[j].at.page * p.c.k_str[0] + m[j].at.slot * p.c.k_str[1] + h * p.c.k_str[2] + 16 * c[j]) = x[j];
+        *reinterpret_cast<u32x4*>(p.c.v + m[j].at.page * p.c.v_str[0] + m[j].at.slot * p.c.v_str[1] + h * p.c.v_str[2] + 16 * c[j]) = y[j];
+        if constexpr (BITS == 4) {         // 16 bytes are 32 elements: their scale
+          p.c.ks[m[j].at.page * p.c.ks_str[0] + m[j].at.slot * p.c.ks_str[1] + h * p.c.ks_str[2] + c[j]] =
+              p.c.ks[m[j].from.page * p.c.ks_str[0] + m[j].from.slot * p.c.ks_str[1] + h * p.c.ks_str[2] + c[j]];
+          p.c.vs[m[j].at.page * p.c.vs_str[0] + m[j].at.slot * p.c.vs_str[1] + h * p.c.vs_str[2] + c[j]] =
+              p.c.vs[m[j].from.page * p.c.vs_str[0] + m[j].from.slot * p.c.vs_str[1] + h * p.c.vs_str[2] + c[j]];
+        }
+        if (c[j] == 0)
+          *reinterpret_cast<float*>(p.w + m[j].at.page * p.w_str[0] + m[j].at.slot * p.w_str[1] + h * p.w_str[2]) =
+              *reinterpret_cast<const float*>(p.w + m[j].from.page * p.w_str[0] + m[j].from.slot * p.w_str[1] + h * p.w_str[2]);
       }
     }
   }
@@ -206,7 +277,7 @@ __global__ __launch_bounds__(256) void paged_evict_slide_kernel(EvictParams p, i
     if (slice == slices - 1) {             // weights and scales
       for (int i0 = 0; i0 < p.keep; i0 += 256) {
         const int i = i0 + (int)threadIdx.x < p.keep ? i0 + (int)threadIdx.x : p.keep - 1;
-        const Move m = move_of(p, b, kept, i);
+        const Move m = move_of(p, b, kept[i], i);
         const char* wf = p.w + m.from.page * p.w_str[0] + m.from.slot * p.w_str[1] + h * p.w_str[2];
         float w = *reinterpret_cast<const float*>(wf);
         uint8_t ks[D / 32], vs[D / 32];
@@ -238,28 +309,50 @@ __global__ __launch_bounds__(256) void paged_evict_slide_kernel(EvictParams p, i
     }
     constexpr int SL = (CH + CS - 1) / CS;
     const bool is_v = slice >= SL;
-    const int c = (is_v ? slice - SL : slice) * CS + threadIdx.x % CS, r0 = threadIdx.x / CS;
-    const bool on = r0 < RPP && c < CH;
+    const int c0 = (is_v ? slice - SL : slice) * CS + threadIdx.x % CS, r0 = threadIdx.x / CS;
+    const bool on = r0 < RPP && c0 < CH;   // some threads have no piece: they read the row's last one
+    const int c = c0 < CH ? c0 : CH - 1;
     char* base = (is_v ? p.c.v + h * p.c.v_str[2] : p.c.k + h * p.c.k_str[2]) + 16 * c;
     const int64_t s0 = is_v ? p.c.v_str[0] : p.c.k_str[0], s1 = is_v ? p.c.v_str[1] : p.c.k_str[1];
-    for (int i0 = 0; i0 < p.keep; i0 += STEP) {
+    // the next batch's rows are on their way while this one's are written: they lie
+    // behind all that is written
+    struct Batch {
       u32x4 x[kMoveDepth];
       char* to[kMoveDepth];
+    };
+    auto place = [&](int i0, int j) __attribute__((always_inline)) {
+      const int i = i0 + j * RPP + r0;
+      return i < p.keep ? i : p.keep - 1;
+    };
+    auto load = [&](int i0, Batch& t) __attribute__((always_inline)) {
+      int old[kMoveDepth];                 // past the end: the last row, which is not written
+#pragma unroll
+      for (int j = 0; j < kMoveDepth; ++j) old[j] = kept[place(i0, j)];
+      Move m[kMoveDepth];
+#pragma unroll
+      for (int j = 0; j < kMoveDepth; ++j) m[j] = move_of(p, b, old[j], place(i0, j));
 #pragma unroll
       for (int j = 0; j < kMoveDepth; ++j) {
-        const int i = i0 + j * RPP + r0;
-        to[j] = nullptr;
-        if (on && i < p.keep) {
-          const Move m = move_of(p, b, kept, i);
-          to[j] = base + m.at.page * s0 + m.at.slot * s1;
-          x[j] = *reinterpret_cast<const u32x4*>(base + m.from.page * s0 + m.from.slot * s1);
-        }
+        t.to[j] = base + m[j].at.page * s0 + m[j].at.slot * s1;
+        t.x[j] = *reinterpret_cast<const u32x4*>(base + m[j].from.page * s0 + m[j].from.slot * s1);
       }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // all rows of the batch are here
+    };
+    auto store = [&](int i0, Batch& t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < kMoveDepth; ++j) asm volatile("" : "+v"(t.x[j]));   // all rows of the batch are here
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < kMoveDepth; ++j)
-        if (to[j]) *reinterpret_cast<u32x4*>(to[j]) = x[j];
+        if (on && i0 + j * RPP + r0 < p.keep) *reinterpret_cast<u32x4*>(t.to[j]) = t.x[j];
+    };
+    Batch a, z;
+    load(0, a);
+    for (int i0 = 0; i0 < p.keep; i0 += 2 * STEP) {
+      load(i0 + STEP, z);
+      store(i0, a);
+      if (i0 + STEP >= p.keep) break;
+      load(i0 + 2 * STEP, a);
+      store(i0 + STEP, z);
     }
   }
 }
@@ -270,7 +363,12 @@ template <int D, typename E, int BITS> struct Evict {
   static int go(const EvictParams& p, hipStream_t stream) {
     const int64_t bh = (int64_t)p.c.B * p.c.Hkv;
     auto grid = [](int64_t n) { return dim3((unsigned)(n < kMostGroups ? n : kMostGroups)); };
-    hipLaunchKernelGGL(paged_evict_select_kernel, grid(bh), dim3(1024), 0, stream, p);
+    // the longest sequence that the table has room for
+    const int64_t cap = (int64_t)p.c.max_pages * p.c.page_size;
+    if (cap <= 4 * 1024) hipLaunchKernelGGL((paged_evict_select_kernel<4>), grid(bh), dim3(1024), 0, stream, p);
+    else if (cap <= 16 * 1024) hipLaunchKernelGGL((paged_evict_select_kernel<16>), grid(bh), dim3(1024), 0, stream, p);
+    else if (cap <= kEvictHeld * 1024) hipLaunchKernelGGL((paged_evict_select_kernel<kEvictHeld>), grid(bh), dim3(1024), 0, stream, p);
+    else hipLaunchKernelGGL((paged_evict_select_kernel<0>), grid(bh), dim3(1024), 0, stream, p);
     int rc = launch_status("lvsa_paged_evict");
     if (rc) return rc;
     constexpr int CH = D * BITS / 128;
