@@ -453,7 +453,7 @@ LVSA_API int lvsa_paged_block_attn_workspace_query(const lvsa_paged_block_attn_a
  * tokens' own weights start from 0, with `accumulate` 0 all of the sequence's do.
  * Rows whose lse is not finite give nothing; sequences without new rows, with a bad
  * length or row range and tokens on a bad page are left alone.  `max_q_len` (0:
- * unknown) only chooses a kernel.                                             */
+ * unknown) only chooses a kernel.  Workspace: as for lvsa_paged_attn_fwd.       */
 typedef struct lvsa_paged_weights_args {
   lvsa_paged_cache cache;
   lvsa_paged_batch batch;
@@ -461,8 +461,11 @@ typedef struct lvsa_paged_weights_args {
   int64_t q_str[2], w_str[3];
   float scale;
   int32_t H, causal, accumulate, max_q_len;
+  void* workspace;
+  int64_t workspace_bytes;
 } lvsa_paged_weights_args;
 LVSA_API int lvsa_paged_weights(const lvsa_paged_weights_args* a, hipStream_t stream);
+LVSA_API int lvsa_paged_weights_workspace_query(const lvsa_paged_weights_args* a, int64_t* bytes);
 
 /* Cuts every sequence to `keep` tokens a head: the first `first`, the newest `last`
  * and of the others those of the largest weights (equal ones by the lower position,

@@ -168,6 +168,7 @@ class PagedWeightsArgs(C.Structure):
         ("cache", PagedCache), ("batch", PagedBatch),
         ("q", C.c_void_p), ("lse", C.c_void_p), ("weights", C.c_void_p), ("q_str", _Str2), ("w_str", _Str3),
         ("scale", C.c_float), ("H", C.c_int32), ("causal", C.c_int32), ("accumulate", C.c_int32), ("max_q_len", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
     ]
 
 
@@ -209,6 +210,7 @@ SIGNATURES = {
     "lvsa_paged_block_attn_fwd": (C.c_int, [C.POINTER(PagedBlockAttnArgs), C.c_void_p]),
     "lvsa_paged_block_attn_workspace_query": (C.c_int, [C.POINTER(PagedBlockAttnArgs), C.POINTER(C.c_int64)]),
     "lvsa_paged_weights": (C.c_int, [C.POINTER(PagedWeightsArgs), C.c_void_p]),
+    "lvsa_paged_weights_workspace_query": (C.c_int, [C.POINTER(PagedWeightsArgs), C.POINTER(C.c_int64)]),
     "lvsa_paged_evict": (C.c_int, [C.POINTER(PagedEvictArgs), C.c_void_p]),
     "lvsa_version": (C.c_char_p, []),
     "lvsa_last_error": (C.c_char_p, []),

@@ -273,8 +273,11 @@ struct WeightsParams {
   const float* lse;
   char* w;
   int64_t w_str[3];                    // bytes
-  int32_t accumulate;
+  int32_t accumulate, many;            // many: rows of a sequence, more than a tile or two
+  int32_t splits;                      // work-groups that share the rows of 128 keys
+  float* ws;                           // their sums: [128 keys][splits][128]
 };
+constexpr int kWeightKeys = 128;
 int paged_weights_d64(const PagedAttnParams& p, const WeightsParams& w, int bits, bool bf16, hipStream_t stream);
 int paged_weights_d96(const PagedAttnParams& p, const WeightsParams& w, int bits, bool bf16, hipStream_t stream);
 int paged_weights_d128(const PagedAttnParams& p, const WeightsParams& w, int bits, bool bf16, hipStream_t stream);
@@ -348,7 +351,7 @@ __device__ __forceinline__ int64_t wave_scan(int64_t x, int lane, int count = 64
 }
 
 // Work-groups take the units of all sequences in turn: `count` says how many a
-// sequence has, `work` does unit i of sequence s.
+// sequence has, `work` does unit i of sequence s, the u-th of all.
 template <typename Count, typename Work>
 __device__ __forceinline__ void walk_units(const PagedView& c, Count count, Work work) {
   const int lane = threadIdx.x & 63;
@@ -365,7 +368,7 @@ __device__ __forceinline__ void walk_units(const PagedView& c, Count count, Work
     const int64_t upto = wave_scan(n, lane), end = base + from_lane(upto, 63);
     for (; u < end; u += gridDim.x) {
       const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(base + upto > u));
-      work(s0 + at, from_lane(mine, at), u - base - from_lane(upto - n, at));
+      work(s0 + at, from_lane(mine, at), u - base - from_lane(upto - n, at), u);
     }
     base = end;
   }

@@ -34,7 +34,7 @@ __global__ __launch_bounds__(256) void paged_means_kernel(MeansParams p) {
     if (s.L == 0 || (p.c.cu && s.n == 0)) return (int64_t)0;
     return ((int64_t)((s.L - 1) / p.block) + 1 - first_block(s)) * p.c.Hkv;
   };
-  walk_units(p.c, count, [&](int seq, const PagedSeq& sq, int64_t u) __attribute__((always_inline)) {
+  walk_units(p.c, count, [&](int seq, const PagedSeq& sq, int64_t u, int64_t) __attribute__((always_inline)) {
     const int i = (int)quotient(u, p.c.Hkv), h = (int)(u - (int64_t)i * p.c.Hkv);
     const int b = first_block(sq) + i, entry = b / p.parts, part = b - entry * p.parts.by;
     const int page = p.c.table[seq * p.c.table_str + entry];
@@ -680,6 +680,41 @@ int block_attn_check(const lvsa_paged_block_attn_args* a, PagedAttnParams* p, Li
   return rc;
 }
 
+int weights_check(const lvsa_paged_weights_args* a, PagedAttnParams* p) {
+  const char* what = "lvsa_paged_weights";
+  LVSA_REQUIRE(a != nullptr, LVSA_ERR_INVALID_ARG, "%s: null args", what);
+  int rc = paged_view(what, &a->cache, &a->batch, true, &p->c);
+  if (!rc) rc = query_view(what, &a->cache, &a->batch, a->q, a->q_str, a->H, p->q_str);
+  if (!rc) rc = scale_check(what, a->scale);
+  return rc;
+}
+
+// How an accumulation runs.
+struct WeightsShape {
+  int many, grid, splits;
+  int64_t bytes;
+};
+WeightsShape weights_shape(const lvsa_paged_weights_args* a) {
+  WeightsShape s{};
+  // rows of a sequence, if unknown: one each where there are no more than sequences, else all of one
+  const int64_t N = a->batch.N, q = a->max_q_len > 0 ? (a->max_q_len < N ? a->max_q_len : N) : N <= a->batch.B ? 1 : N;
+  const int64_t rows = q * (a->H / a->cache.Hkv), B = a->batch.B < N ? a->batch.B : N, cus = cu_count();
+  s.many = rows > 32;
+  s.splits = 1;
+  const int64_t cap = (int64_t)a->batch.max_pages * a->cache.page_size;
+  int64_t units = B * ceil_div(cap, s.many ? kWeightKeys : paged_decode_keys(a->cache.D)) * a->cache.Hkv;
+  if (units < 1) units = 1;
+  if (s.many) {
+    const int64_t want = ceil_div(8 * cus, units), tiles = ceil_div(rows, 128);
+    s.splits = (int)(want < tiles ? want : tiles);
+    s.bytes = s.splits == 1 ? 0 : 4 * units * s.splits * kWeightKeys;
+    units *= s.splits;
+  }
+  const int64_t most = s.many ? 64 * cus : cus * (a->cache.D <= 128 ? 2 : 1);
+  s.grid = (int)(units < most ? units : most);
+  return s;
+}
+
 }  // namespace
 }  // namespace lvsa
 
@@ -791,31 +826,44 @@ int lvsa_paged_block_attn_fwd(const lvsa_paged_block_attn_args* a, hipStream_t s
   }
 }
 
+int lvsa_paged_weights_workspace_query(const lvsa_paged_weights_args* a, int64_t* bytes) {
+  clear_error();
+  LVSA_REQUIRE(bytes != nullptr, LVSA_ERR_INVALID_ARG, "lvsa_paged_weights_workspace_query: null output");
+  PagedAttnParams p{};
+  const int rc = weights_check(a, &p);
+  if (rc) return rc;
+  *bytes = a->batch.N == 0 || a->batch.B == 0 ? 0 : weights_shape(a).bytes;
+  return LVSA_OK;
+}
+
 int lvsa_paged_weights(const lvsa_paged_weights_args* a, hipStream_t stream) {
   clear_error();
   const char* what = "lvsa_paged_weights";
-  LVSA_REQUIRE(a != nullptr, LVSA_ERR_INVALID_ARG, "%s: null args", what);
   PagedAttnParams p{};
   WeightsParams w{};
-  int rc = paged_view(what, &a->cache, &a->batch, true, &p.c);
-  if (!rc) rc = query_view(what, &a->cache, &a->batch, a->q, a->q_str, a->H, p.q_str);
-  if (!rc) rc = scale_check(what, a->scale);
+  const int rc = weights_check(a, &p);
   if (rc) return rc;
-  bool ok = a->weights && ((uintptr_t)a->weights & 3) == 0;
-  LVSA_REQUIRE(ok && (a->lse || a->batch.N == 0), LVSA_ERR_INVALID_ARG, "%s: weights and lse must be non-null, fp32", what);
+  LVSA_REQUIRE(a->weights && ((uintptr_t)a->weights & 3) == 0 && (a->lse || a->batch.N == 0), LVSA_ERR_INVALID_ARG,
+               "%s: weights and lse must be non-null, fp32", what);
   if (a->batch.N == 0 || a->batch.B == 0) return LVSA_OK;
+  const WeightsShape s = weights_shape(a);
+  LVSA_REQUIRE(s.bytes == 0 || (a->workspace && aligned16((int64_t)(uintptr_t)a->workspace)), LVSA_ERR_INVALID_ARG,
+               "%s: %lld bytes of 16-byte aligned workspace needed", what, (long long)s.bytes);
+  LVSA_REQUIRE(s.bytes == 0 || a->workspace_bytes >= s.bytes, LVSA_ERR_CAPACITY, "%s: workspace of %lld bytes < %lld", what,
+               (long long)a->workspace_bytes, (long long)s.bytes);
   p.q = (const char*)a->q;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.H = a->H;
   p.group = a->H / a->cache.Hkv;
   p.causal = a->causal;
+  p.grid = s.grid;
   w.lse = a->lse;
   w.w = (char*)a->weights;
   for (int i = 0; i < 3; ++i) w.w_str[i] = 4 * a->w_str[i];
   w.accumulate = a->accumulate;
-  const int64_t want = (int64_t)a->batch.B * ceil_div((int64_t)a->batch.max_pages * a->cache.page_size, 128) * a->cache.Hkv;
-  const int64_t most = 8LL * cu_count();
-  p.grid = (int)(want < 1 ? 1 : want < most ? want : most);
+  w.many = s.many;
+  w.splits = s.splits;
+  w.ws = (float*)a->workspace;
   const bool bf16 = a->cache.dtype == LVSA_BF16;
   switch (a->cache.D) {
     case 64: return paged_weights_d64(p, w, a->cache.bits, bf16, stream);

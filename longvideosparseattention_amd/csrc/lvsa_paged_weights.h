@@ -1,101 +1,406 @@
 // Weights that the newest rows give to the cached tokens (gfx950): w_j (+)= sum_i
 // exp(scale q_i.k_j - lse_i) over the rows of a sequence and the query heads of a key
-// head.
+// head.  The scores are formed as S^T = K Q^T, so that a row of the matrix is a key and
+// its sum runs over the lanes; nothing is shared between keys.
 #pragma once
 #include "lvsa_paged_attn.h"
 
 namespace lvsa {
 namespace {
 
-constexpr int kWeightTiles = 2;            // 16-key tiles of a wave
+constexpr float kLog2e = 1.4426950408889634f;
 
-// Writes a lane group's sums: lane x < 4 of group g has key 4 g + x of a 16-key tile.
-__device__ __forceinline__ void store_weight(const PagedAttnParams& p, const WeightsParams& wp, const PagedSeq& sq, int h, int key,
-                                             const PagedRow& at, float sum) {
-  float* w = reinterpret_cast<float*>(wp.w + at.page * wp.w_str[0] + at.slot * wp.w_str[1] + h * wp.w_str[2]);
-  *w = (wp.accumulate && key < sq.first ? *w : 0.f) + sum;
-}
-
+// Few rows (a tile of 16, or some of them one after the other): bound by the bytes of
+// the keys.  The launch's work, sum over sequences of key heads x key steps, is cut
+// into equal shares, as in paged_decode_kernel; a wave has 16 T keys of a step and the
+// next step's on their way.  Lane (g = lane / 16, x = lane % 16) holds elements of key
+// x, and the sums of keys 4 g .. + 3, of which it keeps key x's where x / 4 = g: the
+// lane that looked its page up writes its weight.
 template <int D, typename E, int BITS>
-__global__ __launch_bounds__(256) void paged_weights_kernel(PagedAttnParams p, WeightsParams wp) {
-  constexpr int T = kWeightTiles, ND = D / 32, KW = 16 * T, KEYS = 4 * KW;
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_weights_kernel(PagedAttnParams p, WeightsParams wp) {
+  constexpr int T = D >= 192 ? 1 : 2, ND = D / 32, KW = 16 * T, KEYS = 4 * KW;
   constexpr bool kTwoScales = D == 96 || D >= 192;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int g = lane >> 4, x = lane & 15;
-  auto count = [&](const PagedSeq& s) __attribute__((always_inline)) {
-    return s.n ? ((int64_t)s.L + KEYS - 1) / KEYS * p.c.Hkv : (int64_t)0;
+  const bool keeps = (x >> 2) == g;
+  const int B = p.c.B;
+  PagedSeq mine = {};
+  int64_t n_mine = 0, upto = 0, U = 0;
+  int flags = 0;
+  auto units_of = [&](const PagedSeq& s) __attribute__((always_inline)) {
+    return s.n && !s.flags ? (int64_t)p.c.Hkv * (((int64_t)s.L + KEYS - 1) / KEYS) : (int64_t)0;
   };
-  walk_units(p.c, count, [&](int seq, const PagedSeq& sq, int64_t u) __attribute__((always_inline)) {
-    const int chunk = (int)quotient(u, p.c.Hkv), h = (int)(u - (int64_t)chunk * p.c.Hkv);
-    const int key0 = chunk * KEYS + wave * KW;
-    if (key0 >= sq.L) return;
-    const int32_t* table = p.c.table + seq * p.c.table_str;
-    shortx8 kf[T][ND];
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < T; ++j) {
-      const int pos = key_within(key0 + 16 * j + x, sq.L);
-      const PagedRow at = paged_row(p.c, pos, table[page_of(p.c, pos)]);
-      bad |= !at.ok;
-      const char* kr = p.c.k + h * p.c.k_str[2] + at.page * p.c.k_str[0] + at.slot * p.c.k_str[1];
-      if constexpr (BITS == 16) {
-#pragma unroll
-        for (int i = 0; i < ND; ++i) kf[j][i] = *reinterpret_cast<const shortx8*>(kr + 64 * i + 16 * g);
-      } else {
-        const uint32_t* kw = reinterpret_cast<const uint32_t*>(kr + (D / 8) * g);
-        const uint8_t* ks = p.c.ks + h * p.c.ks_str[2] + at.page * p.c.ks_str[0] + at.slot * p.c.ks_str[1];
-        const uint32_t lo = ks[(D / 4) * g / 32], hi = kTwoScales ? ks[((D / 4) * g + D / 4 - 1) / 32] : lo;
-#pragma unroll
-        for (int i = 0; i < ND; ++i)
-          kf[j][i] = decode8<E>(kw[i], kTwoScales && ((D / 4) * g + 8 * i) / 32 != (D / 4) * g / 32 ? hi : lo);
-      }
+  auto read_batch = [&](int s0) __attribute__((always_inline)) {
+    n_mine = 0;
+    if (s0 + lane < B) {
+      mine = paged_seq(p.c, s0 + lane);
+      n_mine = units_of(mine);
+      flags |= mine.flags;
     }
-    if (bad) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
-    float acc[T][4] = {};
+    upto = wave_scan(n_mine, lane, B - s0);
+  };
+  for (int s0 = 0; s0 < B; s0 += 64) {
+    read_batch(s0);
+    U += from_lane(upto, B - s0 < 64 ? B - s0 - 1 : 63);
+  }
+  if (blockIdx.x == 0 && wave == 0 && flags) paged_flag(p.c, flags);
+  if (U == 0) return;
+  const int shares = unit_shares(U, p.grid);
+  if ((int)blockIdx.x >= shares) return;
+  int64_t u = unit_start(U, shares, blockIdx.x);
+  const int64_t u_end = unit_start(U, shares, blockIdx.x + 1);
+  int seq = 0, held = 0;
+  int64_t base = 0;
+  for (int s0 = 0; s0 < B; s0 += 64) {
+    if (B > 64) read_batch(s0);
+    held = s0;
+    const uint64_t above = __builtin_amdgcn_ballot_w64(s0 + lane < B && base + upto > u);
+    if (above) {
+      const int at = __builtin_ctzll(above);
+      seq = s0 + at;
+      base += from_lane(upto - n_mine, at);
+      break;
+    }
+    base += from_lane(upto, 63);
+  }
+
+  struct Keys {
+    u32x4 k[BITS == 16 ? T : 1][ND];
+    uint32_t c[BITS == 4 ? T : 1][ND], s[T][2];
+    float* at[T];
+    float old[T];
+    bool ok[T];
+  };
+  while (u < u_end && seq < B) {
+    if (seq >= held + 64) read_batch(held += 64);
+    const PagedSeq sq = from_lane(mine, seq - held);
+    const int64_t units = units_of(sq);
+    if (u >= base + units) {
+      base += units;
+      ++seq;
+      continue;
+    }
+    const int nb = (int)(((int64_t)sq.L + KEYS - 1) / KEYS);
+    const int h = (int)quotient(u - base, nb), blk0 = (int)(u - base - (int64_t)h * nb);
+    const int blk1 = u_end - u < nb - blk0 ? blk0 + (int)(u_end - u) : nb;
     const int nrows = sq.n * p.group;
-    int from = 0;                          // the first row that attends key0
-    if (p.causal && key0 > sq.first) from = (key0 - sq.first) * p.group / 16 * 16;
-    for (int r0 = from; r0 < nrows; r0 += 16) {
+    const int32_t* table = p.c.table + seq * p.c.table_str;
+    const char* kbase = p.c.k + h * p.c.k_str[2];
+    const uint8_t* sbase = BITS == 4 ? p.c.ks + h * p.c.ks_str[2] : nullptr;
+    char* wbase = wp.w + h * wp.w_str[2];
+    bool bad = false;
+
+    shortx8 qf[ND];
+    float lse = 0.f;                       // times log2(e)
+    int lim = 0;                           // keys that the lane's row gives anything to
+    auto load_rows = [&](int r0) __attribute__((always_inline)) {
       const int r = r0 + x < nrows ? r0 + x : nrows - 1;
       const RowRef ref = row_ref(p, sq, h, r);
       const char* qp = p.q + ref.tok * p.q_str[0] + ref.head * p.q_str[1];
-      shortx8 qf[ND];
 #pragma unroll
       for (int i = 0; i < ND; ++i) qf[i] = *reinterpret_cast<const shortx8*>(qp + 2 * (BITS == 16 ? 32 * i + 8 * g : (D / 4) * g + 8 * i));
-      const float lse = wp.lse[ref.tok * p.H + ref.head] * 1.4426950408889634f;
-      const int lim = r0 + x < nrows && __builtin_fabsf(lse) < __builtin_inff() ? key_limit(p, sq, r) - key0 : 0;
+      lse = wp.lse[ref.tok * p.H + ref.head] * kLog2e;
+      lim = r0 + x < nrows && __builtin_fabsf(lse) < __builtin_inff() ? key_limit(p, sq, r) : 0;
+    };
+    load_rows(0);
+
+    auto key_pos = [&](int b, int j) __attribute__((always_inline)) { return key_within(b * KEYS + wave * KW + 16 * j + x, sq.L); };
+    auto load_pages = [&](int b, int* page) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < T; ++j) page[j] = table[page_of(p.c, key_pos(b, j))];
+    };
+    auto load = [&](int b, const int* page, Keys& st) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < T; ++j) {
-        floatx4 s = {0.f, 0.f, 0.f, 0.f};
+        const int pos = key_pos(b, j);
+        const PagedRow at = paged_row(p.c, pos, page[j]);
+        st.ok[j] = at.ok;
+        bad |= !at.ok;
+        const char* kr = kbase + at.page * p.c.k_str[0] + at.slot * p.c.k_str[1];
+        if constexpr (BITS == 16) {
 #pragma unroll
-        for (int i = 0; i < ND; ++i) s = Mat<E>::mfma16(kf[j][i], qf[i], s);
+          for (int i = 0; i < ND; ++i) st.k[j][i] = *reinterpret_cast<const u32x4*>(kr + 64 * i + 16 * g);
+        } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], p.scale_log2, -lse));
-          acc[j][k] += 16 * j + 4 * g + k < lim ? w : 0.f;
+          for (int i = 0; i < ND; ++i) st.c[j][i] = reinterpret_cast<const uint32_t*>(kr + (D / 8) * g)[i];
+          const uint8_t* s = sbase + at.page * p.c.ks_str[0] + at.slot * p.c.ks_str[1];
+          st.s[j][0] = s[(D / 4) * g / 32];
+          st.s[j][1] = kTwoScales ? s[((D / 4) * g + D / 4 - 1) / 32] : 0;
+        }
+        st.at[j] = reinterpret_cast<float*>(wbase + at.page * wp.w_str[0] + at.slot * wp.w_str[1]);
+        st.old[j] = 0.f;
+        if (keeps && wp.accumulate) st.old[j] = *st.at[j];
+      }
+    };
+    auto compute = [&](int b, const Keys& st) __attribute__((always_inline)) {
+      const int key0 = b * KEYS + wave * KW;
+      if (key0 >= sq.L) return;
+      shortx8 kf[T][ND];
+#pragma unroll
+      for (int j = 0; j < T; ++j)
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+          if constexpr (BITS == 16) kf[j][i] = __builtin_bit_cast(shortx8, st.k[j][i]);
+          else kf[j][i] = decode8<E>(st.c[j][i], kTwoScales && ((D / 4) * g + 8 * i) / 32 != (D / 4) * g / 32 ? st.s[j][1] : st.s[j][0]);
+        }
+      floatx4 acc[T];
+#pragma unroll
+      for (int j = 0; j < T; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+      int from = 0;                        // the first rows that attend key0
+      if (p.causal && key0 > sq.first) from = (key0 - sq.first) * p.group / 16 * 16;
+      for (int r0 = nrows > 16 ? from : 0; r0 < nrows; r0 += 16) {
+        if (nrows > 16) load_rows(r0);
+#pragma unroll
+        for (int j = 0; j < T; ++j) {
+          floatx4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < ND; ++i) s = Mat<E>::mfma16(kf[j][i], qf[i], s);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], p.scale_log2, -lse));
+            acc[j][k] += key0 + 16 * j + 4 * g + k < lim ? w : 0.f;
+          }
         }
       }
-    }
 #pragma unroll
-    for (int j = 0; j < T; ++j) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float a = acc[j][k];
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) a += __shfl_xor(a, d);
-        const int key = key0 + 16 * j + 4 * g + k;
-        if (x == k && key < sq.L) {
-          const PagedRow at = paged_row(p.c, key, table[page_of(p.c, key)]);
-          if (at.ok) store_weight(p, wp, sq, h, key, at, a);
+      for (int j = 0; j < T; ++j) {
+        // sums over the 16 lanes of a group; of the four keys the lane keeps x % 4
+        const float a = (x & 1 ? acc[j][1] : acc[j][0]) + __shfl_xor(x & 1 ? acc[j][0] : acc[j][1], 1);
+        const float c = (x & 1 ? acc[j][3] : acc[j][2]) + __shfl_xor(x & 1 ? acc[j][2] : acc[j][3], 1);
+        float sum = (x & 2 ? c : a) + __shfl_xor(x & 2 ? a : c, 2);
+        sum += __shfl_xor(sum, 4);
+        sum += __shfl_xor(sum, 8);
+        const int key = key0 + 16 * j + x;
+        if (keeps && key < sq.L && st.ok[j]) *st.at[j] = (key < sq.first ? st.old[j] : 0.f) + sum;
+      }
+    };
+
+    Keys a, z;
+    int page[T];
+    load_pages(blk0, page);
+    load(blk0, page, a);
+    load_pages(blk0 + 1, page);
+    for (int b = blk0; b < blk1; b += 2) {
+      if (b + 1 < blk1) {
+        load(b + 1, page, z);
+        load_pages(b + 2, page);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      compute(b, a);
+      if (b + 1 < blk1) {
+        if (b + 2 < blk1) {
+          load(b + 2, page, a);
+          load_pages(b + 3, page);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        compute(b + 1, z);
       }
     }
+    if (bad) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
+    u += blk1 - blk0;
+  }
+}
+
+// Many rows: bound by the exponentials (a lane's 16 per 32 keys and rows take longer
+// than their products).  A work-group has 128 keys of a key head, a wave 32 of them in
+// registers as its matrix operand; the rows come through LDS for all four, 64 at a
+// time (32 of the large heads), and of two tiles of 32 one's exponentials run beside
+// the other's products.  A key's sum stays in a register from the first row to the
+// last; where there are few keys for the card, work-groups share their rows and
+// paged_weights_merge_kernel adds what they found, in their order.
+template <int D, typename E, int BITS>
+__global__ __launch_bounds__(256, D <= 128 ? 4 : 2) void paged_weights_rows_kernel(PagedAttnParams p, WeightsParams wp) {
+  constexpr int NK = D / 16, KEYS = kWeightKeys, RB = 2 * D;       // RB: bytes of a row
+  constexpr int CH = D / 8, NT = D <= 128 ? 2 : 1, ROWS = 32 * NT, NL = (ROWS * CH + 255) / 256;
+  __shared__ __attribute__((aligned(16))) char q_s[2][ROWS * RB];
+  __shared__ float lse_s[2][ROWS];
+  __shared__ int lim_s[2][ROWS];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int half = lane >> 5, i32 = lane & 31;
+  // chunk c (16 bytes) of row r: eight rows' reads of one chunk number cover the banks
+  auto at_lds = [](int r, int c) __attribute__((always_inline)) { return RB * r + 16 * (c ^ (D == 96 ? (r & 3) : (r & 7))); };
+  auto count = [&](const PagedSeq& s) __attribute__((always_inline)) {
+    return s.n ? ((int64_t)s.L + KEYS - 1) / KEYS * p.c.Hkv * wp.splits : (int64_t)0;
+  };
+  walk_units(p.c, count, [&](int seq, const PagedSeq& sq, int64_t u, int64_t id) __attribute__((always_inline)) {
+    const int64_t unit = quotient(u, wp.splits);
+    const int split = (int)(u - unit * wp.splits);
+    const int chunk = (int)quotient(unit, p.c.Hkv), h = (int)(unit - (int64_t)chunk * p.c.Hkv);
+    const int key_wg = chunk * KEYS, key0 = key_wg + 32 * wave;
+    const int32_t* table = p.c.table + seq * p.c.table_str;
+    shortx8 kf[NK];
+    const int pos = key_within(key0 + i32, sq.L);
+    const PagedRow at = paged_row(p.c, pos, table[page_of(p.c, pos)]);
+    {
+      const char* kr = p.c.k + h * p.c.k_str[2] + at.page * p.c.k_str[0] + at.slot * p.c.k_str[1];
+      if constexpr (BITS == 16) {
+#pragma unroll
+        for (int c = 0; c < NK; ++c) kf[c] = *reinterpret_cast<const shortx8*>(kr + 32 * c + 16 * half);
+      } else {
+        const uint8_t* s = p.c.ks + h * p.c.ks_str[2] + at.page * p.c.ks_str[0] + at.slot * p.c.ks_str[1];
+#pragma unroll
+        for (int c = 0; c < NK; ++c) kf[c] = decode8<E>(*reinterpret_cast<const uint32_t*>(kr + 8 * c + 4 * half), s[c / 2]);
+      }
+    }
+    if (!at.ok) paged_flag(p.c, LVSA_PAGED_BAD_PAGE);
+    const int nrows = sq.n * p.group;
+    int from = 0, to = nrows;              // from the first rows that attend any of these keys on
+    if (p.causal && key_wg > sq.first) from = (key_wg - sq.first) * p.group / ROWS * ROWS;
+    if (wp.splits > 1) {
+      const int tiles = (nrows - from + ROWS - 1) / ROWS;
+      const int64_t end = quotient((int64_t)tiles * (split + 1), wp.splits) * ROWS;
+      to = from + end < nrows ? from + (int)end : nrows;
+      from += (int)quotient((int64_t)tiles * split, wp.splits) * ROWS;
+    }
+    // Each thread's rows of the next tiles, and its lse and limit: token and head move on by ROWS.
+    const int step_i = ROWS / p.group, step_j = ROWS - step_i * p.group;
+    struct At {
+      int r, i, j;
+    };
+    At mine[NL], mine_lse;
+    auto start = [&](int row) __attribute__((always_inline)) {
+      const int r = from + row, i = (uint32_t)r / (uint32_t)p.group;
+      return At{r, i, r - i * p.group};
+    };
+    auto advance = [&](At& a) __attribute__((always_inline)) {
+      a.r += ROWS;
+      a.i += step_i;
+      a.j += step_j;
+      if (a.j >= p.group) {
+        a.j -= p.group;
+        ++a.i;
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < NL; ++i) mine[i] = start((threadIdx.x + 256 * i) / CH % ROWS);
+    mine_lse = start(threadIdx.x % ROWS);
+    u32x4 next[NL];
+    float lse_next = 0.f;
+    int lim_next = 0;
+    auto load = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {       // behind the last row: the last token's first head
+        const bool in = mine[i].r < nrows;
+        const int64_t tok = sq.t0 + (in ? mine[i].i : sq.n - 1);
+        next[i] = *reinterpret_cast<const u32x4*>(p.q + tok * p.q_str[0] + (h * p.group + (in ? mine[i].j : 0)) * p.q_str[1] +
+                                                  16 * ((threadIdx.x + 256 * i) % CH));
+        advance(mine[i]);
+      }
+      if (threadIdx.x < ROWS) {
+        const bool in = mine_lse.r < to;
+        const int i = in ? mine_lse.i : sq.n - 1, j = in ? mine_lse.j : 0;
+        lse_next = wp.lse[(int64_t)(sq.t0 + i) * p.H + h * p.group + j] * kLog2e;
+        const int e = p.causal ? (int)((int64_t)sq.first + i + 1 < sq.L ? sq.first + i + 1 : sq.L) : sq.L;
+        lim_next = in && __builtin_fabsf(lse_next) < __builtin_inff() ? e : 0;
+        advance(mine_lse);
+      }
+    };
+    auto store = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int k = threadIdx.x + 256 * i;
+        if (ROWS * CH % 256 == 0 || k < ROWS * CH) *reinterpret_cast<u32x4*>(q_s[s] + at_lds(k / CH, k % CH)) = next[i];
+      }
+      if (threadIdx.x < ROWS) {
+        lse_s[s][threadIdx.x] = lse_next;
+        lim_s[s][threadIdx.x] = lim_next;
+      }
+    };
+    floatx16 acc = floatx16{0};
+    __syncthreads();                       // LDS of the unit before has been read
+    if (from < to) {
+      load();
+      store(0);
+    }
+    __syncthreads();
+    int s = 0;
+    for (int r0 = from; r0 < to; r0 += ROWS, s ^= 1) {
+      if (r0 + ROWS < to) load();
+      __builtin_amdgcn_sched_barrier(0);
+      floatx16 z[NT];
+      float lse[NT];
+      int lim[NT];
+      bool partly = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        lse[t] = lse_s[s][32 * t + i32];
+        lim[t] = lim_s[s][32 * t + i32] - key0 - 4 * half;
+        partly |= lim[t] < 32 - 4 * half;
+        z[t] = floatx16{0};
+#pragma unroll
+        for (int c = 0; c < NK; ++c)
+          z[t] = Mat<E>::mfma32(kf[c], *reinterpret_cast<const shortx8*>(q_s[s] + at_lds(32 * t + i32, 2 * c + half)), z[t]);
+      }
+      if (__builtin_amdgcn_ballot_w64(partly)) {         // keys behind a row, or a row without weights
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(z[t][k], p.scale_log2, -lse[t]));
+            acc[k] += 8 * (k >> 2) + (k & 3) < lim[t] ? w : 0.f;
+          }
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) acc[k] += __builtin_amdgcn_exp2f(__builtin_fmaf(z[t][k], p.scale_log2, -lse[t]));
+      }
+      if (r0 + ROWS < to) store(s ^ 1);
+      __syncthreads();
+    }
+    // Sums over the 32 lanes of a half, in halves of what a lane holds: it ends with key
+    // 8 (i32 >> 3) + 4 half + (i32 & 3) of the tile, which is key i32 where bit 2 of i32
+    // is the half, and that is the key whose page it looked up.
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = acc[k];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = (i32 & 16 ? v[k + 8] : v[k]) + __shfl_xor(i32 & 16 ? v[k] : v[k + 8], 16);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = (i32 & 8 ? v[k + 4] : v[k]) + __shfl_xor(i32 & 8 ? v[k] : v[k + 4], 8);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) v[k] = (i32 & 2 ? v[k + 2] : v[k]) + __shfl_xor(i32 & 2 ? v[k] : v[k + 2], 2);
+    float sum = (i32 & 1 ? v[1] : v[0]) + __shfl_xor(i32 & 1 ? v[0] : v[1], 1);
+    sum += __shfl_xor(sum, 4);
+    const int key = key0 + i32;
+    if (((i32 >> 2) & 1) != half || key >= sq.L) return;
+    if (wp.splits > 1) {
+      wp.ws[id * KEYS + 32 * wave + i32] = sum;
+    } else if (at.ok) {
+      float* w = reinterpret_cast<float*>(wp.w + at.page * wp.w_str[0] + at.slot * wp.w_str[1] + h * wp.w_str[2]);
+      *w = (wp.accumulate && key < sq.first ? *w : 0.f) + sum;
+    }
+  });
+}
+
+// Adds the sums of work-groups that share their rows: a thread per key.
+__global__ __launch_bounds__(kWeightKeys) void paged_weights_merge_kernel(PagedAttnParams p, WeightsParams wp) {
+  auto count = [&](const PagedSeq& s) __attribute__((always_inline)) {
+    return s.n ? ((int64_t)s.L + kWeightKeys - 1) / kWeightKeys * p.c.Hkv : (int64_t)0;
+  };
+  walk_units(p.c, count, [&](int seq, const PagedSeq& sq, int64_t u, int64_t id) __attribute__((always_inline)) {
+    const int chunk = (int)quotient(u, p.c.Hkv), h = (int)(u - (int64_t)chunk * p.c.Hkv);
+    const int key = chunk * kWeightKeys + (int)threadIdx.x;
+    if (key >= sq.L) return;
+    const PagedRow at = paged_row(p.c, key, p.c.table[seq * p.c.table_str + page_of(p.c, key)]);
+    float sum = 0.f;
+    for (int s = 0; s < wp.splits; ++s) sum += wp.ws[(id * wp.splits + s) * kWeightKeys + threadIdx.x];
+    if (!at.ok) return;
+    float* w = reinterpret_cast<float*>(wp.w + at.page * wp.w_str[0] + at.slot * wp.w_str[1] + h * wp.w_str[2]);
+    *w = (wp.accumulate && key < sq.first ? *w : 0.f) + sum;
   });
 }
 
 template <int D, typename E, int BITS>
 int paged_weights_launch(const PagedAttnParams& p, const WeightsParams& w, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_weights_kernel<D, E, BITS>), dim3((unsigned)p.grid), dim3(256), 0, stream, p, w);
+  if (w.many) {
+    hipLaunchKernelGGL((paged_weights_rows_kernel<D, E, BITS>), dim3((unsigned)p.grid), dim3(256), 0, stream, p, w);
+    const int rc = launch_status("lvsa_paged_weights");
+    if (rc || w.splits == 1) return rc;
+    hipLaunchKernelGGL(paged_weights_merge_kernel, dim3((unsigned)p.grid), dim3(kWeightKeys), 0, stream, p, w);
+  } else {
+    hipLaunchKernelGGL((paged_weights_kernel<D, E, BITS>), dim3((unsigned)p.grid), dim3(256), 0, stream, p, w);
+  }
   return launch_status("lvsa_paged_weights");
 }
 

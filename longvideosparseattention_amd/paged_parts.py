@@ -48,7 +48,7 @@ MAX_BLOCKS = 1024                              # of a list (lvsa_paged.h)
 # The C structs behind cache and batch (see include/lvsa_amd.h).
 _SELECT = struct.Struct("@3P5q7i4x")
 _LISTS = struct.Struct("@P3i4x")
-_WEIGHTS = struct.Struct("@3P5qf4i4x")
+_WEIGHTS = struct.Struct("@3P5qf4i4xPq")
 _EVICT = struct.Struct("@4P4q4i")
 assert _ATTN_AT + _SELECT.size == C.sizeof(capi.PagedSelectArgs)
 assert _ATTN_AT + _ATTN.size + _LISTS.size == C.sizeof(capi.PagedBlockAttnArgs)
@@ -119,6 +119,20 @@ def _lists(N: int, B: int, top: int, tile: int) -> int:
     if not 1 <= tile < 1 << 31:
         raise ValueError(f"tiles of {tile} rows")
     return N if tile == 1 else N // tile + B
+
+
+def _needed(query: str, a, cache: PagedKVCache, N: int, H: int, page_table: torch.Tensor, *more: int) -> int:
+    """Bytes of workspace of a call, asked once for its sizes."""
+    key = (query, cache.device.index, cache.bits, cache.head_dim, cache.num_kv_heads, cache.page_size, N, H, *page_table.shape, *more)
+    need = _WORKSPACE.get(key)
+    if need is None:
+        n = C.c_int64(0)
+        with torch.cuda.device(cache.device):            # the size follows its compute units
+            capi.check(query, getattr(capi.lib(), query)(C.byref(a), C.byref(n)))
+        if len(_WORKSPACE) > 1024:
+            _WORKSPACE.clear()
+        need = _WORKSPACE[key] = n.value
+    return need
 
 
 def paged_kv_block_means(cache: PagedKVCache, means: torch.Tensor, kv_lens: torch.Tensor, page_table: torch.Tensor, *,
@@ -225,17 +239,7 @@ def paged_block_attention(q: torch.Tensor, cache: PagedKVCache, blocks: torch.Te
         a = capi.PagedBlockAttnArgs.from_buffer_copy(packed + batch + _ATTN.pack(
             q_ptr, o_ptr, 0 if lse is None else lse.data_ptr(), *q_str, *o_str, scale, H, int(bool(causal)), 1 if fresh else 2, 0, 0,
             0, 0) + _LISTS.pack(blocks.data_ptr(), block_size, top, tile))
-        key = ("blocks", cache.device.index, cache.bits, D, cache.num_kv_heads, cache.page_size, N, H, *page_table.shape, block_size,
-               top, tile)
-        need = _WORKSPACE.get(key)
-        if need is None:
-            n = C.c_int64(0)
-            with torch.cuda.device(cache.device):        # the size follows its compute units
-                capi.check("lvsa_paged_block_attn_workspace_query",
-                           capi.lib().lvsa_paged_block_attn_workspace_query(C.byref(a), C.byref(n)))
-            if len(_WORKSPACE) > 1024:
-                _WORKSPACE.clear()
-            need = _WORKSPACE[key] = n.value
+        need = _needed("lvsa_paged_block_attn_workspace_query", a, cache, N, H, page_table, block_size, top, tile)
         if need:
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
             a.attn.workspace, a.attn.workspace_bytes = ws.data_ptr(), need
@@ -283,7 +287,11 @@ def paged_kv_weights(q: torch.Tensor, lse: torch.Tensor, cache: PagedKVCache, we
     if N and page_table.shape[0]:
         a = capi.PagedWeightsArgs.from_buffer_copy(packed + batch + _WEIGHTS.pack(
             q_ptr, lse.data_ptr(), weights.data_ptr(), *q_str, *strides, scale, H, int(bool(causal)), int(bool(accumulate)),
-            min(mq, 0x7fffffff)))
+            min(mq, 0x7fffffff), 0, 0))
+        need = _needed("lvsa_paged_weights_workspace_query", a, cache, N, H, page_table, mq)
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need
         hip_ops._call(cache.device, "lvsa_paged_weights", C.byref(a))
     return weights
 
