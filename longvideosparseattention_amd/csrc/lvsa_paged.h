@@ -259,8 +259,11 @@ __host__ __device__ inline int list_count(const ListView& v, const PagedSeq& q) 
 struct BlockAttnParams {
   ListView v;
   const int32_t* blocks;               // [lists][Hkv][top]
-  int32_t subs, splits;                // row tiles of a list, work-groups that share its keys
-  int64_t units;                       // lists x subs x key heads
+  // The launch's work is key heads x lists x row tiles of a list (`subs`), each of
+  // `steps` steps, as many as the longest list has (a shorter one's keys are spread
+  // over them); it is cut into equal shares for `grid` work-groups, see DecodeSlots.
+  int32_t subs, steps;
+  int64_t work;
 };
 int paged_block_attn_d64(const PagedAttnParams& p, const BlockAttnParams& l, int bits, int rows, bool bf16, hipStream_t stream);
 int paged_block_attn_d96(const PagedAttnParams& p, const BlockAttnParams& l, int bits, int rows, bool bf16, hipStream_t stream);
@@ -278,6 +281,9 @@ struct WeightsParams {
   float* ws;                           // their sums: [128 keys][splits][128]
 };
 constexpr int kWeightKeys = 128;
+// Work-groups of few rows' weights on a compute unit at once (255, 187, 182 us with 1 to
+// 3 for 45 sequences of up to 16000 keys, 8 heads of 128).
+constexpr int kWeightGroups = 3;
 int paged_weights_d64(const PagedAttnParams& p, const WeightsParams& w, int bits, bool bf16, hipStream_t stream);
 int paged_weights_d96(const PagedAttnParams& p, const WeightsParams& w, int bits, bool bf16, hipStream_t stream);
 int paged_weights_d128(const PagedAttnParams& p, const WeightsParams& w, int bits, bool bf16, hipStream_t stream);

@@ -645,11 +645,12 @@ int scale_check(const char* what, float scale) {
   return LVSA_OK;
 }
 
-// How an attention over lists runs: rows of a tile, row tiles of a list and
-// work-groups that share its keys.
+// How an attention over lists runs: rows of a tile, row tiles of a list, the steps of
+// each, and the work-groups that share them.
 struct BlockShape {
-  int rows, subs, splits;
-  int64_t units, bytes;
+  int rows, subs, steps, grid;
+  int64_t work, o_elems;
+  int64_t bytes(int D) const { return 4 * (o_elems + o_elems / D * 2); }
 };
 BlockShape block_shape(const lvsa_paged_block_attn_args* a, const ListView& v) {
   BlockShape s{};
@@ -658,14 +659,15 @@ BlockShape block_shape(const lvsa_paged_block_attn_args* a, const ListView& v) {
   const int64_t rows = (v.tile.by < N ? v.tile.by : N) * group;
   s.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kPagedTile;
   s.subs = (int)ceil_div(rows, s.rows);
-  s.units = (int64_t)v.lists * s.subs * t.cache.Hkv;
+  const int64_t units = (int64_t)v.lists * s.subs * t.cache.Hkv;
   const int64_t cap = (int64_t)t.batch.max_pages * t.cache.page_size;
-  const int64_t keys = (int64_t)v.top * v.block.by < cap ? (int64_t)v.top * v.block.by : cap;
-  const int64_t steps = ceil_div(keys, s.rows == kPagedTile ? kPagedBlock : paged_decode_keys((int)D));
-  const int64_t want = ceil_div(2 * cus, s.units > 0 ? s.units : 1);
-  s.splits = (int)(want < steps ? want : steps);
-  if (s.splits < 1) s.splits = 1;
-  s.bytes = s.splits == 1 ? 0 : 4 * s.units * s.splits * s.rows * (D + 2);
+  int64_t keys = (int64_t)v.top * v.block.by < cap ? (int64_t)v.top * v.block.by : cap;
+  if (keys < 1) keys = 1;
+  s.steps = (int)ceil_div(keys, s.rows == kPagedTile ? kPagedBlock : paged_decode_keys((int)D));
+  s.work = units * s.steps;
+  const int64_t slots = cus * (s.rows == kPagedTile ? (D >= 192 ? 1 : 2) : paged_decode_groups((int)D, t.cache.bits, s.rows));
+  s.grid = (int)(s.work < slots ? s.work : slots);
+  s.o_elems = s.work == s.grid * (int64_t)s.steps ? 0 : 2LL * s.grid * s.rows * D;
   return s;
 }
 
@@ -710,7 +712,7 @@ WeightsShape weights_shape(const lvsa_paged_weights_args* a) {
     s.bytes = s.splits == 1 ? 0 : 4 * units * s.splits * kWeightKeys;
     units *= s.splits;
   }
-  const int64_t most = s.many ? 64 * cus : cus * (a->cache.D <= 128 ? 2 : 1);
+  const int64_t most = s.many ? 64 * cus : cus * kWeightGroups;
   s.grid = (int)(units < most ? units : most);
   return s;
 }
@@ -775,7 +777,7 @@ int lvsa_paged_block_attn_workspace_query(const lvsa_paged_block_attn_args* a, i
   ListView v{};
   const int rc = block_attn_check(a, &p, &v);
   if (rc) return rc;
-  *bytes = a->attn.batch.N == 0 || a->attn.batch.B == 0 ? 0 : block_shape(a, v).bytes;
+  *bytes = a->attn.batch.N == 0 || a->attn.batch.B == 0 ? 0 : block_shape(a, v).bytes(a->attn.cache.D);
   return LVSA_OK;
 }
 
@@ -797,10 +799,11 @@ int lvsa_paged_block_attn_fwd(const lvsa_paged_block_attn_args* a, hipStream_t s
                "%s: o must not share memory with q", what);
   LVSA_REQUIRE(t.batch.B > 0, LVSA_ERR_INVALID_ARG, "%s: rows of no sequence", what);
   const BlockShape s = block_shape(a, l.v);
-  LVSA_REQUIRE(s.bytes == 0 || (t.workspace && aligned16((int64_t)(uintptr_t)t.workspace)), LVSA_ERR_INVALID_ARG,
-               "%s: %lld bytes of 16-byte aligned workspace needed", what, (long long)s.bytes);
-  LVSA_REQUIRE(s.bytes == 0 || t.workspace_bytes >= s.bytes, LVSA_ERR_CAPACITY, "%s: workspace of %lld bytes < %lld", what,
-               (long long)t.workspace_bytes, (long long)s.bytes);
+  const int64_t need = s.bytes(t.cache.D);
+  LVSA_REQUIRE(need == 0 || (t.workspace && aligned16((int64_t)(uintptr_t)t.workspace)), LVSA_ERR_INVALID_ARG,
+               "%s: %lld bytes of 16-byte aligned workspace needed", what, (long long)need);
+  LVSA_REQUIRE(need == 0 || t.workspace_bytes >= need, LVSA_ERR_CAPACITY, "%s: workspace of %lld bytes < %lld", what,
+               (long long)t.workspace_bytes, (long long)need);
   p.q = (const char*)t.q;
   p.o = (char*)t.o;
   p.lse = t.lse;
@@ -811,11 +814,12 @@ int lvsa_paged_block_attn_fwd(const lvsa_paged_block_attn_args* a, hipStream_t s
   p.fill_tail = t.fill_tail;
   p.short_rows = p.c.k_str[1] >= 0 && p.c.k_str[1] < (1 << 26) && p.c.v_str[1] >= 0 && p.c.v_str[1] < (1 << 26);
   p.ws_o = (float*)t.workspace;
-  p.ws_ml = p.ws_o + s.units * s.splits * s.rows * t.cache.D;
+  p.ws_ml = p.ws_o + s.o_elems;
+  p.grid = s.grid;
   l.blocks = a->blocks;
   l.subs = s.subs;
-  l.splits = s.splits;
-  l.units = s.units;
+  l.steps = s.steps;
+  l.work = s.work;
   const bool bf16 = t.cache.dtype == LVSA_BF16;
   switch (t.cache.D) {
     case 64: return paged_block_attn_d64(p, l, t.cache.bits, s.rows, bf16, stream);

@@ -114,8 +114,8 @@ struct ListKeys {
   }
 };
 
-// One row tile of a list and one of the parts of its keys after the other, `ROWS`
-// rows a tile, `KEYS` keys a step; `work` does a part.
+// The work-group's share: a row tile of a list and some of its key steps after the
+// other, `ROWS` rows a tile, `KEYS` keys a step; `work` does a part.
 template <int D, typename E, int ROWS, int KEYS, typename Work>
 __device__ __forceinline__ void walk_lists(const PagedAttnParams& p, const BlockAttnParams& l, KeyList& list, Work work) {
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -127,14 +127,17 @@ __device__ __forceinline__ void walk_lists(const PagedAttnParams& p, const Block
     return;
   }
   if (p.fill_tail) fill_tail_rows(p, D, lane, wave, 4);
-  const int64_t total = l.units * l.splits;
-  for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
-    const int64_t unit = quotient(w, l.splits);
-    const int split = (int)(w - unit * l.splits);
-    const int64_t ls = quotient(unit, p.c.Hkv);
-    const int h = (int)(unit - ls * p.c.Hkv);
-    const int64_t li = quotient(ls, l.subs);
-    const int sub = (int)(ls - li * l.subs);
+  // (the grid is a multiple of the XCDs, or the shares are in the work-groups' order)
+  const int share = p.grid % 8 ? (int)blockIdx.x : share_of(blockIdx.x, p.grid);
+  const int64_t first = unit_start(l.work, p.grid, share), end = unit_start(l.work, p.grid, share + 1);
+  for (int64_t w = first; w < end;) {
+    const int64_t unit = quotient(w, l.steps), w0 = unit * l.steps;
+    const int s0 = (int)(w - w0), s1 = end - w0 < l.steps ? (int)(end - w0) : l.steps;
+    w = w0 + s1;
+    const int64_t hl = quotient(unit, l.subs);
+    const int sub = (int)(unit - hl * l.subs);
+    const int h = (int)quotient(hl, l.v.lists);
+    const int64_t li = hl - (int64_t)h * l.v.lists;
     PagedSeq sq;
     int i0;
     const int seq = paged_seq_of_list(p.c, l.v, li, lane, &sq, &i0);
@@ -151,8 +154,9 @@ __device__ __forceinline__ void walk_lists(const PagedAttnParams& p, const Block
     k.L = uniform(list.bad ? 0 : k.limit(key_limit(p, sq, r1)));      // keys that the tile's last row attends
     if (list.bad && threadIdx.x == 0) paged_flag(p.c, list.bad);
     const int nb = (k.L + KEYS - 1) / KEYS;
-    const DecodePart part = {sq, h, r0, nrows, (int)quotient((int64_t)split * nb, l.splits), (int)quotient((int64_t)(split + 1) * nb, l.splits),
-                             w, l.splits == 1, list.bad != 0 || (sq.flags & LVSA_PAGED_BAD_LENGTH) != 0};
+    const DecodePart part = {sq, h, r0, nrows, (int)quotient((int64_t)s0 * nb, l.steps), (int)quotient((int64_t)s1 * nb, l.steps),
+                             2 * (int64_t)share + (first < w0 ? 1 : 0),          // see decode_slots
+                             s0 == 0 && s1 == l.steps, list.bad != 0 || (sq.flags & LVSA_PAGED_BAD_LENGTH) != 0};
     work(part, k);
   }
 }
@@ -173,62 +177,80 @@ __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_block_prefill_ker
   });
 }
 
-// Joins the parts of a row: a wave per row, a lane four elements of it.
+// Joins the partials of row tiles that shares divide, 32 rows a work-group: a lane has
+// four elements of a row and a wave R rows at a time, of every partial on their way at
+// once.  Bound by the partials' bytes.
 template <int D, typename E>
 __global__ __launch_bounds__(256) void paged_block_merge_kernel(PagedAttnParams p, BlockAttnParams l, int rows) {
+  typedef E e4 __attribute__((ext_vector_type(4)));
+  constexpr int LR = D / 4, R = 64 / LR;               // lanes per row, rows per wave
+  constexpr int STEPS = 8 / R;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < (int64_t)p.c.N * p.H; row += 4 * (int64_t)gridDim.x) {
-    const int t = (uint32_t)row / (uint32_t)p.H, hq = (int)(row - (int64_t)t * p.H);
-    int flags = 0, seq = -1;
-    PagedSeq sq = {};
-    for (int s0 = 0; s0 < p.c.B; s0 += 64) {
-      PagedSeq q = {};
-      bool in = false;
-      if (s0 + lane < p.c.B) {
-        q = paged_seq(p.c, s0 + lane);
-        in = q.t0 <= t && t < q.t0 + q.n;
-        flags |= q.flags;
+  const int sub = lane / LR, d = 4 * (lane % LR);
+  int bad = 0;
+  for (int s = lane; s < p.c.B; s += 64)
+    bad |= paged_seq(p.c, s).flags & LVSA_PAGED_BAD_CU;
+  if (__builtin_amdgcn_ballot_w64(bad != 0)) return;   // spoiled already
+  const int64_t units = quotient(l.work, l.steps);
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const DecodeSlots parts = decode_slots(l.work, p.grid, unit * l.steps, l.steps);
+    if (parts.count == 0) continue;                    // written by the attention kernel
+    const int64_t hl = quotient(unit, l.subs);
+    const int part = (int)(unit - hl * l.subs), h = (int)quotient(hl, l.v.lists);
+    PagedSeq sq;
+    int i0;
+    if (paged_seq_of_list(p.c, l.v, hl - (int64_t)h * l.v.lists, lane, &sq, &i0) < 0) continue;
+    const int r0 = i0 * p.group + part * rows, i1 = i0 + l.v.tile.by < sq.n ? i0 + l.v.tile.by : sq.n;
+    const int end = i1 * p.group - r0 < rows ? i1 * p.group - r0 : rows;       // rows of the tile
+    if (32 * (int)blockIdx.y >= end || sub >= R) continue;
+    float M[STEPS], sum[STEPS];
+    floatx4 o[STEPS];
+    int r[STEPS];
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+      r[k] = 32 * blockIdx.y + 8 * wave + R * k + sub;
+      M[k] = kNoKeys;
+      sum[k] = 0.f;
+      o[k] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (32 * (int)blockIdx.y + 8 * wave >= end) continue;
+    for (int i = 0; i < parts.count; ++i) {
+      const int64_t slot = (i == 0 ? parts.first : parts.rest + 2 * i) * rows;
+      float m[STEPS], s[STEPS];
+      floatx4 x[STEPS];
+#pragma unroll
+      for (int k = 0; k < STEPS; ++k) {                // rows past the end: the last one
+        const int64_t at = slot + (r[k] < end ? r[k] : end - 1);
+        m[k] = p.ws_ml[2 * at];
+        s[k] = p.ws_ml[2 * at + 1];
+        x[k] = *reinterpret_cast<const floatx4*>(p.ws_o + at * D + d);
       }
-      const uint64_t m = __builtin_amdgcn_ballot_w64(in);
-      if (m && seq < 0) {
-        seq = s0 + __builtin_ctzll(m);
-        sq = from_lane(q, __builtin_ctzll(m));
+#pragma unroll
+      for (int k = 0; k < STEPS; ++k) {
+        const float top = __builtin_fmaxf(M[k], m[k]);
+        const float a = __builtin_amdgcn_exp2f(M[k] - top), b = __builtin_amdgcn_exp2f(m[k] - top);
+        sum[k] = sum[k] * a + s[k] * b;
+        o[k] = o[k] * a + x[k] * b;
+        M[k] = top;
       }
     }
-    if (seq < 0 || __builtin_amdgcn_ballot_w64(flags & LVSA_PAGED_BAD_CU)) continue;    // the attention kernel's
-    const int h = (uint32_t)hq / (uint32_t)p.group, i = t - sq.t0, tile = i / l.v.tile;
-    const int r = (i - tile * l.v.tile.by) * p.group + (hq - h * p.group);
-    const int64_t unit = ((first_list(l.v, seq, sq) + tile) * l.subs + r / rows) * p.c.Hkv + h;
-    const int64_t at = unit * l.splits * rows + r % rows;
-    // maxima and sums of the parts, one a lane
-    float M = kNoKeys, sum = 0.f;
-    for (int k = lane; k < l.splits; k += 64) M = __builtin_fmaxf(M, p.ws_ml[2 * (at + (int64_t)k * rows)]);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) M = __builtin_fmaxf(M, __shfl_xor(M, d));
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < l.splits; ++k) {
-      const int64_t a = at + (int64_t)k * rows;
-      const float w = __builtin_amdgcn_exp2f(p.ws_ml[2 * a] - M);
-      sum += w * p.ws_ml[2 * a + 1];
-      if (4 * lane < D) {
-        const floatx4 o = *reinterpret_cast<const floatx4*>(p.ws_o + a * D + 4 * lane);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] += w * o[j];
-      }
+    for (int k = 0; k < STEPS; ++k) {
+      if (r[k] >= end) continue;
+      const int i = (r0 + r[k]) / p.group, hq = h * p.group + (r0 + r[k]) - i * p.group;
+      const int64_t t = (int64_t)sq.t0 + i;
+      const float inv = sum[k] == 0.f ? 0.f : 1.0f / sum[k];
+      *reinterpret_cast<e4*>(p.o + t * p.o_str[0] + hq * p.o_str[1] + 2 * d) =
+          e4{(E)(o[k][0] * inv), (E)(o[k][1] * inv), (E)(o[k][2] * inv), (E)(o[k][3] * inv)};
+      if (p.lse && d == 0)
+        p.lse[t * p.H + hq] = sum[k] == 0.f ? -__builtin_inff() : (M[k] + __log2f(sum[k])) * 0.69314718055994530942f;
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    if (4 * lane < D)
-      *reinterpret_cast<u32x2*>(p.o + t * p.o_str[0] + hq * p.o_str[1] + 8 * lane) =
-          u32x2{pack2<E>(acc[0] * inv, acc[1] * inv), pack2<E>(acc[2] * inv, acc[3] * inv)};
-    if (p.lse && lane == 0) p.lse[row] = sum == 0.f ? -__builtin_inff() : (M + __log2f(sum)) * 0.69314718055994530942f;
   }
 }
 
 template <int D, typename E, int BITS>
 int paged_block_launch(const PagedAttnParams& p, const BlockAttnParams& l, int rows, hipStream_t stream) {
-  constexpr int64_t most = 1 << 20;
-  const int64_t total = l.units * l.splits;
-  const dim3 grid((unsigned)(total < most ? total : most));
+  const dim3 grid((unsigned)p.grid);
   if (rows == kPagedTile)
     hipLaunchKernelGGL((paged_block_prefill_kernel<D, E, BITS>), grid, dim3(256), 0, stream, p, l);
   else if (rows == 16)
@@ -236,9 +258,10 @@ int paged_block_launch(const PagedAttnParams& p, const BlockAttnParams& l, int r
   else
     hipLaunchKernelGGL((paged_block_decode_kernel<D, E, BITS, 2>), grid, dim3(256), 0, stream, p, l);
   const int rc = launch_status("lvsa_paged_block_attn_fwd");
-  if (rc || l.splits == 1) return rc;
-  const int64_t out = ceil_div((int64_t)p.c.N * p.H, 4);
-  hipLaunchKernelGGL((paged_block_merge_kernel<D, E>), dim3((unsigned)(out < most ? out : most)), dim3(256), 0, stream, p, l, rows);
+  if (rc || l.work == p.grid * (int64_t)l.steps) return rc;      // every share is one unit
+  const int64_t units = l.work / l.steps, most = 1 << 16;
+  hipLaunchKernelGGL((paged_block_merge_kernel<D, E>), dim3((unsigned)(units < most ? units : most), (unsigned)ceil_div(rows, 32)), dim3(256),
+                     0, stream, p, l, rows);
   return launch_status("lvsa_paged_block_attn_fwd");
 }
 
