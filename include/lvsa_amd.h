@@ -399,15 +399,21 @@ LVSA_API int lvsa_paged_attn_workspace_query(const lvsa_paged_attn_args* a, int6
  * of `block` slots (a divisor of the page size); block j of a sequence is its
  * positions j * block .. (j + 1) * block - 1.
  *
- * Writes the mean key (of the tokens there are, in fp32) of
- * every block that holds one of the newest tokens, or of every block of every
- * sequence where the batch has no cu_seqlens.  means: part i, head h of page p at
- * means + p * m_str[0] + i * m_str[1] + h * m_str[2] floats, D of them, rows at
+ * Writes the mean key (of the tokens there are, in fp32) of every block that holds
+ * one of the newest tokens, or of every block of every sequence where the batch has
+ * no cu_seqlens (its N is only a bound of theirs).  means: part i, head h of page p
+ * at means + p * m_str[0] + i * m_str[1] + h * m_str[2] floats, D of them, rows at
  * multiples of 16 bytes.  Blocks of a bad page, length or row range are left out.
  * Sequences that share a page and count different numbers of tokens in one of its
  * blocks leave the mean of either.  The reference has no counterpart.         */
-LVSA_API int lvsa_paged_block_means(const lvsa_paged_cache* cache, const lvsa_paged_batch* batch, float* means,
-                                    const int64_t m_str[3], int32_t block, hipStream_t stream);
+typedef struct lvsa_paged_means_args {
+  lvsa_paged_cache cache;
+  lvsa_paged_batch batch;
+  float* means;
+  int64_t m_str[3];
+  int32_t block;
+} lvsa_paged_means_args;
+LVSA_API int lvsa_paged_block_means(const lvsa_paged_means_args* a, hipStream_t stream);
 
 /* Selects blocks by their means.  Rows of a sequence are taken in tiles of `tile`;
  * tile i of sequence b is list cu_seqlens[b] / tile + b + i of N / tile + B lists,

@@ -148,6 +148,12 @@ class PagedAttnArgs(C.Structure):
     ]
 
 
+class PagedMeansArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("batch", PagedBatch), ("means", C.c_void_p), ("m_str", _Str3), ("block", C.c_int32),
+    ]
+
+
 class PagedSelectArgs(C.Structure):
     _fields_ = [
         ("cache", PagedCache), ("batch", PagedBatch),
@@ -204,8 +210,7 @@ SIGNATURES = {
                                     C.c_void_p]),
     "lvsa_paged_attn_fwd": (C.c_int, [C.POINTER(PagedAttnArgs), C.c_void_p]),
     "lvsa_paged_attn_workspace_query": (C.c_int, [C.POINTER(PagedAttnArgs), C.POINTER(C.c_int64)]),
-    "lvsa_paged_block_means": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedBatch), C.c_void_p, C.POINTER(C.c_int64),
-                                         C.c_int32, C.c_void_p]),
+    "lvsa_paged_block_means": (C.c_int, [C.POINTER(PagedMeansArgs), C.c_void_p]),
     "lvsa_paged_select": (C.c_int, [C.POINTER(PagedSelectArgs), C.c_void_p]),
     "lvsa_paged_block_attn_fwd": (C.c_int, [C.POINTER(PagedBlockAttnArgs), C.c_void_p]),
     "lvsa_paged_block_attn_workspace_query": (C.c_int, [C.POINTER(PagedBlockAttnArgs), C.POINTER(C.c_int64)]),

@@ -722,21 +722,20 @@ WeightsShape weights_shape(const lvsa_paged_weights_args* a) {
 
 extern "C" {
 
-int lvsa_paged_block_means(const lvsa_paged_cache* cache, const lvsa_paged_batch* batch, float* means, const int64_t m_str[3],
-                           int32_t block, hipStream_t stream) {
+int lvsa_paged_block_means(const lvsa_paged_means_args* a, hipStream_t stream) {
   clear_error();
   const char* what = "lvsa_paged_block_means";
-  LVSA_REQUIRE(cache && batch, LVSA_ERR_INVALID_ARG, "%s: null args", what);
+  LVSA_REQUIRE(a != nullptr, LVSA_ERR_INVALID_ARG, "%s: null args", what);
   MeansParams p{};
-  int rc = paged_view(what, cache, batch, false, &p.c);
-  if (!rc) rc = means_view(what, cache, means, m_str, block, p.m_str, &p.block, &p.parts);
+  int rc = paged_view(what, &a->cache, &a->batch, false, &p.c);
+  if (!rc) rc = means_view(what, &a->cache, a->means, a->m_str, a->block, p.m_str, &p.block, &p.parts);
   if (rc) return rc;
-  if (batch->B == 0 || (batch->cu_seqlens && batch->N == 0)) return LVSA_OK;
-  p.means = (char*)means;
-  const int64_t blocks = batch->cu_seqlens ? (int64_t)batch->N / block + 2LL * batch->B
-                                           : (int64_t)batch->B * batch->max_pages * p.parts.by;
-  const int64_t want = blocks * cache->Hkv, most = 16LL * cu_count();
-  return by_type<Means>(cache->D, cache->dtype, cache->bits, p, (unsigned)(want < 1 ? 1 : want < most ? want : most), stream);
+  const lvsa_paged_batch& b = a->batch;
+  if (b.B == 0 || (b.cu_seqlens && b.N == 0)) return LVSA_OK;
+  p.means = (char*)a->means;
+  const int64_t all = (int64_t)b.B * b.max_pages * p.parts.by, touched = (int64_t)b.N / a->block + 2LL * b.B;
+  const int64_t want = (b.cu_seqlens && touched < all ? touched : all) * a->cache.Hkv, most = 4LL * cu_count();
+  return by_type<Means>(a->cache.D, a->cache.dtype, a->cache.bits, p, (unsigned)(want < 1 ? 1 : want < most ? want : most), stream);
 }
 
 int lvsa_paged_select(const lvsa_paged_select_args* a, hipStream_t stream) {

@@ -40,19 +40,33 @@ __device__ __forceinline__ int paged_seq_of_list(const PagedView& c, const ListV
   return -1;
 }
 
+// A thread's part of a list, on its way from memory: blocks tid, tid + 256, ...
+struct ListIds {
+  int id[kListMax / 256];
+  __device__ __forceinline__ void load(const ListView& v, const int32_t* blocks) {
+#pragma unroll
+    for (int k = 0; k < kListMax / 256; ++k) {
+      const int i = threadIdx.x + 256 * k;
+      id[k] = 256 * k < v.top ? blocks[i < v.top ? i : v.top - 1] : 0;
+    }
+  }
+};
+
 // Brings a list into LDS, for a work-group of 256; returns the number of its keys
 // below L.  list.bad: what is wrong with it.
-__device__ __forceinline__ int stage_list(const PagedView& c, const ListView& v, const int32_t* blocks, const int32_t* table,
+__device__ __forceinline__ int stage_list(const PagedView& c, const ListView& v, const ListIds& ids, const int32_t* table,
                                           int L, KeyList& list) {
   if (threadIdx.x == 0) {
     list.n = v.top;
     list.bad = 0;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < v.top; i += 256) {
-    const int id = blocks[i];
-    list.id[i] = id;
-    if (id < 0) atomicMin(&list.n, i);
+#pragma unroll
+  for (int k = 0; k < kListMax / 256; ++k) {
+    const int i = threadIdx.x + 256 * k;
+    if (i >= v.top) continue;
+    list.id[i] = ids.id[k];
+    if (ids.id[k] < 0) atomicMin(&list.n, i);
   }
   __syncthreads();
   const int n = list.n;
@@ -138,6 +152,8 @@ __device__ __forceinline__ void walk_lists(const PagedAttnParams& p, const Block
     const int sub = (int)(unit - hl * l.subs);
     const int h = (int)quotient(hl, l.v.lists);
     const int64_t li = hl - (int64_t)h * l.v.lists;
+    ListIds ids;
+    ids.load(l.v, l.blocks + (li * p.c.Hkv + h) * l.v.top);
     PagedSeq sq;
     int i0;
     const int seq = paged_seq_of_list(p.c, l.v, li, lane, &sq, &i0);
@@ -148,7 +164,7 @@ __device__ __forceinline__ void walk_lists(const PagedAttnParams& p, const Block
     if (r0 >= nrows) continue;
     const int32_t* table = p.c.table + seq * p.c.table_str;
     __syncthreads();                     // the list before has been read
-    const int keys = stage_list(p.c, l.v, l.blocks + (li * p.c.Hkv + h) * l.v.top, table, sq.L, list);
+    const int keys = stage_list(p.c, l.v, ids, table, sq.L, list);
     const int r1 = r0 + ROWS < nrows ? r0 + ROWS - 1 : nrows - 1;
     ListKeys k{list, l.v.block, keys};
     k.L = uniform(list.bad ? 0 : k.limit(key_limit(p, sq, r1)));      // keys that the tile's last row attends

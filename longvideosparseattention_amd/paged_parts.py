@@ -46,10 +46,12 @@ __all__ = ["paged_kv_block_means", "paged_kv_select", "paged_block_attention", "
 MAX_BLOCKS = 1024                              # of a list (lvsa_paged.h)
 
 # The C structs behind cache and batch (see include/lvsa_amd.h).
+_MEANS = struct.Struct("@P3qi4x")
 _SELECT = struct.Struct("@3P5q7i4x")
 _LISTS = struct.Struct("@P3i4x")
 _WEIGHTS = struct.Struct("@3P5qf4i4xPq")
 _EVICT = struct.Struct("@4P4q4i")
+assert _ATTN_AT + _MEANS.size == C.sizeof(capi.PagedMeansArgs)
 assert _ATTN_AT + _SELECT.size == C.sizeof(capi.PagedSelectArgs)
 assert _ATTN_AT + _ATTN.size + _LISTS.size == C.sizeof(capi.PagedBlockAttnArgs)
 assert _ATTN_AT + _WEIGHTS.size == C.sizeof(capi.PagedWeightsArgs)
@@ -67,6 +69,12 @@ def _beside(t: torch.Tensor, name: str, cache: PagedKVCache, shape, rows: bool) 
     if t.requires_grad:
         _no_gradient(t, name)
     s = t.stride()
+    P, S, H = shape[:3]
+    W = shape[3] if rows else 1
+    if s == ((H * S * W, W, S * W, 1) if rows else (H * S, 1, S)) and not t.data_ptr() & 15:
+        lo = t.data_ptr()                    # as allocate_means and allocate_weights lay them out
+        if lo >= cache._high or lo + 4 * P * S * H * W <= cache._low:
+            return s
     if rows and (s[3] != 1 or (t.data_ptr() | (s[0] | s[1] | s[2]) * 4) & 15):
         raise ValueError(f"{name} needs a contiguous last dimension and rows at multiples of 16 bytes")
     at = 1
@@ -82,8 +90,8 @@ def _beside(t: torch.Tensor, name: str, cache: PagedKVCache, shape, rows: bool) 
 def _apart(t: torch.Tensor, name: str, *others: torch.Tensor) -> None:
     lo, hi = _span(t)
     for o in others:
-        a, e = _span(o)
-        if t.numel() and o.numel() and lo < e and a < hi:
+        a, e = _span(o) if o.numel() else (0, 0)
+        if lo < e and a < hi:
             raise ValueError(f"{name} must not share memory with the other tensors of the call")
 
 
@@ -155,11 +163,9 @@ def paged_kv_block_means(cache: PagedKVCache, means: torch.Tensor, kv_lens: torc
     batch = _batch(cache, cu_seqlens, kv_lens, page_table, 0 if cu_seqlens is None else 0x7fffffff)
     if page_table.shape[0] == 0:
         return means
-    packed = cache._pack(cache.dtype or torch.bfloat16)
-    a = capi.PagedAttnArgs()                   # its first two members are what the call takes
-    C.memmove(C.addressof(a), packed + batch, _ATTN_AT)
-    hip_ops._call(cache.device, "lvsa_paged_block_means", C.byref(a.cache), C.byref(a.batch), means.data_ptr(),
-                  capi._Str3(*strides[:3]), block)
+    a = capi.PagedMeansArgs.from_buffer_copy(cache._pack(cache.dtype or torch.bfloat16) + batch +
+                                             _MEANS.pack(means.data_ptr(), *strides[:3], block))
+    hip_ops._call(cache.device, "lvsa_paged_block_means", C.byref(a))
     return means
 
 
