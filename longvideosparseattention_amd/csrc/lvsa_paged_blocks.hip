@@ -665,8 +665,22 @@ BlockShape block_shape(const lvsa_paged_block_attn_args* a, const ListView& v) {
   if (keys < 1) keys = 1;
   s.steps = (int)ceil_div(keys, s.rows == kPagedTile ? kPagedBlock : paged_decode_keys((int)D));
   s.work = units * s.steps;
+  // Shares: one per row tile where these are enough to keep the card busy, which is one
+  // for every compute unit (of 4-bit pages, which need waves to decode, one for every
+  // work-group that runs at once): nothing is to be joined, and each reads one list.
+  // Otherwise as many whole parts of a tile as come near to what runs at once, else
+  // equal shares.  us, with one share a tile and with equal shares:
+  //   16 bits, 128: 444 tiles of 128 rows 195, 214; 384 of 16 rows 86, 86; 800 92, 94;
+  //                 26000 (prompts, each token its own list, of 64) 705, 844
+  //   16 bits, 64:  256 of 16 rows 27, 33; 16 bits, 256: 120 68, 56 and 132 of 128 rows 96, 90
+  //   16 bits, 128: 160 of 16 rows 70, 69; 64 67, 40; 4 37, 22
+  //    4 bits, 128: 800 41, 43; 320 68, 56 (54 in two parts each)
   const int64_t slots = cus * (s.rows == kPagedTile ? (D >= 192 ? 1 : 2) : paged_decode_groups((int)D, t.cache.bits, s.rows));
-  s.grid = (int)(s.work < slots ? s.work : slots);
+  const int64_t enough = t.cache.bits == 16 ? cus : slots, parts = units > 0 ? slots / units : 0;
+  int64_t shares = s.work < slots ? s.work : slots;
+  if (units >= enough && units <= kMostGroups) shares = units;
+  else if (parts >= 2 && parts <= s.steps && 5 * parts * units >= 4 * slots) shares = parts * units;
+  s.grid = (int)shares;
   s.o_elems = s.work == s.grid * (int64_t)s.steps ? 0 : 2LL * s.grid * s.rows * D;
   return s;
 }

@@ -141,8 +141,8 @@ __device__ __forceinline__ void walk_lists(const PagedAttnParams& p, const Block
     return;
   }
   if (p.fill_tail) fill_tail_rows(p, D, lane, wave, 4);
-  // (the grid is a multiple of the XCDs, or the shares are in the work-groups' order)
-  const int share = p.grid % 8 ? (int)blockIdx.x : share_of(blockIdx.x, p.grid);
+  const int share = share_of(blockIdx.x, p.grid);
+  if (share < 0) return;
   const int64_t first = unit_start(l.work, p.grid, share), end = unit_start(l.work, p.grid, share + 1);
   for (int64_t w = first; w < end;) {
     const int64_t unit = quotient(w, l.steps), w0 = unit * l.steps;
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(256) void paged_block_merge_kernel(PagedAttnParams 
 
 template <int D, typename E, int BITS>
 int paged_block_launch(const PagedAttnParams& p, const BlockAttnParams& l, int rows, hipStream_t stream) {
-  const dim3 grid((unsigned)p.grid);
+  const dim3 grid((unsigned)(8 * ceil_div(p.grid, 8)));           // see share_of
   if (rows == kPagedTile)
     hipLaunchKernelGGL((paged_block_prefill_kernel<D, E, BITS>), grid, dim3(256), 0, stream, p, l);
   else if (rows == 16)
