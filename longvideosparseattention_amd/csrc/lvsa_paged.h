@@ -254,6 +254,10 @@ constexpr int kListMax = 1024;         // blocks of a list: what a work-group ke
 __host__ __device__ inline int64_t first_list(const ListView& v, int s, const PagedSeq& q) {
   return v.tile.by == 1 ? q.t0 : (int64_t)(q.t0 / v.tile) + s;
 }
+// End of the rows of a tile that starts at row i0 < q.n of its sequence.
+__host__ __device__ inline int tile_end(const ListView& v, const PagedSeq& q, int i0) {
+  return q.n - i0 > v.tile.by ? i0 + v.tile.by : q.n;
+}
 __host__ __device__ inline int list_count(const ListView& v, const PagedSeq& q) { return (int)(((int64_t)q.n + v.tile.by - 1) / v.tile.by); }
 
 struct BlockAttnParams {

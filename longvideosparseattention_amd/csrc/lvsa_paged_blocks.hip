@@ -111,6 +111,15 @@ __device__ __forceinline__ uint64_t bound_between(uint64_t lo, uint64_t hi, int 
   return mid > lo && mid <= hi ? mid : lo + (hi - lo) / 2 + 1;
 }
 
+// The same for fp32: half way between the numbers for 16 steps, then, where these close
+// in on 0 or stand far apart, half way between their bit patterns.
+__device__ __forceinline__ float float_between(float lo, float hi, int step) {
+  if (step < 16) return 0.5f * lo + 0.5f * hi;
+  auto flip = [](int b) { return b < 0 ? b ^ 0x7fffffff : b; };
+  const int64_t a = flip(__builtin_bit_cast(int, lo)), b = flip(__builtin_bit_cast(int, hi));
+  return __builtin_bit_cast(float, flip((int)((a + b + 1) >> 1)));
+}
+
 struct Span {
   uint64_t lo, hi;
 };
@@ -130,18 +139,20 @@ __device__ __forceinline__ Span wave_span(Span s) {
 // those that are not always selected until a bound cuts off exactly `top`: an fp32
 // comparison and a count per 64 of them, a dozen steps.  Where that does not come out
 // (the border runs between scores that fp32 does not tell apart, infinities, NaN), the
-// ranks themselves are halved.
+// ranks between the two are halved: no step where they are all alike.
 template <int K>
 __device__ __forceinline__ void wave_select(const uint64_t* ranks, int n, int top, int lane, int32_t* out) {
   uint32_t up[K], low[K];
   float x[K];
   float lof = __builtin_inff(), hif = -__builtin_inff();
+  bool nan = false;                        // or -inf
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const bool in = 64 * k + lane < n;
     const uint64_t r = ranks[in ? 64 * k + lane : n - 1];
     x[k] = r == kAlways ? __builtin_inff() : r == 0 ? -__builtin_inff() : (float)score_of(r);
-    lof = __builtin_fminf(lof, x[k]);
+    nan |= x[k] == -__builtin_inff();
+    lof = x[k] > -__builtin_inff() ? __builtin_fminf(lof, x[k]) : lof;
     hif = r != kAlways ? __builtin_fmaxf(hif, x[k]) : hif;
     if (!in) x[k] = -__builtin_inff();     // below what any bound keeps
     up[k] = in ? (uint32_t)(r >> 32) : 0;
@@ -155,9 +166,15 @@ __device__ __forceinline__ void wave_select(const uint64_t* ranks, int n, int to
   int count = n;
   uint64_t bound = 0;                      // at least `top` ranks from it on
   {
+    if (__builtin_amdgcn_ballot_w64(nan)) {      // are the others enough?
+      int fine = 0;
+#pragma unroll
+      for (int k = 0; k < K; ++k) fine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[k] >= lof));
+      if (fine < top) lof = -__builtin_inff();
+    }
     float cut = 0.f;
-    for (;;) {
-      const float mid = 0.5f * lof + 0.5f * hif;
+    for (int step = 0;; ++step) {
+      const float mid = float_between(lof, hif, step);
       if (!(mid > lof && mid <= hif)) break;
       int c = 0;
 #pragma unroll
@@ -169,7 +186,7 @@ __device__ __forceinline__ void wave_select(const uint64_t* ranks, int n, int to
         cut = mid;
         break;
       }
-      if (c < top && mid == hif && !(0.5f * lof + 0.5f * hif < hif)) break;
+      if (c < top && !(float_between(lof, hif, step + 1) < hif)) break;
     }
     if (count == top) {
 #pragma unroll
@@ -179,8 +196,18 @@ __device__ __forceinline__ void wave_select(const uint64_t* ranks, int n, int to
       bound = 1;
     }
   }
-  if (count != top) {
-    uint64_t high = kAlways;
+  if (count != top) {                      // the border lies among the ranks of [lof, hif]
+    Span s = {kAlways, 0};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const uint64_t r = (uint64_t)up[k] << 32 | low[k];
+      const bool in = 64 * k + lane < n && r != kAlways;
+      if (in && x[k] >= lof && r < s.lo) s.lo = r;
+      if (in && x[k] <= hif && r > s.hi) s.hi = r;
+    }
+    s = wave_span(s);
+    bound = s.lo;
+    uint64_t high = s.hi;
     while (bound < high && count != top) {
       const uint64_t mid = bound + (high - bound) / 2 + 1;
       int c = 0;
@@ -366,7 +393,7 @@ __global__ __launch_bounds__(256) void paged_select_kernel(SelectParams p) {
     ListRange range = {0, 0, -1};
     int i1 = 0;
     if (seq >= 0) {
-      i1 = i0 + p.v.tile.by < sq.n ? i0 + p.v.tile.by : sq.n;
+      i1 = tile_end(p.v, sq, i0);
       range = list_range(p, sq, i0, i1);
     }
     const int n = range.n, top = p.v.top;
@@ -490,8 +517,8 @@ __global__ __launch_bounds__(64 * kGroupWaves) void paged_select_group_kernel(Se
     const int tile = p.v.tile.by, lists = list_count(p.v, sq), l0 = r0 / p.v.tile;
     const int64_t list0 = first_list(p.v, seq, sq) + l0;
     auto range_of = [&](int l) __attribute__((always_inline)) {
-      const int i0 = (l0 + l) * tile, i1 = i0 + tile < sq.n ? i0 + tile : sq.n;
-      return list_range(p, sq, i0, i1);
+      const int i0 = (l0 + l) * tile;
+      return list_range(p, sq, i0, tile_end(p.v, sq, i0));
     };
     const int here = lists - l0 < kGroup ? lists - l0 : kGroup;
     const int n = sq.flags ? 0 : range_of(here - 1).n;       // of the last list, which sees the most
@@ -500,7 +527,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void paged_select_group_kernel(Se
     if (n > top) {
       double q[D / 4] = {};
       {
-        const int l = x < here ? x : here - 1, i0 = (l0 + l) * tile, i1 = i0 + tile < sq.n ? i0 + tile : sq.n;
+        const int l = x < here ? x : here - 1, i0 = (l0 + l) * tile, i1 = tile_end(p.v, sq, i0);
         for (int i = i0; i < i1; ++i)
           for (int j = 0; j < p.group; ++j) {
             const char* src = p.q + (int64_t)(sq.t0 + i) * p.q_str[0] + (h * p.group + j) * p.q_str[1] + 8 * g;

@@ -396,6 +396,7 @@ int lvsa_paged_evict(const lvsa_paged_evict_args* a, hipStream_t stream) {
   EvictParams p{};
   const int rc = paged_view(what, &a->cache, &a->batch, false, &p.c);
   if (rc) return rc;
+  LVSA_REQUIRE(a->keep < INT32_MAX - 4096, LVSA_ERR_UNSUPPORTED, "%s: %d tokens to keep: below 2^31 - 4096", what, a->keep);
   LVSA_REQUIRE(a->keep >= 1 && a->first >= 0 && a->last >= 0 && (int64_t)a->first + a->last <= a->keep, LVSA_ERR_INVALID_ARG,
                "%s: %d tokens, the first %d and last %d among them", what, a->keep, a->first, a->last);
   LVSA_REQUIRE(a->weights && ((uintptr_t)a->weights & 3) == 0, LVSA_ERR_INVALID_ARG, "%s: weights must be non-null, fp32", what);

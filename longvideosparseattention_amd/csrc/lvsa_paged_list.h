@@ -159,7 +159,7 @@ __device__ __forceinline__ void walk_lists(const PagedAttnParams& p, const Block
     const int seq = paged_seq_of_list(p.c, l.v, li, lane, &sq, &i0);
     if (seq < 0) continue;
     const int r0 = i0 * p.group + sub * ROWS;
-    const int i1 = i0 + l.v.tile.by < sq.n ? i0 + l.v.tile.by : sq.n;
+    const int i1 = tile_end(l.v, sq, i0);
     const int nrows = i1 * p.group;
     if (r0 >= nrows) continue;
     const int32_t* table = p.c.table + seq * p.c.table_str;
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(256) void paged_block_merge_kernel(PagedAttnParams 
     PagedSeq sq;
     int i0;
     if (paged_seq_of_list(p.c, l.v, hl - (int64_t)h * l.v.lists, lane, &sq, &i0) < 0) continue;
-    const int r0 = i0 * p.group + part * rows, i1 = i0 + l.v.tile.by < sq.n ? i0 + l.v.tile.by : sq.n;
+    const int r0 = i0 * p.group + part * rows, i1 = tile_end(l.v, sq, i0);
     const int end = i1 * p.group - r0 < rows ? i1 * p.group - r0 : rows;       // rows of the tile
     if (32 * (int)blockIdx.y >= end || sub >= R) continue;
     float M[STEPS], sum[STEPS];

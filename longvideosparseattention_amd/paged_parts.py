@@ -329,7 +329,7 @@ def paged_kv_evict(cache: PagedKVCache, weights: torch.Tensor, kv_lens: torch.Te
     strides = _beside(weights, "weights", cache, (cache.num_pages, cache.page_size, cache.num_kv_heads), False)
     batch = _batch(cache, None, kv_lens, page_table, 0)
     B, pages = page_table.shape
-    if not 1 <= keep < 1 << 31 or first < 0 or last < 0 or first + last > keep:
+    if not 1 <= keep < (1 << 31) - 4097 or first < 0 or last < 0 or first + last > keep:
         raise ValueError(f"{keep} tokens to keep, the first {first} and the last {last} among them")
     to = row = new_pages = 0
     if new_table is not None:

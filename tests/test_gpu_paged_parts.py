@@ -108,14 +108,18 @@ def test_select(gpu, i, dtype):
     assert torch.equal(got.cpu(), want)
 
 
-def test_select_takes_the_lower_of_equal_blocks_and_nan_last(gpu):
-    seqs = [(1, 700), (1, 640)]
+@pytest.mark.parametrize("n", [1, 40])
+def test_select_takes_the_lower_of_equal_blocks_and_nan_last(gpu, n):
+    seqs = [(n, 700), (n, 640)]
     b = Batch(gpu, seqs, 64, 2, 1, 10, BF, seed=7)
     q = torch.randint(-2, 3, (b.N, 2, 64), generator=b.gen).to(BF).to(gpu)        # whole numbers: sums are exact
     rows = [torch.randint(-1, 2, (-(-L // 10), 1, 64), generator=b.gen).float() for _, L in seqs]
     rows[0][5:60] = rows[0][5]                                                  # many alike
     rows[1][3:40] = float("nan")
     rows[1][45], rows[1][46] = float("inf"), 0.0
+    rows[0][61] = rows[0][62] = 0.5
+    rows[0][61, 0, 0] += 2.0 ** -24                                             # scores nearer than fp32 tells apart
+    rows[0][8:11] = 0.0                                                         # and scores of 0
     like = b.cache.allocate_means(10)
     like.copy_(ref.paged(b, rows, 10, float("nan"), like))
     for top in (3, 20, 40, 61, 64, 70, 71):
