@@ -173,7 +173,7 @@ __device__ __forceinline__ void wave_select(const uint64_t* ranks, int n, int to
       if (fine < top) lof = -__builtin_inff();
     }
     float cut = 0.f;
-    for (int step = 0;; ++step) {
+    for (int step = 0; step < 48; ++step) {      // 16 and 32 close any range
       const float mid = float_between(lof, hif, step);
       if (!(mid > lof && mid <= hif)) break;
       int c = 0;
@@ -186,7 +186,6 @@ __device__ __forceinline__ void wave_select(const uint64_t* ranks, int n, int to
         cut = mid;
         break;
       }
-      if (c < top && !(float_between(lof, hif, step + 1) < hif)) break;
     }
     if (count == top) {
 #pragma unroll
