@@ -234,8 +234,10 @@ __global__ __launch_bounds__(256, D <= 96 ? 3 : 2) void paged_weights_rows_kerne
   __shared__ int lim_s[2][ROWS];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int half = lane >> 5, i32 = lane & 31;
-  // chunk c (16 bytes) of row r: eight rows' reads of one chunk number cover the banks
-  auto at_lds = [](int r, int c) __attribute__((always_inline)) { return RB * r + 16 * (c ^ (D == 96 ? (r & 3) : (r & 7))); };
+  // chunk c (16 bytes) of row r: sixteen rows' reads of one chunk cover the 64 banks once
+  auto at_lds = [](int r, int c) __attribute__((always_inline)) {
+    return RB * r + 16 * (c ^ (D == 96 ? r >> 2 & 3 : D == 64 || D == 192 ? r >> 1 & 7 : r & 15));
+  };
   auto count = [&](const PagedSeq& s) __attribute__((always_inline)) {
     return s.n ? ((int64_t)s.L + KEYS - 1) / KEYS * p.c.Hkv * wp.splits : (int64_t)0;
   };
