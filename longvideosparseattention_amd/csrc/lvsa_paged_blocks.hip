@@ -22,7 +22,10 @@ struct MeansParams {
 
 // One work-group per block and head: a thread sums 8 elements of every RPP-th key,
 // the sums are joined in LDS.  fp32 within a thread (at most block / RPP keys), 64
-// bits across them, one rounding at the end.  Bound by the keys' bytes.
+// bits across them, one rounding at the end.  Latency where an append touched a few
+// blocks (32 sequences, one token: 4.3 us), else the keys' bytes: 4680 tokens of 12
+// heads of 128 7.3 us, 2.0 TB/s, of which 3 are the launch and the batch.  (Sixteen
+// work-groups a unit instead of four, most without a block: 5.5 us for the former.)
 template <int D, typename E, int BITS>
 __global__ __launch_bounds__(256) void paged_means_kernel(MeansParams p) {
   constexpr int CH = D / 8, RPP = 256 / CH;
@@ -372,6 +375,9 @@ __device__ __forceinline__ void keep_highest(Ranks& r, int n, int top) {
 // with it, eight lanes a block, and keeps the highest.  64-bit sums, so that which of
 // two blocks is the higher does not depend on the order they were summed in (short of
 // differences of 1e-15): a list is the same on every device and beside every batch.
+// Bound by trips to memory one after the other (batch, queries, page table, means) and
+// one wave's search: 45 lists of 8 heads over up to 250 blocks 12 to 14 us for 27 MB.
+// (The first means loaded before the queries: 15.5 us; eight of them at once: 22.)
 template <int D, typename E>
 __global__ __launch_bounds__(256) void paged_select_kernel(SelectParams p) {
   constexpr int CH = D / 8, RPP = 256 / CH, U = D <= 128 ? 4 : 2;    // U: blocks of eight lanes on their way
@@ -485,8 +491,14 @@ __global__ __launch_bounds__(256) void paged_select_kernel(SelectParams p) {
 
 // One work-group per 16 lists of a sequence and key head, for lists of few rows: the
 // scores of 16 blocks for 16 lists on the matrix cores, in 64 bits; a wave then selects
-// for two lists.  A lane of group g = lane / 16 holds elements 16 i + 4 g .. + 3 of
+// for four lists.  A lane of group g = lane / 16 holds elements 16 i + 4 g .. + 3 of
 // block (of list) lane % 16.
+//
+// 6500 tokens of prompts, 4 heads of 64, up to 325 blocks: 78 us (484 with a work-group a
+// list), of which the selection is 35 (a timing variant without it takes 43) and the
+// 64-bit products are 10: MFMA busy 11%, VALU issuing 33%, the rest is waiting on the
+// searches' counts.  (Eight waves, two lists each: 116 us, the queries' sums twice; fp32
+// scores in LDS and the ranks anew where they tie: 95, with 3 to 6 groups a unit 93 to 107.)
 template <int D, typename E>
 __global__ __launch_bounds__(64 * kGroupWaves) void paged_select_group_kernel(SelectParams p, ListView groups, int pitch) {
   extern __shared__ uint64_t group_ranks[];    // [16][pitch]
@@ -741,7 +753,10 @@ WeightsShape weights_shape(const lvsa_paged_weights_args* a) {
   // rows of a sequence, if unknown: one each where there are no more than sequences, else all of one
   const int64_t N = a->batch.N, q = a->max_q_len > 0 ? (a->max_q_len < N ? a->max_q_len : N) : N <= a->batch.B ? 1 : N;
   const int64_t rows = q * (a->H / a->cache.Hkv), B = a->batch.B < N ? a->batch.B : N, cus = cu_count();
-  s.many = rows > 32;
+  // The rows' kernel from 48 rows a sequence and key head on: us, few rows' and rows'
+  // kernel, 8 sequences of 8000 keys, 8 heads of 128: 16 rows 31, 51; 32 42, 51; 48 50,
+  // 51; 64 58, 50; 128 90, 61 (32 sequences of 4000: 32 rows 72, 100; 64 100, 100).
+  s.many = rows > 48;
   s.splits = 1;
   const int64_t cap = (int64_t)a->batch.max_pages * a->cache.page_size;
   int64_t units = B * ceil_div(cap, s.many ? kWeightKeys : paged_decode_keys(a->cache.D)) * a->cache.Hkv;
@@ -803,9 +818,16 @@ int lvsa_paged_select(const lvsa_paged_select_args* a, hipStream_t stream) {
   p.first = a->first;
   p.last = a->last;
   p.causal = a->causal;
-  // Lists together where sequences have many and they are short
+  // Sixteen lists of a sequence together where sequences have many, of few rows, and
+  // there are more of them than one round of single work-groups takes.  us, sixteen
+  // together and one by one, lists of 32 blocks of 64 over 8000 keys, 8 heads of 128:
+  //   lists x heads 256: 17, 12; 512: 18, 12 (of one sequence 25, 11); 1024 (4 and 16 a
+  //   sequence): 20, 19 and 25, 18; 2048 (8 and 256): 24, 33 and 25, 33; 16384: 59, 227
+  //   rows of a list, its tokens x query heads, 16384 lists x heads: 4: 59, 227; 16: 100,
+  //   248; 4096 of 16: 52, 65; 2080 of 32: 50, 36
   const int64_t cap = (int64_t)a->batch.max_pages * p.v.parts.by;
-  const bool grouped = (int64_t)a->tile * p.group <= 16 && p.v.lists >= 8LL * a->batch.B && cap <= kWaveKeys;
+  const bool grouped = (int64_t)a->tile * p.group <= 16 && p.v.lists >= 8LL * a->batch.B &&
+                       (int64_t)p.v.lists * a->cache.Hkv >= 6LL * cu_count() && cap <= kWaveKeys;
   return by_type<Select>(a->cache.D, a->cache.dtype, 16, p, grouped, stream);
 }
 

@@ -177,6 +177,10 @@ __device__ __forceinline__ void walk_lists(const PagedAttnParams& p, const Block
   }
 }
 
+// Few rows: bound by the bytes of the lists' keys and values, and for one list by trips
+// to memory one after the other (batch and list, page table, keys).  45 lists of 8 heads,
+// 32 blocks of 64 of 128, 78 to 85 us, 4.6 TB/s; 4 bits, 40 of 64 blocks, 51 + 5 us, 3.4
+// TB/s; one of 512 keys 11 + 4 us.
 template <int D, typename E, int BITS, int NT>
 __global__ __launch_bounds__(256, D == 256 || (D == 192 && NT == 2) ? 1 : paged_decode_groups(D, BITS, 16 * NT)) void paged_block_decode_kernel(PagedAttnParams p, BlockAttnParams l) {
   __shared__ KeyList list;
@@ -185,6 +189,11 @@ __global__ __launch_bounds__(256, D == 256 || (D == 192 && NT == 2) ? 1 : paged_
   });
 }
 
+// Tiles of many rows: bound as the dense kernel (MFMA busy 33%, VALU issuing 37%), with
+// fewer work-groups than fill it evenly: 4680 tokens of 12 heads of 128, tiles of 128, 48
+// blocks of 104 of 28080 keys 186 to 198 us, 740 TFLOP/s (dense attention over as many
+// keys, in tiles of 256 rows, 183 us).  Copies of 16 keys that cross blocks take the slow
+// way: blocks of 104 cost a tenth more than of 64, 128 or 512.
 template <int D, typename E, int BITS>
 __global__ __launch_bounds__(256, D >= 192 ? 1 : 2) void paged_block_prefill_kernel(PagedAttnParams p, BlockAttnParams l) {
   __shared__ KeyList list;

@@ -80,11 +80,12 @@ SELECT = [  # sequences, D, H, Hkv, page, block, top, tile, first, last, causal
     ([(20, 20), (1, 1513), (40, 800)], 256, 8, 4, 390, 15, 9, 7, 1, 0, True),
     ([(2, 9000)], 64, 1, 1, 8, 1, 1024, 1, 0, 0, False),        # more blocks than are ranked at a time
     ([(1, 30000), (3, 11000)], 64, 4, 2, 64, 2, 100, 2, 1, 2, True),
-    ([(300, 700), (100, 900), (0, 50), (17, 17), (65, 64)], 64, 4, 2, 8, 8, 12, 1, 2, 2, True),    # sixteen lists at a time
-    ([(300, 2000), (210, 250)], 128, 3, 3, 20, 2, 33, 5, 0, 3, False),
-    ([(200, 300), (180, 200)], 96, 4, 1, 3, 1, 7, 3, 1, 0, True),
-    ([(90, 130), (70, 75)], 192, 2, 2, 16, 4, 5, 2, 1, 1, True),
-    ([(64, 700)], 256, 8, 1, 32, 8, 40, 1, 1, 1, False),
+    ([(300, 700), (100, 900), (0, 50), (17, 17), (65, 64)], 64, 4, 2, 8, 8, 12, 1, 2, 2, True),
+    ([(300, 700), (100, 900), (0, 50), (17, 17), (65, 64)], 64, 16, 8, 8, 8, 12, 1, 2, 2, True),   # sixteen lists at a time
+    ([(300, 2000), (210, 250)], 128, 16, 16, 20, 2, 33, 5, 0, 3, False),
+    ([(200, 300), (180, 200)], 96, 32, 16, 3, 1, 7, 3, 1, 0, True),
+    ([(90, 130), (70, 75)], 192, 20, 20, 16, 4, 5, 2, 1, 1, True),
+    ([(64, 700)], 256, 72, 24, 32, 8, 40, 1, 1, 1, False),
 ]
 
 
@@ -108,12 +109,12 @@ def test_select(gpu, i, dtype):
     assert torch.equal(got.cpu(), want)
 
 
-@pytest.mark.parametrize("n", [1, 40])
-def test_select_takes_the_lower_of_equal_blocks_and_nan_last(gpu, n):
+@pytest.mark.parametrize("n,Hkv", [(1, 1), (40, 20)])
+def test_select_takes_the_lower_of_equal_blocks_and_nan_last(gpu, n, Hkv):
     seqs = [(n, 700), (n, 640)]
-    b = Batch(gpu, seqs, 64, 2, 1, 10, BF, seed=7)
-    q = torch.randint(-2, 3, (b.N, 2, 64), generator=b.gen).to(BF).to(gpu)        # whole numbers: sums are exact
-    rows = [torch.randint(-1, 2, (-(-L // 10), 1, 64), generator=b.gen).float() for _, L in seqs]
+    b = Batch(gpu, seqs, 64, 2 * Hkv, Hkv, 10, BF, seed=7)
+    q = torch.randint(-2, 3, (b.N, 2 * Hkv, 64), generator=b.gen).to(BF).to(gpu)  # whole numbers: sums are exact
+    rows = [torch.randint(-1, 2, (-(-L // 10), Hkv, 64), generator=b.gen).float() for _, L in seqs]
     rows[0][5:60] = rows[0][5]                                                  # many alike
     rows[1][3:40] = float("nan")
     rows[1][45], rows[1][46] = float("inf"), 0.0

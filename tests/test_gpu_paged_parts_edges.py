@@ -440,12 +440,12 @@ def test_tiles_longer_than_a_sequence(gpu, tile):
 @pytest.mark.parametrize("blocks", [700, 1000, 1024, 1025])
 def test_selection_among_about_a_thousand_blocks(gpu, blocks):
     """The table's width decides which kernel ranks: sixteen lists at once up to 1024 blocks, in 131 KB of LDS."""
-    b = Batch(gpu, [(40, 4 * blocks - 1)], 64, 2, 2, 4, BF, seed=28)
-    rows = [torch.randn(blocks, 2, 64, generator=b.gen)]
+    b = Batch(gpu, [(100, 4 * blocks - 1)], 64, 16, 16, 4, BF, seed=28)
+    rows = [torch.randn(blocks, 16, 64, generator=b.gen)]
     means = b.cache.allocate_means(4)
     means.copy_(ref.paged(b, rows, 4, 0.0, means))
-    q = b.randn(40, 2, 64)
-    for top in (20, 513, 1024):
+    q = b.randn(100, 16, 64)
+    for top in (20, 1000):
         assert torch.equal(lv.paged_kv_select(q, b.cache, means, *b.call(), top).cpu(), ref.select(b, q, rows, 4, top, 1, 1, 1, True))
 
 
