@@ -268,8 +268,8 @@ def paged_kv_weights(q: torch.Tensor, lse: torch.Tensor, cache: PagedKVCache, we
     Rows whose ``lse`` is not finite give nothing.  Sequences without new rows or with a
     bad length or row range, tokens on bad pages and slots of no sequence are left
     alone.  Sequences that share pages must not be in one call (each would add to the
-    same weights).  Scores and sums are fp32, in an order that does not depend on the
-    batch.  ``max_q_len`` (the most rows of a sequence) only chooses a kernel."""
+    same weights).  Scores and sums are fp32, in an order that follows from the shapes
+    alone.  ``max_q_len`` (the most rows of a sequence) only chooses a kernel."""
     if is_compiling():
         return _outside["weights"](q, lse, cache, weights, cu_seqlens, kv_lens, page_table, causal=causal, scale=scale,
                                    accumulate=accumulate, max_q_len=max_q_len)
