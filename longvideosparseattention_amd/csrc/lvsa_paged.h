@@ -1,7 +1,9 @@
 // What the kernels over the paged key/value cache share (lvsa_paged.hip:
 // append, gather, merge and the C ABI; lvsa_paged_attn.h: attention, one unit
-// per head size): the cache and batch as the device sees them, the lookup of
-// rows through the page table, and the number format of 4-bit pages.
+// per head size; lvsa_paged_blocks.hip, lvsa_paged_list.h, lvsa_paged_weights.h and
+// lvsa_paged_evict.hip: parts of a cache): the cache and batch as the device sees
+// them, the lookup of rows through the page table, and the number format of 4-bit
+// pages.
 //
 // Nothing read from device memory is trusted: page numbers, lengths and row
 // ranges are checked where they are used, so that no address leaves the

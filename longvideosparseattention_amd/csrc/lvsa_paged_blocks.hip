@@ -86,7 +86,7 @@ struct SelectParams {
   const char* means;
   int32_t* blocks;
   int64_t q_str[2], m_str[3];            // bytes
-  int32_t H, group, first, last, causal;
+  int32_t group, first, last, causal;
 };
 
 constexpr int kSelectKeys = 4096;        // blocks ranked at a time
@@ -813,7 +813,6 @@ int lvsa_paged_select(const lvsa_paged_select_args* a, hipStream_t stream) {
   p.q = (const char*)a->q;
   p.means = (const char*)a->means;
   p.blocks = a->blocks;
-  p.H = a->H;
   p.group = a->H / a->cache.Hkv;
   p.first = a->first;
   p.last = a->last;

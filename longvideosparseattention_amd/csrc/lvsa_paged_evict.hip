@@ -15,7 +15,7 @@ struct EvictParams {
   const int32_t* to;                     // new_table, or null: in place
   int64_t to_str;
   int32_t* kept; int32_t* new_lens;
-  int32_t to_pages, keep, first, last, D;
+  int32_t keep, first, last;
 };
 
 // A weight as a number that sorts like it: NaN below -inf, 0 and -0 alike.
@@ -417,7 +417,6 @@ int lvsa_paged_evict(const lvsa_paged_evict_args* a, hipStream_t stream) {
   for (int i = 0; i < 3; ++i) p.w_str[i] = 4 * a->w_str[i];
   p.to = a->new_table;
   p.to_str = a->new_stride;
-  p.to_pages = a->new_pages;
   p.kept = a->kept;
   p.new_lens = a->new_lens;
   p.keep = a->keep;
