@@ -214,8 +214,10 @@ __device__ __forceinline__ Move move_of(const EvictParams& p, int b, int old, in
 
 // To pages of their own: nothing is read that is written, all rows at once.  A thread
 // has a 16-byte piece of a key and of its value; the first ones of a row bring its
-// scales and weight.  Bound by the bytes: 64 heads' 2048 tokens of 128 29 to 32 us, 4.4
-// TB/s (one piece at a time, behind its page numbers: 35).
+// scales and weight.  Bound by the bytes; rows pass the L2 by on their way out, which the
+// next call would find full of them: 64 heads' 2048 tokens of 128 and their selection 60.5
+// us, 65 without.  Four pieces a thread on their way (two: 65, eight: 79; one behind its
+// page numbers: 68).
 template <int D, int BITS>
 __global__ __launch_bounds__(256) void paged_evict_move_kernel(EvictParams p, int per) {
   constexpr int CH = D * BITS / 128;       // 16-byte pieces of a row
@@ -247,8 +249,8 @@ __global__ __launch_bounds__(256) void paged_evict_move_kernel(EvictParams p, in
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         if (k0 + 256 * j >= n) continue;
-        *reinterpret_cast<u32x4*>(p.c.k + m[j].at.page * p.c.k_str[0] + m[j].at.slot * p.c.k_str[1] + h * p.c.k_str[2] + 16 * c[j]) = x[j];
-        *reinterpret_cast<u32x4*>(p.c.v + m[j].at.page * p.c.v_str[0] + m[j].at.slot * p.c.v_str[1] + h * p.c.v_str[2] + 16 * c[j]) = y[j];
+        __builtin_nontemporal_store(x[j], reinterpret_cast<u32x4*>(p.c.k + m[j].at.page * p.c.k_str[0] + m[j].at.slot * p.c.k_str[1] + h * p.c.k_str[2] + 16 * c[j]));
+        __builtin_nontemporal_store(y[j], reinterpret_cast<u32x4*>(p.c.v + m[j].at.page * p.c.v_str[0] + m[j].at.slot * p.c.v_str[1] + h * p.c.v_str[2] + 16 * c[j]));
         if constexpr (BITS == 4) {         // 16 bytes are 32 elements: their scale
           p.c.ks[m[j].at.page * p.c.ks_str[0] + m[j].at.slot * p.c.ks_str[1] + h * p.c.ks_str[2] + c[j]] =
               p.c.ks[m[j].from.page * p.c.ks_str[0] + m[j].from.slot * p.c.ks_str[1] + h * p.c.ks_str[2] + c[j]];
