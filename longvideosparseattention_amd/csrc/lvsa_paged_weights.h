@@ -226,9 +226,9 @@ __global__ __launch_bounds__(256, kWeightGroups) void paged_weights_kernel(Paged
 // last; where there are few keys for the card, work-groups share their rows and
 // paged_weights_merge_kernel adds what they found, in their order.
 //
-// 6500 tokens of prompts over up to 5200 keys, 16 heads over 4 of 64, causal: 84 to 88 us
+// 6500 tokens of prompts over up to 5200 keys, 16 heads over 4 of 64, causal: 78 to 84 us
 // and 5 for the sums (181 with a tile of 16 rows at a time from memory, 97 with a division
-// per row instead of the next row's address): VALU issuing 56%, MFMA 14%.
+// per row instead of the next row's address): VALU issuing 63%, MFMA 15%.
 template <int D, typename E, int BITS>
 __global__ __launch_bounds__(256, D <= 96 ? 3 : 2) void paged_weights_rows_kernel(PagedAttnParams p, WeightsParams wp) {
   constexpr int NK = D / 16, KEYS = kWeightKeys, RB = 2 * D;       // RB: bytes of a row
