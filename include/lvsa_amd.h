@@ -457,9 +457,10 @@ LVSA_API int lvsa_paged_block_attn_workspace_query(const lvsa_paged_block_attn_a
  * sum over the sequence's rows that attend the token and the head's query heads of
  * exp(scale q.k - lse), with lse [N, H] as lvsa_paged_attn_fwd gives it.  The newest
  * tokens' own weights start from 0, with `accumulate` 0 all of the sequence's do.
- * Rows whose lse is not finite give nothing; sequences without new rows, with a bad
- * length or row range and tokens on a bad page are left alone.  `max_q_len` (0:
- * unknown) only chooses a kernel.  Workspace: as for lvsa_paged_attn_fwd.       */
+ * Rows whose lse is not finite give nothing; sequences without new rows or with a bad
+ * length and tokens on a bad page are left alone, and all where cu_seqlens does not
+ * ascend.  `max_q_len` (0: unknown) only chooses a kernel.  Workspace: as for
+ * lvsa_paged_attn_fwd.                                                          */
 typedef struct lvsa_paged_weights_args {
   lvsa_paged_cache cache;
   lvsa_paged_batch batch;

@@ -290,6 +290,13 @@ constexpr int kWeightKeys = 128;
 // Work-groups of few rows' weights on a compute unit at once (255, 187, 182 us with 1 to
 // 3 for 45 sequences of up to 16000 keys, 8 heads of 128).
 constexpr int kWeightGroups = 3;
+// Work of a sequence: its key heads x blocks of `keys` keys.  Over row ranges that
+// ascend there are no more sequences with work than rows or sequences, for which the
+// workspace has room; other batches are refused whole, since each of their ranges may
+// be fine by itself and all of them together more (tests/native/paged_weights_check.cpp).
+__host__ __device__ inline int64_t weight_units(const PagedSeq& s, int Hkv, int keys) {
+  return s.n && !s.flags ? ((int64_t)s.L + keys - 1) / keys * Hkv : 0;
+}
 int paged_weights_d64(const PagedAttnParams& p, const WeightsParams& w, int bits, bool bf16, hipStream_t stream);
 int paged_weights_d96(const PagedAttnParams& p, const WeightsParams& w, int bits, bool bf16, hipStream_t stream);
 int paged_weights_d128(const PagedAttnParams& p, const WeightsParams& w, int bits, bool bf16, hipStream_t stream);
@@ -363,12 +370,15 @@ __device__ __forceinline__ int64_t wave_scan(int64_t x, int lane, int count = 64
 }
 
 // Work-groups take the units of all sequences in turn: `count` says how many a
-// sequence has, `work` does unit i of sequence s, the u-th of all.
-template <typename Count, typename Work>
+// sequence has, `work` does unit i of sequence s, the u-th of all.  WHOLE: row ranges
+// that do not ascend leave the batch no units at all, else those sequences alone.
+template <bool WHOLE, typename Count, typename Work>
 __device__ __forceinline__ void walk_units(const PagedView& c, Count count, Work work) {
   const int lane = threadIdx.x & 63;
   int64_t base = 0, u = blockIdx.x;            // units before these sequences, the next one of this work-group
   int flags = 0;
+  if (WHOLE)                                   // the first 64 are read before any unit
+    for (int s = 64 + lane; s < c.B; s += 64) flags |= paged_seq(c, s).flags;
   for (int s0 = 0; s0 < c.B; s0 += 64) {
     PagedSeq mine = {};
     int64_t n = 0;
@@ -377,6 +387,7 @@ __device__ __forceinline__ void walk_units(const PagedView& c, Count count, Work
       flags |= mine.flags;
       if (!mine.flags) n = count(mine);
     }
+    if (WHOLE && __builtin_amdgcn_ballot_w64(flags & LVSA_PAGED_BAD_CU)) break;
     const int64_t upto = wave_scan(n, lane), end = base + from_lane(upto, 63);
     for (; u < end; u += gridDim.x) {
       const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(base + upto > u));

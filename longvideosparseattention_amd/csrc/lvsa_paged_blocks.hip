@@ -37,7 +37,7 @@ __global__ __launch_bounds__(256) void paged_means_kernel(MeansParams p) {
     if (s.L == 0 || (p.c.cu && s.n == 0)) return (int64_t)0;
     return ((int64_t)((s.L - 1) / p.block) + 1 - first_block(s)) * p.c.Hkv;
   };
-  walk_units(p.c, count, [&](int seq, const PagedSeq& sq, int64_t u, int64_t) __attribute__((always_inline)) {
+  walk_units<false>(p.c, count, [&](int seq, const PagedSeq& sq, int64_t u, int64_t) __attribute__((always_inline)) {
     const int i = (int)quotient(u, p.c.Hkv), h = (int)(u - (int64_t)i * p.c.Hkv);
     const int b = first_block(sq) + i, entry = b / p.parts, part = b - entry * p.parts.by;
     const int page = p.c.table[seq * p.c.table_str + entry];
@@ -752,6 +752,7 @@ WeightsShape weights_shape(const lvsa_paged_weights_args* a) {
   WeightsShape s{};
   // rows of a sequence, if unknown: one each where there are no more than sequences, else all of one
   const int64_t N = a->batch.N, q = a->max_q_len > 0 ? (a->max_q_len < N ? a->max_q_len : N) : N <= a->batch.B ? 1 : N;
+  // sequences that have work: see weight_units
   const int64_t rows = q * (a->H / a->cache.Hkv), B = a->batch.B < N ? a->batch.B : N, cus = cu_count();
   // The rows' kernel from 48 rows a sequence and key head on: us, few rows' and rows'
   // kernel, 8 sequences of 8000 keys, 8 heads of 128: 16 rows 31, 51; 32 42, 51; 48 50,

@@ -32,9 +32,7 @@ __global__ __launch_bounds__(256, kWeightGroups) void paged_weights_kernel(Paged
   PagedSeq mine = {};
   int64_t n_mine = 0, upto = 0, U = 0;
   int flags = 0;
-  auto units_of = [&](const PagedSeq& s) __attribute__((always_inline)) {
-    return s.n && !s.flags ? (int64_t)p.c.Hkv * (((int64_t)s.L + KEYS - 1) / KEYS) : (int64_t)0;
-  };
+  auto units_of = [&](const PagedSeq& s) __attribute__((always_inline)) { return weight_units(s, p.c.Hkv, KEYS); };
   auto read_batch = [&](int s0) __attribute__((always_inline)) {
     n_mine = 0;
     if (s0 + lane < B) {
@@ -49,7 +47,7 @@ __global__ __launch_bounds__(256, kWeightGroups) void paged_weights_kernel(Paged
     U += from_lane(upto, B - s0 < 64 ? B - s0 - 1 : 63);
   }
   if (blockIdx.x == 0 && wave == 0 && flags) paged_flag(p.c, flags);
-  if (U == 0) return;
+  if (U == 0 || __builtin_amdgcn_ballot_w64(flags & LVSA_PAGED_BAD_CU)) return;
   const int shares = unit_shares(U, p.grid);
   if ((int)blockIdx.x >= shares) return;
   int64_t u = unit_start(U, shares, blockIdx.x);
@@ -242,10 +240,8 @@ __global__ __launch_bounds__(256, D <= 96 ? 3 : 2) void paged_weights_rows_kerne
   auto at_lds = [](int r, int c) __attribute__((always_inline)) {
     return RB * r + 16 * (c ^ (D == 96 ? r >> 2 & 3 : D == 64 || D == 192 ? r >> 1 & 7 : r & 15));
   };
-  auto count = [&](const PagedSeq& s) __attribute__((always_inline)) {
-    return s.n ? ((int64_t)s.L + KEYS - 1) / KEYS * p.c.Hkv * wp.splits : (int64_t)0;
-  };
-  walk_units(p.c, count, [&](int seq, const PagedSeq& sq, int64_t u, int64_t id) __attribute__((always_inline)) {
+  auto count = [&](const PagedSeq& s) __attribute__((always_inline)) { return weight_units(s, p.c.Hkv, KEYS) * wp.splits; };
+  walk_units<true>(p.c, count, [&](int seq, const PagedSeq& sq, int64_t u, int64_t id) __attribute__((always_inline)) {
     const int64_t unit = quotient(u, wp.splits);
     const int split = (int)(u - unit * wp.splits);
     const int chunk = (int)quotient(unit, p.c.Hkv), h = (int)(unit - (int64_t)chunk * p.c.Hkv);
@@ -405,10 +401,8 @@ __global__ __launch_bounds__(256, D <= 96 ? 3 : 2) void paged_weights_rows_kerne
 
 // Adds the sums of work-groups that share their rows: a thread per key.
 __global__ __launch_bounds__(kWeightKeys) void paged_weights_merge_kernel(PagedAttnParams p, WeightsParams wp) {
-  auto count = [&](const PagedSeq& s) __attribute__((always_inline)) {
-    return s.n ? ((int64_t)s.L + kWeightKeys - 1) / kWeightKeys * p.c.Hkv : (int64_t)0;
-  };
-  walk_units(p.c, count, [&](int seq, const PagedSeq& sq, int64_t u, int64_t id) __attribute__((always_inline)) {
+  auto count = [&](const PagedSeq& s) __attribute__((always_inline)) { return weight_units(s, p.c.Hkv, kWeightKeys); };
+  walk_units<true>(p.c, count, [&](int seq, const PagedSeq& sq, int64_t u, int64_t id) __attribute__((always_inline)) {
     const int chunk = (int)quotient(u, p.c.Hkv), h = (int)(u - (int64_t)chunk * p.c.Hkv);
     const int key = chunk * kWeightKeys + (int)threadIdx.x;
     if (key >= sq.L) return;

@@ -266,8 +266,8 @@ def paged_kv_weights(q: torch.Tensor, lse: torch.Tensor, cache: PagedKVCache, we
     The newest tokens' own weights start from 0, so slots need no clearing before; with
     ``accumulate=False`` all of the sequence's do (the weights of one chunk alone).
     Rows whose ``lse`` is not finite give nothing.  Sequences without new rows or with a
-    bad length or row range, tokens on bad pages and slots of no sequence are left
-    alone.  Sequences that share pages must not be in one call (each would add to the
+    bad length, tokens on bad pages and slots of no sequence are left alone, and all
+    where ``cu_seqlens`` does not ascend.  Sequences that share pages must not be in one call (each would add to the
     same weights).  Scores and sums are fp32, in an order that follows from the shapes
     alone.  ``max_q_len`` (the most rows of a sequence) only chooses a kernel."""
     if is_compiling():

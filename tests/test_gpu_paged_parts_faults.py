@@ -1,0 +1,67 @@
+"""Calls of the paged cache's parts that once went wrong (see test_gpu_paged_parts_edges.py)."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import longvideosparseattention_amd as lv
+from longvideosparseattention_amd import _capi, hip_ops
+
+from paged_ref import Batch
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+# ── row ranges that do not ascend, each of them fine by itself ───────────────
+
+
+def _weights_args(b, q, lse, weights, cu, max_q_len):
+    a = _capi.PagedWeightsArgs()
+    C.memmove(C.addressof(a), b.cache._pack(b.dtype), C.sizeof(_capi.PagedCache))
+    a.batch.cu_seqlens, a.batch.kv_lens, a.batch.page_table = cu.data_ptr(), b.lens.data_ptr(), b.table_dev.data_ptr()
+    a.batch.table_stride, a.batch.B, a.batch.max_pages = b.table_dev.stride(0), b.table_dev.shape[0], b.table_dev.shape[1]
+    a.batch.N, a.H, a.scale, a.causal, a.accumulate, a.max_q_len = q.shape[0], q.shape[1], 1 / math.sqrt(b.D), 1, 1, max_q_len
+    a.q, a.lse, a.weights = q.data_ptr(), lse.data_ptr(), weights.data_ptr()
+    a.q_str, a.w_str = _capi._Str2(*q.stride()[:2]), _capi._Str3(*weights.stride())
+    return a
+
+
+@pytest.mark.parametrize("B,N,H,L", [(200, 64, 4, 128), (64, 16, 32, 500)])
+def test_weights_stay_within_their_workspace(gpu, B, N, H, L):
+    """Every second sequence has all the rows: more sequences with rows than there are rows."""
+    b = Batch(gpu, [(0, L)] * B, 64, H, 1, 64, BF, seed=40)
+    q, lse = b.randn(N, H, 64), torch.zeros(N, H, device=gpu)
+    weights = b.cache.allocate_weights().fill_(2.0)
+    cu = torch.tensor([N * (i % 2) for i in range(B + 1)], dtype=torch.int32, device=gpu)
+    a, need = _weights_args(b, q, lse, weights, cu, N), C.c_int64()
+    assert _capi.lib().lvsa_paged_weights_workspace_query(C.byref(a), C.byref(need)) == 0 and need.value > 0
+    room = torch.full((4 * need.value // 4,), 77.0, device=gpu)
+    a.workspace, a.workspace_bytes = room.data_ptr(), need.value
+    hip_ops._call(b.cache.device, "lvsa_paged_weights", C.byref(a))
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        b.cache.check()
+    assert (room[need.value // 4:] == 77.0).all()
+    assert (weights == 2.0).all()
+
+
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("hint", [None, 1, 1000])
+@pytest.mark.parametrize("B", [4, 150])
+def test_weights_of_a_batch_whose_rows_do_not_ascend_are_left_alone(gpu, B, hint, n):
+    b = Batch(gpu, [(n, 100)] * B, 64, 4, 2, 16, BF, seed=41)
+    q, lse = b.randn(b.N, 4, 64), torch.zeros(b.N, 4, device=gpu)
+    weights = b.cache.allocate_weights().fill_(2.0)
+    fine = b.cu.tolist()
+    for at, value in ((B - 1, fine[-1] + 1), (1, fine[0] - 1), (B, fine[-1] + 1), (2, 0 if n > 1 else -1), (B - 1, 0)):
+        cu = list(fine)
+        cu[at] = value
+        lv.paged_kv_weights(q, lse, b.cache, weights, torch.tensor(cu, dtype=torch.int32, device=gpu), b.lens, b.table_dev, max_q_len=hint)
+        with pytest.raises(ValueError, match="cu_seqlens"):
+            b.cache.check()
+        assert (weights == 2.0).all(), (at, value)
+    lv.paged_kv_weights(q, lse, b.cache, weights, *b.call(), max_q_len=hint)
+    b.cache.check()
+    got = torch.stack([weights[p, 0, 0] for x in b.pages for p in x[:1]])
+    assert (got != 2.0).all()
