@@ -26,6 +26,63 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
 }
 
 constexpr int kEvictHeld = 32;             // ranks that a thread of the selection holds
+constexpr int kEvictSet = 1024;            // new pages that are few: their set is in LDS
+
+// Page numbers in memory that has twice as many places: each at the first free place
+// from a hash of it on, so that a search ends.  For a work-group of 1024.
+struct PageSet {
+  int* at;
+  uint32_t places;
+  __device__ __forceinline__ uint32_t first(int page) const { return (uint32_t)((uint64_t)((uint32_t)page * 0x9e3779b1u) * places >> 32); }
+  __device__ __forceinline__ uint32_t next(uint32_t i) const { return i + 1 < places ? i + 1 : 0; }
+  __device__ __forceinline__ void clear() const {
+    for (uint32_t i = threadIdx.x; i < places; i += 1024) __hip_atomic_store(&at[i], -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __device__ __forceinline__ void add(int page) const {
+    for (uint32_t i = first(page);; i = next(i)) {
+      const int was = atomicCAS(&at[i], -1, page);
+      if (was == -1 || was == page) return;
+    }
+  }
+  __device__ __forceinline__ bool holds(int page) const {
+    for (uint32_t i = first(page);; i = next(i)) {
+      const int here = __hip_atomic_load(&at[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (here == -1 || here == page) return here == page;
+    }
+  }
+};
+
+// Whether one of many new pages lies outside the cache or is an old one of the
+// sequence, as far as this thread sees, in the time of reading both tables: with a set
+// in `row`, the head's part of `kept`, which has a place for every kept token and is
+// written behind this (half of them at a time where pages are single tokens).
+__device__ __forceinline__ bool many_pages_meet(const PagedView& c, const int32_t* table, int pages, const int32_t* to, int news,
+                                                int32_t* row, int keep) {
+  const PageSet set = {row, (uint32_t)keep};
+  const int some = keep / 2;
+  bool odd = false;
+  auto meet = [&]() __attribute__((always_inline)) {
+    __threadfence();
+    __syncthreads();
+  };
+  for (int i0 = 0; i0 < news; i0 += some) {
+    const int i1 = news - i0 < some ? news : i0 + some;
+    set.clear();
+    meet();
+    for (int i = i0 + (int)threadIdx.x; i < i1; i += 1024) {
+      const int page = to[i];
+      if ((uint32_t)page < (uint32_t)c.n_pages) set.add(page);
+      else odd = true;
+    }
+    meet();
+    for (int e = threadIdx.x; e < pages; e += 1024) {
+      const int page = table[e];
+      if ((uint32_t)page < (uint32_t)c.n_pages) odd |= set.holds(page);
+    }
+    meet();
+  }
+  return odd;
+}
 
 // One work-group per sequence and head: finds the keep-th highest weight by halving the
 // range of the ranks, which its threads hold (R each, or read again in every step where
@@ -40,7 +97,7 @@ __global__ __launch_bounds__(1024) void paged_evict_select_kernel(EvictParams p)
   __shared__ int count_s[2][16];
   __shared__ int gt_s[16], eq_s[16];
   __shared__ uint32_t lo_s[16], hi_s[16];
-  __shared__ int bad_s, new_s[1024];
+  __shared__ int bad_s, set_s[2 * kEvictSet];
   const int Hkv = p.c.Hkv, tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   for (int64_t u = blockIdx.x; u < (int64_t)p.c.B * Hkv; u += gridDim.x) {
     const int b = (int)quotient(u, Hkv), h = (int)(u - (int64_t)b * Hkv);
@@ -75,23 +132,25 @@ __global__ __launch_bounds__(1024) void paged_evict_select_kernel(EvictParams p)
         for (int k = 0; k < R; ++k) held[k] = __builtin_bit_cast(uint32_t, *reinterpret_cast<const float*>(p.w + at[k]));
       }
     }
+    const int pages = L > 0 ? page_of(p.c, L - 1) + 1 : 0, news = left > 0 ? page_of(p.c, left - 1) + 1 : 0;
+    const bool few = to && news <= kEvictSet;
+    const PageSet set = {set_s, 2 * kEvictSet};
+    const int fresh = few && tid < news ? to[tid] : 0;
     __syncthreads();                       // LDS of the head before has been read
     if (tid == 0) bad_s = sq.flags;
+    if (few) set.clear();
     __syncthreads();
-    const int pages = L > 0 ? page_of(p.c, L - 1) + 1 : 0, news = left > 0 ? page_of(p.c, left - 1) + 1 : 0;
-    bool odd = false;
-    for (int e = tid; e < pages; e += 1024) odd |= (uint32_t)table[e] >= (uint32_t)p.c.n_pages;
-    for (int i0 = 0; to && i0 < news; i0 += 1024) {      // a new page that is an old one
-      const int here = news - i0 < 1024 ? news - i0 : 1024;
+    bool odd = (uint32_t)fresh >= (uint32_t)p.c.n_pages;       // a page outside the cache, or a new one that is an old one
+    if (few) {
+      if (tid < news && !odd) set.add(fresh);
       __syncthreads();
-      if (tid < here) new_s[tid] = to[i0 + tid];
-      __syncthreads();
-      odd |= tid < here && (uint32_t)new_s[tid] >= (uint32_t)p.c.n_pages;
-      for (int e = tid; e < pages; e += 1024) {
-        const int page = table[e];
-#pragma unroll 8
-        for (int i = 0; i < here; ++i) odd |= new_s[i] == page;
-      }
+    } else if (to) {
+      odd |= many_pages_meet(p.c, table, pages, to, news, kept, p.keep);
+    }
+    for (int e = tid; e < pages; e += 1024) {
+      const int page = table[e];
+      const bool in = (uint32_t)page < (uint32_t)p.c.n_pages;
+      odd |= !in || (few && set.holds(page));
     }
     if (odd) atomicOr(&bad_s, LVSA_PAGED_BAD_PAGE);
     __syncthreads();

@@ -65,3 +65,65 @@ def test_weights_of_a_batch_whose_rows_do_not_ascend_are_left_alone(gpu, B, hint
     b.cache.check()
     got = torch.stack([weights[p, 0, 0] for x in b.pages for p in x[:1]])
     assert (got != 2.0).all()
+
+
+# ── eviction to new pages of long sequences ──────────────────────────────────
+
+
+def _one_long(gpu, page, L, keep, seed=42):
+    """One sequence over a shuffled pool, random weights, and pages for what is kept of it."""
+    g = torch.Generator().manual_seed(seed)
+    old, new = -(-L // page), -(-keep // page)
+    cache = lv.PagedKVCache.allocate(old + new + 3, page, 1, 64, device=gpu)
+    order = torch.randperm(old + new + 3, generator=g).to(torch.int32)
+    rows = torch.arange(L, dtype=torch.int32)
+    table, to = order[:old], order[old:old + new]
+    at = table.long()[torch.arange(L) // page], torch.arange(L) % page
+    k = torch.zeros(cache.num_pages, page, 1, 2, dtype=torch.int32)
+    k[at[0], at[1], 0, 0] = rows                         # a token's position, in its first four bytes
+    cache.k[..., :4].copy_(k.view(BF).to(gpu))
+    weights, w = cache.allocate_weights(), torch.rand(L, generator=g)
+    like = torch.zeros(cache.num_pages, page, 1)
+    like[at[0], at[1], 0] = w
+    weights.copy_(like)
+    lens = torch.tensor([L], dtype=torch.int32, device=gpu)
+    return cache, weights, w, lens, table[None].to(gpu), to[None].clone()
+
+
+@pytest.mark.parametrize("page,L,keep", [(1, 3000, 2500), (1, 2100, 1025), (2, 9000, 8001), (3, 5000, 3100), (16, 40000, 20001), (1, 40, 30)])
+def test_new_pages_of_a_long_sequence(gpu, page, L, keep):
+    """More new pages than a set in LDS holds: kept ones move, and one old page among them is found wherever it is."""
+    cache, weights, w, lens, table, to = _one_long(gpu, page, L, keep)
+    before = weights.clone()
+    n = to.shape[1]
+    for at, which in ((0, 0), (n - 1, table.shape[1] - 1), (n // 2, 1), (n // 2 - 1, table.shape[1] // 2)):
+        bad = to.clone()
+        bad[0, at] = table[0, which].cpu()
+        got, kept = lv.paged_kv_evict(cache, weights, lens, table, keep, new_table=bad.to(gpu), return_kept=True)
+        with pytest.raises(ValueError, match="page number"):
+            cache.check()
+        assert got.tolist() == [0] and (kept == -1).all() and torch.equal(weights, before)
+    got, kept = lv.paged_kv_evict(cache, weights, lens, table, keep, new_table=to.to(gpu), return_kept=True)
+    cache.check()
+    want = w.sort(descending=True, stable=True)[1][:keep].sort()[0]
+    assert got.tolist() == [keep] and torch.equal(kept[0, 0].cpu().long(), want)
+    i = torch.arange(keep)
+    rows = cache.k[..., :4].cpu()[to[0].long()[i // page], i % page, 0].view(torch.int32)[:, 0]
+    assert torch.equal(rows.long(), want)
+
+
+def test_the_check_of_new_pages_is_linear(gpu):
+    """A million tokens to half a million new pages of one slot: page by page against page that is 5e11 comparisons, about
+    seven seconds by one work-group; the rest of the call is some tens of milliseconds."""
+    cache, weights, w, lens, table, to = _one_long(gpu, 1, 1 << 20, 1 << 19)
+    to = to.to(gpu)
+    lv.paged_kv_evict(cache, weights.clone(), lens[:0], table[:0], 1)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    got, kept = lv.paged_kv_evict(cache, weights, lens, table, 1 << 19, new_table=to, return_kept=True)
+    end.record()
+    torch.cuda.synchronize()
+    cache.check()
+    assert torch.equal(kept[0, 0].cpu().long(), w.sort(descending=True, stable=True)[1][:1 << 19].sort()[0])
+    assert start.elapsed_time(end) < 1500.0, start.elapsed_time(end)
+    print(f"{start.elapsed_time(end):.1f} ms")
