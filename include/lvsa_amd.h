@@ -480,11 +480,11 @@ LVSA_API int lvsa_paged_weights_workspace_query(const lvsa_paged_weights_args* a
  * weights move, in their order, to positions 0 .. keep - 1 on the pages of
  * new_table [B] (rows of new_pages, new_stride apart), or, without it, on the
  * sequence's own first pages.  kept [B, Hkv, keep]: their old positions, -1 behind;
- * new_lens [B]: how many.  A sequence with a bad length or a bad page (a new one
- * that is one of its old ones among them) is not moved: -1, and a length of 0 with
- * new_table, kv_lens' without.  No page of new_table may be another sequence's, in
- * either table, and pages that sequences share are not cut in place.  cu_seqlens
- * and N of the batch are not used.                                            */
+ * new_lens [B]: how many.  A sequence with a bad length or a bad page (of the new
+ * ones that its kept tokens need, one that is an old one of it or comes twice among
+ * them) is not moved: -1, and a length of 0 with new_table, kv_lens' without.  No
+ * page of new_table may be another sequence's, in either table, and pages that
+ * sequences share are not cut in place.  cu_seqlens and N of the batch are not used. */
 typedef struct lvsa_paged_evict_args {
   lvsa_paged_cache cache;
   lvsa_paged_batch batch;

@@ -38,10 +38,11 @@ struct PageSet {
   __device__ __forceinline__ void clear() const {
     for (uint32_t i = threadIdx.x; i < places; i += 1024) __hip_atomic_store(&at[i], -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  __device__ __forceinline__ void add(int page) const {
+  // Whether the page was there already.
+  __device__ __forceinline__ bool add(int page) const {
     for (uint32_t i = first(page);; i = next(i)) {
       const int was = atomicCAS(&at[i], -1, page);
-      if (was == -1 || was == page) return;
+      if (was == -1 || was == page) return was == page;
     }
   }
   __device__ __forceinline__ bool holds(int page) const {
@@ -52,8 +53,8 @@ struct PageSet {
   }
 };
 
-// Whether one of many new pages lies outside the cache or is an old one of the
-// sequence, as far as this thread sees, in the time of reading both tables: with a set
+// Whether one of many new pages lies outside the cache, is an old one of the sequence
+// or comes twice, as far as this thread sees, in the time of reading both tables: with a set
 // in `row`, the head's part of `kept`, which has a place for every kept token and is
 // written behind this (half of them at a time where pages are single tokens).
 __device__ __forceinline__ bool many_pages_meet(const PagedView& c, const int32_t* table, int pages, const int32_t* to, int news,
@@ -71,10 +72,13 @@ __device__ __forceinline__ bool many_pages_meet(const PagedView& c, const int32_
     meet();
     for (int i = i0 + (int)threadIdx.x; i < i1; i += 1024) {
       const int page = to[i];
-      if ((uint32_t)page < (uint32_t)c.n_pages) set.add(page);
-      else odd = true;
+      odd |= (uint32_t)page >= (uint32_t)c.n_pages || set.add(page);
     }
     meet();
+    for (int i = i1 + (int)threadIdx.x; i < news; i += 1024) {
+      const int page = to[i];
+      if ((uint32_t)page < (uint32_t)c.n_pages) odd |= set.holds(page);
+    }
     for (int e = threadIdx.x; e < pages; e += 1024) {
       const int page = table[e];
       if ((uint32_t)page < (uint32_t)c.n_pages) odd |= set.holds(page);
@@ -140,9 +144,9 @@ __global__ __launch_bounds__(1024) void paged_evict_select_kernel(EvictParams p)
     if (tid == 0) bad_s = sq.flags;
     if (few) set.clear();
     __syncthreads();
-    bool odd = (uint32_t)fresh >= (uint32_t)p.c.n_pages;       // a page outside the cache, or a new one that is an old one
+    bool odd = (uint32_t)fresh >= (uint32_t)p.c.n_pages;       // a page outside the cache, or a new one that is an old one or comes twice
     if (few) {
-      if (tid < news && !odd) set.add(fresh);
+      if (tid < news && !odd) odd = set.add(fresh);
       __syncthreads();
     } else if (to) {
       odd |= many_pages_meet(p.c, table, pages, to, news, kept, p.keep);

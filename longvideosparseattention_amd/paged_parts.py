@@ -318,10 +318,11 @@ def paged_kv_evict(cache: PagedKVCache, weights: torch.Tensor, kv_lens: torch.Te
     turned by their positions keep their angles: new tokens' positions go on in
     :func:`paged_kv_append`'s ``positions``.  Means of blocks are the caller's to renew.
 
-    Pages of ``new_table`` belong to nothing else in the call: a sequence that finds
-    one of its old pages there, a page number outside the cache or a bad length is not
-    moved (all ``-1``, its new length 0, in place its old one) and noted in the status;
-    pages of other sequences are not looked for.  Pages that sequences share are not
+    Pages of ``new_table`` belong to nothing else in the call: a sequence that finds,
+    among those that its kept tokens need, one of its old pages, a page twice or a
+    number outside the cache, or has a bad length, is not moved (all ``-1``, its new
+    length 0, in place its old one) and noted in the status; pages of other sequences
+    are not looked for.  Pages that sequences share are not
     to be cut in place."""
     if is_compiling():
         return _outside["evict"](cache, weights, kv_lens, page_table, keep, first=first, last=last, new_table=new_table,

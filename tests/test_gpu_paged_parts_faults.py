@@ -127,3 +127,24 @@ def test_the_check_of_new_pages_is_linear(gpu):
     assert torch.equal(kept[0, 0].cpu().long(), w.sort(descending=True, stable=True)[1][:1 << 19].sort()[0])
     assert start.elapsed_time(end) < 1500.0, start.elapsed_time(end)
     print(f"{start.elapsed_time(end):.1f} ms")
+
+
+@pytest.mark.parametrize("page,L,keep", [(16, 90, 40), (16, 30, 40), (1, 3000, 2500), (2, 9000, 8001), (16, 40000, 20001)])
+def test_a_new_page_that_comes_twice(gpu, page, L, keep):
+    """Two places of the kept tokens in one page: the sequence is not moved.  Behind the pages that it needs anything goes."""
+    cache, weights, w, lens, table, to = _one_long(gpu, page, L, keep, seed=43)
+    before, k = weights.clone(), cache.k.clone()
+    need = -(-min(L, keep) // page)
+    for a, z in {(0, need - 1), (need // 2, need - 1), (0, need // 2), (need - 2, need - 1)} - {(i, i) for i in range(need)}:
+        bad = to.clone()
+        bad[0, z] = bad[0, a]
+        got, kept = lv.paged_kv_evict(cache, weights, lens, table, keep, new_table=bad.to(gpu), return_kept=True)
+        with pytest.raises(ValueError, match="page number"):
+            cache.check()
+        assert got.tolist() == [0] and (kept == -1).all() and torch.equal(weights, before)
+        assert torch.equal(cache.k.view(torch.int16), k.view(torch.int16))          # bits: positions are no numbers
+    more = torch.cat((to[:, :need], to[:, :1].expand(1, to.shape[1] - need + 2)), 1).contiguous()
+    got, kept = lv.paged_kv_evict(cache, weights, lens, table, keep, new_table=more.to(gpu), return_kept=True)
+    cache.check()
+    assert got.tolist() == [min(L, keep)]
+    assert torch.equal(kept[0, 0, :min(L, keep)].cpu().long(), w.sort(descending=True, stable=True)[1][:keep].sort()[0])
