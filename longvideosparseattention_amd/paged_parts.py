@@ -332,6 +332,8 @@ def paged_kv_evict(cache: PagedKVCache, weights: torch.Tensor, kv_lens: torch.Te
     B, pages = page_table.shape
     if not 1 <= keep < (1 << 31) - 4097 or first < 0 or last < 0 or first + last > keep:
         raise ValueError(f"{keep} tokens to keep, the first {first} and the last {last} among them")
+    if keep > pages * cache.page_size and not return_kept:      # all, whatever they are: no list of more than there can be
+        keep, first, last = max(pages * cache.page_size, 1), 0, 0
     to = row = new_pages = 0
     if new_table is not None:
         _int32(new_table, "new_table", 2, cache.device)

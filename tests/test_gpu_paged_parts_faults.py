@@ -148,3 +148,23 @@ def test_a_new_page_that_comes_twice(gpu, page, L, keep):
     cache.check()
     assert got.tolist() == [min(L, keep)]
     assert torch.equal(kept[0, 0, :min(L, keep)].cpu().long(), w.sort(descending=True, stable=True)[1][:keep].sort()[0])
+
+
+@pytest.mark.parametrize("first,last", [(0, 0), (1 << 30, 1 << 29)])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_a_budget_beyond_the_table_costs_no_memory(gpu, in_place, first, last):
+    """As many tokens as there may be, for "all": the list of those that stay would be 343 GB, and nobody asks for it."""
+    b = Batch(gpu, [(0, 20 + i) for i in range(10)], 64, 4, 4, 16, BF, seed=44, spare=40)
+    weights = b.cache.allocate_weights().copy_(torch.rand(b.cache.num_pages, 16, 4, generator=b.gen))
+    free = sorted(set(range(b.cache.num_pages)) - {p for x in b.pages for p in x})
+    to = torch.tensor(free[:20], dtype=torch.int32).view(10, 2)
+    k, w = b.cache.k.cpu(), weights.cpu()
+    got = lv.paged_kv_evict(b.cache, weights, b.lens, b.table_dev, (1 << 31) - 5000, first=first, last=last,
+                            new_table=None if in_place else to.to(gpu))
+    b.cache.check()
+    assert torch.equal(got, b.lens)
+    for s, (_, L) in enumerate(b.seqs):
+        at = b.pages[s] if in_place else to[s].tolist()
+        i = torch.arange(L)
+        now, was = torch.tensor(at)[i // 16], torch.tensor(b.pages[s])[i // 16]
+        assert torch.equal(b.cache.k.cpu()[now, i % 16], k[was, i % 16]) and torch.equal(weights.cpu()[now, i % 16], w[was, i % 16])
