@@ -340,14 +340,14 @@ def paged_kv_evict(cache: PagedKVCache, weights: torch.Tensor, kv_lens: torch.Te
         new_pages = new_table.shape[1]
         if new_table.shape[0] != B:
             raise ValueError(f"new_table has {new_table.shape[0]} sequences, page_table {B}")
-        if B and new_table.data_ptr() == page_table.data_ptr():
+        if B and new_pages and new_table.data_ptr() == page_table.data_ptr():
             raise ValueError("new_table is page_table: leave it out to cut sequences where they lie")
         if new_pages * cache.page_size < min(keep, pages * cache.page_size):
             raise ValueError(f"{new_pages} new pages of {cache.page_size} slots do not hold {keep} tokens")
         row = new_table.stride(0) if B > 1 else new_pages
         if row < new_pages:
             raise ValueError("new_table rows overlap")
-        to = new_table.data_ptr()
+        to = new_table.data_ptr() or kv_lens.data_ptr()          # no page of an empty table is read; null would be "in place"
     lens = torch.empty(B, dtype=torch.int32, device=cache.device)
     kept = torch.empty(B, cache.num_kv_heads, keep, dtype=torch.int32, device=cache.device)
     if B:

@@ -168,3 +168,22 @@ def test_a_budget_beyond_the_table_costs_no_memory(gpu, in_place, first, last):
         i = torch.arange(L)
         now, was = torch.tensor(at)[i // 16], torch.tensor(b.pages[s])[i // 16]
         assert torch.equal(b.cache.k.cpu()[now, i % 16], k[was, i % 16]) and torch.equal(weights.cpu()[now, i % 16], w[was, i % 16])
+
+
+def test_tables_without_pages(gpu):
+    """Sequences that have never had a page, to new pages and in place; a length that says otherwise is a bad one."""
+    cache = lv.PagedKVCache.allocate(3, 16, 2, 64, device=gpu)
+    weights = cache.allocate_weights()
+    none = torch.zeros(2, 0, dtype=torch.int32, device=gpu)
+    some = torch.tensor([[0], [1]], dtype=torch.int32, device=gpu)
+    for lens, fine in (([0, 0], True), ([5, 0], False)):
+        lens = torch.tensor(lens, dtype=torch.int32, device=gpu)
+        for to in (none.clone(), some[:, :0], some, None):
+            for keep in (1, 7):
+                got, kept = lv.paged_kv_evict(cache, weights, lens, none, keep, new_table=to, return_kept=True)
+                assert got.tolist() == ([0, 0] if fine or to is not None else lens.tolist()) and (kept == -1).all()
+        if fine:
+            cache.check()
+        else:
+            with pytest.raises(ValueError, match="kv_lens"):
+                cache.check()
