@@ -484,7 +484,8 @@ LVSA_API int lvsa_paged_weights_workspace_query(const lvsa_paged_weights_args* a
  * ones that its kept tokens need, one that is an old one of it or comes twice among
  * them) is not moved: -1, and a length of 0 with new_table, kv_lens' without.  No
  * page of new_table may be another sequence's, in either table, and pages that
- * sequences share are not cut in place.  cu_seqlens and N of the batch are not used. */
+ * sequences share are not cut in place.  cu_seqlens and N of the batch are not used.
+ * kept and new_lens share no memory with each other, kv_lens and the tables (refused). */
 typedef struct lvsa_paged_evict_args {
   lvsa_paged_cache cache;
   lvsa_paged_batch batch;

@@ -429,6 +429,13 @@ __global__ __launch_bounds__(256) void paged_evict_slide_kernel(EvictParams p, i
 
 constexpr int64_t kMostGroups = 1 << 20;
 
+// An array of a call.
+struct Ints {
+  const int32_t* at;
+  int64_t n;
+  bool meets(const Ints& o) const { return at && o.at && n > 0 && o.n > 0 && at < o.at + o.n && o.at < at + n; }
+};
+
 template <int D, typename E, int BITS> struct Evict {
   static int go(const EvictParams& p, hipStream_t stream) {
     const int64_t bh = (int64_t)p.c.B * p.c.Hkv;
@@ -477,6 +484,13 @@ int lvsa_paged_evict(const lvsa_paged_evict_args* a, hipStream_t stream) {
                "%s: %d new pages of %d slots do not hold %d tokens", what, a->new_pages, a->cache.page_size, a->keep);
   if (a->batch.B == 0) return LVSA_OK;
   LVSA_REQUIRE(a->kept && a->new_lens, LVSA_ERR_INVALID_ARG, "%s: null kept or new_lens", what);
+  // Other heads' work-groups, and the moves, read what the first one would have written over.
+  const int64_t B = a->batch.B;
+  const Ints lens = {a->batch.kv_lens, B}, table = {a->batch.page_table, (B - 1) * a->batch.table_stride + a->batch.max_pages};
+  const Ints to = {a->new_table, (B - 1) * a->new_stride + a->new_pages};
+  const Ints kept = {a->kept, B * a->cache.Hkv * a->keep}, out = {a->new_lens, B};
+  LVSA_REQUIRE(!out.meets(lens) && !out.meets(table) && !out.meets(to) && !out.meets(kept) && !kept.meets(lens) && !kept.meets(table) &&
+                   !kept.meets(to), LVSA_ERR_INVALID_ARG, "%s: kept and new_lens must not share memory with each other, kv_lens and the tables", what);
   p.c.cu = nullptr;
   p.w = (char*)a->weights;
   for (int i = 0; i < 3; ++i) p.w_str[i] = 4 * a->w_str[i];
