@@ -66,8 +66,8 @@ __device__ __forceinline__ bool many_pages_meet(const PagedView& c, const int32_
     __threadfence();
     __syncthreads();
   };
-  for (int i0 = 0; i0 < news; i0 += some) {
-    const int i1 = news - i0 < some ? news : i0 + some;
+  for (int i0 = 0, i1 = 0; i1 < news; i0 = i1) {
+    i1 = news - i0 < some ? news : i0 + some;
     set.clear();
     meet();
     for (int i = i0 + (int)threadIdx.x; i < i1; i += 1024) {
