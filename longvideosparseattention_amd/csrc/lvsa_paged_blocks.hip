@@ -751,6 +751,8 @@ struct WeightsShape {
 WeightsShape weights_shape(const lvsa_paged_weights_args* a) {
   WeightsShape s{};
   // rows of a sequence, if unknown: one each where there are no more than sequences, else all of one
+  // (8 sequences of 2, 4 and 9 rows, 4 query heads a key head, over 8000 keys: 52 to 53 us
+  // without max_q_len, 30, 31 and 47 with it)
   const int64_t N = a->batch.N, q = a->max_q_len > 0 ? (a->max_q_len < N ? a->max_q_len : N) : N <= a->batch.B ? 1 : N;
   // sequences that have work: see weight_units
   const int64_t rows = q * (a->H / a->cache.Hkv), B = a->batch.B < N ? a->batch.B : N, cus = cu_count();
@@ -764,7 +766,10 @@ WeightsShape weights_shape(const lvsa_paged_weights_args* a) {
   if (units < 1) units = 1;
   if (s.many) {
     // 12 work-groups a compute unit, if the table is full: 92, 87, 82, 85 us with 4, 8, 12
-    // and 16 for 6500 tokens of prompts over up to 5200 keys, 4 heads
+    // and 16 for 6500 tokens of prompts over up to 5200 keys, 4 heads of 64 (no other shape
+    // was tried).  A wider table counts as full, too: 113 instead of 85 us in one of 32768
+    // slots and more; one stream's 500 tokens over 5000 keys 66 us, 47, 59 and 88 in tables
+    // of 32768, 65536 and 131072.
     const int64_t want = ceil_div(12 * cus, units), tiles = ceil_div(rows, 128);
     s.splits = (int)(want < tiles ? want : tiles);
     s.bytes = s.splits == 1 ? 0 : 4 * units * s.splits * kWeightKeys;
@@ -827,6 +832,9 @@ int lvsa_paged_select(const lvsa_paged_select_args* a, hipStream_t stream) {
   //   sequence): 20, 19 and 25, 18; 2048 (8 and 256): 24, 33 and 25, 33; 16384: 59, 227
   //   rows of a list, its tokens x query heads, 16384 lists x heads: 4: 59, 227; 16: 100,
   //   248; 4096 of 16: 52, 65; 2080 of 32: 50, 36
+  // LDS has room for 1024 ranks a list: a wider table goes the other way, whatever its
+  // sequences fill of it (6500 tokens of prompts over up to 325 blocks 312 us, 79 in a table
+  // of 325).
   const int64_t cap = (int64_t)a->batch.max_pages * p.v.parts.by;
   const bool grouped = (int64_t)a->tile * p.group <= 16 && p.v.lists >= 8LL * a->batch.B &&
                        (int64_t)p.v.lists * a->cache.Hkv >= 6LL * cu_count() && cap <= kWaveKeys;
