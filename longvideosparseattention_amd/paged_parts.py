@@ -272,9 +272,10 @@ def paged_kv_weights(q: torch.Tensor, lse: torch.Tensor, cache: PagedKVCache, we
     bad length, tokens on bad pages and slots of no sequence are left alone, and all
     where ``cu_seqlens`` does not ascend.  Sequences that share pages must not be in one
     call (each would add to the same weights).  Scores and sums are fp32, in an order that
-    follows from the shapes alone.  ``max_q_len`` (the most rows of a sequence) only chooses a kernel: without it
-    more rows than sequences are taken for one long sequence, which runs slower for a few
-    rows of each (8 sequences of 2 rows over 8000 keys 52 instead of 30 us)."""
+    follows from the shapes alone.  ``max_q_len`` (the most rows of a sequence) only
+    chooses a kernel: without it more rows than sequences are taken for one long sequence,
+    which runs slower for a few rows of each (8 sequences of 2 rows over 8000 keys 52
+    instead of 30 us)."""
     if is_compiling():
         return _outside["weights"](q, lse, cache, weights, cu_seqlens, kv_lens, page_table, causal=causal, scale=scale,
                                    accumulate=accumulate, max_q_len=max_q_len)
@@ -329,8 +330,7 @@ def paged_kv_evict(cache: PagedKVCache, weights: torch.Tensor, kv_lens: torch.Te
     among those that its kept tokens need, one of its old pages, a page twice or a
     number outside the cache, or has a bad length, is not moved (all ``-1``, its new
     length 0, in place its old one) and noted in the status; pages of other sequences
-    are not looked for.  Pages that sequences share are not
-    to be cut in place."""
+    are not looked for.  Pages that sequences share are not to be cut in place."""
     if is_compiling():
         return _outside["evict"](cache, weights, kv_lens, page_table, keep, first=first, last=last, new_table=new_table,
                                  return_kept=return_kept)
